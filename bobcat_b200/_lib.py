@@ -34,6 +34,16 @@ class ProfileEntry(C.Structure):
     _fields_ = [("name", C.c_char_p), ("n_rows", u32), ("n_cols", u32), ("calls", u64), ("seconds", C.c_double), ("bytes", u64)]
 
 
+class KvPool(C.Structure):
+    _fields_ = [("format", i32)] + [(n, u32) for n in ("n_pages", "page_size", "n_kv_heads", "head_dim")] + [
+        ("k", vp), ("k_off", sz), ("v", vp), ("v_off", sz)]
+
+
+class KvRows(C.Structure):
+    _fields_ = [(n, u32) for n in ("n_seqs", "n_rows", "max_queries", "max_pages")] + [
+        ("table", vp), ("table_off", sz), ("starts", vp), ("starts_off", sz), ("lens", vp), ("lens_off", sz)]
+
+
 EMIT_FN = C.CFUNCTYPE(i32, u32, vp)
 
 # name -> (restype, argtypes). `None` restype means void; the default restype is the status code.
@@ -48,6 +58,7 @@ SIGNATURES = {
     "bc_buffer_free": (None, [vp]),
     "bc_buffer_len": (sz, [vp]),
     "bc_buffer_device_ptr": (vp, [vp]),
+    "bc_buffer_at": (i32, [vp, vp, sz, C.POINTER(vp)]),
     "bc_buffer_write": (i32, [vp, sz, vp, sz]),
     "bc_buffer_read": (i32, [vp, sz, vp, sz]),
     "bc_matrix_upload": (i32, [vp, i32, vp, u32, u32, C.POINTER(vp)]),
@@ -73,6 +84,11 @@ SIGNATURES = {
     "bc_op_attention": (i32, [vp] + _VIEW + _VIEW + _VIEW + [i32] + _VIEW + _VIEW + [u32] * 6),
     "bc_attention_scratch_floats": (sz, [u32, u32, u32, u32]),
     "bc_attention_static": (i32, [vp, vp, vp, vp, i32, vp] + [u32] * 6),
+    "bc_kv_pool_bytes": (sz, [i32] + [u32] * 4),
+    "bc_op_kv_write": (i32, [vp, C.POINTER(KvPool), C.POINTER(KvRows)] + _VIEW + _VIEW + [u32] * 2),
+    "bc_op_kv_read": (i32, [vp, C.POINTER(KvPool), C.POINTER(KvRows)] + _VIEW + _VIEW + [i32] + [u32] * 2),
+    "bc_attention_paged_scratch_floats": (sz, [u32] * 3),
+    "bc_op_attention_paged": (i32, [vp, C.POINTER(KvPool), C.POINTER(KvRows)] + _VIEW + _VIEW + _VIEW + [u32] * 3),
     "bc_op_argmax": (i32, [vp] + _VIEW + _VIEW + [u32]),
     "bc_op_sample": (i32, [vp] + _VIEW + [u32] + _VIEW + [u32, C.POINTER(Sampling), f32] + _VIEW),
     "bc_seq_sample": (i32, [vp, C.POINTER(Sampling), f32, vp, sz, C.POINTER(u32)]),

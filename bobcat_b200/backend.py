@@ -11,7 +11,7 @@ import numpy as np
 
 from . import _lib, errors
 
-F32, F16, Q4_0, Q8_0, Q6_K = 0, 1, 2, 8, 14
+F32, F16, Q4_0, Q8_0, Q6_K, I8 = 0, 1, 2, 8, 14, 24
 OVERWRITE, ACCUMULATE, SWIGLU = 0, 1, 2
 
 
@@ -69,6 +69,23 @@ def _v(view):
     return view.buffer._h, view.offset
 
 
+class KvPool(_lib.KvPool):
+    """Pages of keys and values that sequences share (``bc_kv_pool``): ``k`` and ``v`` are views of
+    ``Cuda.kv_pool_bytes`` bytes each."""
+
+    def __init__(self, fmt: int, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, k, v):
+        super().__init__(fmt, n_pages, page_size, n_kv_heads, head_dim, *_v(k), *_v(v))
+        self.holds = (k, v)
+
+
+class KvRows(_lib.KvRows):
+    """The rows of a call over a pool (``bc_kv_rows``): page tables, row starts and lengths are views of 32-bit words."""
+
+    def __init__(self, n_seqs: int, n_rows: int, max_queries: int, max_pages: int, table, starts, lens):
+        super().__init__(n_seqs, n_rows, max_queries, max_pages, *_v(table), *_v(starts), *_v(lens))
+        self.holds = (table, starts, lens)
+
+
 class Readback:
     """Token slots the CPU reads while later recordings still run (``Readback``, backend.rs:324-333)."""
 
@@ -117,6 +134,12 @@ class Cuda:
     def new_buffer(self, n_bytes: int) -> Buffer:
         h = C.c_void_p()
         self._check(self._L.bc_buffer_new(self._h, n_bytes, C.byref(h)))
+        return Buffer(self, h)
+
+    def buffer_at(self, ptr: int, n_bytes: int) -> Buffer:
+        """Device memory of the caller's as a buffer: ops read and write it in place, and the caller keeps it alive."""
+        h = C.c_void_p()
+        self._check(self._L.bc_buffer_at(self._h, ptr, n_bytes, C.byref(h)))
         return Buffer(self, h)
 
     def upload_matrix(self, fmt: int, raw: np.ndarray, n_rows: int, n_cols: int) -> Buffer:
@@ -227,6 +250,22 @@ class Cuda:
 
     def attention_scratch_floats(self, n_heads, head_dim, n_ctx, n_queries) -> int:
         return int(self._L.bc_attention_scratch_floats(n_heads, head_dim, n_ctx, n_queries))
+
+    # ---- a pool of key/value pages (no counterpart in the reference)
+    def kv_pool_bytes(self, fmt, n_pages, page_size, n_kv_heads, head_dim) -> int:
+        return int(self._L.bc_kv_pool_bytes(fmt, n_pages, page_size, n_kv_heads, head_dim))
+
+    def kv_write(self, pool: KvPool, rows: KvRows, k, v, k_stride, v_stride) -> None:
+        self._check(self._L.bc_op_kv_write(self._h, pool, rows, *_v(k), *_v(v), k_stride, v_stride))
+
+    def kv_read(self, pool: KvPool, rows: KvRows, k, v, out_half, k_stride, v_stride) -> None:
+        self._check(self._L.bc_op_kv_read(self._h, pool, rows, *_v(k), *_v(v), int(out_half), k_stride, v_stride))
+
+    def attention_paged(self, pool: KvPool, rows: KvRows, q, scratch, out, n_heads, q_stride, q_head_stride) -> None:
+        self._check(self._L.bc_op_attention_paged(self._h, pool, rows, *_v(q), *_v(scratch), *_v(out), n_heads, q_stride, q_head_stride))
+
+    def attention_paged_scratch_floats(self, n_heads, n_kv_heads, head_dim) -> int:
+        return int(self._L.bc_attention_paged_scratch_floats(n_heads, n_kv_heads, head_dim))
 
     def argmax(self, x, out, n) -> None:
         self._check(self._L.bc_op_argmax(self._h, *_v(x), *_v(out), n))

@@ -40,7 +40,8 @@ bc_status check_range(const bc_backend* backend, const bc_buffer* buffer, size_t
 
 namespace {
 
-// Per device: one word of mapped host memory per kernel file with bounded waits, for the life of the process.
+// Per device: one word of mapped host memory per kernel file with bounded waits, and one for the key/value pool's kernels, for the life of
+// the process.
 constexpr int kWaitWords = 7, kMaxDevices = 64;
 std::atomic<volatile int*> g_wait_words[kMaxDevices];
 
@@ -50,8 +51,8 @@ bc_status set_wait_words(int device) {
     std::lock_guard<std::mutex> lock(mutex);
     if (g_wait_words[device].load()) return BC_OK;
     int* words = nullptr;
-    BC_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&words), kWaitWords * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable));
-    for (int i = 0; i < kWaitWords; ++i) words[i] = 0;
+    BC_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&words), (kWaitWords + 1) * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable));
+    for (int i = 0; i <= kWaitWords; ++i) words[i] = 0;
     BC_CUDA(k::matvec_wait_word(words));
     BC_CUDA(k::matmul_wait_word(words + 1));
     BC_CUDA(k::matmul_half_wait_word(words + 2));
@@ -84,7 +85,16 @@ bc_status kernel_wait_status() {
     if (int code = take(6)) return fail(BC_ERR_EXECUTION, "a delta-rule kernel gave up waiting for its rows (code %d)", code);
     if (int code = take(5)) return fail(BC_ERR_EXECUTION, "a product over experts gave up waiting on its pipeline (code %d)", code);
     if (int code = take(4)) return fail(BC_ERR_EXECUTION, "a product of few rows gave up waiting for its %s (code %d)", code == 2 ? "weights" : "sums", code);
+    if (int code = words[kWaitWords]) {
+        words[kWaitWords] = 0;
+        return fail(BC_ERR_OUT_OF_BOUNDS, code == 1 ? "a page table names a page that the pool does not have" : "a sequence holds more positions than its page table");
+    }
     return BC_OK;
+}
+
+int* page_fault_word(int device) {
+    volatile int* words = device < kMaxDevices ? g_wait_words[device].load() : nullptr;
+    return words ? const_cast<int*>(words) + kWaitWords : nullptr;
 }
 
 }  // namespace bc
@@ -226,7 +236,7 @@ void bc_backend_close(bc_backend* b) {
     if (b->record_start) cudaEventDestroy(b->record_start);
     // Buffers that outlive their backend are orphaned; their frees become no-ops on the pointer.
     for (bc_buffer* buffer : b->buffers) {
-        cudaFree(buffer->ptr);
+        if (buffer->owned) cudaFree(buffer->ptr);
         buffer->ptr = nullptr;
         buffer->expanded.reset();
         buffer->backend = nullptr;
@@ -267,7 +277,7 @@ void bc_buffer_free(bc_buffer* buffer) {
         // until its command buffers complete (crates/bobcat/tests/metal_commands.rs).
         cudaStreamSynchronize(buffer->backend->stream);
         buffer->backend->buffers.erase(buffer);
-        cudaFree(buffer->ptr);
+        if (buffer->owned) cudaFree(buffer->ptr);
     }
     delete buffer;
 }

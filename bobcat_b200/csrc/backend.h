@@ -22,6 +22,7 @@ struct bc_buffer {
     bc_backend* backend = nullptr;
     void* ptr = nullptr;
     size_t len = 0;
+    bool owned = true;  // false: memory of the caller's (bc_buffer_at)
     // Set by bc_matrix_upload: the matrix this buffer holds in the device layout.
     bool is_matrix = false;
     bc::k::Mat matrix;
@@ -95,6 +96,8 @@ namespace bc {
 bc_status check_range(const bc_backend* backend, const bc_buffer* buffer, size_t offset, size_t needed, const char* op);
 // BC_ERR_EXECUTION when a kernel's bounded wait ran out since the last call; clears the record.
 bc_status kernel_wait_status();
+// The word of host memory that the key/value pool's kernels leave a fault in (kv_pool.cuh); null on a device that has none.
+int* page_fault_word(int device);
 
 }  // namespace bc
 

@@ -477,5 +477,29 @@ cudaError_t matmul_exact_experts(cudaStream_t stream, const Mat& w, const Mat* u
 // accumulator, 3: token copy on a free stage, 4: MMA thread on a full stage.
 cudaError_t matmul_wait_word(int* word);
 
+// A pool of key/value pages (bc_kv_pool) and the rows of a call over it (bc_kv_rows).
+struct KvPool {
+    int32_t format;  // BC_F16 or BC_I8
+    uint32_t n_pages, page_shift, n_kv_heads, head_dim;
+    uint32_t row_bytes;   // of one position of one head, without its scale
+    uint64_t page_bytes;  // of a page in either pool
+    uint8_t *k, *v;
+    int* fault;  // word of host memory: a page or a position that is not there (kv_pool.cuh)
+};
+struct KvRows {
+    const uint32_t *table, *starts, *lens;
+    uint32_t n_seqs, n_rows, max_queries, max_pages;
+};
+// New rows into the pool and back (kernels_kv_pool.cu). Strides in elements per token row.
+cudaError_t kv_write(cudaStream_t stream, const KvPool& pool, const KvRows& rows, const float* k, const float* v, uint64_t k_stride, uint64_t v_stride);
+cudaError_t kv_read(cudaStream_t stream, const KvPool& pool, const KvRows& rows, void* k, void* v, bool out_half, uint64_t k_stride, uint64_t v_stride);
+// Attention of the rows over the pool (kernels_attention_paged.cu). Its partial sums depend on the CTAs of a launch alone, of which there are
+// at most kPagedMostCtas on any device.
+constexpr uint32_t kPagedMostCtas = 320;
+uint64_t attention_paged_scratch_floats(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
+int attention_paged_launches(const KvPool& pool, const KvRows& rows, uint32_t n_heads);
+cudaError_t attention_paged(cudaStream_t stream, const KvPool& pool, const KvRows& rows, const float* q, uint64_t q_stride, uint64_t q_head_stride,
+                            float* scratch, float* out, uint32_t n_heads);
+
 }  // namespace k
 }  // namespace bc

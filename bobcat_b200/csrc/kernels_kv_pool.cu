@@ -1,0 +1,241 @@
+// Rows into the pages of a key/value pool, and back.
+//
+// Writing (8 bit). A row is the head_dim elements of one head at one position: d = f32(max |x| / 127), q = the whole number nearest to
+// x / d, ties to even, within +-127. The quotient is rounded exactly without a division per element: q0 = rint(x * (1 / d)) is at most one
+// off, and x - q0 d, which an fma gives without error (a multiple of both operands' last places, no longer than a float), says where x lies.
+// Rows whose d is not a normal number (all elements below 127 * 2^-126) are stored as zeros; a row with an infinity or a NaN gets a scale of
+// NaN, so it reads as NaN throughout. Half pages store the elements rounded to nearest.
+//
+// What bounds it: bytes, 4 read and 1 (+ 4 / head_dim) or 2 written per element, and the look-up of a row's place before the
+// first store. A lane holds 8 elements (two 16-byte loads, one 8- or 16-byte store), a cell (one head's row of keys or of values) is
+// 8, 16 or 32 lanes. A CTA takes neighbouring token rows; its warps look the rows' places up while the first cells' loads are on their way.
+
+#include "kv_pool.cuh"
+
+#include "../../include/bobcat_cuda.h"
+
+namespace bc {
+namespace k {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr uint32_t kRowsPerCta = 8;  // at most: one warp looks up each
+
+// Places of the CTA's rows; the sequence look-up is a warp's.
+__device__ __forceinline__ void look_up(const KvPool& pool, const KvRows& rows, uint32_t row0, uint32_t n, uint2* place) {
+    const uint32_t warp = threadIdx.x >> 5;
+    if (warp < n) {
+        const uint32_t r = row0 + warp, seq = seq_of_row(rows, r);
+        if ((threadIdx.x & 31) == 0) {
+            uint2 at = make_uint2(kNoSlot, 1);  // 1: no such row of any sequence, 0: a row without a place
+            if (seq < rows.n_seqs) {
+                const uint32_t back = rows.starts[seq + 1] - r, len = rows.lens[seq];
+                at = back <= len ? kv_place(pool, rows, seq, len - back) : make_uint2(kNoSlot, 0);
+            }
+            place[warp] = at;
+        }
+    }
+}
+
+struct Sources {
+    const float *k, *v;
+    uint64_t k_stride, v_stride;
+};
+
+template <int FMT, int HD>
+__global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constant__ KvPool pool, const __grid_constant__ KvRows rows,
+                                                            const __grid_constant__ Sources src, uint32_t rows_per_cta) {
+    constexpr uint32_t kLanes = HD / 8, kCellsAtOnce = kThreads / kLanes;
+    __shared__ uint2 place[kRowsPerCta];
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t row0 = blockIdx.x * rows_per_cta, n = min(rows_per_cta, rows.n_rows - row0);
+    const uint32_t per_row = 2 * pool.n_kv_heads, n_cells = n * per_row;
+    const uint32_t lane = threadIdx.x % kLanes, first = threadIdx.x / kLanes;
+    float x[8];
+    auto load = [&](uint32_t cell) {
+        const uint32_t row = cell / per_row, head = cell % per_row;
+        const bool value = head >= pool.n_kv_heads;
+        const float* from = value ? src.v + (row0 + row) * src.v_stride + (head - pool.n_kv_heads) * HD : src.k + (row0 + row) * src.k_stride + head * HD;
+        const float4 a = __ldcs(reinterpret_cast<const float4*>(from) + 2 * lane), b = __ldcs(reinterpret_cast<const float4*>(from) + 2 * lane + 1);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    };
+    if (first < n_cells) load(first);
+    look_up(pool, rows, row0, n, place);
+    __syncthreads();
+    for (uint32_t cell0 = 0; cell0 < n_cells; cell0 += kCellsAtOnce) {
+        const uint32_t cell = cell0 + first;
+        const bool mine = cell < n_cells;
+        if (cell0 > 0 && mine) load(cell);
+        const uint32_t row = mine ? cell / per_row : 0, head = cell % per_row;
+        const bool value = head >= pool.n_kv_heads;
+        const uint2 at = place[row];
+        uint8_t* const to = value ? pool.v : pool.k;
+        const uint32_t kv_head = value ? head - pool.n_kv_heads : head;
+        const bool store = mine && at.x != kNoSlot;
+        if constexpr (FMT == BC_F16) {
+            if (store) {
+                __half2 h[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+                *reinterpret_cast<uint4*>(to + kv_row_at(pool, at.x, kv_head, at.y) + 16 * lane) = *reinterpret_cast<uint4*>(h);
+            }
+        } else {
+            uint32_t top = 0;  // magnitudes as bits: they order as the numbers do, with infinities and NaN on top
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+            for (uint32_t o = kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            float d = __fdiv_rn(__uint_as_float(top), 127.f);
+            if (d < 1.17549435e-38f) d = 0.f;
+            const bool finite = top < 0x7f800000u;
+            const float inverse = d > 0.f && finite ? __frcp_rn(d) : 0.f;
+            uint32_t bytes[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float q = 0.f;
+                if (inverse > 0.f) {
+                    q = rintf(x[i] * inverse);
+                    const float twice = 2.f * fmaf(-q, d, x[i]);
+                    const bool odd = (int)q & 1;
+                    if (twice > d || (twice == d && odd)) q += 1.f;
+                    if (twice < -d || (twice == -d && odd)) q -= 1.f;
+                    q = fminf(fmaxf(q, -127.f), 127.f);
+                }
+                bytes[i / 4] |= (uint32_t)((int)q + 128) << (8 * (i % 4));
+            }
+            if (store) {
+                *reinterpret_cast<uint2*>(to + kv_row_at(pool, at.x, kv_head, at.y) + 8 * lane) = make_uint2(bytes[0], bytes[1]);
+                if (lane == 0) *reinterpret_cast<float*>(to + kv_scale_at(pool, at.x, kv_head, at.y)) = finite ? d : __uint_as_float(0x7fc00000u);
+            }
+        }
+    }
+}
+
+// Reading. Rows of a sequence without a place (before its first position, behind the table, in no page of the pool) read as zeros; rows
+// of no sequence stay as they are.
+struct Targets {
+    void *k, *v;
+    uint64_t k_stride, v_stride;
+};
+
+template <int FMT, int HD, typename Out>
+__global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ KvPool pool, const __grid_constant__ KvRows rows,
+                                                           const __grid_constant__ Targets dst, uint32_t rows_per_cta) {
+    constexpr uint32_t kLanes = HD / 8, kCellsAtOnce = kThreads / kLanes;
+    constexpr int kAhead = 4;  // cells a lane has loads under way for
+    __shared__ uint2 place[kRowsPerCta];
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t row0 = blockIdx.x * rows_per_cta, n = min(rows_per_cta, rows.n_rows - row0);
+    const uint32_t per_row = 2 * pool.n_kv_heads, n_cells = n * per_row;
+    const uint32_t lane = threadIdx.x % kLanes, first = threadIdx.x / kLanes;
+    look_up(pool, rows, row0, n, place);
+    __syncthreads();
+    for (uint32_t cell0 = first; cell0 < n_cells; cell0 += kAhead * kCellsAtOnce) {
+        uint4 raw[kAhead];
+        float scale[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const uint32_t cell = cell0 + j * kCellsAtOnce, row = cell / per_row, head = cell % per_row;
+            raw[j] = make_uint4(0, 0, 0, 0);
+            scale[j] = 0.f;
+            if (cell >= n_cells || place[row].x == kNoSlot) continue;
+            const uint8_t* from = head >= pool.n_kv_heads ? pool.v : pool.k;
+            const uint32_t kv_head = head >= pool.n_kv_heads ? head - pool.n_kv_heads : head;
+            if constexpr (FMT == BC_F16) {
+                raw[j] = *reinterpret_cast<const uint4*>(from + kv_row_at(pool, place[row].x, kv_head, place[row].y) + 16 * lane);
+            } else {
+                const uint2 b = *reinterpret_cast<const uint2*>(from + kv_row_at(pool, place[row].x, kv_head, place[row].y) + 8 * lane);
+                raw[j].x = b.x;
+                raw[j].y = b.y;
+                scale[j] = *reinterpret_cast<const float*>(from + kv_scale_at(pool, place[row].x, kv_head, place[row].y));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const uint32_t cell = cell0 + j * kCellsAtOnce, row = cell / per_row, head = cell % per_row;
+            if (cell >= n_cells) continue;
+            const uint2 at = place[row];
+            if (at.x == kNoSlot && at.y == 1) continue;
+            const bool value = head >= pool.n_kv_heads;
+            void* base = value ? dst.v : dst.k;
+            if (!base) continue;
+            Out* to = static_cast<Out*>(base) + (row0 + row) * (value ? dst.v_stride : dst.k_stride) + (value ? head - pool.n_kv_heads : head) * HD + 8 * lane;
+            float x[8];
+            if constexpr (FMT == BC_F16) {
+                const __half2* h = reinterpret_cast<const __half2*>(&raw[j]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = __half22float2(h[i]);
+                    x[2 * i] = f.x;
+                    x[2 * i + 1] = f.y;
+                }
+            } else {
+                const uint32_t words[2] = {raw[j].x, raw[j].y};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = at.x == kNoSlot ? 0.f : (float)((int)(words[i / 4] >> (8 * (i % 4)) & 0xffu) - 128) * scale[j];
+            }
+            if constexpr (sizeof(Out) == 4) {
+                reinterpret_cast<float4*>(to)[0] = make_float4(x[0], x[1], x[2], x[3]);
+                reinterpret_cast<float4*>(to)[1] = make_float4(x[4], x[5], x[6], x[7]);
+            } else {
+                __half2 h[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+                *reinterpret_cast<uint4*>(to) = *reinterpret_cast<uint4*>(h);
+            }
+        }
+    }
+}
+
+// Token rows per CTA: a CTA works through at most about four rounds of its threads, fewer where that leaves SMs without one.
+uint32_t rows_per_cta(const KvPool& pool, const KvRows& rows) {
+    const uint32_t lanes_per_row = 2 * pool.n_kv_heads * (pool.head_dim / 8);
+    uint32_t n = 4 * kThreads / lanes_per_row;
+    if (n > kRowsPerCta) n = kRowsPerCta;
+    while (n > 1 && (rows.n_rows + n - 1) / n < 2 * (uint32_t)sm_count()) n /= 2;
+    return n < 1 ? 1 : n;
+}
+
+template <int FMT, int HD>
+cudaError_t write_as(cudaStream_t stream, const KvPool& pool, const KvRows& rows, const Sources& src) {
+    const uint32_t n = rows_per_cta(pool, rows);
+    return launch_dependent(kv_write_kernel<FMT, HD>, dim3((rows.n_rows + n - 1) / n), dim3(kThreads), 0, stream, pool, rows, src, n);
+}
+template <int FMT, int HD>
+cudaError_t read_as(cudaStream_t stream, const KvPool& pool, const KvRows& rows, const Targets& dst, bool half) {
+    const uint32_t n = rows_per_cta(pool, rows);
+    const dim3 grid((rows.n_rows + n - 1) / n);
+    return half ? launch_dependent(kv_read_kernel<FMT, HD, __half>, grid, dim3(kThreads), 0, stream, pool, rows, dst, n)
+                : launch_dependent(kv_read_kernel<FMT, HD, float>, grid, dim3(kThreads), 0, stream, pool, rows, dst, n);
+}
+
+}  // namespace
+
+cudaError_t kv_write(cudaStream_t stream, const KvPool& pool, const KvRows& rows, const float* k, const float* v, uint64_t k_stride, uint64_t v_stride) {
+    if (rows.n_rows == 0) return cudaSuccess;
+    const Sources src{k, v, k_stride, v_stride};
+    const bool half = pool.format == BC_F16;
+    switch (pool.head_dim) {
+        case 64: return half ? write_as<BC_F16, 64>(stream, pool, rows, src) : write_as<BC_I8, 64>(stream, pool, rows, src);
+        case 128: return half ? write_as<BC_F16, 128>(stream, pool, rows, src) : write_as<BC_I8, 128>(stream, pool, rows, src);
+        default: return half ? write_as<BC_F16, 256>(stream, pool, rows, src) : write_as<BC_I8, 256>(stream, pool, rows, src);
+    }
+}
+
+cudaError_t kv_read(cudaStream_t stream, const KvPool& pool, const KvRows& rows, void* k, void* v, bool out_half, uint64_t k_stride, uint64_t v_stride) {
+    if (rows.n_rows == 0) return cudaSuccess;
+    const Targets dst{k, v, k_stride, v_stride};
+    const bool half = pool.format == BC_F16;
+    switch (pool.head_dim) {
+        case 64: return half ? read_as<BC_F16, 64>(stream, pool, rows, dst, out_half) : read_as<BC_I8, 64>(stream, pool, rows, dst, out_half);
+        case 128: return half ? read_as<BC_F16, 128>(stream, pool, rows, dst, out_half) : read_as<BC_I8, 128>(stream, pool, rows, dst, out_half);
+        default: return half ? read_as<BC_F16, 256>(stream, pool, rows, dst, out_half) : read_as<BC_I8, 256>(stream, pool, rows, dst, out_half);
+    }
+}
+
+}  // namespace k
+}  // namespace bc

@@ -1,0 +1,63 @@
+// A pool of key/value pages as the kernels see it, and where a row of a call lies in it.
+//
+// A page holds `page_size` positions (a power of two, 16 to 256) of every KV head, [KV head][position][head_dim], keys and
+// values in a pool each. Halves are stored as they are; an 8-bit page stores an element's integer plus 128, which the
+// readers turn into a half with one byte permute and one subtraction, and has f32 scales [KV head][position] behind its elements.
+// A head's positions of one page lie next to each other, so the readers' tiles are runs of up to a whole page.
+#pragma once
+
+#include "device_utils.cuh"
+#include "kernels.h"
+
+namespace bc {
+namespace k {
+
+constexpr uint32_t kNoSlot = 0xffffffffu;
+// Codes left in KvPool::fault.
+constexpr int kFaultPage = 1, kFaultTable = 2;
+
+__device__ __forceinline__ void leave_fault(const KvPool& p, int code) { *reinterpret_cast<volatile int*>(p.fault) = code; }
+
+// Byte offset in a pool of position `slot` of `head` in page `page`, of its elements and of its scale.
+__device__ __forceinline__ uint64_t kv_row_at(const KvPool& p, uint32_t page, uint32_t head, uint32_t slot) {
+    return (uint64_t)page * p.page_bytes + (uint64_t)((head << p.page_shift) + slot) * p.row_bytes;
+}
+__device__ __forceinline__ uint64_t kv_scale_at(const KvPool& p, uint32_t page, uint32_t head, uint32_t slot) {
+    return (uint64_t)page * p.page_bytes + ((uint64_t)(p.n_kv_heads << p.page_shift) * p.row_bytes) + (uint64_t)((head << p.page_shift) + slot) * 4;
+}
+
+// The sequence that row `r` belongs to, by one warp: starts[] ascends, so it is the number of sequences that begin at or before r, less
+// one. n_seqs for a row behind the last sequence. Independent loads; a binary search would wait for each.
+__device__ __forceinline__ uint32_t seq_of_row(const KvRows& rows, uint32_t r) {
+    uint32_t count = 0;
+    for (uint32_t i = threadIdx.x & 31; i <= rows.n_seqs; i += 32) count += rows.starts[i] <= r;
+    count = __reduce_add_sync(0xffffffffu, count);
+    return count == 0 ? rows.n_seqs : count - 1;  // counts the end of the last sequence too: n_seqs for rows behind it
+}
+
+// Page and slot of position `pos` of a sequence; kNoSlot, and a fault left behind, where the table has none.
+__device__ __forceinline__ uint2 kv_place(const KvPool& pool, const KvRows& rows, uint32_t seq, uint32_t pos) {
+    const uint32_t column = pos >> pool.page_shift;
+    if (column >= rows.max_pages) {
+        leave_fault(pool, kFaultTable);
+        return make_uint2(kNoSlot, 0);
+    }
+    const uint32_t page = rows.table[(uint64_t)seq * rows.max_pages + column];
+    if (page >= pool.n_pages) {
+        leave_fault(pool, kFaultPage);
+        return make_uint2(kNoSlot, 0);
+    }
+    return make_uint2(page, pos & ((1u << pool.page_shift) - 1));
+}
+
+// Four stored bytes as two pairs of halves: the bytes become the low mantissa bits of 1024 + byte.
+__device__ __forceinline__ void unpack_i8(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    const __half2 bias = __floats2half2_rn(1152.f, 1152.f);
+    uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+    __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), bias), y = __hsub2(*reinterpret_cast<__half2*>(&b), bias);
+    lo = *reinterpret_cast<uint32_t*>(&x);
+    hi = *reinterpret_cast<uint32_t*>(&y);
+}
+
+}  // namespace k
+}  // namespace bc

@@ -97,6 +97,12 @@ void bc_buffer_free(bc_buffer* buffer);
 size_t bc_buffer_len(const bc_buffer* buffer);
 /* The device address, for callers that share the buffer with their own CUDA code. */
 void* bc_buffer_device_ptr(bc_buffer* buffer);
+/* A buffer over `len` bytes of device memory of the caller's (another library's tensor), for ops that read or
+ * write it in place. No counterpart in the reference, whose buffers share memory with the CPU. `ptr` is memory of the backend's device
+ * and starts at a multiple of 256 bytes, as the backend's own buffers do (a view's offset reaches what lies behind); it stays the
+ * caller's: bc_buffer_free and bc_backend_close wait for the stream and drop the handle alone. Ops run on the backend's stream, so work of
+ * other streams on the memory has to be ordered with it by the caller. */
+bc_status bc_buffer_at(bc_backend* backend, void* ptr, size_t len, bc_buffer** out);
 /* Metal::write / Metal::read (backend.rs:1180-1205): host <-> device copies, complete on return.
  * Fail with BC_ERR_BUSY while a recording is open, BC_ERR_OUT_OF_BOUNDS past the end. */
 bc_status bc_buffer_write(bc_buffer* buffer, size_t offset, const void* data, size_t len);
@@ -220,6 +226,62 @@ size_t bc_attention_scratch_floats(uint32_t n_heads, uint32_t head_dim, uint32_t
 bc_status bc_attention_static(void* stream, const float* q, const void* k_cache, const void* v_cache, int32_t kv_half,
                               float* out, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t first_pos,
                               uint32_t n_queries, uint32_t n_ctx);
+/* ---- a pool of key/value pages that many sequences share. No counterpart in the reference (one contiguous cache per sequence,
+ * crates/bobcat/src/lfm2_metal.rs:1064-1067). Sequences hold pages in any order, named by page tables on the device; a page may
+ * belong to several sequences (a shared prefix). Ops take the new rows of all sequences at once, whatever their numbers and lengths.
+ *
+ * Formats of the pages: BC_F16, halves; BC_I8, whole numbers of -127 to 127 with an f32 scale per position and head: scale = f32(largest
+ * magnitude / 127), element = the whole number nearest to x / scale, ties to even. A row of a head whose scale is below 2^-126 is stored as
+ * zeros, one with an infinity or a NaN reads as NaN.
+ * Layout: keys and values in a pool each of n_pages pages; a page is [n_kv_heads][page_size][head_dim] elements (halves, or bytes that hold
+ * the whole number plus 128), behind them, of BC_I8, [n_kv_heads][page_size] f32 scales. page_size is a power of two of 16 to 256,
+ * head_dim 64, 128 or 256. Views of pages start on 16-byte boundaries. */
+enum { BC_I8 = 24 };
+typedef struct bc_kv_pool {
+    int32_t format;
+    uint32_t n_pages, page_size, n_kv_heads, head_dim;
+    bc_buffer* k;
+    size_t k_off;
+    bc_buffer* v;
+    size_t v_off;
+} bc_kv_pool;
+/* The rows of a call, in device memory of 32-bit words: starts[n_seqs + 1] ascends, sequence s has rows starts[s] .. starts[s + 1] - 1 (none,
+ * one, or more); lens[s] is the number of positions it holds, its rows the last of them: row r is position lens[s] - (starts[s + 1] - r).
+ * table[s][max_pages] names its pages; entries behind its last position are not read. The op takes up to n_rows rows; rows behind
+ * starts[n_seqs] belong to no sequence and are left as they are, in every output. The words are read when the op runs, so a
+ * captured call serves other lengths when it is replayed. max_queries, the most rows of one sequence as far as the caller knows, chooses
+ * among kernels and changes no more than rounding when it is wrong. 1 to 65535 sequences, up to 2^24 rows.
+ * Rows that lie before a sequence's first position (more rows than positions) have no place: they are not written, read as zeros and attend to
+ * nothing. A position behind the table or in a page that the pool does not have (its number is n_pages or more) is treated the same
+ * way, as a key it is left out, and the wait for the recording (bc_wait, bc_end) returns BC_ERR_OUT_OF_BOUNDS. */
+typedef struct bc_kv_rows {
+    uint32_t n_seqs, n_rows, max_queries, max_pages;
+    bc_buffer* table;
+    size_t table_off;
+    bc_buffer* starts;
+    size_t starts_off;
+    bc_buffer* lens;
+    size_t lens_off;
+} bc_kv_rows;
+/* Bytes of the keys' pages, and of the values'; 0 for a shape that pages cannot have. */
+size_t bc_kv_pool_bytes(int32_t format, uint32_t n_pages, uint32_t page_size, uint32_t n_kv_heads, uint32_t head_dim);
+/* Stores the rows' keys and values, f32 [n_rows][n_kv_heads * head_dim] with rows k_stride and v_stride elements apart (multiples of 4).
+ * Rows of one call that share a position of a page (two sequences that both write a shared page) leave it undefined. */
+bc_status bc_op_kv_write(bc_backend* b, const bc_kv_pool* pool, const bc_kv_rows* rows, bc_buffer* k, size_t k_off, bc_buffer* v, size_t v_off,
+                         uint32_t k_stride, uint32_t v_stride);
+/* The inverse: the rows' keys and values as the pages hold them, as f32 or rounded to halves (out_half); strides are multiples of 16
+ * bytes. Either of k and v may be null. With starts that cover whole sequences it reads whole contexts. */
+bc_status bc_op_kv_read(bc_backend* b, const bc_kv_pool* pool, const bc_kv_rows* rows, bc_buffer* k, size_t k_off, bc_buffer* v, size_t v_off,
+                        int32_t out_half, uint32_t k_stride, uint32_t v_stride);
+/* Causal grouped-query attention of the rows over the pages: row r of sequence s sees positions 0 .. its own, which bc_op_kv_write has
+ * stored. q is f32, token rows q_stride and heads q_head_stride elements apart (multiples of 4); out is [n_rows][n_heads * head_dim]
+ * f32, zeros for a row that sees nothing; elements of positions that a row does not see have no part in it, whatever they are, and a value that is
+ * not finite makes its element of the rows that see it not finite. Up to 8 query heads per KV head. Scores and sums are f32; operands keep 22 bits. `scratch` needs
+ * bc_attention_paged_scratch_floats floats (whatever the lengths), for the duration of the call: calls that may overlap, replayed graphs among
+ * them, take one each. */
+size_t bc_attention_paged_scratch_floats(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
+bc_status bc_op_attention_paged(bc_backend* b, const bc_kv_pool* pool, const bc_kv_rows* rows, bc_buffer* q, size_t q_off, bc_buffer* scratch,
+                                size_t s_off, bc_buffer* out, size_t out_off, uint32_t n_heads, uint32_t q_stride, uint32_t q_head_stride);
 /* Sampler::sample (crates/bobcat-cli/src/sampler.rs:45-112) on the device, in llama.cpp's order:
  * the repetition penalty (each distinct token among the last 64 of `recent` once: positive logits
  * divided, the others multiplied), top-k, top-p and min-p on the softmax at temperature one, the
