@@ -42,7 +42,7 @@ namespace {
 
 // Per device: one word of mapped host memory per kernel file with bounded waits, and one for the key/value pool's kernels, for the life of
 // the process.
-constexpr int kWaitWords = 7, kMaxDevices = 64;
+constexpr int kWaitWords = 8, kMaxDevices = 64;
 std::atomic<volatile int*> g_wait_words[kMaxDevices];
 
 bc_status set_wait_words(int device) {
@@ -60,6 +60,7 @@ bc_status set_wait_words(int device) {
     BC_CUDA(k::matmul_few_wait_word(words + 4));
     BC_CUDA(k::matmul_experts_wait_word(words + 5));
     BC_CUDA(k::gdn_chunk_wait_word(words + 6));
+    BC_CUDA(k::attention_chunk_wait_word(words + 7));
     g_wait_words[device].store(words);
     return BC_OK;
 }
@@ -85,6 +86,7 @@ bc_status kernel_wait_status() {
     if (int code = take(6)) return fail(BC_ERR_EXECUTION, "a delta-rule kernel gave up waiting for its rows (code %d)", code);
     if (int code = take(5)) return fail(BC_ERR_EXECUTION, "a product over experts gave up waiting on its pipeline (code %d)", code);
     if (int code = take(4)) return fail(BC_ERR_EXECUTION, "a product of few rows gave up waiting for its %s (code %d)", code == 2 ? "weights" : "sums", code);
+    if (int code = take(7)) return fail(BC_ERR_EXECUTION, "attention over pages gave up waiting on its pipeline (code %d)", code);
     if (int code = words[kWaitWords]) {
         words[kWaitWords] = 0;
         return fail(BC_ERR_OUT_OF_BOUNDS, code == 1 ? "a page table names a page that the pool does not have" : "a sequence holds more positions than its page table");

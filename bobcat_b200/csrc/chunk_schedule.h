@@ -1,0 +1,70 @@
+// The work of attention over pages for sequences of several new rows, as equal runs of key tiles: plain arithmetic, the same on
+// the host, which checks it, and in the kernel.
+//
+// A row tile is the query heads of `per_tile` neighbouring rows of one sequence and KV head. Row tile r sees the key tiles up to its last row's
+// position; the tiles of a head, summed over its row tiles, are a sum of floor((a r + b) / m), which has a closed form by Euclid's steps, so a CTA
+// finds its place without walking through them.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace bc {
+namespace k {
+
+// Sum over i = 0 .. n - 1 of floor((a i + b) / m).
+__host__ __device__ inline uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
+    uint64_t sum = 0;
+    while (n > 0) {
+        sum += a / m * (n * (n - 1) / 2) + b / m * n;
+        a %= m;
+        b %= m;
+        const uint64_t last = a * n + b;
+        n = last / m;
+        b = last % m;
+        const uint64_t other = a;
+        a = m;
+        m = other;
+        if (m == 0) break;
+    }
+    return sum;
+}
+
+struct ChunkSeq {
+    uint32_t row0, n, end;   // rows row0 .. row0 + n - 1 are the sequence's; row `end` would be the position behind its last
+    uint32_t len, held;      // positions, and those that its table can name
+    uint32_t per_tile, row_tiles, key_tile;
+    // Position of the first row, for counting: within what the table holds.
+    __host__ __device__ uint64_t first() const {
+        const uint32_t rows = end - row0;
+        const uint32_t at = len > rows ? len - rows : 0;
+        return at < held ? at : held;
+    }
+    // Key tiles of row tile r, one at least.
+    __host__ __device__ uint32_t tiles(uint32_t r) const {
+        const uint64_t rows = (uint64_t)(r + 1) * per_tile;
+        return (uint32_t)((first() + (rows < n ? rows : n) - 1) / key_tile) + 1;
+    }
+    // Key tiles of row tiles 0 .. r - 1, r < row_tiles.
+    __host__ __device__ uint64_t tiles_before(uint32_t r) const { return r + floor_sum(r, key_tile, per_tile, first() + per_tile - 1); }
+    __host__ __device__ uint64_t tiles_per_head() const { return row_tiles == 0 ? 0 : tiles_before(row_tiles - 1) + tiles(row_tiles - 1); }
+};
+
+// n_rows: rows of the whole call; fewest: sequences of fewer rows are not these kernels' work.
+__host__ __device__ inline ChunkSeq chunk_seq(uint32_t start, uint32_t end, uint32_t len, uint64_t capacity, uint32_t n_rows, uint32_t fewest, uint32_t per_tile, uint32_t key_tile) {
+    ChunkSeq s;
+    s.row0 = start;
+    s.end = end;
+    s.n = start < n_rows && end > start ? (end < n_rows ? end : n_rows) - start : 0;
+    if (end - start < fewest) s.n = 0;
+    s.len = len;
+    s.held = len < capacity ? len : (uint32_t)capacity;
+    s.per_tile = per_tile;
+    s.row_tiles = (s.n + per_tile - 1) / per_tile;
+    s.key_tile = key_tile;
+    return s;
+}
+
+}  // namespace k
+}  // namespace bc

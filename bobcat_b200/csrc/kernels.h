@@ -495,11 +495,18 @@ cudaError_t kv_write(cudaStream_t stream, const KvPool& pool, const KvRows& rows
 cudaError_t kv_read(cudaStream_t stream, const KvPool& pool, const KvRows& rows, void* k, void* v, bool out_half, uint64_t k_stride, uint64_t v_stride);
 // Attention of the rows over the pool (kernels_attention_paged.cu). Its partial sums depend on the CTAs of a launch alone, of which there are
 // at most kPagedMostCtas on any device.
-constexpr uint32_t kPagedMostCtas = 320;
+constexpr uint32_t kPagedMostCtas = 320, kChunkMostCtas = 160;
 uint64_t attention_paged_scratch_floats(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
 int attention_paged_launches(const KvPool& pool, const KvRows& rows, uint32_t n_heads);
 cudaError_t attention_paged(cudaStream_t stream, const KvPool& pool, const KvRows& rows, const float* q, uint64_t q_stride, uint64_t q_head_stride,
                             float* scratch, float* out, uint32_t n_heads);
+// Its sequences of `fewest` rows and more on the tensor cores (kernels_attention_chunk.cu). Codes of its waits: rows on 1: a product with values,
+// 2: scores; loads on 3: free keys, 4: free values; multiplies on 5: probabilities, 6: values, 7: keys, 8: queries.
+cudaError_t attention_chunk_wait_word(int* word);
+uint64_t attention_chunk_scratch_floats(uint32_t head_dim);
+int attention_chunk_launches();
+cudaError_t attention_chunk(cudaStream_t stream, const KvPool& pool, const KvRows& rows, const float* q, uint64_t q_stride, uint64_t q_head_stride, float* scratch,
+                            float* out, uint32_t n_heads, uint32_t fewest);
 
 }  // namespace k
 }  // namespace bc

@@ -1,0 +1,898 @@
+// Attention of sequences' new rows over a pool of key/value pages on the tensor cores: the form for several rows of a sequence, whose time
+// is multiplies.
+//
+// Arithmetic: that of kernels_attention_paged.cu. Elements are exact halves (8-bit ones as whole numbers, their scales multiply scores and
+// probabilities in f32), a query element and a probability (times the value's scale) are two halves, sums are f32. tcgen05 cuts a sum off instead of
+// rounding it, so what it sums stays short: scores over a head, values over one key tile; the tiles' sums are added up in registers.
+//
+// Shape. Persistent CTAs over equal runs of key tiles (chunk_schedule.h): 128 rows, the query heads of neighbouring rows that share a KV head, against
+// 128 positions (64 for heads of 256). Eight warps own the rows, a thread half of a row's scores and half of its sums: they exchange the rows' maxima
+// through shared memory, turn scores into probabilities in place in tensor memory (the A operand of the second product), and add the
+// previous tile's product to their sums. Four warps bring keys and values, which they unpack and, for values, transpose, into the no-swizzle K-major
+// operand layout; its 128-byte core matrices lie 144 bytes apart, so that what neighbouring lanes store falls in distinct banks.
+// One warp issues the multiplies: the scores of the next tile run while the rows' warps work on this one's.
+// Registers are split among the roles: 192 a thread for rows, 96 for loads, 32 for the multiplies.
+
+#include "async_utils.cuh"
+#include "chunk_schedule.h"
+#include "kv_pool.cuh"
+
+#include "../../include/bobcat_cuda.h"
+
+namespace bc {
+namespace k {
+
+namespace {
+
+using namespace async;
+
+constexpr uint32_t kRows = 128;                    // rows of a tile
+constexpr uint32_t kRowWarps = 8, kLoadWarps = 4, kMmaWarp = 12, kThreads = 512;
+constexpr uint32_t kRowThreads = 32 * kRowWarps, kLoadThreads = 32 * kLoadWarps;
+constexpr uint32_t kCore = 144;                    // bytes from one core matrix to the next
+constexpr uint32_t kTmemColumns = 512;
+constexpr uint32_t kMostCtas = kChunkMostCtas;
+constexpr uint32_t kSpinLimit = 1u << 22;
+constexpr uint32_t kRing = 4, kDescRing = 8;       // tiles whose places, scales and masks are kept; whose descriptions are
+
+template <int HD>
+constexpr uint32_t key_tile() { return HD == 256 ? 64 : 128; }
+template <int HD>
+constexpr uint32_t stages() { return HD == 256 ? 1 : 2; }
+
+__device__ int* g_wait_word;  // where a wait that ran out leaves its code (kernels.h), null until set
+
+struct ChunkParams {
+    KvPool pool;
+    KvRows rows;
+    const float* q;
+    float* out;
+    float* parts;  // [2 * CTA + which][kRows][HD] sums, then [2 * CTA + which][kRows] (maximum, sum), then a ChunkHead per CTA
+    uint64_t q_stride, q_head_stride;
+    uint32_t n_heads, group, fewest;
+};
+// The unit that begins in a CTA's run and goes on behind it, for the joining launch; `last` is the CTA it ends in, 0 when there is none.
+struct ChunkHead {
+    uint32_t row0, n, head, last;  // rows of the call from row0, n of them; KV head
+};
+
+// A stretch of key tiles of one row tile.
+struct Unit {
+    uint32_t seq, head, row_tile, tile0, tiles;
+    bool begins, ends;
+};
+
+// Walks a run of key tiles.
+struct Cursor {
+    uint32_t seq, head, row_tile, at, count;
+    uint64_t left;
+    ChunkSeq s;
+    __device__ __forceinline__ bool take(const ChunkParams& p, uint64_t capacity, uint32_t key_tile, Unit& u) {
+        if (left == 0) return false;
+        if (at == count) {  // on to the next row tile
+            at = 0;
+            if (++row_tile == s.row_tiles) {
+                row_tile = 0;
+                if (++head == p.pool.n_kv_heads) {
+                    head = 0;
+                    do {
+                        ++seq;
+                        s = chunk_seq(p.rows.starts[seq], p.rows.starts[seq + 1], p.rows.lens[seq], capacity, p.rows.n_rows, p.fewest, s.per_tile, key_tile);
+                    } while (s.row_tiles == 0);  // tiles are left, so a sequence with some follows
+                }
+            }
+            count = s.tiles(row_tile);
+        }
+        u.seq = seq;
+        u.head = head;
+        u.row_tile = row_tile;
+        u.tile0 = at;
+        u.tiles = (uint32_t)min((uint64_t)(count - at), left);
+        u.begins = at == 0;
+        at += u.tiles;
+        u.ends = at == count;
+        left -= u.tiles;
+        return true;
+    }
+};
+
+// Where the first loading warp is in the run.
+struct Place {
+    Cursor cursor;
+    Unit unit;
+    uint32_t in_unit, unit_number;
+    ChunkHead cut;
+};
+// What a tile is, for every role.
+struct TileDesc {
+    uint32_t key0, end;       // the first position, and the position behind the sequence's last that its table can name
+    uint32_t row0, n, head;   // the row tile's first row of the call, its rows, the KV head
+    int32_t pos0;             // the position of its first row
+    uint32_t unit;            // number within the run
+    uint32_t first, last;     // of the unit
+    uint32_t begins, ends;    // the unit: whether the row tile's first and last key tiles are its
+};
+// What the loads leave behind for a tile.
+template <uint32_t KT, int FMT>
+struct TileInfo {
+    uint64_t rows_at[KT / 16], scales_at[KT / 16];  // in either pool, of every 16 positions; ~0: in no page
+    uint32_t valid[KT / 32];
+    uint32_t top_scale[kLoadWarps];
+    alignas(16) float dk[FMT == BC_I8 ? KT : 4];
+    alignas(16) float dv[FMT == BC_I8 ? KT : 4];
+};
+
+__device__ __forceinline__ void give_up(volatile int* dead, int code) {
+    *dead = 1;
+    if (g_wait_word) *reinterpret_cast<volatile int*>(g_wait_word) = code;
+}
+__device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* dead, int code) {
+    if (__all_sync(0xffffffffu, mbar_wait(bar, parity, kSpinLimit, dead))) return true;
+    if ((threadIdx.x & 31) == 0) give_up(dead, code);
+    return false;
+}
+// A whole warp's wait. Once one has run out the warp goes on without waiting: it takes the same steps as ever, so that nobody waits for it
+// at a barrier, and what it computes is nobody's.
+__device__ __forceinline__ void await(bool& alive, uint32_t bar, uint32_t parity, volatile int* dead, int code) {
+    if (alive) alive = __all_sync(0xffffffffu, mbar_test(bar, parity)) || wait_on(bar, parity, dead, code);
+}
+
+__device__ __forceinline__ void umma_f16_a_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Whole warp: 32 columns of its lanes. The loads may be read after tmem_wait.
+__device__ __forceinline__ void tmem_load_32(uint32_t taddr, float (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]),
+          "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+          "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store_8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+                 "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void split_half2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    __half2 h = __floats2half2_rn(x, y);
+    float2 back = __half22float2(h);
+    __half2 l = __floats2half2_rn(x - back.x, y - back.y);
+    hi = *reinterpret_cast<uint32_t*>(&h);
+    lo = *reinterpret_cast<uint32_t*>(&l);
+}
+__device__ __forceinline__ void rows_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kRowThreads) : "memory"); }
+__device__ __forceinline__ void loads_sync() { asm volatile("bar.sync 2, %0;" ::"n"(kLoadThreads) : "memory"); }
+
+template <int FMT, int HD>
+struct Shared {
+    static constexpr uint32_t KT = key_tile<HD>(), kStages = stages<HD>(), kUnits = kStages == 1 ? 4 : 8;
+    static constexpr uint32_t kQBytes = kRows / 8 * (HD / 8) * kCore, kTileBytes = KT / 8 * (HD / 8) * kCore;
+    uint8_t q_hi[kQBytes], q_lo[kQBytes];
+    uint8_t keys[kStages][kTileBytes], values[kStages][kTileBytes];
+    TileInfo<KT, FMT> info[kRing];
+    TileDesc desc[kDescRing];
+    float most[2][2][kRows];    // [parity][half]: maxima of the halves of a row's scores; at a unit's end, their sums
+    float q_factor[kRows];
+    uint32_t not_finite[FMT == BC_F16 ? kUnits : 1][FMT == BC_F16 ? HD : 1];  // by unit: the first position with such a value, of each element
+    uint32_t any_not_finite[kUnits];
+    uint64_t bars[2 * kStages * 2 + 5];
+    uint64_t total, run_tiles;  // key tiles of the call, and of the CTA's run
+    Place place;
+    uint32_t tmem;
+    int dead;
+};
+
+template <int FMT, int HD>
+__global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __grid_constant__ ChunkParams p) {
+    using S = Shared<FMT, HD>;
+    constexpr uint32_t KT = S::KT, ST = S::kStages, kUnits = S::kUnits;
+    constexpr uint32_t kKeyStep = HD / 8 * kCore;  // between groups of 8 rows of a K-major operand over a head's elements
+    constexpr uint32_t kPv = 2 * KT;               // tensor memory: two tiles of scores, then the product with the values
+    constexpr float kLift = FMT == BC_F16 ? 15.f : 14.f;  // probabilities times 2^15; weights times scales of up to two units
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    S& sh = *reinterpret_cast<S*>(smem_raw);
+    volatile int* dead = &sh.dead;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const KvPool& pool = p.pool;
+    const uint64_t capacity = (uint64_t)p.rows.max_pages << pool.page_shift;
+    const uint32_t per_tile = kRows / p.group;
+    const uint32_t bars = smem_u32(sh.bars);
+    const uint32_t k_full = bars, k_free = k_full + 8 * ST, v_full = k_free + 8 * ST, v_free = v_full + 8 * ST, s_full = v_free + 8 * ST;
+    const uint32_t p_ready = s_full + 16, pv_full = p_ready + 8, q_ready = pv_full + 8;
+
+    pdl_launch_dependents();
+    if (tid == 0) {
+        for (uint32_t s = 0; s < ST; ++s) {
+            mbar_init(k_full + 8 * s, kLoadWarps);
+            mbar_init(k_free + 8 * s, 1);
+            mbar_init(v_full + 8 * s, kLoadWarps);
+            mbar_init(v_free + 8 * s, 1);
+        }
+        mbar_init(s_full, 1);
+        mbar_init(s_full + 8, 1);
+        mbar_init(p_ready, kRowWarps);
+        mbar_init(pv_full, 1);
+        mbar_init(q_ready, kRowWarps);
+        sh.dead = 0;
+        mbar_init_fence();
+    }
+    if (warp == kMmaWarp) tmem_alloc(smem_u32(&sh.tmem), kTmemColumns);
+    pdl_wait();
+    auto seq_at = [&](uint32_t s) {
+        return chunk_seq(p.rows.starts[s], p.rows.starts[s + 1], p.rows.lens[s], capacity, p.rows.n_rows, p.fewest, per_tile, KT);
+    };
+    // The first loading warp looks for the run and describes its tiles, one ahead of the loads. Its place is kept in shared memory.
+    const uint32_t page_slots = (1u << pool.page_shift) - 1;
+    auto describe = [&](uint32_t j) {  // lane l finds the places of 16 positions
+        if (warp != kRowWarps || j >= (uint32_t)sh.run_tiles) return;
+        Place& at = sh.place;
+        if (lane == 0) {
+            if (at.in_unit == at.unit.tiles) {
+                at.cursor.take(p, capacity, KT, at.unit);
+                at.in_unit = 0;
+                ++at.unit_number;
+            }
+            const Unit& u = at.unit;
+            const ChunkSeq& s = at.cursor.s;
+            const uint32_t query0 = u.row_tile * per_tile;
+            const int64_t pos = (int64_t)s.len - (s.end - s.row0) + query0;
+            TileDesc& d = sh.desc[j % kDescRing];
+            d.key0 = (u.tile0 + at.in_unit) * KT;
+            d.end = s.held;
+            d.row0 = s.row0 + query0;
+            d.n = min(per_tile, s.n - query0);
+            d.head = u.head;
+            d.pos0 = (int32_t)min(pos, (int64_t)0x7fffffff);
+            d.unit = at.unit_number;
+            d.first = at.in_unit == 0;
+            d.last = at.in_unit + 1 == u.tiles;
+            d.begins = u.begins;
+            d.ends = u.ends;
+            if (s.held < s.len) leave_fault(pool, kFaultTable);
+            if (u.begins && !u.ends && at.in_unit == 0) {
+                // The CTA whose run holds the row tile's last key tile: run c is [total c / runs, total (c + 1) / runs).
+                const uint64_t total = sh.total, runs = min((uint64_t)gridDim.x, total), last_tile = total * blockIdx.x / runs + j + at.cursor.count - 1;
+                uint32_t last = (uint32_t)(last_tile * runs / total);
+                while (total * (last + 1) / runs <= last_tile) ++last;
+                while (total * last / runs > last_tile) --last;
+                at.cut = ChunkHead{d.row0, d.n, d.head, last};
+            }
+            ++at.in_unit;
+        }
+        __syncwarp();
+        const TileDesc& d = sh.desc[j % kDescRing];
+        TileInfo<KT, FMT>& info = sh.info[j % kRing];
+        if (lane < KT / 16) {
+            const uint32_t key = d.key0 + 16 * lane;
+            uint64_t rows_at = ~0ull, scales_at = ~0ull;
+            if (key < d.end) {
+                const uint32_t page = p.rows.table[(uint64_t)at.unit.seq * p.rows.max_pages + (key >> pool.page_shift)];
+                if (page < pool.n_pages) {
+                    rows_at = kv_row_at(pool, page, d.head, key & page_slots);
+                    scales_at = kv_scale_at(pool, page, d.head, key & page_slots);
+                } else {
+                    leave_fault(pool, kFaultPage);
+                }
+            }
+            info.rows_at[lane] = rows_at;
+            info.scales_at[lane] = scales_at;
+        }
+        __syncwarp();
+    };
+    if (warp == kRowWarps) {
+        uint64_t total = 0, run_tiles = 0;
+        Cursor cur{};
+        for (uint32_t s = lane; s < p.rows.n_seqs; s += 32) total += pool.n_kv_heads * seq_at(s).tiles_per_head();
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        const uint64_t runs = min((uint64_t)gridDim.x, total);
+        if (blockIdx.x < runs) {
+            const uint64_t begin = total * blockIdx.x / runs;
+            run_tiles = total * (blockIdx.x + 1) / runs - begin;
+            uint64_t base = 0;
+            for (uint32_t s0 = 0; s0 < p.rows.n_seqs; s0 += 32) {
+                const uint64_t mine = s0 + lane < p.rows.n_seqs ? pool.n_kv_heads * seq_at(s0 + lane).tiles_per_head() : 0;
+                uint64_t upto = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint64_t other = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= (uint32_t)o) upto += other;
+                }
+                const uint32_t beyond = __ballot_sync(0xffffffffu, base + upto > begin);
+                if (beyond) {
+                    const int who = __ffs(beyond) - 1;
+                    cur.seq = s0 + who;
+                    base += __shfl_sync(0xffffffffu, upto - mine, who);
+                    break;
+                }
+                base += __shfl_sync(0xffffffffu, upto, 31);
+            }
+            cur.s = seq_at(cur.seq);
+            const uint64_t per_head = cur.s.tiles_per_head(), in_seq = begin - base, in_head = in_seq % per_head;
+            cur.head = (uint32_t)(in_seq / per_head);
+            // The last row tile that begins at or before in_head: 32 candidates at a time.
+            uint32_t lo = 0, span = cur.s.row_tiles;
+            while (span > 1) {
+                const uint32_t step = (span + 31) / 32, r = lo + lane * step;
+                const uint32_t below = __ballot_sync(0xffffffffu, lane * step < span && cur.s.tiles_before(r) <= in_head);
+                const uint32_t who = 31 - __clz(below);  // lane 0's holds
+                lo += who * step;
+                span = min(step, span - who * step);
+            }
+            cur.row_tile = lo;
+            cur.at = (uint32_t)(in_head - cur.s.tiles_before(lo));
+            cur.count = cur.s.tiles(lo);
+            cur.left = run_tiles;
+        }
+        if (lane == 0) {
+            sh.total = total;
+            sh.run_tiles = run_tiles;
+            sh.place.cut = ChunkHead{0, 0, 0, 0};
+            sh.place.cursor = cur;
+            sh.place.unit.tiles = sh.place.in_unit = 0;
+            sh.place.unit_number = ~0u;
+        }
+        __syncwarp();
+        describe(0);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = sh.tmem;
+    const uint32_t n_tiles = (uint32_t)sh.run_tiles;
+    bool alive = true;
+
+    if (warp < kRowWarps) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        const uint32_t half = warp >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lanes = tmem + ((warp & 3) << 21);
+        const float scale = 1.4426950408889634f / sqrtf((float)HD) / 16384.f;
+        // A warp takes 16 rows; a row's largest element goes to 2^14 (see kernels_attention_paged.cu).
+        auto load_queries = [&](const TileDesc& d) {
+            constexpr uint32_t kEach = HD / 32;
+#pragma unroll 4
+            for (uint32_t i = 0; i < 16; ++i) {
+                const uint32_t r = warp * 16 + i, query = r / p.group;
+                const bool there = query < d.n;
+                float x[kEach];
+                const float* from = p.q + (uint64_t)(d.row0 + query) * p.q_stride + (uint64_t)(d.head * p.group + r % p.group) * p.q_head_stride + lane * kEach;
+                if constexpr (kEach == 2) {
+                    const float2 v = there ? *reinterpret_cast<const float2*>(from) : make_float2(0.f, 0.f);
+                    x[0] = v.x, x[1] = v.y;
+                } else {
+#pragma unroll
+                    for (uint32_t e = 0; e < kEach; e += 4) {
+                        const float4 v = there ? *reinterpret_cast<const float4*>(from + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        x[e] = v.x, x[e + 1] = v.y, x[e + 2] = v.z, x[e + 3] = v.w;
+                    }
+                }
+                uint32_t top = 0;
+#pragma unroll
+                for (uint32_t e = 0; e < kEach; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+                const uint32_t exponent = min(max(__reduce_max_sync(0xffffffffu, top) >> 23, 1u), 253u);
+                const float up = __uint_as_float((254u - exponent) << 23);
+                if (lane == 0) sh.q_factor[r] = __uint_as_float(exponent << 23) * scale;
+                const uint32_t at = (r >> 3) * kKeyStep + (lane * kEach / 8) * kCore + (r & 7) * 16 + (lane * kEach % 8) * 2;
+#pragma unroll
+                for (uint32_t e = 0; e < kEach; e += 2) {
+                    uint32_t hi, lo;
+                    split_half2(x[e] * up * 16384.f, x[e + 1] * up * 16384.f, hi, lo);
+                    *reinterpret_cast<uint32_t*>(sh.q_hi + at + e * 2) = hi;
+                    *reinterpret_cast<uint32_t*>(sh.q_lo + at + e * 2) = lo;
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_ready);
+        };
+        if (n_tiles > 0) load_queries(sh.desc[0]);
+        float o[HD / 2], factor = 0.f, top = 0.f, total = 0.f, unit = 0.f;
+        float keep = 0.f, grow = 0.f;  // how the last tile's product joins the sums: o keep + product grow
+        int32_t limit = 0;             // the last position that the row sees, negative for none
+        auto add_product = [&](uint32_t tile) {
+            await(alive, pv_full, tile & 1, dead, 1);
+            tc_fence_after_sync();
+#pragma unroll
+            for (uint32_t c = 0; c < HD / 2; c += 16) {
+                float v[16];
+                tmem_load_16(lanes + kPv + half * (HD / 2) + c, v);
+#pragma unroll
+                for (uint32_t i = 0; i < 16; ++i) o[c + i] = fmaf(o[c + i], keep, v[i] * grow);
+            }
+            tc_fence_before_sync();
+        };
+        for (uint32_t tile = 0; tile < n_tiles; ++tile) {
+            const TileDesc& desc = sh.desc[tile % kDescRing];
+            const bool first = desc.first;
+            if (first) {
+                rows_sync();  // q_factor is there
+                factor = sh.q_factor[row];
+                // (Rows that are nobody's see all there is: no tile is masked for them.)
+                const uint32_t query = row / p.group;
+                limit = (int32_t)min((int64_t)desc.pos0 + (query < desc.n ? query : 0x40000000u), (int64_t)desc.end - 1);
+#pragma unroll
+                for (uint32_t i = 0; i < HD / 2; ++i) o[i] = 0.f;
+                top = -INFINITY;
+                total = unit = 0.f;
+            }
+            const uint32_t buffer = tile & 1;
+            const TileInfo<KT, FMT>& info = sh.info[tile % kRing];
+            await(alive, s_full + 8 * buffer, (tile >> 1) & 1, dead, 2);
+            tc_fence_after_sync();
+            const uint32_t scores_at = lanes + buffer * KT;
+            float x[KT / 2];
+#pragma unroll
+            for (uint32_t c = 0; c < KT / 2; c += 32) tmem_load_32(scores_at + half * (KT / 2) + c, *reinterpret_cast<float(*)[32]>(x + c));
+            const uint32_t key0 = desc.key0 + half * (KT / 2);
+            uint32_t seen[KT / 64];  // positions of this half that the row sees
+            uint32_t all = 0xffffffffu;
+#pragma unroll
+            for (uint32_t w = 0; w < KT / 64; ++w) {
+                const int64_t behind = (int64_t)limit - (key0 + 32 * w) + 1;  // positions of the word up to the limit
+                seen[w] = info.valid[half * (KT / 64) + w] & (behind >= 32 ? 0xffffffffu : behind <= 0 ? 0u : (1u << behind) - 1);
+                all &= seen[w];
+            }
+            const bool masked = __any_sync(0xffffffffu, all != 0xffffffffu);
+            if constexpr (FMT == BC_I8) {
+#pragma unroll
+                for (uint32_t i = 0; i < KT / 2; i += 4) {
+                    const float4 d = *reinterpret_cast<const float4*>(info.dk + half * (KT / 2) + i);
+                    x[i] *= d.x, x[i + 1] *= d.y, x[i + 2] *= d.z, x[i + 3] *= d.w;
+                }
+            }
+            if (masked) {
+#pragma unroll
+                for (uint32_t i = 0; i < KT / 2; ++i)
+                    if (!(seen[i / 32] >> (i % 32) & 1)) x[i] = -INFINITY;
+            }
+            float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (uint32_t i = 0; i < KT / 2; i += 4)
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) most[j] = fmaxf(most[j], x[i + j]);
+            const float mine_most = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * factor;
+            sh.most[tile & 1][half][row] = mine_most;
+            rows_sync();  // and every thread has read its scores: probabilities may take their place
+            const float now = fmaxf(top, fmaxf(mine_most, sh.most[tile & 1][half ^ 1][row]));
+            const float shift = now == -INFINITY ? 0.f : now;
+            const float fall = exp2f(top - shift);
+            top = now;
+            // 8-bit values: weights are counted in the power of two below the tile's largest scale.
+            float down = kLift - shift, tile_unit = 1.f;
+            if constexpr (FMT == BC_I8) {
+                uint32_t largest = 0;
+#pragma unroll
+                for (uint32_t w = 0; w < kLoadWarps; ++w) largest = max(largest, info.top_scale[w]);
+                const uint32_t exponent = min(max(largest >> 23, 27u), 227u);  // 2^-100 to 2^100
+                tile_unit = __uint_as_float(exponent << 23);
+                down -= (float)((int)exponent - 127);
+            }
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (uint32_t i = 0; i < KT / 2; i += 16) {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (uint32_t j = 0; j < 16; j += 4) {
+                    float w[4];
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) {
+                        w[e] = exp2_fast(fmaf(x[i + j + e], factor, down));
+                        sum[e] += w[e];
+                    }
+                    if constexpr (FMT == BC_I8) {
+                        const float4 d = *reinterpret_cast<const float4*>(info.dv + half * (KT / 2) + i + j);
+                        w[0] *= d.x, w[1] *= d.y, w[2] *= d.z, w[3] *= d.w;
+                        if (masked) {
+#pragma unroll
+                            for (uint32_t e = 0; e < 4; ++e)
+                                if (!(seen[(i + j + e) / 32] >> ((i + j + e) % 32) & 1)) w[e] = 0.f;  // a scale may be no number
+                        }
+                    }
+                    split_half2(w[0], w[1], hi[j / 2], lo[j / 2]);
+                    split_half2(w[2], w[3], hi[j / 2 + 1], lo[j / 2 + 1]);
+                }
+                tmem_store_8(scores_at + half * (KT / 4) + i / 2, hi);
+                tmem_store_8(scores_at + KT / 2 + half * (KT / 4) + i / 2, lo);
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            total = total * fall + ((sum[0] + sum[1]) + (sum[2] + sum[3])) * tile_unit;
+            if (!first) add_product(tile - 1);  // before the next one may take its place
+            if constexpr (FMT == BC_I8) {
+                // The sums' unit follows the larger of what they were and what this tile brings.
+                const float target = fmaxf(unit * fall, tile_unit);
+                const float next = __uint_as_float(min(max(__float_as_uint(target) >> 23, 1u), 253u) << 23);
+                keep = fall * (unit / next);
+                grow = tile_unit / next;
+                unit = next;
+            } else {
+                keep = fall;
+                grow = 1.f;
+                unit = 1.f;
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_ready);
+            if (!desc.last) continue;
+            // The next unit's queries go ahead of this one's end: the last scores are done.
+            rows_sync();  // q_factor has been read
+            if (tile + 1 < n_tiles) load_queries(sh.desc[(tile + 1) % kDescRing]);
+            add_product(tile);
+            // A row's two sums of probabilities meet.
+            sh.most[0][half][row] = total;
+            rows_sync();
+            total = sh.most[0][0][row] + sh.most[0][1][row];
+            rows_sync();  // the next unit writes there
+            if constexpr (FMT == BC_F16) {
+                const uint32_t slot = desc.unit % kUnits;
+                if (sh.any_not_finite[slot]) {
+#pragma unroll
+                    for (uint32_t i = 0; i < HD / 2; ++i)
+                        if ((int64_t)sh.not_finite[slot][half * (HD / 2) + i] <= limit) o[i] = __uint_as_float(0x7fc00000u);
+                }
+            }
+            if (desc.begins && desc.ends) {
+                if (row / p.group < desc.n) {
+                    const float inverse = top == -INFINITY && total == 0.f ? 0.f : unit / total;
+                    float* to = p.out + (uint64_t)(desc.row0 + row / p.group) * p.n_heads * HD + (desc.head * p.group + row % p.group) * HD + half * (HD / 2);
+#pragma unroll
+                    for (uint32_t i = 0; i < HD / 2; i += 4)
+                        *reinterpret_cast<float4*>(to + i) = make_float4(o[i] * inverse, o[i + 1] * inverse, o[i + 2] * inverse, o[i + 3] * inverse);
+                }
+            } else {
+                const uint32_t slot = 2 * blockIdx.x + (desc.begins ? 1 : 0);
+                float* to = p.parts + ((uint64_t)slot * kRows + row) * HD + half * (HD / 2);
+#pragma unroll
+                for (uint32_t i = 0; i < HD / 2; i += 4) *reinterpret_cast<float4*>(to + i) = make_float4(o[i] * unit, o[i + 1] * unit, o[i + 2] * unit, o[i + 3] * unit);
+                if (half == 0) *reinterpret_cast<float2*>(p.parts + (uint64_t)2 * kMostCtas * kRows * HD + ((uint64_t)slot * kRows + row) * 2) = make_float2(top, total);
+            }
+        }
+    } else if (warp < kMmaWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        // ---- keys and values
+        const uint32_t ltid = tid - kRowThreads, lwarp = ltid >> 5;
+        constexpr uint32_t kUnitsOfKeys = KT * (HD / 8) / kLoadThreads;        // pieces of 8 elements of a key that a thread brings
+        constexpr uint32_t kBlocks = KT / 8 * (HD / 8) / kLoadThreads;         // blocks of 8 positions x 8 elements of values
+        constexpr uint32_t kPiece = FMT == BC_F16 ? 16 : 8, kPieceWords = kPiece / 4;
+        uint32_t k_raw[FMT == BC_F16 ? 1 : kUnitsOfKeys][2];
+        uint32_t v_raw[kBlocks][8][kPieceWords];
+        float dk = 0.f, dv = 0.f;
+
+        auto key_there = [&](uint32_t j, uint32_t key) {
+            return sh.info[j % kRing].rows_at[key >> 4] != ~0ull && sh.desc[j % kDescRing].key0 + key < sh.desc[j % kDescRing].end;
+        };
+        // What a tile's loads are, into registers (or, halves of keys, straight to shared memory).
+        auto load_scales = [&](uint32_t j) {
+            const TileInfo<KT, FMT>& info = sh.info[j % kRing];
+            dk = dv = 0.f;
+            if (FMT == BC_I8 && ltid < KT && key_there(j, ltid)) {
+                const uint64_t at = info.scales_at[ltid >> 4] + 4 * (ltid & 15);
+                dk = *reinterpret_cast<const float*>(pool.k + at);
+                dv = *reinterpret_cast<const float*>(pool.v + at);
+            }
+        };
+        auto load_keys = [&](uint32_t j) {
+            const TileInfo<KT, FMT>& info = sh.info[j % kRing];
+#pragma unroll
+            for (uint32_t n = 0; n < kUnitsOfKeys; ++n) {
+                const uint32_t i = ltid + n * kLoadThreads, piece = i % (HD / 8), key = i / (HD / 8);
+                const bool there = key_there(j, key);
+                const uint8_t* from = pool.k + info.rows_at[key >> 4] + (key & 15) * pool.row_bytes + piece * kPiece;
+                if constexpr (FMT == BC_F16) {
+                    if (there) cp_async_16(smem_u32(sh.keys[j % ST]) + (key >> 3) * kKeyStep + piece * kCore + (key & 7) * 16, from);
+                } else {
+                    const uint2 w = there ? *reinterpret_cast<const uint2*>(from) : make_uint2(0, 0);
+                    k_raw[n][0] = w.x;
+                    k_raw[n][1] = w.y;
+                }
+            }
+        };
+        auto load_values = [&](uint32_t j) {
+            const TileInfo<KT, FMT>& info = sh.info[j % kRing];
+#pragma unroll
+            for (uint32_t n = 0; n < kBlocks; ++n) {
+                const uint32_t i = ltid + n * kLoadThreads, piece = i % (HD / 8), key = i / (HD / 8) * 8;
+                const uint8_t* from = pool.v + info.rows_at[key >> 4] + (key & 15) * pool.row_bytes + piece * kPiece;
+#pragma unroll
+                for (uint32_t r = 0; r < 8; ++r) {
+                    const bool there = key_there(j, key + r);
+                    if constexpr (FMT == BC_F16) {
+                        const uint4 w = there ? *reinterpret_cast<const uint4*>(from + r * pool.row_bytes) : make_uint4(0, 0, 0, 0);
+                        v_raw[n][r][0] = w.x, v_raw[n][r][1] = w.y, v_raw[n][r][kPieceWords - 2] = w.z, v_raw[n][r][kPieceWords - 1] = w.w;
+                    } else {
+                        const uint2 w = there ? *reinterpret_cast<const uint2*>(from + r * pool.row_bytes) : make_uint2(0x80808080u, 0x80808080u);
+                        v_raw[n][r][0] = w.x, v_raw[n][r][1] = w.y;
+                    }
+                }
+            }
+        };
+        auto store_values = [&](uint32_t j) {
+            const TileDesc& desc = sh.desc[j % kDescRing];
+            uint8_t* const to = sh.values[j % ST];
+            // A value that is not finite would reach rows that do not see it: zero times it is no number. Tiles that end behind the row tile's
+            // first row keep such values apart.
+            const bool apart = FMT == BC_F16 && (int64_t)desc.key0 + KT - 1 > desc.pos0;
+#pragma unroll
+            for (uint32_t n = 0; n < kBlocks; ++n) {
+                const uint32_t i = ltid + n * kLoadThreads, piece = i % (HD / 8), key = i / (HD / 8) * 8;
+                uint4* const core = reinterpret_cast<uint4*>(to + piece * kCore + (key >> 3) * kKeyStep);  // 8 elements x 8 positions
+                if constexpr (FMT == BC_F16) {
+                    if (apart) {
+#pragma unroll
+                        for (uint32_t r = 0; r < 8; ++r)
+#pragma unroll
+                            for (uint32_t w = 0; w < kPieceWords; ++w)
+#pragma unroll
+                                for (uint32_t e = 0; e < 2; ++e)
+                                    if ((v_raw[n][r][w] >> (16 * e) & 0x7c00u) == 0x7c00u) {
+                                        const uint32_t slot = desc.unit % kUnits;
+                                        atomicMin(&sh.not_finite[slot][FMT == BC_F16 ? 8 * piece + 2 * w + e : 0], desc.key0 + key + r);
+                                        sh.any_not_finite[slot] = 1;
+                                        v_raw[n][r][w] &= ~(0xffffu << (16 * e));
+                                    }
+                    }
+#pragma unroll
+                    for (uint32_t w = 0; w < 4; ++w) {
+                        uint32_t even[4], odd[4];
+#pragma unroll
+                        for (uint32_t r = 0; r < 4; ++r) {
+                            even[r] = __byte_perm(v_raw[n][2 * r][w % kPieceWords], v_raw[n][2 * r + 1][w % kPieceWords], 0x5410);
+                            odd[r] = __byte_perm(v_raw[n][2 * r][w % kPieceWords], v_raw[n][2 * r + 1][w % kPieceWords], 0x7632);
+                        }
+                        core[2 * w] = make_uint4(even[0], even[1], even[2], even[3]);
+                        core[2 * w + 1] = make_uint4(odd[0], odd[1], odd[2], odd[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t w = 0; w < 2; ++w)
+#pragma unroll
+                        for (uint32_t h = 0; h < 2; ++h) {  // elements 4w + 2h and the next
+                            uint32_t even[4], odd[4];
+#pragma unroll
+                            for (uint32_t r = 0; r < 4; ++r)
+                                unpack_i8(__byte_perm(v_raw[n][2 * r][w], v_raw[n][2 * r + 1][w], h ? 0x7362 : 0x5140), even[r], odd[r]);
+                            core[4 * w + 2 * h] = make_uint4(even[0], even[1], even[2], even[3]);
+                            core[4 * w + 2 * h + 1] = make_uint4(odd[0], odd[1], odd[2], odd[3]);
+                        }
+                }
+            }
+        };
+        if (n_tiles > 0) {
+            load_scales(0);
+            if (FMT == BC_I8) load_keys(0);
+            load_values(0);
+        }
+        for (uint32_t j = 0; j <= n_tiles; ++j) {
+            if (j < n_tiles) {
+                const uint32_t st = j % ST;
+                TileInfo<KT, FMT>& info = sh.info[j % kRing];
+                describe(j + 1);
+                // Free keys: their scores are done, so the rows' warps are done with the tile before those, and the ring's fourth is nobody's.
+                await(alive, k_free + 8 * st, ((j / ST) & 1) ^ 1, dead, 3);
+                if (FMT == BC_F16 && sh.desc[j % kDescRing].first) {
+                    const uint32_t slot = sh.desc[j % kDescRing].unit % kUnits;
+                    for (uint32_t i = ltid; i < (FMT == BC_F16 ? HD : 1); i += kLoadThreads) sh.not_finite[slot][i] = 0xffffffffu;
+                    if (ltid == 0) sh.any_not_finite[slot] = 0;
+                    // The barrier below comes before the unit's first values are stored.
+                }
+                // Masks and scales of the tile's positions.
+                const bool there = ltid < KT && key_there(j, ltid);
+                const uint32_t votes = __ballot_sync(0xffffffffu, there);
+                if (lane == 0 && lwarp < KT / 32) info.valid[lwarp] = votes;
+                if (FMT == BC_I8) {
+                    if (ltid < KT) {
+                        info.dk[ltid] = dk;
+                        info.dv[ltid] = dv;
+                    }
+                    // The largest finite one.
+                    const uint32_t bits = __float_as_uint(dv) & 0x7fffffffu, largest = __reduce_max_sync(0xffffffffu, bits < 0x7f800000u ? bits : 0u);
+                    if (lane == 0) info.top_scale[lwarp] = largest;
+                }
+                if constexpr (FMT == BC_F16) {
+                    load_keys(j);
+                    cp_async_commit();
+                } else {
+                    uint8_t* const to = sh.keys[st];
+#pragma unroll
+                    for (uint32_t n = 0; n < kUnitsOfKeys; ++n) {
+                        const uint32_t i = ltid + n * kLoadThreads, piece = i % (HD / 8), key = i / (HD / 8);
+                        uint4 w;
+                        unpack_i8(k_raw[n][0], w.x, w.y);
+                        unpack_i8(k_raw[n][1], w.z, w.w);
+                        *reinterpret_cast<uint4*>(to + (key >> 3) * kKeyStep + piece * kCore + (key & 7) * 16) = w;
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(k_full + 8 * st);
+                }
+            }
+            loads_sync();  // tile j + 1 is described
+            if (FMT == BC_I8 && j + 1 < n_tiles) {
+                load_scales(j + 1);
+                load_keys(j + 1);
+            }
+            if (j > 0) {
+                const uint32_t st = (j - 1) % ST;
+                await(alive, v_free + 8 * st, (((j - 1) / ST) & 1) ^ 1, dead, 4);
+                store_values(j - 1);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_full + 8 * st);
+                if (j < n_tiles) load_values(j);
+            }
+            if (FMT == BC_F16 && j < n_tiles) {
+                cp_async_wait<0>();
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(k_full + 8 * (j % ST));
+            }
+        }
+        if (ltid == 0) reinterpret_cast<ChunkHead*>(p.parts + (uint64_t)2 * kMostCtas * kRows * (HD + 2))[blockIdx.x] = sh.place.cut;
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+        if (warp == kMmaWarp) {
+            // ---- the tensor core
+            const uint32_t scores_idesc = umma_idesc_f16(kRows, KT), values_idesc = umma_idesc_f16(kRows, HD);
+            const uint64_t q_hi = umma_desc(smem_u32(sh.q_hi), kCore, kKeyStep), q_lo = umma_desc(smem_u32(sh.q_lo), kCore, kKeyStep);
+            uint32_t units = 0;
+            auto product = [&](uint32_t j) {  // P V of tile j
+                await(alive, p_ready, j & 1, dead, 5);
+                await(alive, v_full + 8 * (j % ST), (j / ST) & 1, dead, 6);
+                tc_fence_after_sync();
+                if (elect_one()) {
+                    const uint64_t v = umma_desc(smem_u32(sh.values[j % ST]), kKeyStep, kCore);
+                    const uint32_t weights = tmem + (j & 1) * KT;
+#pragma unroll 1
+                    for (uint32_t part = 0; part < 2; ++part)
+#pragma unroll
+                        for (uint32_t ks = 0; ks < KT / 16; ++ks)
+                            umma_f16_a_tmem(tmem + kPv, weights + part * (KT / 2) + ks * 8, v + (uint64_t)(ks * 2 * kKeyStep >> 4), values_idesc, part | ks);
+                    umma_commit(v_free + 8 * (j % ST));
+                    umma_commit(pv_full);
+                }
+                __syncwarp();
+            };
+            for (uint32_t j = 0; j < n_tiles; ++j) {
+                await(alive, k_full + 8 * (j % ST), (j / ST) & 1, dead, 7);
+                const bool first = sh.desc[j % kDescRing].first;
+                if (first) {
+                    if (j > 0) product(j - 1);
+                    await(alive, q_ready, units & 1, dead, 8);
+                    ++units;
+                }
+                tc_fence_after_sync();
+                if (elect_one()) {
+                    const uint64_t keys = umma_desc(smem_u32(sh.keys[j % ST]), kCore, kKeyStep);
+#pragma unroll 1
+                    for (uint32_t part = 0; part < 2; ++part)
+#pragma unroll
+                        for (uint32_t ks = 0; ks < HD / 16; ++ks)
+                            umma_f16(tmem + (j & 1) * KT, (part ? q_lo : q_hi) + (uint64_t)(ks * 2 * kCore >> 4), keys + (uint64_t)(ks * 2 * kCore >> 4), scores_idesc, part | ks);
+                    umma_commit(k_free + 8 * (j % ST));
+                    umma_commit(s_full + 8 * (j & 1));
+                }
+                __syncwarp();
+                if (!first) product(j - 1);
+            }
+            if (n_tiles > 0) product(n_tiles - 1);
+        }
+    }
+    // Whoever waited for the last product has seen all multiplies end; after a wait that ran out, they get a limited time to.
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        if (sh.dead && n_tiles > 0) {
+            if (elect_one()) {
+                mbar_init(q_ready, 1);
+                mbar_init_fence();
+                umma_commit(q_ready);
+                for (uint32_t spin = 0; spin < kSpinLimit && !mbar_test(q_ready, 0); ++spin) {}
+            }
+            __syncwarp();
+        }
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, kTmemColumns);
+    }
+}
+
+// Joins the parts of a unit that begins in CTA c's run: a warp to a row.
+template <int HD>
+__global__ void __launch_bounds__(256) attention_chunk_join_kernel(const float* __restrict__ parts, float* __restrict__ out, uint32_t n_heads, uint32_t group) {
+    constexpr int kPairs = HD / 64;
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5), c = blockIdx.x;
+    const ChunkHead cut = reinterpret_cast<const ChunkHead*>(parts + (uint64_t)2 * kMostCtas * kRows * (HD + 2))[c];
+    if (cut.last == 0 || r >= cut.n * group) return;
+    const float2* stats = reinterpret_cast<const float2*>(parts + (uint64_t)2 * kMostCtas * kRows * HD);
+    const uint32_t n = cut.last - c + 1;
+    auto slot_of = [&](uint32_t i) { return (uint64_t)(2 * (c + i) + (i == 0 ? 1 : 0)); };
+    float top = -INFINITY;
+    for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, stats[slot_of(i) * kRows + r].x);
+    top = warp_max(top);
+    const float shift = top == -INFINITY ? 0.f : top;
+    float total = 0.f;
+    float2 sum[kPairs];
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) sum[i] = make_float2(0.f, 0.f);
+    for (uint32_t i0 = 0; i0 < n; i0 += 32) {
+        float2 st = make_float2(-INFINITY, 0.f);
+        if (i0 + lane < n) st = stats[slot_of(i0 + lane) * kRows + r];
+        const float weight = st.x == -INFINITY ? 0.f : exp2f(st.x - shift);
+        total += weight * st.y;
+        const uint32_t many = min(32u, n - i0);
+#pragma unroll 4
+        for (uint32_t i = 0; i < many; ++i) {
+            const float w = __shfl_sync(0xffffffffu, weight, i);
+            const bool any = __shfl_sync(0xffffffffu, st.x, i) != -INFINITY;
+            const float2* from = reinterpret_cast<const float2*>(parts + (slot_of(i0 + i) * kRows + r) * HD) + lane;
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) {
+                const float2 v = from[32 * k];
+                if (any) {
+                    sum[k].x += w * v.x;
+                    sum[k].y += w * v.y;
+                }
+            }
+        }
+    }
+    total = warp_sum(total);
+    const float inverse = top == -INFINITY && total == 0.f ? 0.f : 1.f / total;
+    float2* to = reinterpret_cast<float2*>(out + (uint64_t)(cut.row0 + r / group) * n_heads * HD + (cut.head * group + r % group) * HD) + lane;
+#pragma unroll
+    for (int k = 0; k < kPairs; ++k) to[32 * k] = make_float2(sum[k].x * inverse, sum[k].y * inverse);
+}
+
+uint32_t chunk_ctas() {
+    const uint32_t sms = (uint32_t)sm_count();
+    return sms < kMostCtas ? sms : kMostCtas;
+}
+
+template <int FMT, int HD>
+cudaError_t launch_chunk(cudaStream_t stream, const ChunkParams& p) {
+    constexpr size_t smem = sizeof(Shared<FMT, HD>);
+    static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+    static_assert(2 * key_tile<HD>() + HD <= kTmemColumns, "tensor memory");
+    cudaError_t e = ensure_dynamic_smem((const void*)attention_chunk_kernel<FMT, HD>, smem);
+    if (e != cudaSuccess) return e;
+    const uint32_t ctas = chunk_ctas();
+    e = launch_dependent(attention_chunk_kernel<FMT, HD>, dim3(ctas), dim3(kThreads), smem, stream, p);
+    if (e != cudaSuccess || ctas == 1) return e;
+    return launch_dependent(attention_chunk_join_kernel<HD>, dim3(ctas - 1, kRows / 8), dim3(256), 0, stream, static_cast<const float*>(p.parts), p.out, p.n_heads, p.group);
+}
+
+}  // namespace
+
+uint64_t attention_chunk_scratch_floats(uint32_t head_dim) {
+    return (uint64_t)2 * kMostCtas * kRows * (head_dim + 2) + (uint64_t)kMostCtas * sizeof(ChunkHead) / 4;
+}
+
+int attention_chunk_launches() { return chunk_ctas() == 1 ? 1 : 2; }
+
+cudaError_t attention_chunk(cudaStream_t stream, const KvPool& pool, const KvRows& rows, const float* q, uint64_t q_stride, uint64_t q_head_stride, float* scratch,
+                            float* out, uint32_t n_heads, uint32_t fewest) {
+    const ChunkParams p{pool, rows, q, out, scratch, q_stride, q_head_stride, n_heads, n_heads / pool.n_kv_heads, fewest};
+    const bool half = pool.format == BC_F16;
+    switch (pool.head_dim) {
+        case 64: return half ? launch_chunk<BC_F16, 64>(stream, p) : launch_chunk<BC_I8, 64>(stream, p);
+        case 128: return half ? launch_chunk<BC_F16, 128>(stream, p) : launch_chunk<BC_I8, 128>(stream, p);
+        default: return half ? launch_chunk<BC_F16, 256>(stream, p) : launch_chunk<BC_I8, 256>(stream, p);
+    }
+}
+
+cudaError_t attention_chunk_wait_word(int* word) { return cudaMemcpyToSymbol(g_wait_word, &word, sizeof word); }
+
+}  // namespace k
+}  // namespace bc

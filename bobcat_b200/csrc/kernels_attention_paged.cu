@@ -44,6 +44,7 @@ struct TokenParams {
     float* parts;  // [2 * CTA + which][kRows][HD] sums, then [2 * CTA + which][kRows] (maximum, sum), then a PartsHead per CTA
     uint64_t q_stride, q_head_stride;
     uint32_t n_heads, group;
+    uint32_t most;  // sequences of more rows are the other kernel's (kernels_attention_chunk.cu)
 };
 // What the joining launch needs of the unit that begins in a CTA's run and goes on behind it; `last` is the CTA it ends in, 0 when there is none.
 struct PartsHead {
@@ -68,11 +69,11 @@ struct Seq {
     uint32_t row0, n, end, len;
     uint32_t blocks;
 };
-__device__ __forceinline__ Seq seq_at(const KvPool& pool, const KvRows& rows, uint32_t s) {
+__device__ __forceinline__ Seq seq_at(const KvPool& pool, const KvRows& rows, uint32_t s, uint32_t most) {
     Seq q;
     q.row0 = rows.starts[s];
     q.end = rows.starts[s + 1];
-    q.n = q.row0 < rows.n_rows && q.end > q.row0 ? min(q.end, rows.n_rows) - q.row0 : 0;
+    q.n = q.row0 < rows.n_rows && q.end > q.row0 && q.end - q.row0 <= most ? min(q.end, rows.n_rows) - q.row0 : 0;
     q.len = rows.lens[s];
     const uint32_t held = min((uint64_t)q.len, (uint64_t)rows.max_pages << pool.page_shift);
     q.blocks = max(1u, (held + kBlock - 1) / kBlock);
@@ -111,7 +112,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(FMT, HD)) attention_toke
 
     // This CTA's run of blocks, and the sequence that it begins in. Every warp works it out for itself.
     uint64_t total = 0;
-    for (uint32_t s = lane; s < rows.n_seqs; s += 32) total += blocks_of(pool, seq_at(pool, rows, s));
+    for (uint32_t s = lane; s < rows.n_seqs; s += 32) total += blocks_of(pool, seq_at(pool, rows, s, p.most));
     total = warp_sum_u64(total);
     const uint64_t runs = min((uint64_t)gridDim.x, total);  // none of them empty
     uint64_t at = blockIdx.x < runs ? total * blockIdx.x / runs : total;
@@ -124,7 +125,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(FMT, HD)) attention_toke
     uint32_t seq = 0;
     uint64_t base = 0;  // blocks of the sequences before `seq`
     for (uint32_t s0 = 0; s0 < rows.n_seqs; s0 += 32) {
-        const uint64_t mine = s0 + lane < rows.n_seqs ? blocks_of(pool, seq_at(pool, rows, s0 + lane)) : 0;
+        const uint64_t mine = s0 + lane < rows.n_seqs ? blocks_of(pool, seq_at(pool, rows, s0 + lane, p.most)) : 0;
         uint64_t upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -143,10 +144,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(FMT, HD)) attention_toke
     PartsHead cut{0, 0, 0, 0};
 
     while (at < end) {
-        Seq sq = seq_at(pool, rows, seq);
+        Seq sq = seq_at(pool, rows, seq, p.most);
         while (base + blocks_of(pool, sq) <= at) {  // sequences without rows have no blocks
             base += blocks_of(pool, sq);
-            sq = seq_at(pool, rows, ++seq);
+            sq = seq_at(pool, rows, ++seq, p.most);
         }
         // The unit, and the blocks of it that are this CTA's. Rows of a head are neighbours.
         const uint64_t in_seq = at - base;
@@ -516,24 +517,43 @@ cudaError_t launch_token(cudaStream_t stream, const TokenParams& p) {
     return launch_dependent(attention_token_join_kernel<HD>, dim3(ctas - 1), dim3(32 * kRows), 0, stream, static_cast<const float*>(p.parts), p.out, p.n_heads, p.group);
 }
 
-}  // namespace
-
-uint64_t attention_paged_scratch_floats(uint32_t, uint32_t, uint32_t head_dim) {
+uint64_t token_floats(uint32_t head_dim) {
     return (uint64_t)2 * kMostCtas * kRows * (head_dim + 2) + (uint64_t)kMostCtas * sizeof(PartsHead) / 4;
 }
 
-int attention_paged_launches(const KvPool& pool, const KvRows& rows, uint32_t) { return token_ctas(pool, rows) == 1 ? 1 : 2; }
+}  // namespace
+
+// Rows of a sequence up to which each is a unit of its own. The tensor-core kernel reads the positions once for all rows, and takes
+// the time of 128.
+constexpr uint32_t kTokenRows = 1;
+
+uint64_t attention_paged_scratch_floats(uint32_t, uint32_t, uint32_t head_dim) {
+    return token_floats(head_dim) + attention_chunk_scratch_floats(head_dim);
+}
+
+int attention_paged_launches(const KvPool& pool, const KvRows& rows, uint32_t) {
+    const int tokens = token_ctas(pool, rows) == 1 ? 1 : 2;
+    if (rows.max_queries <= kTokenRows) return tokens;
+    return attention_chunk_launches() + (rows.n_seqs > 1 ? tokens : 0);
+}
 
 cudaError_t attention_paged(cudaStream_t stream, const KvPool& pool, const KvRows& rows, const float* q, uint64_t q_stride, uint64_t q_head_stride,
                             float* scratch, float* out, uint32_t n_heads) {
     if (rows.n_rows == 0 || rows.n_seqs == 0) return cudaSuccess;
-    const TokenParams p{pool, rows, q, out, scratch, q_stride, q_head_stride, n_heads, n_heads / pool.n_kv_heads};
+    // What the caller says of the rows decides which kernels run; the rows themselves, on the device, which of them takes a sequence.
+    const bool chunks = rows.max_queries > kTokenRows, tokens = !chunks || rows.n_seqs > 1;
+    const TokenParams p{pool, rows, q, out, scratch, q_stride, q_head_stride, n_heads, n_heads / pool.n_kv_heads, chunks ? kTokenRows : 0xffffffffu};
     const bool half = pool.format == BC_F16;
-    switch (pool.head_dim) {
-        case 64: return half ? launch_token<BC_F16, 64>(stream, p) : launch_token<BC_I8, 64>(stream, p);
-        case 128: return half ? launch_token<BC_F16, 128>(stream, p) : launch_token<BC_I8, 128>(stream, p);
-        default: return half ? launch_token<BC_F16, 256>(stream, p) : launch_token<BC_I8, 256>(stream, p);
+    cudaError_t e = cudaSuccess;
+    if (tokens) {
+        switch (pool.head_dim) {
+            case 64: e = half ? launch_token<BC_F16, 64>(stream, p) : launch_token<BC_I8, 64>(stream, p); break;
+            case 128: e = half ? launch_token<BC_F16, 128>(stream, p) : launch_token<BC_I8, 128>(stream, p); break;
+            default: e = half ? launch_token<BC_F16, 256>(stream, p) : launch_token<BC_I8, 256>(stream, p);
+        }
     }
+    if (e != cudaSuccess || !chunks) return e;
+    return attention_chunk(stream, pool, rows, q, q_stride, q_head_stride, scratch + token_floats(pool.head_dim), out, n_heads, tokens ? kTokenRows + 1 : 0);
 }
 
 }  // namespace k
