@@ -6,12 +6,13 @@
 // rounding it, so what it sums stays short: scores over a head, values over one key tile; the tiles' sums are added up in registers.
 //
 // Shape. Persistent CTAs over equal runs of key tiles (chunk_schedule.h): 128 rows, the query heads of neighbouring rows that share a KV head, against
-// 128 positions (64 for heads of 256). Eight warps own the rows, a thread half of a row's scores and half of its sums: they exchange the rows' maxima
-// through shared memory, turn scores into probabilities in place in tensor memory (the A operand of the second product), and add the
-// previous tile's product to their sums. Four warps bring keys and values, which they unpack and, for values, transpose, into the no-swizzle K-major
-// operand layout; its 128-byte core matrices lie 144 bytes apart, so that what neighbouring lanes store falls in distinct banks.
-// One warp issues the multiplies: the scores of the next tile run while the rows' warps work on this one's.
-// Registers are split among the roles: 192 a thread for rows, 96 for loads, 32 for the multiplies.
+// 128 positions (64 for heads of 256). One warp walks the run, looks the pages up and brings a tile's bytes into shared memory by bulk copies, 16
+// positions each. Four warps unpack them and, of values, transpose them, into the no-swizzle K-major operand layout; its 128-byte core matrices lie
+// 144 bytes apart, so that what neighbouring lanes store falls in distinct banks. One warp issues the multiplies. Eight warps own the rows, a thread half
+// of a row's scores and half of its sums: they exchange the rows' maxima through shared memory, turn scores into probabilities in place in
+// tensor memory, and add the previous tile's product to their sums, while the scores of the next tile run.
+// Queries and probabilities are A operands in tensor memory: both operands in shared memory would take its 128 bytes a cycle whole. (Heads of 256
+// leave room for the queries' upper halves alone.)
 
 #include "async_utils.cuh"
 #include "chunk_schedule.h"
@@ -27,18 +28,21 @@ namespace {
 using namespace async;
 
 constexpr uint32_t kRows = 128;                    // rows of a tile
-constexpr uint32_t kRowWarps = 8, kLoadWarps = 4, kMmaWarp = 12, kThreads = 512;
-constexpr uint32_t kRowThreads = 32 * kRowWarps, kLoadThreads = 32 * kLoadWarps;
+constexpr uint32_t kRowWarps = 8, kUnpackWarps = 4, kMmaWarp = 12, kCopyWarp = 13, kThreads = 512;
+constexpr uint32_t kRowThreads = 32 * kRowWarps, kUnpackThreads = 32 * kUnpackWarps;
 constexpr uint32_t kCore = 144;                    // bytes from one core matrix to the next
 constexpr uint32_t kTmemColumns = 512;
 constexpr uint32_t kMostCtas = kChunkMostCtas;
 constexpr uint32_t kSpinLimit = 1u << 22;
-constexpr uint32_t kRing = 4, kDescRing = 8;       // tiles whose places, scales and masks are kept; whose descriptions are
+constexpr uint32_t kRing = 4, kDescRing = 8;       // tiles whose scales and masks are kept; whose descriptions are
 
 template <int HD>
 constexpr uint32_t key_tile() { return HD == 256 ? 64 : 128; }
-template <int HD>
-constexpr uint32_t stages() { return HD == 256 ? 1 : 2; }
+// Operand tiles and tiles of bytes on their way, as many as shared memory holds.
+template <int FMT, int HD>
+constexpr uint32_t stages() { return HD == 256 || (HD == 128 && FMT == BC_F16) ? 1 : 2; }
+template <int FMT, int HD>
+constexpr uint32_t raw_tiles() { return HD == 256 && FMT == BC_F16 ? 1 : 2; }
 
 __device__ int* g_wait_word;  // where a wait that ran out leaves its code (kernels.h), null until set
 
@@ -106,20 +110,27 @@ struct Place {
 // What a tile is, for every role.
 struct TileDesc {
     uint32_t key0, end;       // the first position, and the position behind the sequence's last that its table can name
+    uint32_t groups;          // of 16 positions, a bit each: in a page of the pool
     uint32_t row0, n, head;   // the row tile's first row of the call, its rows, the KV head
     int32_t pos0;             // the position of its first row
     uint32_t unit;            // number within the run
     uint32_t first, last;     // of the unit
     uint32_t begins, ends;    // the unit: whether the row tile's first and last key tiles are its
 };
-// What the loads leave behind for a tile.
+// What the unpacking warps leave behind for a tile.
 template <uint32_t KT, int FMT>
 struct TileInfo {
-    uint64_t rows_at[KT / 16], scales_at[KT / 16];  // in either pool, of every 16 positions; ~0: in no page
     uint32_t valid[KT / 32];
-    uint32_t top_scale[kLoadWarps];
+    uint32_t top_scale[kUnpackWarps];
     alignas(16) float dk[FMT == BC_I8 ? KT : 4];
     alignas(16) float dv[FMT == BC_I8 ? KT : 4];
+};
+// A tile's bytes as they lie in the pages.
+template <uint32_t KT, int FMT, int HD>
+struct RawTile {
+    static constexpr uint32_t kRowBytes = FMT == BC_F16 ? 2 * HD : HD;
+    uint8_t keys[KT * kRowBytes], values[KT * kRowBytes];
+    float dk[FMT == BC_I8 ? KT : 4], dv[FMT == BC_I8 ? KT : 4];
 };
 
 __device__ __forceinline__ void give_up(volatile int* dead, int code) {
@@ -146,13 +157,11 @@ __device__ __forceinline__ void umma_f16_a_tmem(uint32_t tmem_d, uint32_t tmem_a
         : "memory");
 }
 // Whole warp: 32 columns of its lanes. The loads may be read after tmem_wait.
-__device__ __forceinline__ void tmem_load_32(uint32_t taddr, float (&v)[32]) {
+__device__ __forceinline__ void tmem_load_32(uint32_t taddr, float2* v) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
-        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]),
-          "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
-          "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "=f"(v[0].x), "=f"(v[0].y), "=f"(v[1].x), "=f"(v[1].y), "=f"(v[2].x), "=f"(v[2].y), "=f"(v[3].x), "=f"(v[3].y), "=f"(v[4].x), "=f"(v[4].y), "=f"(v[5].x), "=f"(v[5].y), "=f"(v[6].x), "=f"(v[6].y), "=f"(v[7].x), "=f"(v[7].y), "=f"(v[8].x), "=f"(v[8].y), "=f"(v[9].x), "=f"(v[9].y), "=f"(v[10].x), "=f"(v[10].y), "=f"(v[11].x), "=f"(v[11].y), "=f"(v[12].x), "=f"(v[12].y), "=f"(v[13].x), "=f"(v[13].y), "=f"(v[14].x), "=f"(v[14].y), "=f"(v[15].x), "=f"(v[15].y)
         : "r"(taddr)
         : "memory");
 }
@@ -160,6 +169,27 @@ __device__ __forceinline__ void tmem_store_8(uint32_t taddr, const uint32_t (&v)
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
                  "r"(v[6]), "r"(v[7])
                  : "memory");
+}
+__device__ __forceinline__ void tmem_store_4(uint32_t taddr, const uint32_t (&v)[4]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+// Pairs of f32 in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(r)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(r)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+    return r;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -173,34 +203,44 @@ __device__ __forceinline__ void split_half2(float x, float y, uint32_t& hi, uint
     hi = *reinterpret_cast<uint32_t*>(&h);
     lo = *reinterpret_cast<uint32_t*>(&l);
 }
+// (x, y) as halves of the upper 11 bits, cut off, and of what they leave over.
+__device__ __forceinline__ void cut_half2(float2 x, uint32_t& hi, uint32_t& lo) {
+    const float2 upper = make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffffe000u), __uint_as_float(__float_as_uint(x.y) & 0xffffe000u));
+    const __half2 h = __floats2half2_rn(upper.x, upper.y);
+    const float2 rest = add2(x, make_float2(-upper.x, -upper.y));
+    const __half2 l = __floats2half2_rn(rest.x, rest.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
 __device__ __forceinline__ void rows_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kRowThreads) : "memory"); }
-__device__ __forceinline__ void loads_sync() { asm volatile("bar.sync 2, %0;" ::"n"(kLoadThreads) : "memory"); }
-
 template <int FMT, int HD>
 struct Shared {
-    static constexpr uint32_t KT = key_tile<HD>(), kStages = stages<HD>(), kUnits = kStages == 1 ? 4 : 8;
-    static constexpr uint32_t kQBytes = kRows / 8 * (HD / 8) * kCore, kTileBytes = KT / 8 * (HD / 8) * kCore;
-    uint8_t q_hi[kQBytes], q_lo[kQBytes];
+    static constexpr uint32_t KT = key_tile<HD>(), kStages = stages<FMT, HD>(), kRaw = raw_tiles<FMT, HD>(), kUnits = 8;
+    static constexpr uint32_t kTileBytes = KT / 8 * (HD / 8) * kCore;
+    uint8_t q_lo[HD == 256 ? kRows / 8 * (HD / 8) * kCore : 16];
     uint8_t keys[kStages][kTileBytes], values[kStages][kTileBytes];
+    alignas(16) RawTile<KT, FMT, HD> raw[kRaw];
     TileInfo<KT, FMT> info[kRing];
     TileDesc desc[kDescRing];
-    float most[2][2][kRows];    // [parity][half]: maxima of the halves of a row's scores; at a unit's end, their sums
-    float q_factor[kRows];
+    float most[2][2][kRows];    // [parity][half]: maxima of the halves of a row's scores; at a unit's ends, other exchanges
     uint32_t not_finite[FMT == BC_F16 ? kUnits : 1][FMT == BC_F16 ? HD : 1];  // by unit: the first position with such a value, of each element
     uint32_t any_not_finite[kUnits];
-    uint64_t bars[2 * kStages * 2 + 5];
+    uint64_t bars[4 * kStages + 2 * kRaw + 5 + kDescRing];
     uint64_t total, run_tiles;  // key tiles of the call, and of the CTA's run
     Place place;
     uint32_t tmem;
-    int dead;
+    int dead, never;            // whether a wait has run out; a flag that nobody raises
 };
 
 template <int FMT, int HD>
 __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __grid_constant__ ChunkParams p) {
     using S = Shared<FMT, HD>;
-    constexpr uint32_t KT = S::KT, ST = S::kStages, kUnits = S::kUnits;
+    constexpr uint32_t KT = S::KT, ST = S::kStages, RAW = S::kRaw, kUnits = S::kUnits;
     constexpr uint32_t kKeyStep = HD / 8 * kCore;  // between groups of 8 rows of a K-major operand over a head's elements
-    constexpr uint32_t kPv = 2 * KT;               // tensor memory: two tiles of scores, then the product with the values
+    // Tensor memory: two tiles of scores, the product with the values, the queries' halves.
+    constexpr uint32_t kPv = 2 * KT, kQHi = kPv + HD, kQLo = kQHi + HD / 2;
+    constexpr bool kQLoShared = HD == 256;
+    static_assert(kQLo + (kQLoShared ? 0 : HD / 2) <= kTmemColumns, "tensor memory");
     constexpr float kLift = FMT == BC_F16 ? 15.f : 14.f;  // probabilities times 2^15; weights times scales of up to two units
     extern __shared__ __align__(128) uint8_t smem_raw[];
     S& sh = *reinterpret_cast<S*>(smem_raw);
@@ -210,89 +250,37 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
     const uint64_t capacity = (uint64_t)p.rows.max_pages << pool.page_shift;
     const uint32_t per_tile = kRows / p.group;
     const uint32_t bars = smem_u32(sh.bars);
-    const uint32_t k_full = bars, k_free = k_full + 8 * ST, v_full = k_free + 8 * ST, v_free = v_full + 8 * ST, s_full = v_free + 8 * ST;
-    const uint32_t p_ready = s_full + 16, pv_full = p_ready + 8, q_ready = pv_full + 8;
+    const uint32_t k_full = bars, k_free = k_full + 8 * ST, v_full = k_free + 8 * ST, v_free = v_full + 8 * ST, raw_full = v_free + 8 * ST, raw_free = raw_full + 8 * RAW;
+    const uint32_t s_full = raw_free + 8 * RAW, p_ready = s_full + 16, pv_full = p_ready + 8, q_ready = pv_full + 8, described = q_ready + 8;
 
     pdl_launch_dependents();
     if (tid == 0) {
         for (uint32_t s = 0; s < ST; ++s) {
-            mbar_init(k_full + 8 * s, kLoadWarps);
+            mbar_init(k_full + 8 * s, kUnpackWarps);
             mbar_init(k_free + 8 * s, 1);
-            mbar_init(v_full + 8 * s, kLoadWarps);
+            mbar_init(v_full + 8 * s, kUnpackWarps);
             mbar_init(v_free + 8 * s, 1);
+        }
+        for (uint32_t r = 0; r < RAW; ++r) {
+            mbar_init(raw_full + 8 * r, 1);
+            mbar_init(raw_free + 8 * r, kUnpackWarps);
         }
         mbar_init(s_full, 1);
         mbar_init(s_full + 8, 1);
         mbar_init(p_ready, kRowWarps);
         mbar_init(pv_full, 1);
         mbar_init(q_ready, kRowWarps);
-        sh.dead = 0;
+        for (uint32_t d = 0; d < kDescRing; ++d) mbar_init(described + 8 * d, 1);
+        sh.dead = sh.never = 0;
         mbar_init_fence();
     }
     if (warp == kMmaWarp) tmem_alloc(smem_u32(&sh.tmem), kTmemColumns);
     pdl_wait();
-    auto seq_at = [&](uint32_t s) {
-        return chunk_seq(p.rows.starts[s], p.rows.starts[s + 1], p.rows.lens[s], capacity, p.rows.n_rows, p.fewest, per_tile, KT);
-    };
-    // The first loading warp looks for the run and describes its tiles, one ahead of the loads. Its place is kept in shared memory.
-    const uint32_t page_slots = (1u << pool.page_shift) - 1;
-    auto describe = [&](uint32_t j) {  // lane l finds the places of 16 positions
-        if (warp != kRowWarps || j >= (uint32_t)sh.run_tiles) return;
-        Place& at = sh.place;
-        if (lane == 0) {
-            if (at.in_unit == at.unit.tiles) {
-                at.cursor.take(p, capacity, KT, at.unit);
-                at.in_unit = 0;
-                ++at.unit_number;
-            }
-            const Unit& u = at.unit;
-            const ChunkSeq& s = at.cursor.s;
-            const uint32_t query0 = u.row_tile * per_tile;
-            const int64_t pos = (int64_t)s.len - (s.end - s.row0) + query0;
-            TileDesc& d = sh.desc[j % kDescRing];
-            d.key0 = (u.tile0 + at.in_unit) * KT;
-            d.end = s.held;
-            d.row0 = s.row0 + query0;
-            d.n = min(per_tile, s.n - query0);
-            d.head = u.head;
-            d.pos0 = (int32_t)min(pos, (int64_t)0x7fffffff);
-            d.unit = at.unit_number;
-            d.first = at.in_unit == 0;
-            d.last = at.in_unit + 1 == u.tiles;
-            d.begins = u.begins;
-            d.ends = u.ends;
-            if (s.held < s.len) leave_fault(pool, kFaultTable);
-            if (u.begins && !u.ends && at.in_unit == 0) {
-                // The CTA whose run holds the row tile's last key tile: run c is [total c / runs, total (c + 1) / runs).
-                const uint64_t total = sh.total, runs = min((uint64_t)gridDim.x, total), last_tile = total * blockIdx.x / runs + j + at.cursor.count - 1;
-                uint32_t last = (uint32_t)(last_tile * runs / total);
-                while (total * (last + 1) / runs <= last_tile) ++last;
-                while (total * last / runs > last_tile) --last;
-                at.cut = ChunkHead{d.row0, d.n, d.head, last};
-            }
-            ++at.in_unit;
-        }
-        __syncwarp();
-        const TileDesc& d = sh.desc[j % kDescRing];
-        TileInfo<KT, FMT>& info = sh.info[j % kRing];
-        if (lane < KT / 16) {
-            const uint32_t key = d.key0 + 16 * lane;
-            uint64_t rows_at = ~0ull, scales_at = ~0ull;
-            if (key < d.end) {
-                const uint32_t page = p.rows.table[(uint64_t)at.unit.seq * p.rows.max_pages + (key >> pool.page_shift)];
-                if (page < pool.n_pages) {
-                    rows_at = kv_row_at(pool, page, d.head, key & page_slots);
-                    scales_at = kv_scale_at(pool, page, d.head, key & page_slots);
-                } else {
-                    leave_fault(pool, kFaultPage);
-                }
-            }
-            info.rows_at[lane] = rows_at;
-            info.scales_at[lane] = scales_at;
-        }
-        __syncwarp();
-    };
-    if (warp == kRowWarps) {
+    if (warp == kCopyWarp) {
+        // The run, and where it begins.
+        auto seq_at = [&](uint32_t s) {
+            return chunk_seq(p.rows.starts[s], p.rows.starts[s + 1], p.rows.lens[s], capacity, p.rows.n_rows, p.fewest, per_tile, KT);
+        };
         uint64_t total = 0, run_tiles = 0;
         Cursor cur{};
         for (uint32_t s = lane; s < p.rows.n_seqs; s += 32) total += pool.n_kv_heads * seq_at(s).tiles_per_head();
@@ -345,8 +333,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             sh.place.unit.tiles = sh.place.in_unit = 0;
             sh.place.unit_number = ~0u;
         }
-        __syncwarp();
-        describe(0);
     }
     tc_fence_before_sync();
     __syncthreads();
@@ -356,86 +342,101 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
     bool alive = true;
 
     if (warp < kRowWarps) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
         const uint32_t half = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((warp & 3) << 21);
         const float scale = 1.4426950408889634f / sqrtf((float)HD) / 16384.f;
-        // A warp takes 16 rows; a row's largest element goes to 2^14 (see kernels_attention_paged.cu).
-        auto load_queries = [&](const TileDesc& d) {
-            constexpr uint32_t kEach = HD / 32;
-#pragma unroll 4
-            for (uint32_t i = 0; i < 16; ++i) {
-                const uint32_t r = warp * 16 + i, query = r / p.group;
-                const bool there = query < d.n;
-                float x[kEach];
-                const float* from = p.q + (uint64_t)(d.row0 + query) * p.q_stride + (uint64_t)(d.head * p.group + r % p.group) * p.q_head_stride + lane * kEach;
-                if constexpr (kEach == 2) {
-                    const float2 v = there ? *reinterpret_cast<const float2*>(from) : make_float2(0.f, 0.f);
-                    x[0] = v.x, x[1] = v.y;
-                } else {
+        float factor = 0.f;
+
+        // The next unit's queries, a thread half of a row: its largest element goes to 2^14 (see kernels_attention_paged.cu). The other half's
+        // largest comes through shared memory.
+        auto load_queries = [&](uint32_t tile) {
+            await(alive, described + 8 * (tile % kDescRing), (tile / kDescRing) & 1, dead, 9);
+            const TileDesc& d = sh.desc[tile % kDescRing];
+            const uint32_t query = row / p.group;
+            const bool there = query < d.n;
+            const float4* from = reinterpret_cast<const float4*>(p.q + (there ? (uint64_t)(d.row0 + query) * p.q_stride + (uint64_t)(d.head * p.group + row % p.group) * p.q_head_stride
+                                                                               : 0) + half * (HD / 2));
+            uint32_t top = 0;
+#pragma unroll 8
+            for (uint32_t i = 0; i < HD / 8; ++i) {
+                const float4 v = there ? from[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+                top = max(max(top, __float_as_uint(v.x) & 0x7fffffffu), max(__float_as_uint(v.y) & 0x7fffffffu, max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu)));
+            }
+            sh.most[0][half][row] = __uint_as_float(top);
+            rows_sync();
+            top = max(top, __float_as_uint(sh.most[0][half ^ 1][row]));
+            rows_sync();
+            const uint32_t exponent = min(max(top >> 23, 1u), 253u);
+            const float up = __uint_as_float((254u - exponent) << 23);
+            factor = __uint_as_float(exponent << 23) * scale;
+#pragma unroll 2
+            for (uint32_t i = 0; i < HD / 32; ++i) {  // 16 elements: 8 columns
+                uint32_t hi[8], lo[8];
 #pragma unroll
-                    for (uint32_t e = 0; e < kEach; e += 4) {
-                        const float4 v = there ? *reinterpret_cast<const float4*>(from + e) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        x[e] = v.x, x[e + 1] = v.y, x[e + 2] = v.z, x[e + 3] = v.w;
-                    }
+                for (uint32_t e = 0; e < 4; ++e) {
+                    const float4 v = there ? from[4 * i + e] : make_float4(0.f, 0.f, 0.f, 0.f);
+                    split_half2(v.x * up * 16384.f, v.y * up * 16384.f, hi[2 * e], lo[2 * e]);
+                    split_half2(v.z * up * 16384.f, v.w * up * 16384.f, hi[2 * e + 1], lo[2 * e + 1]);
                 }
-                uint32_t top = 0;
-#pragma unroll
-                for (uint32_t e = 0; e < kEach; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-                const uint32_t exponent = min(max(__reduce_max_sync(0xffffffffu, top) >> 23, 1u), 253u);
-                const float up = __uint_as_float((254u - exponent) << 23);
-                if (lane == 0) sh.q_factor[r] = __uint_as_float(exponent << 23) * scale;
-                const uint32_t at = (r >> 3) * kKeyStep + (lane * kEach / 8) * kCore + (r & 7) * 16 + (lane * kEach % 8) * 2;
-#pragma unroll
-                for (uint32_t e = 0; e < kEach; e += 2) {
-                    uint32_t hi, lo;
-                    split_half2(x[e] * up * 16384.f, x[e + 1] * up * 16384.f, hi, lo);
-                    *reinterpret_cast<uint32_t*>(sh.q_hi + at + e * 2) = hi;
-                    *reinterpret_cast<uint32_t*>(sh.q_lo + at + e * 2) = lo;
+                tmem_store_8(lanes + kQHi + half * (HD / 4) + 8 * i, hi);
+                if constexpr (kQLoShared) {
+                    uint8_t* to = sh.q_lo + (row >> 3) * kKeyStep + (half * (HD / 16) + 2 * i) * kCore + (row & 7) * 16;
+                    *reinterpret_cast<uint4*>(to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    *reinterpret_cast<uint4*>(to + kCore) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+                } else {
+                    tmem_store_8(lanes + kQLo + half * (HD / 4) + 8 * i, lo);
                 }
             }
-            fence_proxy_async();
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            if (kQLoShared) fence_proxy_async();
+            tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_ready);
         };
-        if (n_tiles > 0) load_queries(sh.desc[0]);
-        float o[HD / 2], factor = 0.f, top = 0.f, total = 0.f, unit = 0.f;
+        if (n_tiles > 0) load_queries(0);
+        float2 o[HD / 4];
+        float row_factor = 0.f, top = 0.f, total = 0.f, unit = 0.f;
         float keep = 0.f, grow = 0.f;  // how the last tile's product joins the sums: o keep + product grow
         int32_t limit = 0;             // the last position that the row sees, negative for none
         auto add_product = [&](uint32_t tile) {
             await(alive, pv_full, tile & 1, dead, 1);
             tc_fence_after_sync();
+            const float2 keep2 = make_float2(keep, keep), grow2 = make_float2(grow, grow);
 #pragma unroll
             for (uint32_t c = 0; c < HD / 2; c += 16) {
                 float v[16];
                 tmem_load_16(lanes + kPv + half * (HD / 2) + c, v);
 #pragma unroll
-                for (uint32_t i = 0; i < 16; ++i) o[c + i] = fmaf(o[c + i], keep, v[i] * grow);
+                for (uint32_t i = 0; i < 16; i += 2) {
+                    float2 add = make_float2(v[i], v[i + 1]);
+                    if (FMT == BC_I8) add = mul2(add, grow2);
+                    o[(c + i) / 2] = fma2(o[(c + i) / 2], keep2, add);
+                }
             }
             tc_fence_before_sync();
         };
         for (uint32_t tile = 0; tile < n_tiles; ++tile) {
             const TileDesc& desc = sh.desc[tile % kDescRing];
-            const bool first = desc.first;
-            if (first) {
-                rows_sync();  // q_factor is there
-                factor = sh.q_factor[row];
-                // (Rows that are nobody's see all there is: no tile is masked for them.)
-                const uint32_t query = row / p.group;
-                limit = (int32_t)min((int64_t)desc.pos0 + (query < desc.n ? query : 0x40000000u), (int64_t)desc.end - 1);
-#pragma unroll
-                for (uint32_t i = 0; i < HD / 2; ++i) o[i] = 0.f;
-                top = -INFINITY;
-                total = unit = 0.f;
-            }
             const uint32_t buffer = tile & 1;
             const TileInfo<KT, FMT>& info = sh.info[tile % kRing];
             await(alive, s_full + 8 * buffer, (tile >> 1) & 1, dead, 2);
             tc_fence_after_sync();
-            const uint32_t scores_at = lanes + buffer * KT;
-            float x[KT / 2];
+            const bool first = desc.first;
+            if (first) {
+                // (Rows that are nobody's see all there is: no tile is masked for them.)
+                const uint32_t query = row / p.group;
+                limit = (int32_t)min((int64_t)desc.pos0 + (query < desc.n ? query : 0x40000000u), (int64_t)desc.end - 1);
+                row_factor = factor;
 #pragma unroll
-            for (uint32_t c = 0; c < KT / 2; c += 32) tmem_load_32(scores_at + half * (KT / 2) + c, *reinterpret_cast<float(*)[32]>(x + c));
+                for (uint32_t i = 0; i < HD / 4; ++i) o[i] = make_float2(0.f, 0.f);
+                top = -INFINITY;
+                total = unit = 0.f;
+            }
+            const uint32_t scores_at = lanes + buffer * KT;
+            float2 x[KT / 4];
+#pragma unroll
+            for (uint32_t c = 0; c < KT / 4; c += 16) tmem_load_32(scores_at + half * (KT / 2) + 2 * c, x + c);
             const uint32_t key0 = desc.key0 + half * (KT / 2);
             uint32_t seen[KT / 64];  // positions of this half that the row sees
             uint32_t all = 0xffffffffu;
@@ -448,22 +449,25 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             const bool masked = __any_sync(0xffffffffu, all != 0xffffffffu);
             if constexpr (FMT == BC_I8) {
 #pragma unroll
-                for (uint32_t i = 0; i < KT / 2; i += 4) {
-                    const float4 d = *reinterpret_cast<const float4*>(info.dk + half * (KT / 2) + i);
-                    x[i] *= d.x, x[i + 1] *= d.y, x[i + 2] *= d.z, x[i + 3] *= d.w;
+                for (uint32_t i = 0; i < KT / 4; i += 2) {
+                    const float4 d = *reinterpret_cast<const float4*>(info.dk + half * (KT / 2) + 2 * i);
+                    x[i] = mul2(x[i], make_float2(d.x, d.y));
+                    x[i + 1] = mul2(x[i + 1], make_float2(d.z, d.w));
                 }
             }
             if (masked) {
 #pragma unroll
-                for (uint32_t i = 0; i < KT / 2; ++i)
-                    if (!(seen[i / 32] >> (i % 32) & 1)) x[i] = -INFINITY;
+                for (uint32_t i = 0; i < KT / 4; ++i) {
+                    if (!(seen[i / 16] >> (2 * i % 32) & 1)) x[i].x = -INFINITY;
+                    if (!(seen[i / 16] >> (2 * i % 32 + 1) & 1)) x[i].y = -INFINITY;
+                }
             }
             float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (uint32_t i = 0; i < KT / 2; i += 4)
+            for (uint32_t i = 0; i < KT / 4; i += 4)
 #pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) most[j] = fmaxf(most[j], x[i + j]);
-            const float mine_most = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * factor;
+                for (uint32_t j = 0; j < 4; ++j) most[j] = fmaxf(most[j], fmaxf(x[i + j].x, x[i + j].y));
+            const float mine_most = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * row_factor;
             sh.most[tile & 1][half][row] = mine_most;
             rows_sync();  // and every thread has read its scores: probabilities may take their place
             const float now = fmaxf(top, fmaxf(mine_most, sh.most[tile & 1][half ^ 1][row]));
@@ -475,40 +479,45 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             if constexpr (FMT == BC_I8) {
                 uint32_t largest = 0;
 #pragma unroll
-                for (uint32_t w = 0; w < kLoadWarps; ++w) largest = max(largest, info.top_scale[w]);
+                for (uint32_t w = 0; w < kUnpackWarps; ++w) largest = max(largest, info.top_scale[w]);
                 const uint32_t exponent = min(max(largest >> 23, 27u), 227u);  // 2^-100 to 2^100
                 tile_unit = __uint_as_float(exponent << 23);
                 down -= (float)((int)exponent - 127);
             }
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const float2 factor2 = make_float2(row_factor, row_factor), down2 = make_float2(down, down);
+            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-            for (uint32_t i = 0; i < KT / 2; i += 16) {
-                uint32_t hi[8], lo[8];
+            for (uint32_t i = 0; i < KT / 4; i += 4) {  // 8 positions
+                float2 d2[4];
+                if constexpr (FMT == BC_I8) {
 #pragma unroll
-                for (uint32_t j = 0; j < 16; j += 4) {
-                    float w[4];
-#pragma unroll
-                    for (uint32_t e = 0; e < 4; ++e) {
-                        w[e] = exp2_fast(fmaf(x[i + j + e], factor, down));
-                        sum[e] += w[e];
+                    for (uint32_t j = 0; j < 4; j += 2) {
+                        const float4 d = *reinterpret_cast<const float4*>(info.dv + half * (KT / 2) + 2 * (i + j));
+                        d2[j] = make_float2(d.x, d.y);
+                        d2[j + 1] = make_float2(d.z, d.w);
                     }
-                    if constexpr (FMT == BC_I8) {
-                        const float4 d = *reinterpret_cast<const float4*>(info.dv + half * (KT / 2) + i + j);
-                        w[0] *= d.x, w[1] *= d.y, w[2] *= d.z, w[3] *= d.w;
-                        if (masked) {
+                }
+                uint32_t hi[4], lo[4];
 #pragma unroll
-                            for (uint32_t e = 0; e < 4; ++e)
-                                if (!(seen[(i + j + e) / 32] >> ((i + j + e) % 32) & 1)) w[e] = 0.f;  // a scale may be no number
+                for (uint32_t j = 0; j < 4; ++j) {
+                    float2 w = fma2(x[i + j], factor2, down2);
+                    w.x = exp2_fast(w.x);
+                    w.y = exp2_fast(w.y);
+                    sum[j & 1] = add2(sum[j & 1], w);
+                    if constexpr (FMT == BC_I8) {
+                        w = mul2(w, d2[j]);
+                        if (masked) {  // a scale may be no number
+                            if (!(seen[(i + j) / 16] >> (2 * (i + j) % 32) & 1)) w.x = 0.f;
+                            if (!(seen[(i + j) / 16] >> (2 * (i + j) % 32 + 1) & 1)) w.y = 0.f;
                         }
                     }
-                    split_half2(w[0], w[1], hi[j / 2], lo[j / 2]);
-                    split_half2(w[2], w[3], hi[j / 2 + 1], lo[j / 2 + 1]);
+                    cut_half2(w, hi[j], lo[j]);
                 }
-                tmem_store_8(scores_at + half * (KT / 4) + i / 2, hi);
-                tmem_store_8(scores_at + KT / 2 + half * (KT / 4) + i / 2, lo);
+                tmem_store_4(scores_at + half * (KT / 4) + i, hi);
+                tmem_store_4(scores_at + KT / 2 + half * (KT / 4) + i, lo);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            total = total * fall + ((sum[0] + sum[1]) + (sum[2] + sum[3])) * tile_unit;
+            total = total * fall + ((sum[0].x + sum[1].x) + (sum[0].y + sum[1].y)) * tile_unit;
             if (!first) add_product(tile - 1);  // before the next one may take its place
             if constexpr (FMT == BC_I8) {
                 // The sums' unit follows the larger of what they were and what this tile brings.
@@ -519,16 +528,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 unit = next;
             } else {
                 keep = fall;
-                grow = 1.f;
                 unit = 1.f;
             }
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(p_ready);
+
             if (!desc.last) continue;
             // The next unit's queries go ahead of this one's end: the last scores are done.
-            rows_sync();  // q_factor has been read
-            if (tile + 1 < n_tiles) load_queries(sh.desc[(tile + 1) % kDescRing]);
+            rows_sync();  // the maxima have been read
+            if (tile + 1 < n_tiles) load_queries(tile + 1);
             add_product(tile);
             // A row's two sums of probabilities meet.
             sh.most[0][half][row] = total;
@@ -539,117 +548,143 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 const uint32_t slot = desc.unit % kUnits;
                 if (sh.any_not_finite[slot]) {
 #pragma unroll
-                    for (uint32_t i = 0; i < HD / 2; ++i)
-                        if ((int64_t)sh.not_finite[slot][half * (HD / 2) + i] <= limit) o[i] = __uint_as_float(0x7fc00000u);
-                }
-            }
-            if (desc.begins && desc.ends) {
-                if (row / p.group < desc.n) {
-                    const float inverse = top == -INFINITY && total == 0.f ? 0.f : unit / total;
-                    float* to = p.out + (uint64_t)(desc.row0 + row / p.group) * p.n_heads * HD + (desc.head * p.group + row % p.group) * HD + half * (HD / 2);
-#pragma unroll
-                    for (uint32_t i = 0; i < HD / 2; i += 4)
-                        *reinterpret_cast<float4*>(to + i) = make_float4(o[i] * inverse, o[i + 1] * inverse, o[i + 2] * inverse, o[i + 3] * inverse);
-                }
-            } else {
-                const uint32_t slot = 2 * blockIdx.x + (desc.begins ? 1 : 0);
-                float* to = p.parts + ((uint64_t)slot * kRows + row) * HD + half * (HD / 2);
-#pragma unroll
-                for (uint32_t i = 0; i < HD / 2; i += 4) *reinterpret_cast<float4*>(to + i) = make_float4(o[i] * unit, o[i + 1] * unit, o[i + 2] * unit, o[i + 3] * unit);
-                if (half == 0) *reinterpret_cast<float2*>(p.parts + (uint64_t)2 * kMostCtas * kRows * HD + ((uint64_t)slot * kRows + row) * 2) = make_float2(top, total);
-            }
-        }
-    } else if (warp < kMmaWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-        // ---- keys and values
-        const uint32_t ltid = tid - kRowThreads, lwarp = ltid >> 5;
-        constexpr uint32_t kUnitsOfKeys = KT * (HD / 8) / kLoadThreads;        // pieces of 8 elements of a key that a thread brings
-        constexpr uint32_t kBlocks = KT / 8 * (HD / 8) / kLoadThreads;         // blocks of 8 positions x 8 elements of values
-        constexpr uint32_t kPiece = FMT == BC_F16 ? 16 : 8, kPieceWords = kPiece / 4;
-        uint32_t k_raw[FMT == BC_F16 ? 1 : kUnitsOfKeys][2];
-        uint32_t v_raw[kBlocks][8][kPieceWords];
-        float dk = 0.f, dv = 0.f;
-
-        auto key_there = [&](uint32_t j, uint32_t key) {
-            return sh.info[j % kRing].rows_at[key >> 4] != ~0ull && sh.desc[j % kDescRing].key0 + key < sh.desc[j % kDescRing].end;
-        };
-        // What a tile's loads are, into registers (or, halves of keys, straight to shared memory).
-        auto load_scales = [&](uint32_t j) {
-            const TileInfo<KT, FMT>& info = sh.info[j % kRing];
-            dk = dv = 0.f;
-            if (FMT == BC_I8 && ltid < KT && key_there(j, ltid)) {
-                const uint64_t at = info.scales_at[ltid >> 4] + 4 * (ltid & 15);
-                dk = *reinterpret_cast<const float*>(pool.k + at);
-                dv = *reinterpret_cast<const float*>(pool.v + at);
-            }
-        };
-        auto load_keys = [&](uint32_t j) {
-            const TileInfo<KT, FMT>& info = sh.info[j % kRing];
-#pragma unroll
-            for (uint32_t n = 0; n < kUnitsOfKeys; ++n) {
-                const uint32_t i = ltid + n * kLoadThreads, piece = i % (HD / 8), key = i / (HD / 8);
-                const bool there = key_there(j, key);
-                const uint8_t* from = pool.k + info.rows_at[key >> 4] + (key & 15) * pool.row_bytes + piece * kPiece;
-                if constexpr (FMT == BC_F16) {
-                    if (there) cp_async_16(smem_u32(sh.keys[j % ST]) + (key >> 3) * kKeyStep + piece * kCore + (key & 7) * 16, from);
-                } else {
-                    const uint2 w = there ? *reinterpret_cast<const uint2*>(from) : make_uint2(0, 0);
-                    k_raw[n][0] = w.x;
-                    k_raw[n][1] = w.y;
-                }
-            }
-        };
-        auto load_values = [&](uint32_t j) {
-            const TileInfo<KT, FMT>& info = sh.info[j % kRing];
-#pragma unroll
-            for (uint32_t n = 0; n < kBlocks; ++n) {
-                const uint32_t i = ltid + n * kLoadThreads, piece = i % (HD / 8), key = i / (HD / 8) * 8;
-                const uint8_t* from = pool.v + info.rows_at[key >> 4] + (key & 15) * pool.row_bytes + piece * kPiece;
-#pragma unroll
-                for (uint32_t r = 0; r < 8; ++r) {
-                    const bool there = key_there(j, key + r);
-                    if constexpr (FMT == BC_F16) {
-                        const uint4 w = there ? *reinterpret_cast<const uint4*>(from + r * pool.row_bytes) : make_uint4(0, 0, 0, 0);
-                        v_raw[n][r][0] = w.x, v_raw[n][r][1] = w.y, v_raw[n][r][kPieceWords - 2] = w.z, v_raw[n][r][kPieceWords - 1] = w.w;
-                    } else {
-                        const uint2 w = there ? *reinterpret_cast<const uint2*>(from + r * pool.row_bytes) : make_uint2(0x80808080u, 0x80808080u);
-                        v_raw[n][r][0] = w.x, v_raw[n][r][1] = w.y;
+                    for (uint32_t i = 0; i < HD / 4; ++i) {
+                        if ((int64_t)sh.not_finite[slot][half * (HD / 2) + 2 * i] <= limit) o[i].x = __uint_as_float(0x7fc00000u);
+                        if ((int64_t)sh.not_finite[slot][half * (HD / 2) + 2 * i + 1] <= limit) o[i].y = __uint_as_float(0x7fc00000u);
                     }
                 }
             }
-        };
-        auto store_values = [&](uint32_t j) {
+            const bool whole = desc.begins && desc.ends;
+            const uint32_t slot = 2 * blockIdx.x + (desc.begins ? 1 : 0);
+            const float times = whole ? (top == -INFINITY && total == 0.f ? 0.f : unit / total) : unit;
+            float* to = (whole ? p.out + (uint64_t)(desc.row0 + row / p.group) * p.n_heads * HD + (desc.head * p.group + row % p.group) * HD
+                               : p.parts + ((uint64_t)slot * kRows + row) * HD) + half * (HD / 2);
+            if (row / p.group < desc.n) {
+#pragma unroll
+                for (uint32_t i = 0; i < HD / 4; i += 2)
+                    *reinterpret_cast<float4*>(to + 2 * i) = make_float4(o[i].x * times, o[i].y * times, o[i + 1].x * times, o[i + 1].y * times);
+            }
+            if (!whole && half == 0)
+                *reinterpret_cast<float2*>(p.parts + (uint64_t)2 * kMostCtas * kRows * HD + ((uint64_t)slot * kRows + row) * 2) = make_float2(top, total);
+        }
+    } else if (warp < kMmaWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        // ---- bytes to operands
+        const uint32_t utid = tid - kRowThreads, uwarp = utid >> 5;
+        constexpr uint32_t kPieces = KT * (HD / 8) / kUnpackThreads;           // pieces of 8 elements of a key that a thread unpacks
+        constexpr uint32_t kBlocks = KT / 8 * (HD / 8) / kUnpackThreads;       // blocks of 8 positions x 8 elements of values
+        constexpr uint32_t kPiece = FMT == BC_F16 ? 16 : 8, kWords = kPiece / 4, kRowBytes = RawTile<KT, FMT, HD>::kRowBytes;
+        for (uint32_t j = 0; j < n_tiles; ++j) {
+            const uint32_t st = j % ST;
+            TileInfo<KT, FMT>& info = sh.info[j % kRing];
+            const RawTile<KT, FMT, HD>& raw = sh.raw[j % RAW];
+            await(alive, raw_full + 8 * (j % RAW), (j / RAW) & 1, dead, 10);
             const TileDesc& desc = sh.desc[j % kDescRing];
-            uint8_t* const to = sh.values[j % ST];
+            const uint32_t key0 = desc.key0, end = desc.end, groups = desc.groups;
+            auto key_there = [&](uint32_t key) { return (groups >> (key >> 4) & 1) && key0 + key < end; };
+            const bool whole = groups == (1u << KT / 16) - 1 && end - key0 >= KT;  // every position is there
+            // Free keys: their scores are done, so the rows' warps are done with the tile before those, and the ring's fourth is nobody's.
+            await(alive, k_free + 8 * st, ((j / ST) & 1) ^ 1, dead, 3);
+            if constexpr (FMT == BC_F16) {
+                if (desc.first) {
+                    const uint32_t slot = desc.unit % kUnits;
+                    for (uint32_t i = utid; i < HD; i += kUnpackThreads) sh.not_finite[slot][i] = 0xffffffffu;
+                    if (utid == 0) sh.any_not_finite[slot] = 0;
+                    asm volatile("bar.sync 2, %0;" ::"n"(kUnpackThreads) : "memory");  // before any of them finds one
+                }
+            }
+            // Masks and scales of the tile's positions.
+            const bool there = utid < KT && key_there(utid);
+            const uint32_t votes = __ballot_sync(0xffffffffu, there);
+            if (lane == 0 && uwarp < KT / 32) info.valid[uwarp] = votes;
+            if constexpr (FMT == BC_I8) {
+                const float dv = there ? raw.dv[utid] : 0.f;
+                if (utid < KT) {
+                    info.dk[utid] = there ? raw.dk[utid] : 0.f;
+                    info.dv[utid] = dv;
+                }
+                // The largest finite one.
+                const uint32_t bits = __float_as_uint(dv) & 0x7fffffffu, largest = __reduce_max_sync(0xffffffffu, bits < 0x7f800000u ? bits : 0u);
+                if (lane == 0) info.top_scale[uwarp] = largest;
+            }
+            {  // What is there of positions that are not is masked in the scores, whatever it is.
+                const uint8_t* from = raw.keys + utid * kPiece;
+                uint8_t* const to = sh.keys[st];
+#pragma unroll
+                for (uint32_t n = 0; n < kPieces; ++n) {
+                    const uint32_t i = utid + n * kUnpackThreads, piece = i % (HD / 8), key = i / (HD / 8);
+                    uint4 w;
+                    if constexpr (FMT == BC_F16) {
+                        w = *reinterpret_cast<const uint4*>(from + n * kUnpackThreads * kPiece);
+                    } else {
+                        const uint2 b = *reinterpret_cast<const uint2*>(from + n * kUnpackThreads * kPiece);
+                        unpack_i8(b.x, w.x, w.y);
+                        unpack_i8(b.y, w.z, w.w);
+                    }
+                    *reinterpret_cast<uint4*>(to + (key >> 3) * kKeyStep + piece * kCore + (key & 7) * 16) = w;
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(k_full + 8 * st);
+
+            await(alive, v_free + 8 * st, ((j / ST) & 1) ^ 1, dead, 4);
+            uint8_t* const to = sh.values[st];
             // A value that is not finite would reach rows that do not see it: zero times it is no number. Tiles that end behind the row tile's
             // first row keep such values apart.
-            const bool apart = FMT == BC_F16 && (int64_t)desc.key0 + KT - 1 > desc.pos0;
+            const bool apart = FMT == BC_F16 && (int64_t)key0 + KT - 1 > desc.pos0;
 #pragma unroll
             for (uint32_t n = 0; n < kBlocks; ++n) {
-                const uint32_t i = ltid + n * kLoadThreads, piece = i % (HD / 8), key = i / (HD / 8) * 8;
+                const uint32_t i = utid + n * kUnpackThreads, piece = i % (HD / 8), key = i / (HD / 8) * 8;
+                const uint8_t* from = raw.values + key * kRowBytes + piece * kPiece;
                 uint4* const core = reinterpret_cast<uint4*>(to + piece * kCore + (key >> 3) * kKeyStep);  // 8 elements x 8 positions
+                uint32_t v[8][kWords];
+#pragma unroll
+                for (uint32_t r = 0; r < 8; ++r) {
+                    if constexpr (FMT == BC_F16) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(from + r * kRowBytes);
+                        v[r][0] = w.x, v[r][1] = w.y, v[r][2] = w.z, v[r][3] = w.w;
+                    } else {
+                        const uint2 w = *reinterpret_cast<const uint2*>(from + r * kRowBytes);
+                        v[r][0] = w.x, v[r][1] = w.y;
+                    }
+                }
+                if (!whole) {
+#pragma unroll
+                    for (uint32_t r = 0; r < 8; ++r)
+                        if (!key_there(key + r))
+#pragma unroll
+                            for (uint32_t w = 0; w < kWords; ++w) v[r][w] = FMT == BC_F16 ? 0u : 0x80808080u;
+                }
                 if constexpr (FMT == BC_F16) {
                     if (apart) {
+                        uint32_t any = 0;
 #pragma unroll
                         for (uint32_t r = 0; r < 8; ++r)
 #pragma unroll
-                            for (uint32_t w = 0; w < kPieceWords; ++w)
+                            for (uint32_t w = 0; w < kWords; ++w) any |= (v[r][w] & 0x7c007c00u) + 0x04000400u;  // exponents of all ones carry
+                        if (any & 0x80008000u) {
 #pragma unroll
-                                for (uint32_t e = 0; e < 2; ++e)
-                                    if ((v_raw[n][r][w] >> (16 * e) & 0x7c00u) == 0x7c00u) {
-                                        const uint32_t slot = desc.unit % kUnits;
-                                        atomicMin(&sh.not_finite[slot][FMT == BC_F16 ? 8 * piece + 2 * w + e : 0], desc.key0 + key + r);
-                                        sh.any_not_finite[slot] = 1;
-                                        v_raw[n][r][w] &= ~(0xffffu << (16 * e));
-                                    }
+                            for (uint32_t r = 0; r < 8; ++r)
+#pragma unroll
+                                for (uint32_t w = 0; w < kWords; ++w)
+#pragma unroll
+                                    for (uint32_t e = 0; e < 2; ++e)
+                                        if ((v[r][w] >> (16 * e) & 0x7c00u) == 0x7c00u) {
+                                            const uint32_t slot = desc.unit % kUnits;
+                                            atomicMin(&sh.not_finite[slot][8 * piece + 2 * w + e], key0 + key + r);
+                                            sh.any_not_finite[slot] = 1;
+                                            v[r][w] &= ~(0xffffu << (16 * e));
+                                        }
+                        }
                     }
 #pragma unroll
                     for (uint32_t w = 0; w < 4; ++w) {
                         uint32_t even[4], odd[4];
 #pragma unroll
                         for (uint32_t r = 0; r < 4; ++r) {
-                            even[r] = __byte_perm(v_raw[n][2 * r][w % kPieceWords], v_raw[n][2 * r + 1][w % kPieceWords], 0x5410);
-                            odd[r] = __byte_perm(v_raw[n][2 * r][w % kPieceWords], v_raw[n][2 * r + 1][w % kPieceWords], 0x7632);
+                            even[r] = __byte_perm(v[2 * r][w], v[2 * r + 1][w], 0x5410);
+                            odd[r] = __byte_perm(v[2 * r][w], v[2 * r + 1][w], 0x7632);
                         }
                         core[2 * w] = make_uint4(even[0], even[1], even[2], even[3]);
                         core[2 * w + 1] = make_uint4(odd[0], odd[1], odd[2], odd[3]);
@@ -661,91 +696,25 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                         for (uint32_t h = 0; h < 2; ++h) {  // elements 4w + 2h and the next
                             uint32_t even[4], odd[4];
 #pragma unroll
-                            for (uint32_t r = 0; r < 4; ++r)
-                                unpack_i8(__byte_perm(v_raw[n][2 * r][w], v_raw[n][2 * r + 1][w], h ? 0x7362 : 0x5140), even[r], odd[r]);
+                            for (uint32_t r = 0; r < 4; ++r) unpack_i8(__byte_perm(v[2 * r][w], v[2 * r + 1][w], h ? 0x7362 : 0x5140), even[r], odd[r]);
                             core[4 * w + 2 * h] = make_uint4(even[0], even[1], even[2], even[3]);
                             core[4 * w + 2 * h + 1] = make_uint4(odd[0], odd[1], odd[2], odd[3]);
                         }
                 }
             }
-        };
-        if (n_tiles > 0) {
-            load_scales(0);
-            if (FMT == BC_I8) load_keys(0);
-            load_values(0);
-        }
-        for (uint32_t j = 0; j <= n_tiles; ++j) {
-            if (j < n_tiles) {
-                const uint32_t st = j % ST;
-                TileInfo<KT, FMT>& info = sh.info[j % kRing];
-                describe(j + 1);
-                // Free keys: their scores are done, so the rows' warps are done with the tile before those, and the ring's fourth is nobody's.
-                await(alive, k_free + 8 * st, ((j / ST) & 1) ^ 1, dead, 3);
-                if (FMT == BC_F16 && sh.desc[j % kDescRing].first) {
-                    const uint32_t slot = sh.desc[j % kDescRing].unit % kUnits;
-                    for (uint32_t i = ltid; i < (FMT == BC_F16 ? HD : 1); i += kLoadThreads) sh.not_finite[slot][i] = 0xffffffffu;
-                    if (ltid == 0) sh.any_not_finite[slot] = 0;
-                    // The barrier below comes before the unit's first values are stored.
-                }
-                // Masks and scales of the tile's positions.
-                const bool there = ltid < KT && key_there(j, ltid);
-                const uint32_t votes = __ballot_sync(0xffffffffu, there);
-                if (lane == 0 && lwarp < KT / 32) info.valid[lwarp] = votes;
-                if (FMT == BC_I8) {
-                    if (ltid < KT) {
-                        info.dk[ltid] = dk;
-                        info.dv[ltid] = dv;
-                    }
-                    // The largest finite one.
-                    const uint32_t bits = __float_as_uint(dv) & 0x7fffffffu, largest = __reduce_max_sync(0xffffffffu, bits < 0x7f800000u ? bits : 0u);
-                    if (lane == 0) info.top_scale[lwarp] = largest;
-                }
-                if constexpr (FMT == BC_F16) {
-                    load_keys(j);
-                    cp_async_commit();
-                } else {
-                    uint8_t* const to = sh.keys[st];
-#pragma unroll
-                    for (uint32_t n = 0; n < kUnitsOfKeys; ++n) {
-                        const uint32_t i = ltid + n * kLoadThreads, piece = i % (HD / 8), key = i / (HD / 8);
-                        uint4 w;
-                        unpack_i8(k_raw[n][0], w.x, w.y);
-                        unpack_i8(k_raw[n][1], w.z, w.w);
-                        *reinterpret_cast<uint4*>(to + (key >> 3) * kKeyStep + piece * kCore + (key & 7) * 16) = w;
-                    }
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(k_full + 8 * st);
-                }
-            }
-            loads_sync();  // tile j + 1 is described
-            if (FMT == BC_I8 && j + 1 < n_tiles) {
-                load_scales(j + 1);
-                load_keys(j + 1);
-            }
-            if (j > 0) {
-                const uint32_t st = (j - 1) % ST;
-                await(alive, v_free + 8 * st, (((j - 1) / ST) & 1) ^ 1, dead, 4);
-                store_values(j - 1);
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(v_full + 8 * st);
-                if (j < n_tiles) load_values(j);
-            }
-            if (FMT == BC_F16 && j < n_tiles) {
-                cp_async_wait<0>();
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(k_full + 8 * (j % ST));
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(v_full + 8 * st);
+                mbar_arrive(raw_free + 8 * (j % RAW));
             }
         }
-        if (ltid == 0) reinterpret_cast<ChunkHead*>(p.parts + (uint64_t)2 * kMostCtas * kRows * (HD + 2))[blockIdx.x] = sh.place.cut;
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         if (warp == kMmaWarp) {
-            // ---- the tensor core
+            // ---- the tensor core. Lower halves first: what a sum cuts off grows with what is there already.
             const uint32_t scores_idesc = umma_idesc_f16(kRows, KT), values_idesc = umma_idesc_f16(kRows, HD);
-            const uint64_t q_hi = umma_desc(smem_u32(sh.q_hi), kCore, kKeyStep), q_lo = umma_desc(smem_u32(sh.q_lo), kCore, kKeyStep);
+            const uint64_t q_lo = umma_desc(smem_u32(sh.q_lo), kCore, kKeyStep);
             uint32_t units = 0;
             auto product = [&](uint32_t j) {  // P V of tile j
                 await(alive, p_ready, j & 1, dead, 5);
@@ -758,7 +727,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                     for (uint32_t part = 0; part < 2; ++part)
 #pragma unroll
                         for (uint32_t ks = 0; ks < KT / 16; ++ks)
-                            umma_f16_a_tmem(tmem + kPv, weights + part * (KT / 2) + ks * 8, v + (uint64_t)(ks * 2 * kKeyStep >> 4), values_idesc, part | ks);
+                            umma_f16_a_tmem(tmem + kPv, weights + (part ^ 1) * (KT / 2) + ks * 8, v + (uint64_t)(ks * 2 * kKeyStep >> 4), values_idesc, part | ks);
                     umma_commit(v_free + 8 * (j % ST));
                     umma_commit(pv_full);
                 }
@@ -775,11 +744,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 tc_fence_after_sync();
                 if (elect_one()) {
                     const uint64_t keys = umma_desc(smem_u32(sh.keys[j % ST]), kCore, kKeyStep);
-#pragma unroll 1
-                    for (uint32_t part = 0; part < 2; ++part)
+                    const uint32_t to = tmem + (j & 1) * KT;
 #pragma unroll
-                        for (uint32_t ks = 0; ks < HD / 16; ++ks)
-                            umma_f16(tmem + (j & 1) * KT, (part ? q_lo : q_hi) + (uint64_t)(ks * 2 * kCore >> 4), keys + (uint64_t)(ks * 2 * kCore >> 4), scores_idesc, part | ks);
+                    for (uint32_t ks = 0; ks < HD / 16; ++ks) {
+                        if constexpr (kQLoShared)
+                            umma_f16(to, q_lo + (uint64_t)(ks * 2 * kCore >> 4), keys + (uint64_t)(ks * 2 * kCore >> 4), scores_idesc, ks);
+                        else
+                            umma_f16_a_tmem(to, tmem + kQLo + ks * 8, keys + (uint64_t)(ks * 2 * kCore >> 4), scores_idesc, ks);
+                    }
+#pragma unroll
+                    for (uint32_t ks = 0; ks < HD / 16; ++ks) umma_f16_a_tmem(to, tmem + kQHi + ks * 8, keys + (uint64_t)(ks * 2 * kCore >> 4), scores_idesc, 1);
                     umma_commit(k_free + 8 * (j % ST));
                     umma_commit(s_full + 8 * (j & 1));
                 }
@@ -787,6 +761,82 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 if (!first) product(j - 1);
             }
             if (n_tiles > 0) product(n_tiles - 1);
+        } else if (warp == kCopyWarp) {
+            // ---- the walk through the run, and the pages' bytes: a lane per 16 positions of keys, values, and either's scales.
+            Place& at = sh.place;
+            constexpr uint32_t kGroups = KT / 16, kRowBytes = RawTile<KT, FMT, HD>::kRowBytes;
+            const uint32_t page_slots = (1u << pool.page_shift) - 1;
+            for (uint32_t j = 0; j < n_tiles; ++j) {
+                TileDesc& d = sh.desc[j % kDescRing];
+                if (lane == 0) {
+                    if (at.in_unit == at.unit.tiles) {
+                        at.cursor.take(p, capacity, KT, at.unit);
+                        at.in_unit = 0;
+                        ++at.unit_number;
+                    }
+                    const Unit& u = at.unit;
+                    const ChunkSeq& s = at.cursor.s;
+                    const uint32_t query0 = u.row_tile * per_tile;
+                    const int64_t pos = (int64_t)s.len - (s.end - s.row0) + query0;
+                    d.key0 = (u.tile0 + at.in_unit) * KT;
+                    d.end = s.held;
+                    d.row0 = s.row0 + query0;
+                    d.n = min(per_tile, s.n - query0);
+                    d.head = u.head;
+                    d.pos0 = (int32_t)min(pos, (int64_t)0x7fffffff);
+                    d.unit = at.unit_number;
+                    d.first = at.in_unit == 0;
+                    d.last = at.in_unit + 1 == u.tiles;
+                    d.begins = u.begins;
+                    d.ends = u.ends;
+                    if (s.held < s.len) leave_fault(pool, kFaultTable);
+                    if (u.begins && !u.ends && at.in_unit == 0) {
+                        // The CTA whose run holds the row tile's last key tile: run c is [total c / runs, total (c + 1) / runs).
+                        const uint64_t total = sh.total, runs = min((uint64_t)gridDim.x, total), last_tile = total * blockIdx.x / runs + j + at.cursor.count - 1;
+                        uint32_t last = (uint32_t)(last_tile * runs / total);
+                        while (total * (last + 1) / runs <= last_tile) ++last;
+                        while (total * last / runs > last_tile) --last;
+                        at.cut = ChunkHead{d.row0, d.n, d.head, last};
+                    }
+                    ++at.in_unit;
+                }
+                __syncwarp();
+                // Every lane looks up its group's page.
+                const uint32_t group = lane % kGroups, what = lane / kGroups, key = d.key0 + 16 * group;
+                uint32_t page = ~0u;
+                if (key < d.end && what < 4) {
+                    page = p.rows.table[(uint64_t)at.unit.seq * p.rows.max_pages + (key >> pool.page_shift)];
+                    if (page >= pool.n_pages) leave_fault(pool, kFaultPage);
+                }
+                const bool there = page < pool.n_pages;
+                const uint32_t groups = __ballot_sync(0xffffffffu, there) & ((1u << kGroups) - 1);
+                const uint32_t slot = j % RAW, bar = raw_full + 8 * slot;
+                await(alive, raw_free + 8 * slot, ((j / RAW) & 1) ^ 1, dead, 11);
+                if (lane == 0) {
+                    d.groups = groups;
+                    mbar_arrive(described + 8 * (j % kDescRing));
+                    mbar_arrive_expect(bar, __popc(groups) * 16 * 2 * (kRowBytes + (FMT == BC_I8 ? 4 : 0)));
+                }
+                __syncwarp();
+                if (there && alive) {
+                    RawTile<KT, FMT, HD>& raw = sh.raw[slot];
+                    const uint64_t rows_at = kv_row_at(pool, page, d.head, key & page_slots);
+                    if (what < 2) {
+                        bulk_load(smem_u32(what ? raw.values : raw.keys) + group * 16 * kRowBytes, (what ? pool.v : pool.k) + rows_at, 16 * kRowBytes, bar);
+                    } else if (FMT == BC_I8 && what < 4) {
+                        bulk_load(smem_u32(what == 3 ? raw.dv : raw.dk) + group * 64, (what == 3 ? pool.v : pool.k) + kv_scale_at(pool, page, d.head, key & page_slots), 64, bar);
+                    }
+                }
+                __syncwarp();
+            }
+            if (lane == 0) reinterpret_cast<ChunkHead*>(p.parts + (uint64_t)2 * kMostCtas * kRows * (HD + 2))[blockIdx.x] = at.cut;
+            // Copies in flight end before the CTA does: their tiles are waited for by the unpacking warps, or here when those gave up.
+            for (uint32_t r = 0; r < RAW && r < n_tiles; ++r) {
+                const uint32_t j = n_tiles - 1 - r;
+                bool patient = true;
+                if (!alive || *dead) patient = mbar_wait(raw_full + 8 * (j % RAW), (j / RAW) & 1, kSpinLimit, &sh.never);
+                (void)patient;
+            }
         }
     }
     // Whoever waited for the last product has seen all multiplies end; after a wait that ran out, they get a limited time to.
@@ -864,7 +914,6 @@ template <int FMT, int HD>
 cudaError_t launch_chunk(cudaStream_t stream, const ChunkParams& p) {
     constexpr size_t smem = sizeof(Shared<FMT, HD>);
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
-    static_assert(2 * key_tile<HD>() + HD <= kTmemColumns, "tensor memory");
     cudaError_t e = ensure_dynamic_smem((const void*)attention_chunk_kernel<FMT, HD>, smem);
     if (e != cudaSuccess) return e;
     const uint32_t ctas = chunk_ctas();
