@@ -14,6 +14,8 @@
 // Queries and probabilities are A operands in tensor memory: both operands in shared memory would take its 128 bytes a cycle whole. (Heads of 256
 // leave room for the queries' upper halves alone.)
 
+#include <type_traits>
+
 #include "async_utils.cuh"
 #include "chunk_schedule.h"
 #include "kv_pool.cuh"
@@ -165,13 +167,13 @@ __device__ __forceinline__ void tmem_load_32(uint32_t taddr, float2* v) {
         : "r"(taddr)
         : "memory");
 }
+// Loads and stores of memory may move across these; tcgen05.wait::st keeps what follows behind.
 __device__ __forceinline__ void tmem_store_8(uint32_t taddr, const uint32_t (&v)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
-                 "r"(v[6]), "r"(v[7])
-                 : "memory");
+                 "r"(v[6]), "r"(v[7]));
 }
 __device__ __forceinline__ void tmem_store_4(uint32_t taddr, const uint32_t (&v)[4]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]));
 }
 // Pairs of f32 in one instruction.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
@@ -207,7 +209,7 @@ __device__ __forceinline__ void split_half2(float x, float y, uint32_t& hi, uint
 __device__ __forceinline__ void cut_half2(float2 x, uint32_t& hi, uint32_t& lo) {
     const float2 upper = make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffffe000u), __uint_as_float(__float_as_uint(x.y) & 0xffffe000u));
     const __half2 h = __floats2half2_rn(upper.x, upper.y);
-    const float2 rest = add2(x, make_float2(-upper.x, -upper.y));
+    const float2 rest = fma2(upper, make_float2(-1.f, -1.f), x);
     const __half2 l = __floats2half2_rn(rest.x, rest.y);
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&l);
@@ -486,45 +488,52 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             }
             const float2 factor2 = make_float2(row_factor, row_factor), down2 = make_float2(down, down);
             float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            auto probabilities = [&](auto some_unseen) {
 #pragma unroll
-            for (uint32_t i = 0; i < KT / 4; i += 4) {  // 8 positions
-                float2 d2[4];
-                if constexpr (FMT == BC_I8) {
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; j += 2) {
-                        const float4 d = *reinterpret_cast<const float4*>(info.dv + half * (KT / 2) + 2 * (i + j));
-                        d2[j] = make_float2(d.x, d.y);
-                        d2[j + 1] = make_float2(d.z, d.w);
-                    }
-                }
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) {
-                    float2 w = fma2(x[i + j], factor2, down2);
-                    w.x = exp2_fast(w.x);
-                    w.y = exp2_fast(w.y);
-                    sum[j & 1] = add2(sum[j & 1], w);
+                for (uint32_t i = 0; i < KT / 4; i += 4) {  // 8 positions
+                    float2 d2[4];
                     if constexpr (FMT == BC_I8) {
-                        w = mul2(w, d2[j]);
-                        if (masked) {  // a scale may be no number
-                            if (!(seen[(i + j) / 16] >> (2 * (i + j) % 32) & 1)) w.x = 0.f;
-                            if (!(seen[(i + j) / 16] >> (2 * (i + j) % 32 + 1) & 1)) w.y = 0.f;
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; j += 2) {
+                            const float4 d = *reinterpret_cast<const float4*>(info.dv + half * (KT / 2) + 2 * (i + j));
+                            d2[j] = make_float2(d.x, d.y);
+                            d2[j + 1] = make_float2(d.z, d.w);
                         }
                     }
-                    cut_half2(w, hi[j], lo[j]);
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        float2 w = fma2(x[i + j], factor2, down2);
+                        w.x = exp2_fast(w.x);
+                        w.y = exp2_fast(w.y);
+                        sum[j & 1] = add2(sum[j & 1], w);
+                        if constexpr (FMT == BC_I8) {
+                            w = mul2(w, d2[j]);
+                            if (decltype(some_unseen)::value) {  // a scale may be no number
+                                if (!(seen[(i + j) / 16] >> (2 * (i + j) % 32) & 1)) w.x = 0.f;
+                                if (!(seen[(i + j) / 16] >> (2 * (i + j) % 32 + 1) & 1)) w.y = 0.f;
+                            }
+                        }
+                        cut_half2(w, hi[j], lo[j]);
+                    }
+                    tmem_store_4(scores_at + half * (KT / 4) + i, hi);
+                    tmem_store_4(scores_at + KT / 2 + half * (KT / 4) + i, lo);
                 }
-                tmem_store_4(scores_at + half * (KT / 4) + i, hi);
-                tmem_store_4(scores_at + KT / 2 + half * (KT / 4) + i, lo);
-            }
+            };
+            if (FMT == BC_I8 && masked)
+                probabilities(std::true_type{});
+            else
+                probabilities(std::false_type{});
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             total = total * fall + ((sum[0].x + sum[1].x) + (sum[0].y + sum[1].y)) * tile_unit;
             if (!first) add_product(tile - 1);  // before the next one may take its place
             if constexpr (FMT == BC_I8) {
                 // The sums' unit follows the larger of what they were and what this tile brings.
                 const float target = fmaxf(unit * fall, tile_unit);
-                const float next = __uint_as_float(min(max(__float_as_uint(target) >> 23, 1u), 253u) << 23);
-                keep = fall * (unit / next);
-                grow = tile_unit / next;
+                const uint32_t exponent = min(max(__float_as_uint(target) >> 23, 1u), 253u);
+                const float next = __uint_as_float(exponent << 23), inverse = __uint_as_float((254u - exponent) << 23);
+                keep = fall * (unit * inverse);
+                grow = tile_unit * inverse;
                 unit = next;
             } else {
                 keep = fall;
