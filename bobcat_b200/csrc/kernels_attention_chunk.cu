@@ -14,8 +14,6 @@
 // Queries and probabilities are A operands in tensor memory: both operands in shared memory would take its 128 bytes a cycle whole. (Heads of 256
 // leave room for the queries' upper halves alone.)
 
-#include <type_traits>
-
 #include "async_utils.cuh"
 #include "chunk_schedule.h"
 #include "kv_pool.cuh"
@@ -30,8 +28,11 @@ namespace {
 using namespace async;
 
 constexpr uint32_t kRows = 128;                    // rows of a tile
-constexpr uint32_t kRowWarps = 8, kUnpackWarps = 4, kMmaWarp = 12, kCopyWarp = 13, kThreads = 512;
+constexpr uint32_t kParts = 2;                     // threads of a row
+constexpr uint32_t kRowWarps = 4 * kParts, kUnpackWarps = 4, kMmaWarp = kRowWarps + kUnpackWarps, kCopyWarp = kMmaWarp + 1, kThreads = 32 * (kMmaWarp + 4);
 constexpr uint32_t kRowThreads = 32 * kRowWarps, kUnpackThreads = 32 * kUnpackWarps;
+// Registers of a thread after the split, 128 before: 256 threads x 184 + 128 x 96 + 128 x 48 = 512 x 128.
+constexpr int kRowRegisters = 184, kUnpackRegisters = 96, kOtherRegisters = 48;
 constexpr uint32_t kCore = 144;                    // bytes from one core matrix to the next
 constexpr uint32_t kTmemColumns = 512;
 constexpr uint32_t kMostCtas = kChunkMostCtas;
@@ -123,7 +124,8 @@ struct TileDesc {
 template <uint32_t KT, int FMT>
 struct TileInfo {
     uint32_t valid[KT / 32];
-    uint32_t top_scale[kUnpackWarps];
+    uint32_t masked;          // whether some row does not see some of its positions
+    alignas(16) uint32_t top_scale[kUnpackWarps];
     alignas(16) float dk[FMT == BC_I8 ? KT : 4];
     alignas(16) float dv[FMT == BC_I8 ? KT : 4];
 };
@@ -144,8 +146,8 @@ __device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile 
     if ((threadIdx.x & 31) == 0) give_up(dead, code);
     return false;
 }
-// A whole warp's wait. Once one has run out the warp goes on without waiting: it takes the same steps as ever, so that nobody waits for it
-// at a barrier, and what it computes is nobody's.
+// A whole warp's wait. One that runs out takes the warp out of its loop, and the others with it: all that warps wait for are mbarriers, so nobody
+// waits for it for good. It touches nothing after that: what it would go by may not be there.
 __device__ __forceinline__ void await(bool& alive, uint32_t bar, uint32_t parity, volatile int* dead, int code) {
     if (alive) alive = __all_sync(0xffffffffu, mbar_test(bar, parity)) || wait_on(bar, parity, dead, code);
 }
@@ -158,22 +160,10 @@ __device__ __forceinline__ void umma_f16_a_tmem(uint32_t tmem_d, uint32_t tmem_a
         "r"(tmem_a), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// Whole warp: 32 columns of its lanes. The loads may be read after tmem_wait.
-__device__ __forceinline__ void tmem_load_32(uint32_t taddr, float2* v) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=f"(v[0].x), "=f"(v[0].y), "=f"(v[1].x), "=f"(v[1].y), "=f"(v[2].x), "=f"(v[2].y), "=f"(v[3].x), "=f"(v[3].y), "=f"(v[4].x), "=f"(v[4].y), "=f"(v[5].x), "=f"(v[5].y), "=f"(v[6].x), "=f"(v[6].y), "=f"(v[7].x), "=f"(v[7].y), "=f"(v[8].x), "=f"(v[8].y), "=f"(v[9].x), "=f"(v[9].y), "=f"(v[10].x), "=f"(v[10].y), "=f"(v[11].x), "=f"(v[11].y), "=f"(v[12].x), "=f"(v[12].y), "=f"(v[13].x), "=f"(v[13].y), "=f"(v[14].x), "=f"(v[14].y), "=f"(v[15].x), "=f"(v[15].y)
-        : "r"(taddr)
-        : "memory");
-}
 // Loads and stores of memory may move across these; tcgen05.wait::st keeps what follows behind.
 __device__ __forceinline__ void tmem_store_8(uint32_t taddr, const uint32_t (&v)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
                  "r"(v[6]), "r"(v[7]));
-}
-__device__ __forceinline__ void tmem_store_4(uint32_t taddr, const uint32_t (&v)[4]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]));
 }
 // Pairs of f32 in one instruction.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
@@ -214,7 +204,25 @@ __device__ __forceinline__ void cut_half2(float2 x, uint32_t& hi, uint32_t& lo) 
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
-__device__ __forceinline__ void rows_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kRowThreads) : "memory"); }
+// Which of 16 scores a row sees: those of positions that exist, up to the last it may.
+template <uint32_t KT, int FMT>
+__device__ __forceinline__ uint32_t seen_bits(const TileInfo<KT, FMT>& info, uint32_t score, int32_t upto) {
+    const uint32_t there = info.valid[score / 32] >> (score % 32), n = (uint32_t)max(upto + 1, 0);  // scores up to the limit
+    return there & (n >= 16 ? 0xffffu : (1u << n) - 1);
+}
+
+// A barrier of several warps that a warp may leave: an mbarrier with an arrival of each.
+struct WarpsBarrier {
+    uint32_t bar, phase;
+    int code;
+    __device__ __forceinline__ void sync(bool& alive, volatile int* dead) {
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+        await(alive, bar, phase, dead, code);
+        phase ^= 1;
+    }
+};
+
 template <int FMT, int HD>
 struct Shared {
     static constexpr uint32_t KT = key_tile<HD>(), kStages = stages<FMT, HD>(), kRaw = raw_tiles<FMT, HD>(), kUnits = 8;
@@ -224,10 +232,10 @@ struct Shared {
     alignas(16) RawTile<KT, FMT, HD> raw[kRaw];
     TileInfo<KT, FMT> info[kRing];
     TileDesc desc[kDescRing];
-    float most[2][2][kRows];    // [parity][half]: maxima of the halves of a row's scores; at a unit's ends, other exchanges
+    float most[2][kParts][kRows];  // [parity][part]: maxima of the parts of a row's scores; at a unit's ends, other exchanges
     uint32_t not_finite[FMT == BC_F16 ? kUnits : 1][FMT == BC_F16 ? HD : 1];  // by unit: the first position with such a value, of each element
     uint32_t any_not_finite[kUnits];
-    uint64_t bars[4 * kStages + 2 * kRaw + 5 + kDescRing];
+    uint64_t bars[4 * kStages + 2 * kRaw + 10 + kDescRing];
     uint64_t total, run_tiles;  // key tiles of the call, and of the CTA's run
     Place place;
     uint32_t tmem;
@@ -253,7 +261,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
     const uint32_t per_tile = kRows / p.group;
     const uint32_t bars = smem_u32(sh.bars);
     const uint32_t k_full = bars, k_free = k_full + 8 * ST, v_full = k_free + 8 * ST, v_free = v_full + 8 * ST, raw_full = v_free + 8 * ST, raw_free = raw_full + 8 * RAW;
-    const uint32_t s_full = raw_free + 8 * RAW, p_ready = s_full + 16, pv_full = p_ready + 8, q_ready = pv_full + 8, described = q_ready + 8;
+    const uint32_t s_full = raw_free + 8 * RAW, p_ready = s_full + 16, pv_full = p_ready + 16, pv_free = pv_full + 16, q_ready = pv_free + 8;
+    const uint32_t rows_bar = q_ready + 8, unpack_bar = rows_bar + 8, described = unpack_bar + 8;
 
     pdl_launch_dependents();
     if (tid == 0) {
@@ -270,8 +279,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
         mbar_init(s_full, 1);
         mbar_init(s_full + 8, 1);
         mbar_init(p_ready, kRowWarps);
+        mbar_init(p_ready + 8, kRowWarps);
         mbar_init(pv_full, 1);
+        mbar_init(pv_full + 8, 1);
+        mbar_init(pv_free, kRowWarps);
         mbar_init(q_ready, kRowWarps);
+        mbar_init(rows_bar, kRowWarps);
+        mbar_init(unpack_bar, kUnpackWarps);
         for (uint32_t d = 0; d < kDescRing; ++d) mbar_init(described + 8 * d, 1);
         sh.dead = sh.never = 0;
         mbar_init_fence();
@@ -344,36 +358,43 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
     bool alive = true;
 
     if (warp < kRowWarps) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
-        const uint32_t half = warp >> 2, row = (warp & 3) * 32 + lane;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegisters));
+        const uint32_t part = warp >> 2, row = (warp & 3) * 32 + lane;
+        constexpr uint32_t kScores = KT / kParts, kSums = HD / kParts;  // of a thread
+        const uint32_t first_score = part * kScores, first_sum = part * kSums;
         const uint32_t lanes = tmem + ((warp & 3) << 21);
         const float scale = 1.4426950408889634f / sqrtf((float)HD) / 16384.f;
         float factor = 0.f;
+        WarpsBarrier everyone{rows_bar, 0, 13};
+        auto rows_sync = [&]() { everyone.sync(alive, dead); };
 
         // The next unit's queries, a thread half of a row: its largest element goes to 2^14 (see kernels_attention_paged.cu). The other half's
         // largest comes through shared memory.
         auto load_queries = [&](uint32_t tile) {
             await(alive, described + 8 * (tile % kDescRing), (tile / kDescRing) & 1, dead, 9);
+            if (!alive) return;
             const TileDesc& d = sh.desc[tile % kDescRing];
             const uint32_t query = row / p.group;
             const bool there = query < d.n;
             const float4* from = reinterpret_cast<const float4*>(p.q + (there ? (uint64_t)(d.row0 + query) * p.q_stride + (uint64_t)(d.head * p.group + row % p.group) * p.q_head_stride
-                                                                               : 0) + half * (HD / 2));
+                                                                               : 0) + part * kSums);
             uint32_t top = 0;
 #pragma unroll 8
-            for (uint32_t i = 0; i < HD / 8; ++i) {
+            for (uint32_t i = 0; i < kSums / 4; ++i) {
                 const float4 v = there ? from[i] : make_float4(0.f, 0.f, 0.f, 0.f);
                 top = max(max(top, __float_as_uint(v.x) & 0x7fffffffu), max(__float_as_uint(v.y) & 0x7fffffffu, max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu)));
             }
-            sh.most[0][half][row] = __uint_as_float(top);
+            sh.most[0][part][row] = __uint_as_float(top);
             rows_sync();
-            top = max(top, __float_as_uint(sh.most[0][half ^ 1][row]));
+#pragma unroll
+            for (uint32_t i = 0; i < kParts; ++i) top = max(top, __float_as_uint(sh.most[0][i][row]));
             rows_sync();
+            if (!alive) return;
             const uint32_t exponent = min(max(top >> 23, 1u), 253u);
             const float up = __uint_as_float((254u - exponent) << 23);
             factor = __uint_as_float(exponent << 23) * scale;
 #pragma unroll 2
-            for (uint32_t i = 0; i < HD / 32; ++i) {  // 16 elements: 8 columns
+            for (uint32_t i = 0; i < kSums / 16; ++i) {  // 16 elements: 8 columns
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (uint32_t e = 0; e < 4; ++e) {
@@ -381,13 +402,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                     split_half2(v.x * up * 16384.f, v.y * up * 16384.f, hi[2 * e], lo[2 * e]);
                     split_half2(v.z * up * 16384.f, v.w * up * 16384.f, hi[2 * e + 1], lo[2 * e + 1]);
                 }
-                tmem_store_8(lanes + kQHi + half * (HD / 4) + 8 * i, hi);
+                tmem_store_8(lanes + kQHi + part * (kSums / 2) + 8 * i, hi);
                 if constexpr (kQLoShared) {
-                    uint8_t* to = sh.q_lo + (row >> 3) * kKeyStep + (half * (HD / 16) + 2 * i) * kCore + (row & 7) * 16;
+                    uint8_t* to = sh.q_lo + (row >> 3) * kKeyStep + (part * (kSums / 8) + 2 * i) * kCore + (row & 7) * 16;
                     *reinterpret_cast<uint4*>(to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     *reinterpret_cast<uint4*>(to + kCore) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
                 } else {
-                    tmem_store_8(lanes + kQLo + half * (HD / 4) + 8 * i, lo);
+                    tmem_store_8(lanes + kQLo + part * (kSums / 2) + 8 * i, lo);
                 }
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -396,19 +417,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             __syncwarp();
             if (lane == 0) mbar_arrive(q_ready);
         };
-        if (n_tiles > 0) load_queries(0);
-        float2 o[HD / 4];
-        float row_factor = 0.f, top = 0.f, total = 0.f, unit = 0.f;
-        float keep = 0.f, grow = 0.f;  // how the last tile's product joins the sums: o keep + product grow
-        int32_t limit = 0;             // the last position that the row sees, negative for none
-        auto add_product = [&](uint32_t tile) {
-            await(alive, pv_full, tile & 1, dead, 1);
+        float2 o[kSums / 2];
+        float top = 0.f, total = 0.f, unit = 0.f;
+        int32_t limit = 0;  // the last position that the row sees, negative for none
+        // Sums become o keep + product grow.
+        auto add_product = [&](uint32_t tile, float keep, float grow) {
+            await(alive, pv_full + 8 * (tile & 1), (tile >> 1) & 1, dead, 1);
+            if (!alive) return;
             tc_fence_after_sync();
             const float2 keep2 = make_float2(keep, keep), grow2 = make_float2(grow, grow);
 #pragma unroll
-            for (uint32_t c = 0; c < HD / 2; c += 16) {
+            for (uint32_t c = 0; c < kSums; c += 16) {
                 float v[16];
-                tmem_load_16(lanes + kPv + half * (HD / 2) + c, v);
+                tmem_load_16(lanes + kPv + first_sum + c, v);
 #pragma unroll
                 for (uint32_t i = 0; i < 16; i += 2) {
                     float2 add = make_float2(v[i], v[i + 1]);
@@ -417,116 +438,99 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 }
             }
             tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pv_free);
         };
-        for (uint32_t tile = 0; tile < n_tiles; ++tile) {
-            const TileDesc& desc = sh.desc[tile % kDescRing];
-            const uint32_t buffer = tile & 1;
-            const TileInfo<KT, FMT>& info = sh.info[tile % kRing];
-            await(alive, s_full + 8 * buffer, (tile >> 1) & 1, dead, 2);
-            tc_fence_after_sync();
-            const bool first = desc.first;
-            if (first) {
-                // (Rows that are nobody's see all there is: no tile is masked for them.)
-                const uint32_t query = row / p.group;
-                limit = (int32_t)min((int64_t)desc.pos0 + (query < desc.n ? query : 0x40000000u), (int64_t)desc.end - 1);
-                row_factor = factor;
-#pragma unroll
-                for (uint32_t i = 0; i < HD / 4; ++i) o[i] = make_float2(0.f, 0.f);
-                top = -INFINITY;
-                total = unit = 0.f;
-            }
-            const uint32_t scores_at = lanes + buffer * KT;
-            float2 x[KT / 4];
-#pragma unroll
-            for (uint32_t c = 0; c < KT / 4; c += 16) tmem_load_32(scores_at + half * (KT / 2) + 2 * c, x + c);
-            const uint32_t key0 = desc.key0 + half * (KT / 2);
-            uint32_t seen[KT / 64];  // positions of this half that the row sees
-            uint32_t all = 0xffffffffu;
-#pragma unroll
-            for (uint32_t w = 0; w < KT / 64; ++w) {
-                const int64_t behind = (int64_t)limit - (key0 + 32 * w) + 1;  // positions of the word up to the limit
-                seen[w] = info.valid[half * (KT / 64) + w] & (behind >= 32 ? 0xffffffffu : behind <= 0 ? 0u : (1u << behind) - 1);
-                all &= seen[w];
-            }
-            const bool masked = __any_sync(0xffffffffu, all != 0xffffffffu);
+        // 16 scores of a tile from score c on, scaled and masked.
+        auto load_scores = [&](uint32_t scores_at, const TileInfo<KT, FMT>& info, int32_t see, uint32_t c, float2 (&x)[8]) {
+            tmem_load_16(scores_at + c, reinterpret_cast<float(&)[16]>(x));
             if constexpr (FMT == BC_I8) {
 #pragma unroll
-                for (uint32_t i = 0; i < KT / 4; i += 2) {
-                    const float4 d = *reinterpret_cast<const float4*>(info.dk + half * (KT / 2) + 2 * i);
+                for (uint32_t i = 0; i < 8; i += 2) {
+                    const float4 d = *reinterpret_cast<const float4*>(info.dk + first_score + c + 2 * i);
                     x[i] = mul2(x[i], make_float2(d.x, d.y));
                     x[i + 1] = mul2(x[i + 1], make_float2(d.z, d.w));
                 }
             }
-            if (masked) {
+            if (info.masked) {
+                const uint32_t bits = seen_bits(info, first_score + c, see - (int32_t)c);
 #pragma unroll
-                for (uint32_t i = 0; i < KT / 4; ++i) {
-                    if (!(seen[i / 16] >> (2 * i % 32) & 1)) x[i].x = -INFINITY;
-                    if (!(seen[i / 16] >> (2 * i % 32 + 1) & 1)) x[i].y = -INFINITY;
+                for (uint32_t i = 0; i < 8; ++i) {
+                    if (!(bits >> (2 * i) & 1)) x[i].x = -INFINITY;
+                    if (!(bits >> (2 * i + 1) & 1)) x[i].y = -INFINITY;
                 }
             }
-            float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        };
+        // The tile's scores to probabilities, in place: of each 16 the upper halves, then the lower. 16 at a time, twice (for their maximum, then again), in loops:
+        // warps that run through a thousand instructions in a line wait for those more than for anything else.
+        auto take = [&](uint32_t tile, float& keep, float& grow) {
+            const uint32_t buffer = tile & 1, scores_at = lanes + buffer * KT + first_score;
+            const TileInfo<KT, FMT>& info = sh.info[tile % kRing];
+            await(alive, s_full + 8 * buffer, (tile >> 1) & 1, dead, 2);
+            if (!alive) return;
+            tc_fence_after_sync();
+            const int32_t see = (int32_t)max(min((int64_t)limit - sh.desc[tile % kDescRing].key0 - first_score, (int64_t)KT), (int64_t)-1);  // the last score seen
+            float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll 4
+            for (uint32_t c = 0; c < kScores; c += 16) {
+                float2 x[8];
+                load_scores(scores_at, info, see, c, x);
 #pragma unroll
-            for (uint32_t i = 0; i < KT / 4; i += 4)
-#pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) most[j] = fmaxf(most[j], fmaxf(x[i + j].x, x[i + j].y));
-            const float mine_most = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * row_factor;
-            sh.most[tile & 1][half][row] = mine_most;
-            rows_sync();  // and every thread has read its scores: probabilities may take their place
-            const float now = fmaxf(top, fmaxf(mine_most, sh.most[tile & 1][half ^ 1][row]));
+                for (uint32_t i = 0; i < 8; ++i) most[i & 1] = fmaxf(most[i & 1], fmaxf(x[i].x, x[i].y));
+            }
+            float now = fmaxf(top, fmaxf(most[0], most[1]) * factor);
+            sh.most[tile & 1][part][row] = now;
+            rows_sync();
+            if (!alive) return;
+            now = fmaxf(now, sh.most[tile & 1][part ^ 1][row]);
             const float shift = now == -INFINITY ? 0.f : now;
-            const float fall = exp2f(top - shift);
+            const float fall = exp2_fast(top - shift);
             top = now;
             // 8-bit values: weights are counted in the power of two below the tile's largest scale.
             float down = kLift - shift, tile_unit = 1.f;
             if constexpr (FMT == BC_I8) {
-                uint32_t largest = 0;
-#pragma unroll
-                for (uint32_t w = 0; w < kUnpackWarps; ++w) largest = max(largest, info.top_scale[w]);
-                const uint32_t exponent = min(max(largest >> 23, 27u), 227u);  // 2^-100 to 2^100
+                const uint4 tops = *reinterpret_cast<const uint4*>(info.top_scale);
+                const uint32_t exponent = min(max(max(max(tops.x, tops.y), max(tops.z, tops.w)) >> 23, 27u), 227u);  // 2^-100 to 2^100
                 tile_unit = __uint_as_float(exponent << 23);
                 down -= (float)((int)exponent - 127);
             }
-            const float2 factor2 = make_float2(row_factor, row_factor), down2 = make_float2(down, down);
+            const float2 factor2 = make_float2(factor, factor), down2 = make_float2(down, down);
             float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-            auto probabilities = [&](auto some_unseen) {
+#pragma unroll 1
+            for (uint32_t c = 0; c < kScores; c += 16) {
+                float2 x[8];
+                load_scores(scores_at, info, see, c, x);
+                uint32_t hi[8], lo[8];
 #pragma unroll
-                for (uint32_t i = 0; i < KT / 4; i += 4) {  // 8 positions
-                    float2 d2[4];
-                    if constexpr (FMT == BC_I8) {
-#pragma unroll
-                        for (uint32_t j = 0; j < 4; j += 2) {
-                            const float4 d = *reinterpret_cast<const float4*>(info.dv + half * (KT / 2) + 2 * (i + j));
-                            d2[j] = make_float2(d.x, d.y);
-                            d2[j + 1] = make_float2(d.z, d.w);
-                        }
-                    }
-                    uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) {
-                        float2 w = fma2(x[i + j], factor2, down2);
-                        w.x = exp2_fast(w.x);
-                        w.y = exp2_fast(w.y);
-                        sum[j & 1] = add2(sum[j & 1], w);
-                        if constexpr (FMT == BC_I8) {
-                            w = mul2(w, d2[j]);
-                            if (decltype(some_unseen)::value) {  // a scale may be no number
-                                if (!(seen[(i + j) / 16] >> (2 * (i + j) % 32) & 1)) w.x = 0.f;
-                                if (!(seen[(i + j) / 16] >> (2 * (i + j) % 32 + 1) & 1)) w.y = 0.f;
-                            }
-                        }
-                        cut_half2(w, hi[j], lo[j]);
-                    }
-                    tmem_store_4(scores_at + half * (KT / 4) + i, hi);
-                    tmem_store_4(scores_at + KT / 2 + half * (KT / 4) + i, lo);
+                for (uint32_t i = 0; i < 8; ++i) {
+                    x[i] = fma2(x[i], factor2, down2);
+                    x[i].x = exp2_fast(x[i].x);
+                    x[i].y = exp2_fast(x[i].y);
+                    sum[i & 1] = add2(sum[i & 1], x[i]);
                 }
-            };
-            if (FMT == BC_I8 && masked)
-                probabilities(std::true_type{});
-            else
-                probabilities(std::false_type{});
+                if constexpr (FMT == BC_I8) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; i += 2) {
+                        const float4 d = *reinterpret_cast<const float4*>(info.dv + first_score + c + 2 * i);
+                        x[i] = mul2(x[i], make_float2(d.x, d.y));
+                        x[i + 1] = mul2(x[i + 1], make_float2(d.z, d.w));
+                    }
+                    if (info.masked) {  // a scale may be no number
+                        const uint32_t bits = seen_bits(info, first_score + c, see - (int32_t)c);
+#pragma unroll
+                        for (uint32_t i = 0; i < 8; ++i) {
+                            if (!(bits >> (2 * i) & 1)) x[i].x = 0.f;
+                            if (!(bits >> (2 * i + 1) & 1)) x[i].y = 0.f;
+                        }
+                    }
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) cut_half2(x[i], hi[i], lo[i]);
+                tmem_store_8(scores_at + c, hi);
+                tmem_store_8(scores_at + c + 8, lo);
+            }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             total = total * fall + ((sum[0].x + sum[1].x) + (sum[0].y + sum[1].y)) * tile_unit;
-            if (!first) add_product(tile - 1);  // before the next one may take its place
             if constexpr (FMT == BC_I8) {
                 // The sums' unit follows the larger of what they were and what this tile brings.
                 const float target = fmaxf(unit * fall, tile_unit);
@@ -537,75 +541,119 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 unit = next;
             } else {
                 keep = fall;
+                grow = 1.f;
                 unit = 1.f;
             }
+        };
+        auto publish = [&](uint32_t tile) {
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_ready);
-
-            if (!desc.last) continue;
-            // The next unit's queries go ahead of this one's end: the last scores are done.
-            rows_sync();  // the maxima have been read
-            if (tile + 1 < n_tiles) load_queries(tile + 1);
-            add_product(tile);
-            // A row's two sums of probabilities meet.
-            sh.most[0][half][row] = total;
-            rows_sync();
-            total = sh.most[0][0][row] + sh.most[0][1][row];
-            rows_sync();  // the next unit writes there
-            if constexpr (FMT == BC_F16) {
-                const uint32_t slot = desc.unit % kUnits;
-                if (sh.any_not_finite[slot]) {
-#pragma unroll
-                    for (uint32_t i = 0; i < HD / 4; ++i) {
-                        if ((int64_t)sh.not_finite[slot][half * (HD / 2) + 2 * i] <= limit) o[i].x = __uint_as_float(0x7fc00000u);
-                        if ((int64_t)sh.not_finite[slot][half * (HD / 2) + 2 * i + 1] <= limit) o[i].y = __uint_as_float(0x7fc00000u);
-                    }
-                }
-            }
+            if (lane == 0) mbar_arrive(p_ready + 8 * (tile & 1));
+        };
+        // A row's results: whole, or a part for the joining launch. `sums` are those of the row's elements from first_element on.
+        auto store = [&](const TileDesc& desc, uint32_t first_element, const float2 (&sums)[HD / kParts / 2], float times, bool stats) {
             const bool whole = desc.begins && desc.ends;
             const uint32_t slot = 2 * blockIdx.x + (desc.begins ? 1 : 0);
-            const float times = whole ? (top == -INFINITY && total == 0.f ? 0.f : unit / total) : unit;
+            if (whole) times *= top == -INFINITY && total == 0.f ? 0.f : 1.f / total;
             float* to = (whole ? p.out + (uint64_t)(desc.row0 + row / p.group) * p.n_heads * HD + (desc.head * p.group + row % p.group) * HD
-                               : p.parts + ((uint64_t)slot * kRows + row) * HD) + half * (HD / 2);
+                               : p.parts + ((uint64_t)slot * kRows + row) * HD) + first_element;
+            const bool any = FMT == BC_F16 && sh.any_not_finite[desc.unit % kUnits];
             if (row / p.group < desc.n) {
 #pragma unroll
-                for (uint32_t i = 0; i < HD / 4; i += 2)
-                    *reinterpret_cast<float4*>(to + 2 * i) = make_float4(o[i].x * times, o[i].y * times, o[i + 1].x * times, o[i + 1].y * times);
+                for (uint32_t i = 0; i < HD / kParts / 2; i += 2) {
+                    float4 v = make_float4(sums[i].x * times, sums[i].y * times, sums[i + 1].x * times, sums[i + 1].y * times);
+                    if constexpr (FMT == BC_F16) {
+                        if (any) {
+                            const uint32_t* at = sh.not_finite[desc.unit % kUnits] + first_element + 2 * i;
+                            if ((int64_t)at[0] <= limit) v.x = __uint_as_float(0x7fc00000u);
+                            if ((int64_t)at[1] <= limit) v.y = __uint_as_float(0x7fc00000u);
+                            if ((int64_t)at[2] <= limit) v.z = __uint_as_float(0x7fc00000u);
+                            if ((int64_t)at[3] <= limit) v.w = __uint_as_float(0x7fc00000u);
+                        }
+                    }
+                    *reinterpret_cast<float4*>(to + 2 * i) = v;
+                }
             }
-            if (!whole && half == 0)
+            if (!whole && stats)
                 *reinterpret_cast<float2*>(p.parts + (uint64_t)2 * kMostCtas * kRows * HD + ((uint64_t)slot * kRows + row) * 2) = make_float2(top, total);
+        };
+        auto start_unit = [&](uint32_t tile) {
+            // (Rows that are nobody's see all there is: no tile is masked for them.)
+            const TileDesc& desc = sh.desc[tile % kDescRing];
+            const uint32_t query = row / p.group;
+            limit = (int32_t)min((int64_t)desc.pos0 + (query < desc.n ? query : 0x40000000u), (int64_t)desc.end - 1);
+#pragma unroll
+            for (uint32_t i = 0; i < kSums / 2; ++i) o[i] = make_float2(0.f, 0.f);
+            top = -INFINITY;
+            total = unit = 0.f;
+        };
+        {
+            // All rows' threads take every tile; the last product is added to the sums when the next tile's probabilities are there.
+            bool first = true;
+            float keep = 0.f, grow = 0.f;
+            for (uint32_t tile = 0; tile <= n_tiles && n_tiles > 0; ++tile) {
+                if (first) {
+                    // The next unit's queries go ahead of the last one's end: its scores are done.
+                    if (tile > 0) rows_sync();  // the maxima have been read
+                    if (tile < n_tiles && alive) load_queries(tile);
+                    if (tile > 0 && alive) {
+                        add_product(tile - 1, keep, grow);
+                        // A row's sums of probabilities meet.
+                        sh.most[0][part][row] = total;
+                        rows_sync();
+                        total = sh.most[0][0][row] + sh.most[0][1][row];
+                        rows_sync();  // the next unit writes there
+                        if (!alive) break;
+                        store(sh.desc[(tile - 1) % kDescRing], first_sum, o, unit, part == 0);
+                    }
+                    if (tile == n_tiles || !alive) break;
+                    start_unit(tile);
+                }
+                float next_keep, next_grow;
+                take(tile, next_keep, next_grow);
+                if (!first && alive) add_product(tile - 1, keep, grow);  // before the next one may take its place
+                if (!alive) break;
+                keep = next_keep;
+                grow = next_grow;
+                publish(tile);
+                first = sh.desc[tile % kDescRing].last;
+            }
         }
     } else if (warp < kMmaWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUnpackRegisters));
         // ---- bytes to operands
         const uint32_t utid = tid - kRowThreads, uwarp = utid >> 5;
         constexpr uint32_t kPieces = KT * (HD / 8) / kUnpackThreads;           // pieces of 8 elements of a key that a thread unpacks
         constexpr uint32_t kBlocks = KT / 8 * (HD / 8) / kUnpackThreads;       // blocks of 8 positions x 8 elements of values
         constexpr uint32_t kPiece = FMT == BC_F16 ? 16 : 8, kWords = kPiece / 4, kRowBytes = RawTile<KT, FMT, HD>::kRowBytes;
+        WarpsBarrier everyone{unpack_bar, 0, 14};
         for (uint32_t j = 0; j < n_tiles; ++j) {
             const uint32_t st = j % ST;
             TileInfo<KT, FMT>& info = sh.info[j % kRing];
             const RawTile<KT, FMT, HD>& raw = sh.raw[j % RAW];
             await(alive, raw_full + 8 * (j % RAW), (j / RAW) & 1, dead, 10);
+            if (!alive) break;
             const TileDesc& desc = sh.desc[j % kDescRing];
             const uint32_t key0 = desc.key0, end = desc.end, groups = desc.groups;
             auto key_there = [&](uint32_t key) { return (groups >> (key >> 4) & 1) && key0 + key < end; };
             const bool whole = groups == (1u << KT / 16) - 1 && end - key0 >= KT;  // every position is there
             // Free keys: their scores are done, so the rows' warps are done with the tile before those, and the ring's fourth is nobody's.
             await(alive, k_free + 8 * st, ((j / ST) & 1) ^ 1, dead, 3);
+            if (!alive) break;
             if constexpr (FMT == BC_F16) {
                 if (desc.first) {
                     const uint32_t slot = desc.unit % kUnits;
                     for (uint32_t i = utid; i < HD; i += kUnpackThreads) sh.not_finite[slot][i] = 0xffffffffu;
                     if (utid == 0) sh.any_not_finite[slot] = 0;
-                    asm volatile("bar.sync 2, %0;" ::"n"(kUnpackThreads) : "memory");  // before any of them finds one
+                    everyone.sync(alive, dead);  // before any of them finds one
+                    if (!alive) break;
                 }
             }
             // Masks and scales of the tile's positions.
             const bool there = utid < KT && key_there(utid);
             const uint32_t votes = __ballot_sync(0xffffffffu, there);
             if (lane == 0 && uwarp < KT / 32) info.valid[uwarp] = votes;
+            if (utid == 0) info.masked = !whole || (int64_t)key0 + KT - 1 > desc.pos0;
             if constexpr (FMT == BC_I8) {
                 const float dv = there ? raw.dv[utid] : 0.f;
                 if (utid < KT) {
@@ -619,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             {  // What is there of positions that are not is masked in the scores, whatever it is.
                 const uint8_t* from = raw.keys + utid * kPiece;
                 uint8_t* const to = sh.keys[st];
-#pragma unroll
+#pragma unroll 4
                 for (uint32_t n = 0; n < kPieces; ++n) {
                     const uint32_t i = utid + n * kUnpackThreads, piece = i % (HD / 8), key = i / (HD / 8);
                     uint4 w;
@@ -638,11 +686,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             if (lane == 0) mbar_arrive(k_full + 8 * st);
 
             await(alive, v_free + 8 * st, ((j / ST) & 1) ^ 1, dead, 4);
+            if (!alive) break;
             uint8_t* const to = sh.values[st];
             // A value that is not finite would reach rows that do not see it: zero times it is no number. Tiles that end behind the row tile's
             // first row keep such values apart.
             const bool apart = FMT == BC_F16 && (int64_t)key0 + KT - 1 > desc.pos0;
-#pragma unroll
+#pragma unroll 1
             for (uint32_t n = 0; n < kBlocks; ++n) {
                 const uint32_t i = utid + n * kUnpackThreads, piece = i % (HD / 8), key = i / (HD / 8) * 8;
                 const uint8_t* from = raw.values + key * kRowBytes + piece * kPiece;
@@ -719,41 +768,51 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
         if (warp == kMmaWarp) {
-            // ---- the tensor core. Lower halves first: what a sum cuts off grows with what is there already.
+            // ---- the tensor core. Lower halves first: what a sum cuts off grows with what is there already. Every loop and branch goes by a vote: the
+            // compiler then keeps the descriptors in uniform registers, where the instruction wants them (without, an instruction took 106 cycles
+            // to issue, of the 64 that it runs).
             const uint32_t scores_idesc = umma_idesc_f16(kRows, KT), values_idesc = umma_idesc_f16(kRows, HD);
-            const uint64_t q_lo = umma_desc(smem_u32(sh.q_lo), kCore, kKeyStep);
+            const uint64_t q_lo = umma_desc(smem_u32(sh.q_lo), kCore, kKeyStep), keys0 = umma_desc(smem_u32(sh.keys), kCore, kKeyStep),
+                           values0 = umma_desc(smem_u32(sh.values), kKeyStep, kCore);
             uint32_t units = 0;
             auto product = [&](uint32_t j) {  // P V of tile j
-                await(alive, p_ready, j & 1, dead, 5);
+                await(alive, p_ready + 8 * (j & 1), (j >> 1) & 1, dead, 5);
+                if (j > 0) await(alive, pv_free, (j - 1) & 1, dead, 12);
                 await(alive, v_full + 8 * (j % ST), (j / ST) & 1, dead, 6);
+                if (__any_sync(0xffffffffu, !alive)) return;
                 tc_fence_after_sync();
+                const uint64_t v = values0 + (j % ST) * (S::kTileBytes >> 4);
+                const uint32_t weights = tmem + (j & 1) * KT;
                 if (elect_one()) {
-                    const uint64_t v = umma_desc(smem_u32(sh.values[j % ST]), kKeyStep, kCore);
-                    const uint32_t weights = tmem + (j & 1) * KT;
-#pragma unroll 1
+#pragma unroll
                     for (uint32_t part = 0; part < 2; ++part)
 #pragma unroll
                         for (uint32_t ks = 0; ks < KT / 16; ++ks)
-                            umma_f16_a_tmem(tmem + kPv, weights + (part ^ 1) * (KT / 2) + ks * 8, v + (uint64_t)(ks * 2 * kKeyStep >> 4), values_idesc, part | ks);
+                            umma_f16_a_tmem(tmem + kPv, weights + ks * 16 + (part ^ 1) * 8, v + (uint64_t)(ks * 2 * kKeyStep >> 4), values_idesc, part | ks);
+                }
+                __syncwarp();
+                if (elect_one()) {
                     umma_commit(v_free + 8 * (j % ST));
-                    umma_commit(pv_full);
+                    umma_commit(pv_full + 8 * (j & 1));
                 }
                 __syncwarp();
             };
-            for (uint32_t j = 0; j < n_tiles; ++j) {
+            for (uint32_t j = 0; __all_sync(0xffffffffu, j < n_tiles && alive); ++j) {
                 await(alive, k_full + 8 * (j % ST), (j / ST) & 1, dead, 7);
-                const bool first = sh.desc[j % kDescRing].first;
+                if (__any_sync(0xffffffffu, !alive)) break;
+                const bool first = __any_sync(0xffffffffu, sh.desc[j % kDescRing].first != 0);
                 if (first) {
                     if (j > 0) product(j - 1);
                     await(alive, q_ready, units & 1, dead, 8);
                     ++units;
                 }
+                if (__any_sync(0xffffffffu, !alive)) break;
                 tc_fence_after_sync();
+                const uint64_t keys = keys0 + (j % ST) * (S::kTileBytes >> 4);
+                const uint32_t to = tmem + (j & 1) * KT;
                 if (elect_one()) {
-                    const uint64_t keys = umma_desc(smem_u32(sh.keys[j % ST]), kCore, kKeyStep);
-                    const uint32_t to = tmem + (j & 1) * KT;
 #pragma unroll
                     for (uint32_t ks = 0; ks < HD / 16; ++ks) {
                         if constexpr (kQLoShared)
@@ -763,18 +822,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                     }
 #pragma unroll
                     for (uint32_t ks = 0; ks < HD / 16; ++ks) umma_f16_a_tmem(to, tmem + kQHi + ks * 8, keys + (uint64_t)(ks * 2 * kCore >> 4), scores_idesc, 1);
+                }
+                __syncwarp();
+                if (elect_one()) {
                     umma_commit(k_free + 8 * (j % ST));
                     umma_commit(s_full + 8 * (j & 1));
                 }
                 __syncwarp();
                 if (!first) product(j - 1);
             }
-            if (n_tiles > 0) product(n_tiles - 1);
+            if (__all_sync(0xffffffffu, n_tiles > 0 && alive)) product(n_tiles - 1);
         } else if (warp == kCopyWarp) {
             // ---- the walk through the run, and the pages' bytes: a lane per 16 positions of keys, values, and either's scales.
             Place& at = sh.place;
             constexpr uint32_t kGroups = KT / 16, kRowBytes = RawTile<KT, FMT, HD>::kRowBytes;
             const uint32_t page_slots = (1u << pool.page_shift) - 1;
+            uint32_t issued = 0;
             for (uint32_t j = 0; j < n_tiles; ++j) {
                 TileDesc& d = sh.desc[j % kDescRing];
                 if (lane == 0) {
@@ -821,13 +884,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 const uint32_t groups = __ballot_sync(0xffffffffu, there) & ((1u << kGroups) - 1);
                 const uint32_t slot = j % RAW, bar = raw_full + 8 * slot;
                 await(alive, raw_free + 8 * slot, ((j / RAW) & 1) ^ 1, dead, 11);
+                if (!alive) break;
+                ++issued;
                 if (lane == 0) {
                     d.groups = groups;
                     mbar_arrive(described + 8 * (j % kDescRing));
                     mbar_arrive_expect(bar, __popc(groups) * 16 * 2 * (kRowBytes + (FMT == BC_I8 ? 4 : 0)));
                 }
                 __syncwarp();
-                if (there && alive) {
+                if (there) {
                     RawTile<KT, FMT, HD>& raw = sh.raw[slot];
                     const uint64_t rows_at = kv_row_at(pool, page, d.head, key & page_slots);
                     if (what < 2) {
@@ -838,13 +903,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 }
                 __syncwarp();
             }
-            if (lane == 0) reinterpret_cast<ChunkHead*>(p.parts + (uint64_t)2 * kMostCtas * kRows * (HD + 2))[blockIdx.x] = at.cut;
-            // Copies in flight end before the CTA does: their tiles are waited for by the unpacking warps, or here when those gave up.
-            for (uint32_t r = 0; r < RAW && r < n_tiles; ++r) {
-                const uint32_t j = n_tiles - 1 - r;
-                bool patient = true;
-                if (!alive || *dead) patient = mbar_wait(raw_full + 8 * (j % RAW), (j / RAW) & 1, kSpinLimit, &sh.never);
-                (void)patient;
+            if (lane == 0) reinterpret_cast<ChunkHead*>(p.parts + (uint64_t)2 * kMostCtas * kRows * (HD + 2))[blockIdx.x] = alive ? at.cut : ChunkHead{0, 0, 0, 0};
+            // Copies in flight end before the CTA does: the unpacking warps wait for them, or this one does when those gave up.
+            for (uint32_t r = 0; r < RAW && r < issued && *dead; ++r) {
+                const uint32_t j = issued - 1 - r;
+                mbar_wait(raw_full + 8 * (j % RAW), (j / RAW) & 1, kSpinLimit, &sh.never);
             }
         }
     }

@@ -77,11 +77,33 @@ class Pool:
                 self.put(self.k_raw, s, pos, (rng.standard_normal((self.kv, self.hd)) * amplitude).astype(np.float32))
                 self.put(self.v_raw, s, pos, (rng.standard_normal((self.kv, self.hd)) * amplitude).astype(np.float32))
 
+    def fill_at_once(self, rng, amplitude=1.0):
+        """The same for long contexts: every position of a sequence in one go."""
+        for s, n in enumerate(self.lens):
+            pos = np.arange(n)
+            page, slot = self.table[s, pos // self.page_size], pos % self.page_size
+            for which in (self.k_raw, self.v_raw):
+                held, scales = stored((rng.standard_normal((n, self.kv, self.hd)) * amplitude).astype(np.float32), self.fmt)
+                m = self.kv * self.page_size * self.row_bytes
+                view = np.lib.stride_tricks.as_strided(which, (self.n_pages, self.kv, self.page_size, self.row_bytes),
+                                                       (self.page_bytes, self.page_size * self.row_bytes, self.row_bytes, 1))
+                view[page, :, slot] = held.view(np.uint8).reshape(n, self.kv, self.row_bytes)
+                if scales is not None:
+                    view = np.lib.stride_tricks.as_strided(which[:, m:], (self.n_pages, self.kv, self.page_size, 4), (self.page_bytes, self.page_size * 4, 4, 1))
+                    view[page, :, slot] = scales.astype(np.float32).reshape(n, self.kv, 1).view(np.uint8).reshape(n, self.kv, 4)
+
     def context(self, which, seq, length) -> np.ndarray:
         """[length][kv][hd] in 64 bits."""
         if length == 0:
             return np.zeros((0, self.kv, self.hd))
-        return np.stack([self.get(which, seq, pos) for pos in range(length)])
+        pos = np.arange(length)
+        page, slot = self.table[seq, pos // self.page_size], pos % self.page_size
+        m = self.kv * self.page_size * self.row_bytes
+        held = np.ascontiguousarray(which[:, :m].reshape(self.n_pages, self.kv, self.page_size, self.row_bytes)[page, :, slot])
+        if self.fmt == F16:
+            return held.view(np.float16).astype(np.float64)
+        scales = np.ascontiguousarray(which[:, m:].reshape(self.n_pages, self.kv, self.page_size, 4)[page, :, slot]).view(np.float32).reshape(length, self.kv)
+        return values(held, scales)
 
     def upload(self):
         self.k, self.v = self.cuda.buffer_from(self.k_raw), self.cuda.buffer_from(self.v_raw)
@@ -107,20 +129,23 @@ def attention(q, k, v, first):
     the exponential's two last places; its products with values are sums over at most n / 64 + 64 steps, each off by
     the last place, relative to the sum of magnitudes."""
     n, heads, hd = q.shape
-    kv = k.shape[1]
+    kv, group = k.shape[1], heads // k.shape[1]
     q = q.astype(np.float64)
     out, bound = np.zeros((n, heads, hd)), np.zeros((n, heads, hd))
-    for i in range(n):
-        see = min(first + i + 1, len(k))
-        if see <= 0:
-            continue
-        for h in range(heads):
-            kk, vv = k[:see, h // (heads // kv)], v[:see, h // (heads // kv)]
-            s = kk @ q[i, h] / np.sqrt(hd)
-            p = np.exp(s - s.max())
-            total = p.sum()
-            out[i, h] = p @ vv / total
-            magnitude = np.abs(kk) @ np.abs(q[i, h]) / np.sqrt(hd)
-            ds = (magnitude * (2.0 ** -22 + (hd / 8 + 8) * 2.0 ** -23) + 2.0 ** -25 * np.abs(q[i, h]).max() * np.abs(kk).sum(axis=1) / np.sqrt(hd)).max()
-            bound[i, h] = (2 * ds + 2.0 ** -20 + (see / 64 + 64) * 2.0 ** -23) * (p @ np.abs(vv)) / total
+    see = np.clip(first + np.arange(n) + 1, 0, len(k))
+    rows = np.flatnonzero(see > 0)
+    if rows.size == 0:
+        return out, bound
+    unseen = np.arange(len(k)) >= see[rows, None]
+    for h in range(heads):
+        kk, vv = k[:, h // group], v[:, h // group]
+        x = q[rows, h]
+        magnitude = np.where(unseen, 0.0, np.abs(x) @ np.abs(kk).T) / np.sqrt(hd)
+        floor = np.abs(x).max(axis=1, keepdims=True) * np.where(unseen, 0.0, np.abs(kk).sum(axis=1)) / np.sqrt(hd)
+        ds = (magnitude * (2.0 ** -22 + (hd / 8 + 8) * 2.0 ** -23) + 2.0 ** -25 * floor).max(axis=1, keepdims=True)
+        s = np.where(unseen, -np.inf, x @ kk.T / np.sqrt(hd))
+        p = np.exp(s - s.max(axis=1, keepdims=True))
+        total = p.sum(axis=1, keepdims=True)
+        out[rows, h] = p @ vv / total
+        bound[rows, h] = (2 * ds + 2.0 ** -20 + (see[rows, None] / 64 + 64) * 2.0 ** -23) * (p @ np.abs(vv)) / total
     return out, bound

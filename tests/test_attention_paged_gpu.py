@@ -92,6 +92,23 @@ def test_chunks(cuda, fmt, page_size, heads, kv, hd, seqs):
 
 
 @pytest.mark.parametrize("fmt", [F16, I8])
+@pytest.mark.parametrize("page_size, heads, kv, hd, seqs", [
+    (64, 8, 8, 64, [(70, 30000)]),                # one head a group: two row tiles of 235 key tiles and eight heads over the device
+    (128, 16, 8, 128, [(40, 40000)]),
+    (256, 8, 4, 256, [(20, 20000)]),              # key tiles of 64
+    (16, 16, 4, 128, [(3, 9000), (90, 17000), (1, 12000), (5, 33)]),
+])
+def test_long_contexts(cuda, fmt, page_size, heads, kv, hd, seqs):
+    """Many key tiles to a CTA, so that every ring of the pipeline wraps many times."""
+    news, lens = [n for n, _ in seqs], [length for _, length in seqs]
+    case = Pool(cuda, fmt, page_size, kv, hd, lens, np.random.default_rng(30))
+    case.fill_at_once(np.random.default_rng(31))
+    case.upload()
+    q = (np.random.default_rng(32).standard_normal((sum(news), heads * hd)) * 1.5).astype(np.float32)
+    check(case, news, heads, q, attend(cuda, case, news, heads, q))
+
+
+@pytest.mark.parametrize("fmt", [F16, I8])
 @pytest.mark.parametrize("news", [[1, 1], [70, 9]])
 def test_what_the_caller_says_of_the_rows_is_no_more_than_a_hint(cuda, fmt, news):
     case = build(cuda, fmt, 32, 2, 128, [150, 37], seed=3)
