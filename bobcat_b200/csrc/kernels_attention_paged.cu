@@ -13,13 +13,15 @@
 // to the upper end of their range by a power of two first: a query row's largest element to 2^14, the largest probability to 2^15, the largest weight of
 // 8-bit values to 2^11 or more (`unit` follows it). What is 2^25 times smaller than these still keeps 22 bits or is lost beside them.
 //
-// A warp takes 16 positions at a time, from global memory straight into the fragments of mma.m16n8k16, no shared memory between.
-// Scores: the 16 rows of A are the group's 8 query heads' hi parts, then their lo parts, so one multiply gives both sums and a thread adds
-// its two. A lane's 16 bytes of a key are neighbouring elements; the order of elements within a product is free, and the queries
-// are stored in the same order. Values are the A operand (elements x positions), for which pairs of positions are woven together by byte permutes;
-// B is the probabilities as the scores left them, hi then lo. The next keys' loads are issued when the scores are done, the next values'
-// when the sums are: a warp always has about a step's half under way.
+// A warp takes 16 positions at a time. Their bytes come by cp.async into a ring of the warp's own, rows as far apart as keeps the fragments'
+// loads off one another's banks, and go from there into the fragments of mma.m16n8k16 without another arrangement: elements' order within a product is
+// free, and a page's rows hold what a lane needs in 8 or 16 neighbouring bytes. Scores: the 16 rows of A are the group's 8 query heads' hi parts,
+// then their lo parts, so one multiply gives both sums and a thread adds its two. Values are the A operand (elements x positions), for which
+// pairs of positions are woven together by byte permutes; B is the probabilities as the scores left them, hi and lo: up to four query heads share the 8
+// columns (hi in the first four, lo in the others, from rows of queries given twice), more take two multiplies. The tensor cores cut sums
+// off: what they add up is one step, and steps are added in f32, rounding.
 
+#include "async_utils.cuh"
 #include "kv_pool.cuh"
 
 #include "../../include/bobcat_cuda.h"
@@ -56,6 +58,35 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same from zero.
+__device__ __forceinline__ void mma_f16_new(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// Whole numbers: 32 signed bytes a row times 32 unsigned ones a column; from `upper` in rows 0 to 7, `lower` in the others.
+__device__ __forceinline__ void mma_i8_new(uint32_t (&c)[4], const uint4& a, uint32_t b0, uint32_t b1, uint32_t upper, uint32_t lower) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%11,%11};"
+                 : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+                 : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "r"(upper), "r"(lower));
+}
+__device__ __forceinline__ void mma_i8(uint32_t (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_fast(float x) {  // results below the normal numbers are zero
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {  // two in one instruction
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+    return r;
+}
 __device__ __forceinline__ void split_half2(float x, float y, uint32_t& hi, uint32_t& lo) {
     __half2 h = __floats2half2_rn(x, y);
     float2 back = __half22float2(h);
@@ -87,22 +118,37 @@ __device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
     return v;
 }
 
-// CTAs that an SM holds, by their registers.
-constexpr uint32_t ctas_per_sm(int32_t format, uint32_t head_dim) { return head_dim == 64 || (head_dim == 128 && format == BC_I8) ? 2 : 1; }
+// A warp's ring: steps under way, and where a step's keys, values and scales lie in it. Two rows of keys that a load's phase covers fall 64
+// bytes apart, four of values (every other one) 32.
+template <int FMT, int HD>
+struct Ring {
+    static constexpr uint32_t kRowBytes = FMT == BC_F16 ? 2 * HD : HD;
+    static constexpr uint32_t kKeyPitch = kRowBytes == 64 ? 64 : kRowBytes + 64, kValuePitch = kRowBytes + 16;
+    static constexpr uint32_t kValues = kStep * kKeyPitch, kScales = kValues + kStep * kValuePitch, kBytes = kScales + (FMT == BC_I8 ? 8 * kStep : 0);
+    static constexpr uint32_t kSteps = kBytes <= 2560 ? 4 : kBytes <= 5632 ? 2 : 1;
+};
+// CTAs that an SM holds, by their registers: heads of 256 take more than half (131072 positions of four 8-bit heads 60 us, 86 with two CTAs and spills).
+constexpr uint32_t ctas_per_sm(uint32_t head_dim) { return head_dim == 256 ? 1 : 2; }
 
 // Registers of a warp's step of keys, and of values: 32-bit words per lane.
 template <int FMT, int HD>
 constexpr int step_words() { return FMT == BC_F16 ? HD / 4 : HD / 8; }
 
-template <int FMT, int HD>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(FMT, HD)) attention_token_paged_kernel(const __grid_constant__ TokenParams p) {
-    constexpr int kWords = step_words<FMT, HD>();
+// PACKED: up to four query heads a KV head.
+template <int FMT, int HD, bool PACKED>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_paged_kernel(const __grid_constant__ TokenParams p) {
+    using R = Ring<FMT, HD>;
+    constexpr int kWords = step_words<FMT, HD>(), D = R::kSteps;
+    constexpr uint32_t kSumPitch = HD + 4;
     constexpr int kKSteps = HD / 16, kTiles = HD / 16;
-    extern __shared__ __align__(16) float token_smem[];
+    extern __shared__ __align__(16) uint8_t token_smem[];
     uint4* q_frag = reinterpret_cast<uint4*>(token_smem);                                    // [kKSteps][32]
-    float* sums = token_smem + kKSteps * 32 * 4;                                             // [kWarps][kRows][HD + 4]
-    float2* stats = reinterpret_cast<float2*>(sums + kWarps * kRows * (HD + 4));             // [kWarps][kRows]
+    uint8_t* rings = token_smem + kKSteps * 32 * 16;                                         // [kWarps][D] steps; at a unit's end:
+    float* sums = reinterpret_cast<float*>(rings);                                           // [kWarps][kRows][kSumPitch]
+    __shared__ float2 stats[kWarps * kRows];
     __shared__ float q_factor[kRows];
+    __shared__ uint32_t page_ids[kWarps][64];
+    __shared__ int digit_sums[kRows][4];
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -159,247 +205,343 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(FMT, HD)) attention_toke
         const uint32_t n_keys = back <= sq.len ? min(sq.len - back + 1, held) : 0;
         if (held < sq.len) leave_fault(pool, kFaultTable);
 
-        // Query fragments in the order of a lane's key elements, a warp per query head. A pair of elements is a word of hi and one of lo parts.
-        __syncthreads();  // the previous unit's fragments have been read
+        // Query fragments in the order of a lane's key elements, a warp per query head (PACKED: two). A pair of elements is a word of hi and one of
+        // lo parts.
+        __syncthreads();  // the previous unit's fragments and sums have been read
+        const uint32_t q_head = PACKED ? warp & 3 : warp;
         {
             float2 x[HD / 64];
             uint32_t most = 0;
 #pragma unroll
             for (int i = 0; i < HD / 64; ++i) {
-                x[i] = warp < p.group ? *reinterpret_cast<const float2*>(p.q + row * p.q_stride + (head * p.group + warp) * p.q_head_stride + 64 * i + 2 * lane)
+                x[i] = q_head < p.group ? *reinterpret_cast<const float2*>(p.q + row * p.q_stride + (head * p.group + q_head) * p.q_head_stride + 64 * i + 2 * lane)
                                       : make_float2(0.f, 0.f);
                 most = max(most, max(__float_as_uint(x[i].x) & 0x7fffffffu, __float_as_uint(x[i].y) & 0x7fffffffu));
             }
-            const uint32_t exponent = min(max(__reduce_max_sync(0xffffffffu, most) >> 23, 1u), 253u);
-            const float up = __uint_as_float((254u - exponent) << 23);  // times 2^14 below: together they may pass the largest float
-            if (lane == 0) q_factor[warp] = __uint_as_float(exponent << 23) * (scale / 16384.f);
+            most = __reduce_max_sync(0xffffffffu, most);
+            const uint32_t exponent = min(max(most >> 23, 1u), 253u);
+            const float up = __uint_as_float((254u - exponent) << 23);  // times 2^14 or 2^29 below: together they may pass the largest float
+            const float back = FMT == BC_F16 ? 1.f / 16384.f : 1.f / 536870912.f;
+            if (lane == 0) q_factor[warp] = most < 0x7f800000u ? __uint_as_float(exponent << 23) * (scale * back) : __uint_as_float(0x7fc00000u);
+            int sum[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int i = 0; i < HD / 64; ++i) {
-                uint32_t hi, lo;
-                split_half2(x[i].x * up * 16384.f, x[i].y * up * 16384.f, hi, lo);
                 const uint32_t e = 2 * lane;  // element 64 i + e
-                const uint32_t ks = FMT == BC_F16 ? 4 * i + 2 * (e >> 5) + ((e & 7) >> 2) : 4 * i + ((e & 15) >> 2);
-                const uint32_t of_lane = 4 * warp + (FMT == BC_F16 ? (e & 31) >> 3 : e >> 4);
-                uint32_t* to = reinterpret_cast<uint32_t*>(q_frag + ks * 32 + of_lane) + (e & 3);  // e & 3 is 0 or 2
-                to[0] = hi;
-                to[1] = lo;
+                if constexpr (FMT == BC_F16) {
+                    uint32_t hi, lo;
+                    split_half2(x[i].x * up * 16384.f, x[i].y * up * 16384.f, hi, lo);
+                    uint32_t* to = reinterpret_cast<uint32_t*>(q_frag + (4 * i + 2 * (e >> 5) + ((e & 7) >> 2)) * 32 + 4 * warp + ((e & 31) >> 3)) + (e & 3);  // e & 3 is 0 or 2
+                    to[0] = hi;
+                    to[1] = lo;
+                } else {
+                    // Signed digits of base 256, of whole numbers up to 2^30; most significant first.
+                    int v[2] = {__float2int_rn(x[i].x * up * 536870912.f), __float2int_rn(x[i].y * up * 536870912.f)};
+                    uint32_t digits[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int d = 3; d >= 0; --d)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const int digit = (int)((uint32_t)v[k] << 24) >> 24;
+                            v[k] = (v[k] - digit) >> 8;
+                            digits[d] |= (uint32_t)(digit & 0xff) << (8 * k);
+                            sum[d] += digit;
+                        }
+                    // Words 0 and 2 of a lane's four are rows 0 to 7 of A, 1 and 3 rows 8 to 15: digits 0 and 1 (of the upper four warps when PACKED: 2 and 3).
+                    uint8_t* to = reinterpret_cast<uint8_t*>(q_frag + (2 * i + ((e & 15) >> 3)) * 32 + 4 * warp + (e >> 4)) + ((e & 7) >> 2) * 8 + (e & 3);
+                    const bool lower = PACKED && warp >= 4;
+                    *reinterpret_cast<uint16_t*>(to) = (uint16_t)(lower ? digits[2] : digits[0]);
+                    *reinterpret_cast<uint16_t*>(to + 4) = (uint16_t)(lower ? digits[3] : digits[1]);
+                    if (!PACKED) {
+                        *reinterpret_cast<uint16_t*>(to + kKSteps / 2 * 32 * 16) = (uint16_t)digits[2];
+                        *reinterpret_cast<uint16_t*>(to + kKSteps / 2 * 32 * 16 + 4) = (uint16_t)digits[3];
+                    }
+                }
+            }
+            if constexpr (FMT == BC_I8) {
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    sum[d] = __reduce_add_sync(0xffffffffu, sum[d]);
+                    if (lane == 0) digit_sums[warp][d] = sum[d];
+                }
             }
         }
         __syncthreads();
         const float factor_q = q_factor[g];
+        // What sums of digits begin with: a float of 1.5 * 2^23, less 128 times the digits (an element is stored as its number plus 128). They end
+        // as floats of 1.5 * 2^23 plus the sum.
+        constexpr uint32_t kMagic = 0x4b400000u;
+        uint32_t begin_sums[4] = {0, 0, 0, 0};
+        if constexpr (FMT == BC_I8) {
+#pragma unroll
+            for (int d = 0; d < (PACKED ? 2 : 4); ++d) begin_sums[d] = kMagic - 128u * (uint32_t)digit_sums[g][PACKED && g >= 4 ? d + 2 : d];
+        }
 
-        float o[kTiles][4];
+        float2 o[kTiles][2];
 #pragma unroll
-        for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
+        for (int n = 0; n < kTiles; ++n) o[n][0] = o[n][1] = make_float2(0.f, 0.f);
         float top = -INFINITY, total_p = 0.f;  // of query head g, the sum over this lane's positions
         float unit = FMT == BC_I8 ? 0.f : 1.f, inverse_unit = unit;  // the sums of query head g are counted in these
 
-        uint32_t kw[kWords], vw[kWords];
-        float2 dk[2], dv[2];
         const uint32_t* table = rows.table + (uint64_t)seq * rows.max_pages;
         const uint32_t slots = (1u << pool.page_shift) - 1;
-        // The warp's steps are one block apart; `pos` is the first position of one.
-        const uint32_t pos_end = min((block0 + blocks) * kBlock, n_keys);
-        auto page_of = [&](uint32_t pos) { return pos < pos_end ? table[pos >> pool.page_shift] : 0u; };
-        auto load_keys = [&](uint32_t pos, uint32_t page) {
-            const uint8_t* from = pool.k + kv_row_at(pool, page, head, pos & slots);
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int c = 0; c < kWords / 8; ++c) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(from + (8 * j + g) * pool.row_bytes + 64 * c + 16 * t);
-                    kw[(j * (kWords / 8) + c) * 4 + 0] = w.x;
-                    kw[(j * (kWords / 8) + c) * 4 + 1] = w.y;
-                    kw[(j * (kWords / 8) + c) * 4 + 2] = w.z;
-                    kw[(j * (kWords / 8) + c) * 4 + 3] = w.w;
-                }
-            if (FMT == BC_I8) {
-                const float* s = reinterpret_cast<const float*>(pool.k + kv_scale_at(pool, page, head, pos & slots));
-                dk[0] = *reinterpret_cast<const float2*>(s + 2 * t);
-                dk[1] = *reinterpret_cast<const float2*>(s + 8 + 2 * t);
+        // The warp's steps are one block apart: step n has positions pos0 + n * kBlock .. 15 on.
+        const uint32_t pos0 = block0 * kBlock + warp * kStep, pos_end = min((block0 + blocks) * kBlock, n_keys);
+        const uint32_t n_steps = pos0 < pos_end ? (pos_end - pos0 + kBlock - 1) / kBlock : 0;
+        uint8_t* const ring = rings + warp * (D * R::kBytes);
+        // The page of a step, 32 steps looked up at a time: by the copies of step 0, 32, ..., before anything asks.
+        auto look_up = [&](uint32_t n) {
+            if (n % 32 == 0 && n < n_steps) {
+                if (n + lane < n_steps) page_ids[warp][(n + lane) % 64] = table[(pos0 + (n + lane) * kBlock) >> pool.page_shift];
+                __syncwarp();
             }
         };
-        // Position 2t + (i & 1) + 8 (i >> 1) of the step, i = 0 .. 3; a lane's 8 elements 8g .. of every 64.
-        auto load_values = [&](uint32_t pos, uint32_t page) {
-            const uint8_t* from = pool.v + kv_row_at(pool, page, head, pos & slots);
+        constexpr uint32_t kPieces = R::kRowBytes / 16;  // of a row; a lane brings every 32nd of the step's
+        const uint32_t ring_at = async::smem_u32(ring), key_to = ring_at + lane / kPieces * R::kKeyPitch + lane % kPieces * 16,
+                       value_to = ring_at + R::kValues + lane / kPieces * R::kValuePitch + lane % kPieces * 16;
+        const uint64_t head_at = (uint64_t)(head << pool.page_shift) * pool.row_bytes + 16 * lane;
+        const uint64_t scales_at = (uint64_t)(pool.n_kv_heads << pool.page_shift) * pool.row_bytes + (uint64_t)(head << pool.page_shift) * 4 + 16 * (lane & 3);
+        const uint8_t* const scale_pool = lane < 4 ? pool.k : pool.v;
+        // Keys (and both scales) of a step, then its values: a group of copies each, empty behind the last step.
+        uint64_t rows_at = 0;
+        bool there = false;
+        auto copy_keys = [&](uint32_t n) {
+            look_up(n);
+            const uint32_t page = n < n_steps ? page_ids[warp][n % 64] : ~0u, slot = (pos0 + n * kBlock) & slots, in_ring = n % D * R::kBytes;
+            there = page < pool.n_pages;
+            if (there) {
+                const uint64_t page_at = page * pool.page_bytes;
+                rows_at = page_at + head_at + slot * pool.row_bytes;
+                const uint8_t* from = pool.k + rows_at;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint8_t* at_row = from + (2 * t + (i & 1) + 8 * (i >> 1)) * pool.row_bytes;
+                for (uint32_t i = 0; i < kPieces / 2; ++i) async::cp_async_16(key_to + in_ring + i * (32 / kPieces) * R::kKeyPitch, from + 512 * i);
+                if (FMT == BC_I8 && lane < 8) async::cp_async_16(ring_at + in_ring + R::kScales + 16 * lane, scale_pool + page_at + scales_at + slot * 4);
+            }
+            async::cp_async_commit();
+        };
+        auto copy_values = [&](uint32_t n) {  // behind the same step's copy_keys
+            if (there) {
+                const uint8_t* from = pool.v + rows_at;
 #pragma unroll
-                for (int c = 0; c < HD / 64; ++c) {
-                    if constexpr (FMT == BC_F16) {
-                        const uint4 w = *reinterpret_cast<const uint4*>(at_row + 128 * c + 16 * g);
-                        vw[(i * (HD / 64) + c) * 4 + 0] = w.x;
-                        vw[(i * (HD / 64) + c) * 4 + 1] = w.y;
-                        vw[(i * (HD / 64) + c) * 4 + 2] = w.z;
-                        vw[(i * (HD / 64) + c) * 4 + 3] = w.w;
-                    } else {
-                        const uint2 w = *reinterpret_cast<const uint2*>(at_row + 64 * c + 8 * g);
-                        vw[(i * (HD / 64) + c) * 2 + 0] = w.x;
-                        vw[(i * (HD / 64) + c) * 2 + 1] = w.y;
+                for (uint32_t i = 0; i < kPieces / 2; ++i) async::cp_async_16(value_to + n % D * R::kBytes + i * (32 / kPieces) * R::kValuePitch, from + 512 * i);
+            }
+            async::cp_async_commit();
+        };
+#pragma unroll
+        for (uint32_t n = 0; n < D; ++n) {
+            copy_keys(n);
+            copy_values(n);
+        }
+        for (uint32_t n = 0; n < n_steps; ++n) {
+            const uint8_t* const here = ring + n % D * R::kBytes;
+            const bool good = page_ids[warp][n % 64] < pool.n_pages;  // a page that the pool does not have holds nothing
+            async::cp_async_wait<2 * D - 1>();
+            __syncwarp();  // everyone's copies of the keys
+            float x[4];  // scores of positions 2t, 2t + 1, 8 + 2t, 9 + 2t for query head g
+            float2 dk[2], dv[2];
+            if (good) {
+                if constexpr (FMT == BC_F16) {
+                    float s[2][4];
+#pragma unroll
+                    for (int c = 0; c < kWords / 8; ++c) {  // 64 bytes of a key: 32 elements
+                        uint4 kw[2];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) kw[j] = *reinterpret_cast<const uint4*>(here + (8 * j + g) * R::kKeyPitch + 64 * c + 16 * t);
+                        const uint4 f0 = q_frag[2 * c * 32 + lane], f1 = q_frag[(2 * c + 1) * 32 + lane];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            if (c == 0)
+                                mma_f16_new(s[j], f0.x, f0.y, f0.z, f0.w, kw[j].x, kw[j].y);
+                            else
+                                mma_f16(s[j], f0.x, f0.y, f0.z, f0.w, kw[j].x, kw[j].y);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) mma_f16(s[j], f1.x, f1.y, f1.z, f1.w, kw[j].z, kw[j].w);
                     }
-                }
-            }
-            if (FMT == BC_I8) {
-                const float* s = reinterpret_cast<const float*>(pool.v + kv_scale_at(pool, page, head, pos & slots));
-                dv[0] = *reinterpret_cast<const float2*>(s + 2 * t);
-                dv[1] = *reinterpret_cast<const float2*>(s + 8 + 2 * t);
-            }
-        };
-
-        uint32_t pos = block0 * kBlock + warp * kStep;
-        uint32_t page = page_of(pos), next_page = page_of(pos + kBlock);
-        bool good = page < pool.n_pages;  // a page that the pool does not have holds nothing
-        if (pos < pos_end && good) load_keys(pos, page);
-        while (pos < pos_end) {  // uniform in the warp
-            const uint32_t next = pos + kBlock;
-            const bool next_good = next_page < pool.n_pages;
-            if (!good) {
-                if (lane == 0) leave_fault(pool, kFaultPage);
-                if (next < pos_end && next_good) load_keys(next, next_page);
-            } else {
-                load_values(pos, page);
-                float s[2][4];
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[j][i] = 0.f;
-#pragma unroll
-                for (int ks = 0; ks < kKSteps; ++ks) {
-                    const uint4 f = q_frag[ks * 32 + lane];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        uint32_t b0, b1;
-                        if constexpr (FMT == BC_F16) {
-                            b0 = kw[j * (kWords / 2) + 2 * ks];
-                            b1 = kw[j * (kWords / 2) + 2 * ks + 1];
-                        } else {
-                            unpack_i8(kw[j * (kWords / 2) + ks], b0, b1);
-                        }
-                        mma_f16(s[j], f.x, f.y, f.z, f.w, b0, b1);
-                    }
-                }
-                float x[4];  // scores of positions 2t, 2t + 1, 8 + 2t, 9 + 2t for query head g
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    x[2 * j] = (s[j][0] + s[j][2]) * factor_q;
-                    x[2 * j + 1] = (s[j][1] + s[j][3]) * factor_q;
-                    if (FMT == BC_I8) {
-                        x[2 * j] *= dk[j].x;
-                        x[2 * j + 1] *= dk[j].y;
-                    }
-                }
-                if (next < pos_end && next_good) load_keys(next, next_page);
-                const uint32_t left = n_keys - pos;  // positions of the step that exist, if fewer than 16
-                if (left < kStep) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (2 * t + (i & 1) + 8 * (i >> 1) >= left) x[i] = -INFINITY;
-                }
-                float most = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                const float now = fmaxf(top, most);
-                const float shift = now == -INFINITY ? 0.f : now;
-                float factor = exp2f(top - shift);
-                bool moved = now > top;
-                top = now;
-                float total_step = 0.f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[i] = exp2f(x[i] - shift + kLift);  // the sums are lifted alike
-                    total_step += x[i];
-                }
-                total_p = total_p * factor + total_step;
-                if (FMT == BC_I8) {
-                    float largest = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float d = i & 1 ? dv[i >> 1].y : dv[i >> 1].x;
-                        x[i] = 2 * t + (i & 1) + 8 * (i >> 1) < left ? x[i] * d : 0.f;  // scales behind the last position may be anything
-                        largest = fmaxf(largest, fabsf(x[i]));
-                    }
-                    largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-                    largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-                    if (moved || largest > 32768.f * unit) {  // weights of 2^15 units at most: halves end at 2^16
-                        // A row's largest weight so far, what went before scaled to the new maximum, is 2^11 to 2^12 units.
-                        const uint32_t exponent = __float_as_uint(fmaxf(2048.f * unit * factor, largest)) >> 23;
-                        const bool any = exponent > 11;  // smaller ones weigh nothing
-                        const float before = unit;
-                        unit = any ? __uint_as_float((min(exponent, 253u) - 11u) << 23) : 0.f;
-                        inverse_unit = any ? __uint_as_float((265u - min(exponent, 253u)) << 23) : 0.f;
-                        factor *= before * inverse_unit;
-                        moved = true;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] *= inverse_unit;
-                }
-                if (__any_sync(0xffffffffu, moved)) {
-                    const float f0 = __shfl_sync(0xffffffffu, factor, 8 * t), f1 = __shfl_sync(0xffffffffu, factor, 8 * t + 4);
-#pragma unroll
-                    for (int n = 0; n < kTiles; ++n) {
-                        o[n][0] *= f0;
-                        o[n][1] *= f1;
-                        o[n][2] *= f0;
-                        o[n][3] *= f1;
-                    }
-                }
-                uint32_t hi0, lo0, hi1, lo1;
-                split_half2(x[0], x[1], hi0, lo0);
-                split_half2(x[2], x[3], hi1, lo1);
-                if constexpr (FMT == BC_F16) {
-                    if (left < kStep) {  // elements behind the last position may be anything
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (2 * t + (i & 1) + 8 * (i >> 1) >= left) {
-#pragma unroll
-                                for (int w = 0; w < kWords / 4; ++w) vw[i * (kWords / 4) + w] = 0;
-                            }
-                    }
-#pragma unroll
-                    for (int w = 0; w < kWords / 4; ++w) {  // elements 2w, 2w + 1 of the lane's: rows g and g + 8 of a tile
-                        const uint32_t a = vw[w], b = vw[kWords / 4 + w], c = vw[2 * (kWords / 4) + w], d = vw[3 * (kWords / 4) + w];
-                        const uint32_t a0 = __byte_perm(a, b, 0x5410), a1 = __byte_perm(a, b, 0x7632), a2 = __byte_perm(c, d, 0x5410), a3 = __byte_perm(c, d, 0x7632);
-                        mma_f16(o[w], a0, a1, a2, a3, hi0, hi1);
-                        mma_f16(o[w], a0, a1, a2, a3, lo0, lo1);
+                        x[2 * j] = s[j][0] + s[j][2];
+                        x[2 * j + 1] = s[j][1] + s[j][3];
                     }
                 } else {
+                    uint32_t s[2][PACKED ? 1 : 2][4];
 #pragma unroll
-                    for (int w = 0; w < kWords / 4; ++w) {  // elements 4w .. 4w + 3 of the lane's: two tiles
-                        const uint32_t a = vw[w], b = vw[kWords / 4 + w], c = vw[2 * (kWords / 4) + w], d = vw[3 * (kWords / 4) + w];
-                        const uint32_t ab_lo = __byte_perm(a, b, 0x5140), ab_hi = __byte_perm(a, b, 0x7362);  // a0 b0 a1 b1, a2 b2 a3 b3
-                        const uint32_t cd_lo = __byte_perm(c, d, 0x5140), cd_hi = __byte_perm(c, d, 0x7362);
-                        uint32_t a0, a1, a2, a3;
-                        unpack_i8(ab_lo, a0, a1);
-                        unpack_i8(cd_lo, a2, a3);
-                        mma_f16(o[2 * w], a0, a1, a2, a3, hi0, hi1);
-                        mma_f16(o[2 * w], a0, a1, a2, a3, lo0, lo1);
-                        unpack_i8(ab_hi, a0, a1);
-                        unpack_i8(cd_hi, a2, a3);
-                        mma_f16(o[2 * w + 1], a0, a1, a2, a3, hi0, hi1);
-                        mma_f16(o[2 * w + 1], a0, a1, a2, a3, lo0, lo1);
+                    for (int c = 0; c < kWords / 8; ++c) {  // 64 bytes of a key: 64 elements
+                        uint4 kw[2];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) kw[j] = *reinterpret_cast<const uint4*>(here + (8 * j + g) * R::kKeyPitch + 64 * c + 16 * t);
+#pragma unroll
+                        for (int m = 0; m < (PACKED ? 1 : 2); ++m) {
+                            const uint4 f0 = q_frag[(m * (kKSteps / 2) + 2 * c) * 32 + lane], f1 = q_frag[(m * (kKSteps / 2) + 2 * c + 1) * 32 + lane];
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                if (c == 0)
+                                    mma_i8_new(s[j][m], f0, kw[j].x, kw[j].y, begin_sums[2 * m], begin_sums[2 * m + 1]);
+                                else
+                                    mma_i8(s[j][m], f0, kw[j].x, kw[j].y);
+                            }
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) mma_i8(s[j][m], f1, kw[j].z, kw[j].w);
+                        }
                     }
+                    // The digits' sums together: two here, the other two in the lane of the row four on, or here too.
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int j = i >> 1, k = i & 1;
+                        x[i] = fmaf(__uint_as_float(s[j][0][k]) - 12582912.f, 256.f, __uint_as_float(s[j][0][k + 2]) - 12582912.f);
+                        if constexpr (PACKED) {
+                            x[i] *= g < 4 ? 65536.f : 1.f;
+                            x[i] += __shfl_xor_sync(0xffffffffu, x[i], 16);
+                        } else {
+                            x[i] = fmaf(x[i], 65536.f, fmaf(__uint_as_float(s[j][1][k]) - 12582912.f, 256.f, __uint_as_float(s[j][1][k + 2]) - 12582912.f));
+                        }
+                    }
+                    const float* scales = reinterpret_cast<const float*>(here + R::kScales);
+                    dk[0] = *reinterpret_cast<const float2*>(scales + 2 * t);
+                    dk[1] = *reinterpret_cast<const float2*>(scales + 8 + 2 * t);
+                    dv[0] = *reinterpret_cast<const float2*>(scales + kStep + 2 * t);
+                    dv[1] = *reinterpret_cast<const float2*>(scales + kStep + 8 + 2 * t);
                 }
             }
-            pos = next;
-            page = next_page;
-            good = next_good;
-            next_page = page_of(pos + kBlock);
+            __syncwarp();  // the keys have been read
+            copy_keys(n + D);
+            if (!good) {
+                if (lane == 0) leave_fault(pool, kFaultPage);
+                copy_values(n + D);
+                continue;
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                x[2 * j] *= factor_q;
+                x[2 * j + 1] *= factor_q;
+                if (FMT == BC_I8) {
+                    x[2 * j] *= dk[j].x;
+                    x[2 * j + 1] *= dk[j].y;
+                }
+            }
+            const uint32_t left = n_keys - (pos0 + n * kBlock);  // positions of the step that exist, if fewer than 16
+            if (left < kStep) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (2 * t + (i & 1) + 8 * (i >> 1) >= left) x[i] = -INFINITY;
+            }
+            float most = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const float now = fmaxf(top, most);
+            const float shift = now == -INFINITY ? 0.f : now, down = shift - kLift;
+            float factor = exp2_fast(top - shift);
+            const bool moved = now > top;
+            top = now;
+            float total_step = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = exp2_fast(x[i] - down);  // the sums are lifted alike
+                total_step += x[i];
+            }
+            total_p = total_p * factor + total_step;
+            if constexpr (FMT == BC_I8) {
+                float largest = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float d = i & 1 ? dv[i >> 1].y : dv[i >> 1].x;
+                    x[i] *= d;
+                }
+                if (left < kStep) {  // scales behind the last position may be anything
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (2 * t + (i & 1) + 8 * (i >> 1) >= left) x[i] = 0.f;
+                }
+                largest = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+                if (moved || largest > 32768.f * unit) {  // weights of 2^15 units at most: halves end at 2^16
+                    // A row's largest weight so far, what went before scaled to the new maximum, is 2^11 to 2^12 units.
+                    const uint32_t exponent = __float_as_uint(fmaxf(2048.f * unit * factor, largest)) >> 23;
+                    const bool any = exponent > 11;  // smaller ones weigh nothing
+                    const float before = unit;
+                    unit = any ? __uint_as_float((min(exponent, 253u) - 11u) << 23) : 0.f;
+                    inverse_unit = any ? __uint_as_float((265u - min(exponent, 253u)) << 23) : 0.f;
+                    factor *= before * inverse_unit;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] *= inverse_unit;
+            }
+            const float2 f = make_float2(__shfl_sync(0xffffffffu, factor, 8 * t), __shfl_sync(0xffffffffu, factor, 8 * t + 4));  // of columns 2t and 2t + 1
+            uint32_t hi0, lo0, hi1, lo1;
+            split_half2(x[0], x[1], hi0, lo0);
+            split_half2(x[2], x[3], hi1, lo1);
+            if (PACKED && g >= 4) {
+                hi0 = lo0;
+                hi1 = lo1;
+            }
+            async::cp_async_wait<2 * D - 1>();
+            __syncwarp();  // everyone's copies of the values
+            // Position 2t + (i & 1) + 8 (i >> 1) of the step, i = 0 .. 3; a lane's 8 elements 8g .. of every 64.
+            uint32_t vw[4][kWords / 4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint8_t* at_row = here + R::kValues + (2 * t + (i & 1) + 8 * (i >> 1)) * R::kValuePitch;
+#pragma unroll
+                for (int c = 0; c < HD / 64; ++c) {
+                    if constexpr (FMT == BC_F16)
+                        *reinterpret_cast<uint4*>(&vw[i][4 * c]) = *reinterpret_cast<const uint4*>(at_row + 128 * c + 16 * g);
+                    else
+                        *reinterpret_cast<uint2*>(&vw[i][2 * c]) = *reinterpret_cast<const uint2*>(at_row + 64 * c + 8 * g);
+                }
+            }
+            __syncwarp();  // the values have been read
+            copy_values(n + D);
+            // A step's sums, from zero, join the others rounded.
+            auto product = [&](int tile, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+                float d[4];
+                if (PACKED) {
+                    mma_f16_new(d, a0, a1, a2, a3, hi0, hi1);
+                } else {
+                    mma_f16_new(d, a0, a1, a2, a3, lo0, lo1);
+                    mma_f16(d, a0, a1, a2, a3, hi0, hi1);
+                }
+                o[tile][0] = fma2(o[tile][0], f, make_float2(d[0], d[1]));
+                o[tile][1] = fma2(o[tile][1], f, make_float2(d[2], d[3]));
+            };
+            if constexpr (FMT == BC_F16) {
+                if (left < kStep) {  // elements behind the last position may be anything
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (2 * t + (i & 1) + 8 * (i >> 1) >= left) {
+#pragma unroll
+                            for (int w = 0; w < kWords / 4; ++w) vw[i][w] = 0;
+                        }
+                }
+#pragma unroll
+                for (int w = 0; w < kWords / 4; ++w)  // elements 2w, 2w + 1 of the lane's: rows g and g + 8 of a tile
+                    product(w, __byte_perm(vw[0][w], vw[1][w], 0x5410), __byte_perm(vw[0][w], vw[1][w], 0x7632), __byte_perm(vw[2][w], vw[3][w], 0x5410),
+                            __byte_perm(vw[2][w], vw[3][w], 0x7632));
+            } else {
+#pragma unroll
+                for (int w = 0; w < kWords / 4; ++w)  // elements 4w .. 4w + 3 of the lane's: two tiles
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t a0, a1, a2, a3;  // elements 2h and 2h + 1 of two positions
+                        unpack_i8(__byte_perm(vw[0][w], vw[1][w], h ? 0x7362 : 0x5140), a0, a1);
+                        unpack_i8(__byte_perm(vw[2][w], vw[3][w], h ? 0x7362 : 0x5140), a2, a3);
+                        product(2 * w + h, a0, a1, a2, a3);
+                    }
+            }
         }
+        async::cp_async_wait<0>();
 
-        // The warps' sums, joined through shared memory. Tile n's rows g and g + 8 are elements 2n' and 2n' + 1 of the lane's eight: see load_values.
+        // The warps' sums, joined through shared memory, in the rings' place. Tile n's rows g and g + 8 are elements 2n' and 2n' + 1 of the lane's eight.
         total_p += __shfl_xor_sync(0xffffffffu, total_p, 1);
         total_p += __shfl_xor_sync(0xffffffffu, total_p, 2);
         if (t == 0) stats[warp * kRows + g] = make_float2(top, total_p);
         const float u0 = __shfl_sync(0xffffffffu, unit, 8 * t), u1 = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
+        __syncthreads();  // every ring has been read
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
             const uint32_t d = (n / 4) * 64 + 8 * g + 2 * (n % 4);  // elements d and d + 1
-            float* to = sums + (warp * kRows + 2 * t) * (HD + 4) + d;
-            *reinterpret_cast<float2*>(to) = make_float2(o[n][0] * u0, o[n][2] * u0);
-            *reinterpret_cast<float2*>(to + HD + 4) = make_float2(o[n][1] * u1, o[n][3] * u1);
+            float* to = sums + (warp * kRows + 2 * t) * kSumPitch + d;
+            *reinterpret_cast<float2*>(to) = make_float2(o[n][0].x * u0, o[n][1].x * u0);
+            *reinterpret_cast<float2*>(to + kSumPitch) = make_float2(o[n][0].y * u1, o[n][1].y * u1);
         }
         __syncthreads();
         const bool begins = block0 == 0, ends = block0 + blocks == sq.blocks;
@@ -416,7 +558,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(FMT, HD)) attention_toke
             for (int w = 0; w < kWarps; ++w) {
                 const float2 st = stats[w * kRows + r];
                 const float weight = st.x == -INFINITY ? 0.f : exp2f(st.x - shift);
-                const float4 v = *reinterpret_cast<const float4*>(sums + (w * kRows + r) * (HD + 4) + d);
+                float4 v = *reinterpret_cast<const float4*>(sums + (w * kRows + r) * kSumPitch + d);
+                if (PACKED) {  // the lower halves' sums
+                    const float4 l = *reinterpret_cast<const float4*>(sums + (w * kRows + r + 4) * kSumPitch + d);
+                    v = make_float4(v.x + l.x, v.y + l.y, v.z + l.z, v.w + l.w);
+                }
                 if (st.x != -INFINITY) {
                     sum.x += weight * v.x;
                     sum.y += weight * v.y;
@@ -496,23 +642,32 @@ __global__ void __launch_bounds__(32 * kRows) attention_token_join_kernel(const 
     for (int k = 0; k < kPairs; ++k) to[32 * k] = make_float2(sum[k].x * inverse, sum[k].y * inverse);
 }
 
-template <int HD>
-constexpr size_t token_smem_bytes() { return (size_t)(HD / 16) * 32 * 16 + (size_t)kWarps * kRows * (HD + 4) * 4 + kWarps * kRows * 8; }
+template <int FMT, int HD>
+constexpr size_t token_smem_bytes() {
+    using R = Ring<FMT, HD>;
+    constexpr size_t rings = (size_t)kWarps * R::kSteps * R::kBytes, sums = (size_t)kWarps * kRows * (HD + 4) * 4;
+    return (size_t)(HD / 16) * 32 * 16 + (rings > sums ? rings : sums);
+}
 
 // CTAs of a launch: no more than the blocks that the tables could hold.
 uint32_t token_ctas(const KvPool& pool, const KvRows& rows) {
     const uint64_t most = (uint64_t)rows.n_rows * pool.n_kv_heads * ((((uint64_t)rows.max_pages << pool.page_shift) + kBlock - 1) / kBlock);
-    uint64_t ctas = (uint64_t)sm_count() * ctas_per_sm(pool.format, pool.head_dim);
+    uint64_t ctas = (uint64_t)sm_count() * ctas_per_sm(pool.head_dim);
     if (ctas > kMostCtas) ctas = kMostCtas;
     return (uint32_t)(ctas > most ? most : ctas);
 }
 
+template <int FMT, int HD, bool PACKED>
+cudaError_t launch_token_as(cudaStream_t stream, const TokenParams& p, uint32_t ctas) {
+    static_assert((token_smem_bytes<FMT, HD>() + 4096) * ctas_per_sm(HD) <= 228 * 1024, "shared memory of an SM");
+    cudaError_t e = ensure_dynamic_smem((const void*)attention_token_paged_kernel<FMT, HD, PACKED>, token_smem_bytes<FMT, HD>());
+    if (e != cudaSuccess) return e;
+    return launch_dependent(attention_token_paged_kernel<FMT, HD, PACKED>, dim3(ctas), dim3(kThreads), token_smem_bytes<FMT, HD>(), stream, p);
+}
 template <int FMT, int HD>
 cudaError_t launch_token(cudaStream_t stream, const TokenParams& p) {
-    cudaError_t e = ensure_dynamic_smem((const void*)attention_token_paged_kernel<FMT, HD>, token_smem_bytes<HD>());
-    if (e != cudaSuccess) return e;
     const uint32_t ctas = token_ctas(p.pool, p.rows);
-    e = launch_dependent(attention_token_paged_kernel<FMT, HD>, dim3(ctas), dim3(kThreads), token_smem_bytes<HD>(), stream, p);
+    cudaError_t e = p.group <= 4 ? launch_token_as<FMT, HD, true>(stream, p, ctas) : launch_token_as<FMT, HD, false>(stream, p, ctas);
     if (e != cudaSuccess || ctas == 1) return e;
     return launch_dependent(attention_token_join_kernel<HD>, dim3(ctas - 1), dim3(32 * kRows), 0, stream, static_cast<const float*>(p.parts), p.out, p.n_heads, p.group);
 }
