@@ -32,8 +32,7 @@ namespace k {
 namespace {
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
-constexpr uint32_t kStep = 16;                 // positions a warp takes at a time
-constexpr uint32_t kBlock = kStep * kWarps;    // positions of a block, the unit that work is counted in
+constexpr uint32_t kHalf = 16;                 // positions in a fragment, always of one page
 constexpr float kLift = 15.f;                  // probabilities are taken times 2^15
 constexpr uint32_t kRows = 8;                  // query heads of a KV head, at most
 constexpr uint32_t kMostCtas = kPagedMostCtas;
@@ -95,19 +94,31 @@ __device__ __forceinline__ void split_half2(float x, float y, uint32_t& hi, uint
     lo = *reinterpret_cast<uint32_t*>(&l);
 }
 
+// A warp's ring: steps under way, and where a step's keys, values and scales lie in it. Two rows of keys that a load's phase covers fall 64
+// bytes apart, four of values (every other one) 32.
+template <int FMT, int HD>
+struct Ring {
+    // Positions of a step: two fragments where registers and shared memory hold them, which halves what a step costs beside its multiplies. A block, the
+    // unit that work is counted in, is a step of each warp.
+    static constexpr uint32_t kStep = HD == 64 || (HD == 128 && FMT == BC_I8) ? 2 * kHalf : kHalf, kBlock = kStep * kWarps, kHalves = kStep / kHalf;
+    static constexpr uint32_t kRowBytes = FMT == BC_F16 ? 2 * HD : HD;
+    static constexpr uint32_t kKeyPitch = kRowBytes == 64 ? 64 : kRowBytes + 64, kValuePitch = kRowBytes + 16;
+    static constexpr uint32_t kValues = kStep * kKeyPitch, kScales = kValues + kStep * kValuePitch, kBytes = kScales + (FMT == BC_I8 ? 8 * kStep : 0);
+    static constexpr uint32_t kSteps = kBytes <= 5632 ? 2 : 1;
+};
 // A sequence of the call: its rows, the positions it holds, the blocks its longest row takes.
 struct Seq {
     uint32_t row0, n, end, len;
     uint32_t blocks;
 };
-__device__ __forceinline__ Seq seq_at(const KvPool& pool, const KvRows& rows, uint32_t s, uint32_t most) {
+__device__ __forceinline__ Seq seq_at(const KvPool& pool, const KvRows& rows, uint32_t s, uint32_t most, uint32_t block) {
     Seq q;
     q.row0 = rows.starts[s];
     q.end = rows.starts[s + 1];
     q.n = q.row0 < rows.n_rows && q.end > q.row0 && q.end - q.row0 <= most ? min(q.end, rows.n_rows) - q.row0 : 0;
     q.len = rows.lens[s];
     const uint32_t held = min((uint64_t)q.len, (uint64_t)rows.max_pages << pool.page_shift);
-    q.blocks = max(1u, (held + kBlock - 1) / kBlock);
+    q.blocks = max(1u, (held + block - 1) / block);
     return q;
 }
 __device__ __forceinline__ uint64_t blocks_of(const KvPool& pool, const Seq& q) { return (uint64_t)q.n * pool.n_kv_heads * q.blocks; }
@@ -118,15 +129,6 @@ __device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
     return v;
 }
 
-// A warp's ring: steps under way, and where a step's keys, values and scales lie in it. Two rows of keys that a load's phase covers fall 64
-// bytes apart, four of values (every other one) 32.
-template <int FMT, int HD>
-struct Ring {
-    static constexpr uint32_t kRowBytes = FMT == BC_F16 ? 2 * HD : HD;
-    static constexpr uint32_t kKeyPitch = kRowBytes == 64 ? 64 : kRowBytes + 64, kValuePitch = kRowBytes + 16;
-    static constexpr uint32_t kValues = kStep * kKeyPitch, kScales = kValues + kStep * kValuePitch, kBytes = kScales + (FMT == BC_I8 ? 8 * kStep : 0);
-    static constexpr uint32_t kSteps = kBytes <= 2560 ? 4 : kBytes <= 5632 ? 2 : 1;
-};
 // CTAs that an SM holds, by their registers: heads of 256 take more than half (131072 positions of four 8-bit heads 60 us, 86 with two CTAs and spills).
 constexpr uint32_t ctas_per_sm(uint32_t head_dim) { return head_dim == 256 ? 1 : 2; }
 
@@ -139,7 +141,7 @@ template <int FMT, int HD, bool PACKED>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_paged_kernel(const __grid_constant__ TokenParams p) {
     using R = Ring<FMT, HD>;
     constexpr int kWords = step_words<FMT, HD>(), D = R::kSteps;
-    constexpr uint32_t kSumPitch = HD + 4;
+    constexpr uint32_t kSumPitch = HD + 4, kStep = R::kStep, kBlock = R::kBlock, kHalves = R::kHalves;
     constexpr int kKSteps = HD / 16, kTiles = HD / 16;
     extern __shared__ __align__(16) uint8_t token_smem[];
     uint4* q_frag = reinterpret_cast<uint4*>(token_smem);                                    // [kKSteps][32]
@@ -158,7 +160,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
 
     // This CTA's run of blocks, and the sequence that it begins in. Every warp works it out for itself.
     uint64_t total = 0;
-    for (uint32_t s = lane; s < rows.n_seqs; s += 32) total += blocks_of(pool, seq_at(pool, rows, s, p.most));
+    for (uint32_t s = lane; s < rows.n_seqs; s += 32) total += blocks_of(pool, seq_at(pool, rows, s, p.most, kBlock));
     total = warp_sum_u64(total);
     const uint64_t runs = min((uint64_t)gridDim.x, total);  // none of them empty
     uint64_t at = blockIdx.x < runs ? total * blockIdx.x / runs : total;
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
     uint32_t seq = 0;
     uint64_t base = 0;  // blocks of the sequences before `seq`
     for (uint32_t s0 = 0; s0 < rows.n_seqs; s0 += 32) {
-        const uint64_t mine = s0 + lane < rows.n_seqs ? blocks_of(pool, seq_at(pool, rows, s0 + lane, p.most)) : 0;
+        const uint64_t mine = s0 + lane < rows.n_seqs ? blocks_of(pool, seq_at(pool, rows, s0 + lane, p.most, kBlock)) : 0;
         uint64_t upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -190,10 +192,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
     PartsHead cut{0, 0, 0, 0};
 
     while (at < end) {
-        Seq sq = seq_at(pool, rows, seq, p.most);
+        Seq sq = seq_at(pool, rows, seq, p.most, kBlock);
         while (base + blocks_of(pool, sq) <= at) {  // sequences without rows have no blocks
             base += blocks_of(pool, sq);
-            sq = seq_at(pool, rows, ++seq, p.most);
+            sq = seq_at(pool, rows, ++seq, p.most, kBlock);
         }
         // The unit, and the blocks of it that are this CTA's. Rows of a head are neighbours.
         const uint64_t in_seq = at - base;
@@ -288,10 +290,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
         const uint32_t pos0 = block0 * kBlock + warp * kStep, pos_end = min((block0 + blocks) * kBlock, n_keys);
         const uint32_t n_steps = pos0 < pos_end ? (pos_end - pos0 + kBlock - 1) / kBlock : 0;
         uint8_t* const ring = rings + warp * (D * R::kBytes);
-        // The page of a step, 32 steps looked up at a time: by the copies of step 0, 32, ..., before anything asks.
+        // The pages of a step's halves, 32 halves looked up at a time, by the copies of the first of them, before anything asks. A half behind the
+        // last position has none.
+        constexpr uint32_t kAtOnce = 32 / kHalves;  // steps
         auto look_up = [&](uint32_t n) {
-            if (n % 32 == 0 && n < n_steps) {
-                if (n + lane < n_steps) page_ids[warp][(n + lane) % 64] = table[(pos0 + (n + lane) * kBlock) >> pool.page_shift];
+            if (n % kAtOnce == 0 && n < n_steps) {
+                const uint32_t at = pos0 + (n + lane / kHalves) * kBlock + lane % kHalves * kHalf;
+                page_ids[warp][(n * kHalves + lane) % 64] = at < pos_end ? table[at >> pool.page_shift] : kNoSlot;
                 __syncwarp();
             }
         };
@@ -302,28 +307,36 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
         const uint64_t scales_at = (uint64_t)(pool.n_kv_heads << pool.page_shift) * pool.row_bytes + (uint64_t)(head << pool.page_shift) * 4 + 16 * (lane & 3);
         const uint8_t* const scale_pool = lane < 4 ? pool.k : pool.v;
         // Keys (and both scales) of a step, then its values: a group of copies each, empty behind the last step.
-        uint64_t rows_at = 0;
-        bool there = false;
+        uint64_t rows_at[kHalves] = {};
+        bool there[kHalves] = {};
         auto copy_keys = [&](uint32_t n) {
             look_up(n);
-            const uint32_t page = n < n_steps ? page_ids[warp][n % 64] : ~0u, slot = (pos0 + n * kBlock) & slots, in_ring = n % D * R::kBytes;
-            there = page < pool.n_pages;
-            if (there) {
-                const uint64_t page_at = page * pool.page_bytes;
-                rows_at = page_at + head_at + slot * pool.row_bytes;
-                const uint8_t* from = pool.k + rows_at;
+            const uint32_t in_ring = n % D * R::kBytes;
 #pragma unroll
-                for (uint32_t i = 0; i < kPieces / 2; ++i) async::cp_async_16(key_to + in_ring + i * (32 / kPieces) * R::kKeyPitch, from + 512 * i);
-                if (FMT == BC_I8 && lane < 8) async::cp_async_16(ring_at + in_ring + R::kScales + 16 * lane, scale_pool + page_at + scales_at + slot * 4);
+            for (uint32_t h = 0; h < kHalves; ++h) {
+                const uint32_t page = n < n_steps ? page_ids[warp][(n * kHalves + h) % 64] : kNoSlot, slot = (pos0 + n * kBlock + h * kHalf) & slots;
+                there[h] = page < pool.n_pages;
+                if (there[h]) {
+                    const uint64_t page_at = page * pool.page_bytes;
+                    rows_at[h] = page_at + head_at + slot * pool.row_bytes;
+                    const uint8_t* from = pool.k + rows_at[h];
+#pragma unroll
+                    for (uint32_t i = 0; i < kPieces / 2; ++i) async::cp_async_16(key_to + in_ring + (h * kHalf + i * (32 / kPieces)) * R::kKeyPitch, from + 512 * i);
+                    if (FMT == BC_I8 && lane < 8)
+                        async::cp_async_16(ring_at + in_ring + R::kScales + h * 4 * kHalf + (lane >> 2) * 4 * kStep + 16 * (lane & 3), scale_pool + page_at + scales_at + slot * 4);
+                }
             }
             async::cp_async_commit();
         };
         auto copy_values = [&](uint32_t n) {  // behind the same step's copy_keys
-            if (there) {
-                const uint8_t* from = pool.v + rows_at;
 #pragma unroll
-                for (uint32_t i = 0; i < kPieces / 2; ++i) async::cp_async_16(value_to + n % D * R::kBytes + i * (32 / kPieces) * R::kValuePitch, from + 512 * i);
-            }
+            for (uint32_t h = 0; h < kHalves; ++h)
+                if (there[h]) {
+                    const uint8_t* from = pool.v + rows_at[h];
+#pragma unroll
+                    for (uint32_t i = 0; i < kPieces / 2; ++i)
+                        async::cp_async_16(value_to + n % D * R::kBytes + (h * kHalf + i * (32 / kPieces)) * R::kValuePitch, from + 512 * i);
+                }
             async::cp_async_commit();
         };
 #pragma unroll
@@ -333,98 +346,99 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
         }
         for (uint32_t n = 0; n < n_steps; ++n) {
             const uint8_t* const here = ring + n % D * R::kBytes;
-            const bool good = page_ids[warp][n % 64] < pool.n_pages;  // a page that the pool does not have holds nothing
+            // Positions of the step that exist, from its first on; halves whose page the pool does not have hold nothing.
+            const uint32_t left = pos_end - (pos0 + n * kBlock);
+            uint32_t missing = 0;
+#pragma unroll
+            for (uint32_t h = 0; h < kHalves; ++h) missing |= page_ids[warp][(n * kHalves + h) % 64] >= pool.n_pages ? 1u << h : 0u;
             async::cp_async_wait<2 * D - 1>();
             __syncwarp();  // everyone's copies of the keys
-            float x[4];  // scores of positions 2t, 2t + 1, 8 + 2t, 9 + 2t for query head g
-            float2 dk[2], dv[2];
-            if (good) {
-                if constexpr (FMT == BC_F16) {
-                    float s[2][4];
+            // Scores of positions 16h + 2t + (i & 1) + 8 (i >> 1), x[4h + i], for query head g.
+            constexpr int kTilesOfKeys = 2 * kHalves, kScores = 4 * kHalves;
+            float x[kScores];
+            float2 dk[kTilesOfKeys], dv[kTilesOfKeys];
+            if constexpr (FMT == BC_F16) {
+                float s[kTilesOfKeys][4];
 #pragma unroll
-                    for (int c = 0; c < kWords / 8; ++c) {  // 64 bytes of a key: 32 elements
-                        uint4 kw[2];
+                for (int c = 0; c < kWords / 8; ++c) {  // 64 bytes of a key: 32 elements
+                    const uint4 f0 = q_frag[2 * c * 32 + lane], f1 = q_frag[(2 * c + 1) * 32 + lane];
+                    uint4 kw[kTilesOfKeys];
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) kw[j] = *reinterpret_cast<const uint4*>(here + (8 * j + g) * R::kKeyPitch + 64 * c + 16 * t);
-                        const uint4 f0 = q_frag[2 * c * 32 + lane], f1 = q_frag[(2 * c + 1) * 32 + lane];
+                    for (int j = 0; j < kTilesOfKeys; ++j) kw[j] = *reinterpret_cast<const uint4*>(here + (8 * j + g) * R::kKeyPitch + 64 * c + 16 * t);
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
+                    for (int j = 0; j < kTilesOfKeys; ++j) {
+                        if (c == 0)
+                            mma_f16_new(s[j], f0.x, f0.y, f0.z, f0.w, kw[j].x, kw[j].y);
+                        else
+                            mma_f16(s[j], f0.x, f0.y, f0.z, f0.w, kw[j].x, kw[j].y);
+                    }
+#pragma unroll
+                    for (int j = 0; j < kTilesOfKeys; ++j) mma_f16(s[j], f1.x, f1.y, f1.z, f1.w, kw[j].z, kw[j].w);
+                }
+#pragma unroll
+                for (int j = 0; j < kTilesOfKeys; ++j) {
+                    x[2 * j] = s[j][0] + s[j][2];
+                    x[2 * j + 1] = s[j][1] + s[j][3];
+                }
+            } else {
+                constexpr int kSets = PACKED ? 1 : 2;
+                uint32_t s[kTilesOfKeys][kSets][4];
+#pragma unroll
+                for (int c = 0; c < kWords / 8; ++c) {  // 64 bytes of a key: 64 elements
+                    uint4 kw[kTilesOfKeys];
+#pragma unroll
+                    for (int j = 0; j < kTilesOfKeys; ++j) kw[j] = *reinterpret_cast<const uint4*>(here + (8 * j + g) * R::kKeyPitch + 64 * c + 16 * t);
+#pragma unroll
+                    for (int m = 0; m < kSets; ++m) {
+                        const uint4 f0 = q_frag[(m * (kKSteps / 2) + 2 * c) * 32 + lane], f1 = q_frag[(m * (kKSteps / 2) + 2 * c + 1) * 32 + lane];
+#pragma unroll
+                        for (int j = 0; j < kTilesOfKeys; ++j) {
                             if (c == 0)
-                                mma_f16_new(s[j], f0.x, f0.y, f0.z, f0.w, kw[j].x, kw[j].y);
+                                mma_i8_new(s[j][m], f0, kw[j].x, kw[j].y, begin_sums[2 * m], begin_sums[2 * m + 1]);
                             else
-                                mma_f16(s[j], f0.x, f0.y, f0.z, f0.w, kw[j].x, kw[j].y);
+                                mma_i8(s[j][m], f0, kw[j].x, kw[j].y);
                         }
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) mma_f16(s[j], f1.x, f1.y, f1.z, f1.w, kw[j].z, kw[j].w);
+                        for (int j = 0; j < kTilesOfKeys; ++j) mma_i8(s[j][m], f1, kw[j].z, kw[j].w);
                     }
+                }
+                // The digits' sums together: two here, the other two in the lane of the row four on, or here too.
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        x[2 * j] = s[j][0] + s[j][2];
-                        x[2 * j + 1] = s[j][1] + s[j][3];
+                for (int i = 0; i < kScores; ++i) {
+                    const int j = i >> 1, k = i & 1;
+                    x[i] = fmaf(__uint_as_float(s[j][0][k]) - 12582912.f, 256.f, __uint_as_float(s[j][0][k + 2]) - 12582912.f);
+                    if constexpr (PACKED) {
+                        x[i] *= g < 4 ? 65536.f : 1.f;
+                        x[i] += __shfl_xor_sync(0xffffffffu, x[i], 16);
+                    } else {
+                        x[i] = fmaf(x[i], 65536.f, fmaf(__uint_as_float(s[j][1][k]) - 12582912.f, 256.f, __uint_as_float(s[j][1][k + 2]) - 12582912.f));
                     }
-                } else {
-                    uint32_t s[2][PACKED ? 1 : 2][4];
+                }
+                const float* scales = reinterpret_cast<const float*>(here + R::kScales);
 #pragma unroll
-                    for (int c = 0; c < kWords / 8; ++c) {  // 64 bytes of a key: 64 elements
-                        uint4 kw[2];
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) kw[j] = *reinterpret_cast<const uint4*>(here + (8 * j + g) * R::kKeyPitch + 64 * c + 16 * t);
-#pragma unroll
-                        for (int m = 0; m < (PACKED ? 1 : 2); ++m) {
-                            const uint4 f0 = q_frag[(m * (kKSteps / 2) + 2 * c) * 32 + lane], f1 = q_frag[(m * (kKSteps / 2) + 2 * c + 1) * 32 + lane];
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                if (c == 0)
-                                    mma_i8_new(s[j][m], f0, kw[j].x, kw[j].y, begin_sums[2 * m], begin_sums[2 * m + 1]);
-                                else
-                                    mma_i8(s[j][m], f0, kw[j].x, kw[j].y);
-                            }
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) mma_i8(s[j][m], f1, kw[j].z, kw[j].w);
-                        }
-                    }
-                    // The digits' sums together: two here, the other two in the lane of the row four on, or here too.
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int j = i >> 1, k = i & 1;
-                        x[i] = fmaf(__uint_as_float(s[j][0][k]) - 12582912.f, 256.f, __uint_as_float(s[j][0][k + 2]) - 12582912.f);
-                        if constexpr (PACKED) {
-                            x[i] *= g < 4 ? 65536.f : 1.f;
-                            x[i] += __shfl_xor_sync(0xffffffffu, x[i], 16);
-                        } else {
-                            x[i] = fmaf(x[i], 65536.f, fmaf(__uint_as_float(s[j][1][k]) - 12582912.f, 256.f, __uint_as_float(s[j][1][k + 2]) - 12582912.f));
-                        }
-                    }
-                    const float* scales = reinterpret_cast<const float*>(here + R::kScales);
-                    dk[0] = *reinterpret_cast<const float2*>(scales + 2 * t);
-                    dk[1] = *reinterpret_cast<const float2*>(scales + 8 + 2 * t);
-                    dv[0] = *reinterpret_cast<const float2*>(scales + kStep + 2 * t);
-                    dv[1] = *reinterpret_cast<const float2*>(scales + kStep + 8 + 2 * t);
+                for (int j = 0; j < kTilesOfKeys; ++j) {
+                    dk[j] = *reinterpret_cast<const float2*>(scales + 8 * j + 2 * t);
+                    dv[j] = *reinterpret_cast<const float2*>(scales + kStep + 8 * j + 2 * t);
                 }
             }
             __syncwarp();  // the keys have been read
             copy_keys(n + D);
-            if (!good) {
-                if (lane == 0) leave_fault(pool, kFaultPage);
-                copy_values(n + D);
-                continue;
-            }
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                x[2 * j] *= factor_q;
-                x[2 * j + 1] *= factor_q;
-                if (FMT == BC_I8) {
-                    x[2 * j] *= dk[j].x;
-                    x[2 * j + 1] *= dk[j].y;
-                }
+            for (int i = 0; i < kScores; ++i) {
+                x[i] *= factor_q;
+                if (FMT == BC_I8) x[i] *= i & 1 ? dk[i >> 1].y : dk[i >> 1].x;
             }
-            const uint32_t left = n_keys - (pos0 + n * kBlock);  // positions of the step that exist, if fewer than 16
-            if (left < kStep) {
+            const bool some_unseen = left < kStep || missing;  // uniform
+            auto seen = [&](int i) { return 16 * (i >> 2) + 2 * t + (i & 1) + 8 * (i >> 1 & 1) < left && !(missing >> (i >> 2) & 1); };
+            if (some_unseen) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (2 * t + (i & 1) + 8 * (i >> 1) >= left) x[i] = -INFINITY;
+                for (int i = 0; i < kScores; ++i)
+                    if (!seen(i)) x[i] = -INFINITY;
+                if (missing & ((left + kHalf - 1) / kHalf >= 2 ? 3u : 1u) && lane == 0) leave_fault(pool, kFaultPage);
             }
-            float most = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+            float most = x[0];
+#pragma unroll
+            for (int i = 1; i < kScores; ++i) most = fmaxf(most, x[i]);
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
             const float now = fmaxf(top, most);
@@ -434,24 +448,22 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
             top = now;
             float total_step = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < kScores; ++i) {
                 x[i] = exp2_fast(x[i] - down);  // the sums are lifted alike
                 total_step += x[i];
             }
             total_p = total_p * factor + total_step;
             if constexpr (FMT == BC_I8) {
-                float largest = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float d = i & 1 ? dv[i >> 1].y : dv[i >> 1].x;
-                    x[i] *= d;
-                }
-                if (left < kStep) {  // scales behind the last position may be anything
+                for (int i = 0; i < kScores; ++i) x[i] *= i & 1 ? dv[i >> 1].y : dv[i >> 1].x;
+                if (some_unseen) {  // scales behind the last position may be anything
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (2 * t + (i & 1) + 8 * (i >> 1) >= left) x[i] = 0.f;
+                    for (int i = 0; i < kScores; ++i)
+                        if (!seen(i)) x[i] = 0.f;
                 }
-                largest = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+                float largest = fabsf(x[0]);
+#pragma unroll
+                for (int i = 1; i < kScores; ++i) largest = fmaxf(largest, fabsf(x[i]));
                 largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
                 largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
                 if (moved || largest > 32768.f * unit) {  // weights of 2^15 units at most: halves end at 2^16
@@ -464,68 +476,86 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
                     factor *= before * inverse_unit;
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] *= inverse_unit;
+                for (int i = 0; i < kScores; ++i) x[i] *= inverse_unit;
             }
             const float2 f = make_float2(__shfl_sync(0xffffffffu, factor, 8 * t), __shfl_sync(0xffffffffu, factor, 8 * t + 4));  // of columns 2t and 2t + 1
-            uint32_t hi0, lo0, hi1, lo1;
-            split_half2(x[0], x[1], hi0, lo0);
-            split_half2(x[2], x[3], hi1, lo1);
-            if (PACKED && g >= 4) {
-                hi0 = lo0;
-                hi1 = lo1;
+            uint32_t hi[2 * kHalves], lo[2 * kHalves];
+#pragma unroll
+            for (int j = 0; j < kTilesOfKeys; ++j) {
+                split_half2(x[2 * j], x[2 * j + 1], hi[j], lo[j]);
+                if (PACKED && g >= 4) hi[j] = lo[j];
             }
             async::cp_async_wait<2 * D - 1>();
             __syncwarp();  // everyone's copies of the values
-            // Position 2t + (i & 1) + 8 (i >> 1) of the step, i = 0 .. 3; a lane's 8 elements 8g .. of every 64.
-            uint32_t vw[4][kWords / 4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint8_t* at_row = here + R::kValues + (2 * t + (i & 1) + 8 * (i >> 1)) * R::kValuePitch;
-#pragma unroll
-                for (int c = 0; c < HD / 64; ++c) {
-                    if constexpr (FMT == BC_F16)
-                        *reinterpret_cast<uint4*>(&vw[i][4 * c]) = *reinterpret_cast<const uint4*>(at_row + 128 * c + 16 * g);
-                    else
-                        *reinterpret_cast<uint2*>(&vw[i][2 * c]) = *reinterpret_cast<const uint2*>(at_row + 64 * c + 8 * g);
-                }
-            }
-            __syncwarp();  // the values have been read
-            copy_values(n + D);
-            // A step's sums, from zero, join the others rounded.
-            auto product = [&](int tile, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+            // A step's sums, from zero, join the others rounded: of 16 elements, by the fragments of both halves.
+            auto product = [&](int tile, const uint32_t (&a)[kHalves][4]) {
                 float d[4];
                 if (PACKED) {
-                    mma_f16_new(d, a0, a1, a2, a3, hi0, hi1);
+                    mma_f16_new(d, a[0][0], a[0][1], a[0][2], a[0][3], hi[0], hi[1]);
+                    if (kHalves == 2) mma_f16(d, a[kHalves - 1][0], a[kHalves - 1][1], a[kHalves - 1][2], a[kHalves - 1][3], hi[2 * kHalves - 2], hi[2 * kHalves - 1]);
                 } else {
-                    mma_f16_new(d, a0, a1, a2, a3, lo0, lo1);
-                    mma_f16(d, a0, a1, a2, a3, hi0, hi1);
+                    mma_f16_new(d, a[0][0], a[0][1], a[0][2], a[0][3], lo[0], lo[1]);
+                    if (kHalves == 2) mma_f16(d, a[kHalves - 1][0], a[kHalves - 1][1], a[kHalves - 1][2], a[kHalves - 1][3], lo[2 * kHalves - 2], lo[2 * kHalves - 1]);
+                    mma_f16(d, a[0][0], a[0][1], a[0][2], a[0][3], hi[0], hi[1]);
+                    if (kHalves == 2) mma_f16(d, a[kHalves - 1][0], a[kHalves - 1][1], a[kHalves - 1][2], a[kHalves - 1][3], hi[2 * kHalves - 2], hi[2 * kHalves - 1]);
                 }
                 o[tile][0] = fma2(o[tile][0], f, make_float2(d[0], d[1]));
                 o[tile][1] = fma2(o[tile][1], f, make_float2(d[2], d[3]));
             };
-            if constexpr (FMT == BC_F16) {
-                if (left < kStep) {  // elements behind the last position may be anything
+            // Position 16h + 2t + (i & 1) + 8 (i >> 1) of the step, i = 0 .. 3; a lane's 8 elements 8g .. of every 64.
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (2 * t + (i & 1) + 8 * (i >> 1) >= left) {
+            for (int c = 0; c < HD / 64; ++c) {
+                constexpr int kOfRow = FMT == BC_F16 ? 4 : 2;  // words
+                uint32_t vw[kHalves][4][kOfRow];
 #pragma unroll
-                            for (int w = 0; w < kWords / 4; ++w) vw[i][w] = 0;
+                for (int h = 0; h < (int)kHalves; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint8_t* from = here + R::kValues + (16 * h + 2 * t + (i & 1) + 8 * (i >> 1)) * R::kValuePitch;
+                        if constexpr (FMT == BC_F16) {
+                            const uint4 w = *reinterpret_cast<const uint4*>(from + 128 * c + 16 * g);
+                            vw[h][i][0] = w.x, vw[h][i][1] = w.y, vw[h][i][kOfRow - 2] = w.z, vw[h][i][kOfRow - 1] = w.w;
+                            if (some_unseen) {  // elements behind the last position may be anything
+#pragma unroll
+                                for (int k = 0; k < kOfRow; ++k)
+                                    if (!seen(4 * h + i)) vw[h][i][k] = 0;
+                            }
+                        } else {
+                            const uint2 w = *reinterpret_cast<const uint2*>(from + 64 * c + 8 * g);
+                            vw[h][i][0] = w.x, vw[h][i][1] = w.y;
+                        }
+                    }
+                if (c == HD / 64 - 1) {
+                    __syncwarp();  // the values have been read
+                    copy_values(n + D);
+                }
+                if constexpr (FMT == BC_F16) {
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {  // elements 2w, 2w + 1 of the lane's: rows g and g + 8 of a tile
+                        uint32_t a[kHalves][4];
+#pragma unroll
+                        for (int h = 0; h < (int)kHalves; ++h) {
+                            a[h][0] = __byte_perm(vw[h][0][w], vw[h][1][w], 0x5410);
+                            a[h][1] = __byte_perm(vw[h][0][w], vw[h][1][w], 0x7632);
+                            a[h][2] = __byte_perm(vw[h][2][w], vw[h][3][w], 0x5410);
+                            a[h][3] = __byte_perm(vw[h][2][w], vw[h][3][w], 0x7632);
+                        }
+                        product(4 * c + w, a);
+                    }
+                } else {
+#pragma unroll
+                    for (int w = 0; w < 2; ++w)  // elements 4w .. 4w + 3 of the lane's: two tiles
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            uint32_t a[kHalves][4];  // elements 2e and 2e + 1 of two positions
+#pragma unroll
+                            for (int h = 0; h < (int)kHalves; ++h) {
+                                unpack_i8(__byte_perm(vw[h][0][w], vw[h][1][w], e ? 0x7362 : 0x5140), a[h][0], a[h][1]);
+                                unpack_i8(__byte_perm(vw[h][2][w], vw[h][3][w], e ? 0x7362 : 0x5140), a[h][2], a[h][3]);
+                            }
+                            product(4 * c + 2 * w + e, a);
                         }
                 }
-#pragma unroll
-                for (int w = 0; w < kWords / 4; ++w)  // elements 2w, 2w + 1 of the lane's: rows g and g + 8 of a tile
-                    product(w, __byte_perm(vw[0][w], vw[1][w], 0x5410), __byte_perm(vw[0][w], vw[1][w], 0x7632), __byte_perm(vw[2][w], vw[3][w], 0x5410),
-                            __byte_perm(vw[2][w], vw[3][w], 0x7632));
-            } else {
-#pragma unroll
-                for (int w = 0; w < kWords / 4; ++w)  // elements 4w .. 4w + 3 of the lane's: two tiles
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t a0, a1, a2, a3;  // elements 2h and 2h + 1 of two positions
-                        unpack_i8(__byte_perm(vw[0][w], vw[1][w], h ? 0x7362 : 0x5140), a0, a1);
-                        unpack_i8(__byte_perm(vw[2][w], vw[3][w], h ? 0x7362 : 0x5140), a2, a3);
-                        product(2 * w + h, a0, a1, a2, a3);
-                    }
             }
         }
         async::cp_async_wait<0>();
@@ -649,9 +679,19 @@ constexpr size_t token_smem_bytes() {
     return (size_t)(HD / 16) * 32 * 16 + (rings > sums ? rings : sums);
 }
 
+uint32_t block_of(const KvPool& pool) {
+    const bool half = pool.format == BC_F16;
+    switch (pool.head_dim) {
+        case 64: return half ? Ring<BC_F16, 64>::kBlock : Ring<BC_I8, 64>::kBlock;
+        case 128: return half ? Ring<BC_F16, 128>::kBlock : Ring<BC_I8, 128>::kBlock;
+        default: return half ? Ring<BC_F16, 256>::kBlock : Ring<BC_I8, 256>::kBlock;
+    }
+}
+
 // CTAs of a launch: no more than the blocks that the tables could hold.
 uint32_t token_ctas(const KvPool& pool, const KvRows& rows) {
-    const uint64_t most = (uint64_t)rows.n_rows * pool.n_kv_heads * ((((uint64_t)rows.max_pages << pool.page_shift) + kBlock - 1) / kBlock);
+    const uint32_t block = block_of(pool);
+    const uint64_t most = (uint64_t)rows.n_rows * pool.n_kv_heads * ((((uint64_t)rows.max_pages << pool.page_shift) + block - 1) / block);
     uint64_t ctas = (uint64_t)sm_count() * ctas_per_sm(pool.head_dim);
     if (ctas > kMostCtas) ctas = kMostCtas;
     return (uint32_t)(ctas > most ? most : ctas);
