@@ -129,8 +129,24 @@ __device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
     return v;
 }
 
+// Rows of sums that a warp leaves at a unit's end.
+template <bool PACKED>
+constexpr uint32_t sum_rows() { return PACKED ? kRows / 2 : kRows; }
+template <int FMT, int HD>
+constexpr size_t rings_bytes() { return (size_t)kWarps * Ring<FMT, HD>::kSteps * Ring<FMT, HD>::kBytes; }
+template <int HD, bool PACKED>
+constexpr size_t sums_bytes() { return (size_t)kWarps * sum_rows<PACKED>() * (HD + 4) * 4; }
 // CTAs that an SM holds, by their registers: heads of 256 take more than half (131072 positions of four 8-bit heads 60 us, 86 with two CTAs and spills).
 constexpr uint32_t ctas_per_sm(uint32_t head_dim) { return head_dim == 256 ? 1 : 2; }
+
+// Whether the sums have room beside the rings: the next unit's copies are then under way while a unit ends.
+template <int FMT, int HD, bool PACKED>
+constexpr bool sums_beside() { return (size_t)HD * 32 + rings_bytes<FMT, HD>() + sums_bytes<HD, PACKED>() <= 228 * 1024 / ctas_per_sm(HD) - 4096; }
+template <int FMT, int HD, bool PACKED>
+constexpr size_t token_smem_bytes() {
+    constexpr size_t rings = rings_bytes<FMT, HD>(), sums = sums_bytes<HD, PACKED>();
+    return (size_t)HD * 32 + (sums_beside<FMT, HD, PACKED>() ? rings + sums : rings > sums ? rings : sums);
+}
 
 // Registers of a warp's step of keys, and of values: 32-bit words per lane.
 template <int FMT, int HD>
@@ -145,8 +161,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
     constexpr int kKSteps = HD / 16, kTiles = HD / 16;
     extern __shared__ __align__(16) uint8_t token_smem[];
     uint4* q_frag = reinterpret_cast<uint4*>(token_smem);                                    // [kKSteps][32]
-    uint8_t* rings = token_smem + kKSteps * 32 * 16;                                         // [kWarps][D] steps; at a unit's end:
-    float* sums = reinterpret_cast<float*>(rings);                                           // [kWarps][kRows][kSumPitch]
+    uint8_t* rings = token_smem + kKSteps * 32 * 16;                                         // [kWarps][D] steps
+    constexpr bool kBeside = sums_beside<FMT, HD, PACKED>();
+    constexpr uint32_t kSumRows = sum_rows<PACKED>();
+    float* sums = reinterpret_cast<float*>(rings + (kBeside ? rings_bytes<FMT, HD>() : 0));  // [kWarps][kSumRows][kSumPitch], or in the rings' place
     __shared__ float2 stats[kWarps * kRows];
     __shared__ float q_factor[kRows];
     __shared__ uint32_t page_ids[kWarps][64];
@@ -191,22 +209,104 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
     }
     PartsHead cut{0, 0, 0, 0};
 
-    while (at < end) {
+    // The unit at `at`, and the blocks of it that are this CTA's. Rows of a head are neighbours.
+    struct Work {
+        uint32_t seq, row, head, n_keys, block0, blocks, all_blocks;
+    };
+    auto find = [&]() {
+        Work w;
         Seq sq = seq_at(pool, rows, seq, p.most, kBlock);
         while (base + blocks_of(pool, sq) <= at) {  // sequences without rows have no blocks
             base += blocks_of(pool, sq);
             sq = seq_at(pool, rows, ++seq, p.most, kBlock);
         }
-        // The unit, and the blocks of it that are this CTA's. Rows of a head are neighbours.
         const uint64_t in_seq = at - base;
-        const uint32_t which = (uint32_t)(in_seq / sq.blocks), block0 = (uint32_t)(in_seq % sq.blocks);
-        const uint32_t blocks = (uint32_t)min((uint64_t)(sq.blocks - block0), end - at);
-        const uint32_t head = which / sq.n, row = sq.row0 + which % sq.n;
-        const uint32_t back = sq.end - row;  // the row's distance from the end: it sees positions 0 .. len - back
+        const uint32_t which = (uint32_t)(in_seq / sq.blocks);
+        w.seq = seq;
+        w.block0 = (uint32_t)(in_seq % sq.blocks);
+        w.blocks = (uint32_t)min((uint64_t)(sq.blocks - w.block0), end - at);
+        w.all_blocks = sq.blocks;
+        w.head = which / sq.n;
+        w.row = sq.row0 + which % sq.n;
+        const uint32_t back = sq.end - w.row;  // the row's distance from the end: it sees positions 0 .. len - back
         const uint32_t held = min((uint64_t)sq.len, (uint64_t)rows.max_pages << pool.page_shift);
-        const uint32_t n_keys = back <= sq.len ? min(sq.len - back + 1, held) : 0;
+        w.n_keys = back <= sq.len ? min(sq.len - back + 1, held) : 0;
         if (held < sq.len) leave_fault(pool, kFaultTable);
+        return w;
+    };
 
+    // What the copies go by: the warp's steps of a unit are one block apart, step n has positions pos0 + n * kBlock on.
+    const uint32_t slots = (1u << pool.page_shift) - 1;
+    uint8_t* const ring = rings + warp * (D * R::kBytes);
+    constexpr uint32_t kPieces = R::kRowBytes / 16;  // of a row; a lane brings every 32nd of the step's
+    const uint32_t ring_at = async::smem_u32(ring), key_to = ring_at + lane / kPieces * R::kKeyPitch + lane % kPieces * 16,
+                   value_to = ring_at + R::kValues + lane / kPieces * R::kValuePitch + lane % kPieces * 16;
+    const uint8_t* const scale_pool = lane < 4 ? pool.k : pool.v;
+    const uint32_t* table = nullptr;
+    uint32_t pos0 = 0, pos_end = 0, n_steps = 0;
+    uint64_t head_at = 0, scales_at = 0;
+    auto aim = [&](const Work& w) {
+        table = rows.table + (uint64_t)w.seq * rows.max_pages;
+        pos0 = w.block0 * kBlock + warp * kStep;
+        pos_end = min((w.block0 + w.blocks) * kBlock, w.n_keys);
+        n_steps = pos0 < pos_end ? (pos_end - pos0 + kBlock - 1) / kBlock : 0;
+        head_at = (uint64_t)(w.head << pool.page_shift) * pool.row_bytes + 16 * lane;
+        scales_at = (uint64_t)(pool.n_kv_heads << pool.page_shift) * pool.row_bytes + (uint64_t)(w.head << pool.page_shift) * 4 + 16 * (lane & 3);
+    };
+    // The pages of a step's halves, 32 halves looked up at a time, by the copies of the first of them, before anything asks. A half behind the
+    // last position has none.
+    constexpr uint32_t kAtOnce = 32 / kHalves;  // steps
+    auto look_up = [&](uint32_t n) {
+        if (n % kAtOnce == 0 && n < n_steps) {
+            const uint32_t at = pos0 + (n + lane / kHalves) * kBlock + lane % kHalves * kHalf;
+            page_ids[warp][(n * kHalves + lane) % 64] = at < pos_end ? table[at >> pool.page_shift] : kNoSlot;
+            __syncwarp();
+        }
+    };
+    // Keys (and both scales) of a step, then its values: a group of copies each, empty behind the last step.
+    uint64_t rows_at[kHalves] = {};
+    bool there[kHalves] = {};
+    auto copy_keys = [&](uint32_t n) {
+        look_up(n);
+        const uint32_t in_ring = n % D * R::kBytes;
+#pragma unroll
+        for (uint32_t h = 0; h < kHalves; ++h) {
+            const uint32_t page = n < n_steps ? page_ids[warp][(n * kHalves + h) % 64] : kNoSlot, slot = (pos0 + n * kBlock + h * kHalf) & slots;
+            there[h] = page < pool.n_pages;
+            if (there[h]) {
+                const uint64_t page_at = page * pool.page_bytes;
+                rows_at[h] = page_at + head_at + slot * pool.row_bytes;
+                const uint8_t* from = pool.k + rows_at[h];
+#pragma unroll
+                for (uint32_t i = 0; i < kPieces / 2; ++i) async::cp_async_16(key_to + in_ring + (h * kHalf + i * (32 / kPieces)) * R::kKeyPitch, from + 512 * i);
+                if (FMT == BC_I8 && lane < 8)
+                    async::cp_async_16(ring_at + in_ring + R::kScales + h * 4 * kHalf + (lane >> 2) * 4 * kStep + 16 * (lane & 3), scale_pool + page_at + scales_at + slot * 4);
+            }
+        }
+        async::cp_async_commit();
+    };
+    auto copy_values = [&](uint32_t n) {  // behind the same step's copy_keys
+#pragma unroll
+        for (uint32_t h = 0; h < kHalves; ++h)
+            if (there[h]) {
+                const uint8_t* from = pool.v + rows_at[h];
+#pragma unroll
+                for (uint32_t i = 0; i < kPieces / 2; ++i)
+                    async::cp_async_16(value_to + n % D * R::kBytes + (h * kHalf + i * (32 / kPieces)) * R::kValuePitch, from + 512 * i);
+            }
+        async::cp_async_commit();
+    };
+    auto begin_copies = [&](const Work& w) {
+        aim(w);
+#pragma unroll
+        for (uint32_t n = 0; n < D; ++n) {
+            copy_keys(n);
+            copy_values(n);
+        }
+    };
+    Work w = find();
+    begin_copies(w);
+    while (true) {
         // Query fragments in the order of a lane's key elements, a warp per query head (PACKED: two). A pair of elements is a word of hi and one of
         // lo parts.
         __syncthreads();  // the previous unit's fragments and sums have been read
@@ -216,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
             uint32_t most = 0;
 #pragma unroll
             for (int i = 0; i < HD / 64; ++i) {
-                x[i] = q_head < p.group ? *reinterpret_cast<const float2*>(p.q + row * p.q_stride + (head * p.group + q_head) * p.q_head_stride + 64 * i + 2 * lane)
+                x[i] = q_head < p.group ? *reinterpret_cast<const float2*>(p.q + w.row * p.q_stride + (w.head * p.group + q_head) * p.q_head_stride + 64 * i + 2 * lane)
                                       : make_float2(0.f, 0.f);
                 most = max(most, max(__float_as_uint(x[i].x) & 0x7fffffffu, __float_as_uint(x[i].y) & 0x7fffffffu));
             }
@@ -284,66 +384,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
         float top = -INFINITY, total_p = 0.f;  // of query head g, the sum over this lane's positions
         float unit = FMT == BC_I8 ? 0.f : 1.f, inverse_unit = unit;  // the sums of query head g are counted in these
 
-        const uint32_t* table = rows.table + (uint64_t)seq * rows.max_pages;
-        const uint32_t slots = (1u << pool.page_shift) - 1;
-        // The warp's steps are one block apart: step n has positions pos0 + n * kBlock .. 15 on.
-        const uint32_t pos0 = block0 * kBlock + warp * kStep, pos_end = min((block0 + blocks) * kBlock, n_keys);
-        const uint32_t n_steps = pos0 < pos_end ? (pos_end - pos0 + kBlock - 1) / kBlock : 0;
-        uint8_t* const ring = rings + warp * (D * R::kBytes);
-        // The pages of a step's halves, 32 halves looked up at a time, by the copies of the first of them, before anything asks. A half behind the
-        // last position has none.
-        constexpr uint32_t kAtOnce = 32 / kHalves;  // steps
-        auto look_up = [&](uint32_t n) {
-            if (n % kAtOnce == 0 && n < n_steps) {
-                const uint32_t at = pos0 + (n + lane / kHalves) * kBlock + lane % kHalves * kHalf;
-                page_ids[warp][(n * kHalves + lane) % 64] = at < pos_end ? table[at >> pool.page_shift] : kNoSlot;
-                __syncwarp();
-            }
-        };
-        constexpr uint32_t kPieces = R::kRowBytes / 16;  // of a row; a lane brings every 32nd of the step's
-        const uint32_t ring_at = async::smem_u32(ring), key_to = ring_at + lane / kPieces * R::kKeyPitch + lane % kPieces * 16,
-                       value_to = ring_at + R::kValues + lane / kPieces * R::kValuePitch + lane % kPieces * 16;
-        const uint64_t head_at = (uint64_t)(head << pool.page_shift) * pool.row_bytes + 16 * lane;
-        const uint64_t scales_at = (uint64_t)(pool.n_kv_heads << pool.page_shift) * pool.row_bytes + (uint64_t)(head << pool.page_shift) * 4 + 16 * (lane & 3);
-        const uint8_t* const scale_pool = lane < 4 ? pool.k : pool.v;
-        // Keys (and both scales) of a step, then its values: a group of copies each, empty behind the last step.
-        uint64_t rows_at[kHalves] = {};
-        bool there[kHalves] = {};
-        auto copy_keys = [&](uint32_t n) {
-            look_up(n);
-            const uint32_t in_ring = n % D * R::kBytes;
-#pragma unroll
-            for (uint32_t h = 0; h < kHalves; ++h) {
-                const uint32_t page = n < n_steps ? page_ids[warp][(n * kHalves + h) % 64] : kNoSlot, slot = (pos0 + n * kBlock + h * kHalf) & slots;
-                there[h] = page < pool.n_pages;
-                if (there[h]) {
-                    const uint64_t page_at = page * pool.page_bytes;
-                    rows_at[h] = page_at + head_at + slot * pool.row_bytes;
-                    const uint8_t* from = pool.k + rows_at[h];
-#pragma unroll
-                    for (uint32_t i = 0; i < kPieces / 2; ++i) async::cp_async_16(key_to + in_ring + (h * kHalf + i * (32 / kPieces)) * R::kKeyPitch, from + 512 * i);
-                    if (FMT == BC_I8 && lane < 8)
-                        async::cp_async_16(ring_at + in_ring + R::kScales + h * 4 * kHalf + (lane >> 2) * 4 * kStep + 16 * (lane & 3), scale_pool + page_at + scales_at + slot * 4);
-                }
-            }
-            async::cp_async_commit();
-        };
-        auto copy_values = [&](uint32_t n) {  // behind the same step's copy_keys
-#pragma unroll
-            for (uint32_t h = 0; h < kHalves; ++h)
-                if (there[h]) {
-                    const uint8_t* from = pool.v + rows_at[h];
-#pragma unroll
-                    for (uint32_t i = 0; i < kPieces / 2; ++i)
-                        async::cp_async_16(value_to + n % D * R::kBytes + (h * kHalf + i * (32 / kPieces)) * R::kValuePitch, from + 512 * i);
-                }
-            async::cp_async_commit();
-        };
-#pragma unroll
-        for (uint32_t n = 0; n < D; ++n) {
-            copy_keys(n);
-            copy_values(n);
-        }
         for (uint32_t n = 0; n < n_steps; ++n) {
             const uint8_t* const here = ring + n % D * R::kBytes;
             // Positions of the step that exist, from its first on; halves whose page the pool does not have hold nothing.
@@ -559,40 +599,50 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
             }
         }
         async::cp_async_wait<0>();
+        const Work done = w;
+        at += done.blocks;
+        const bool more = at < end;  // uniform in the CTA
+        if (more) w = find();
+        if (kBeside && more) begin_copies(w);
 
-        // The warps' sums, joined through shared memory, in the rings' place. Tile n's rows g and g + 8 are elements 2n' and 2n' + 1 of the lane's eight.
+        // The warps' sums, joined through shared memory. Tile n's rows g and g + 8 are elements 2n' and 2n' + 1 of the lane's eight.
         total_p += __shfl_xor_sync(0xffffffffu, total_p, 1);
         total_p += __shfl_xor_sync(0xffffffffu, total_p, 2);
         if (t == 0) stats[warp * kRows + g] = make_float2(top, total_p);
         const float u0 = __shfl_sync(0xffffffffu, unit, 8 * t), u1 = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
-        __syncthreads();  // every ring has been read
+        if (!kBeside) __syncthreads();  // every ring has been read
 #pragma unroll
         for (int n = 0; n < kTiles; ++n) {
             const uint32_t d = (n / 4) * 64 + 8 * g + 2 * (n % 4);  // elements d and d + 1
-            float* to = sums + (warp * kRows + 2 * t) * kSumPitch + d;
-            *reinterpret_cast<float2*>(to) = make_float2(o[n][0].x * u0, o[n][1].x * u0);
-            *reinterpret_cast<float2*>(to + kSumPitch) = make_float2(o[n][0].y * u1, o[n][1].y * u1);
+            float2 even = make_float2(o[n][0].x * u0, o[n][1].x * u0), odd = make_float2(o[n][0].y * u1, o[n][1].y * u1);
+            if (PACKED) {  // the lower halves' sums, two lanes on
+                even.x += __shfl_xor_sync(0xffffffffu, even.x, 2);
+                even.y += __shfl_xor_sync(0xffffffffu, even.y, 2);
+                odd.x += __shfl_xor_sync(0xffffffffu, odd.x, 2);
+                odd.y += __shfl_xor_sync(0xffffffffu, odd.y, 2);
+            }
+            if (!PACKED || t < 2) {
+                float* to = sums + (warp * kSumRows + 2 * t) * kSumPitch + d;
+                *reinterpret_cast<float2*>(to) = even;
+                *reinterpret_cast<float2*>(to + kSumPitch) = odd;
+            }
         }
         __syncthreads();
-        const bool begins = block0 == 0, ends = block0 + blocks == sq.blocks;
+        const bool begins = done.block0 == 0, ends = done.block0 + done.blocks == done.all_blocks;
         const uint32_t slot = 2 * blockIdx.x + (begins ? 1 : 0);
-        for (uint32_t i = tid; i < p.group * (HD / 4); i += kThreads) {
-            const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4;
+        for (uint32_t quad = tid; quad < p.group * (HD / 4); quad += kThreads) {
+            const uint32_t r = quad / (HD / 4), d = quad % (HD / 4) * 4;
             float most = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) most = fmaxf(most, stats[w * kRows + r].x);
+            for (int i = 0; i < kWarps; ++i) most = fmaxf(most, stats[i * kRows + r].x);
             const float shift = most == -INFINITY ? 0.f : most;
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
             float sum_p = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float2 st = stats[w * kRows + r];
+            for (int i = 0; i < kWarps; ++i) {
+                const float2 st = stats[i * kRows + r];
                 const float weight = st.x == -INFINITY ? 0.f : exp2f(st.x - shift);
-                float4 v = *reinterpret_cast<const float4*>(sums + (w * kRows + r) * kSumPitch + d);
-                if (PACKED) {  // the lower halves' sums
-                    const float4 l = *reinterpret_cast<const float4*>(sums + (w * kRows + r + 4) * kSumPitch + d);
-                    v = make_float4(v.x + l.x, v.y + l.y, v.z + l.z, v.w + l.w);
-                }
+                const float4 v = *reinterpret_cast<const float4*>(sums + (i * kSumRows + r) * kSumPitch + d);
                 if (st.x != -INFINITY) {
                     sum.x += weight * v.x;
                     sum.y += weight * v.y;
@@ -604,7 +654,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
             if (begins && ends) {
                 // A row that sees nothing is zeros.
                 const float inverse = most == -INFINITY && sum_p == 0.f ? 0.f : 1.f / sum_p;
-                *reinterpret_cast<float4*>(p.out + (uint64_t)row * p.n_heads * HD + (head * p.group + r) * HD + d) =
+                *reinterpret_cast<float4*>(p.out + (uint64_t)done.row * p.n_heads * HD + (done.head * p.group + r) * HD + d) =
                     make_float4(sum.x * inverse, sum.y * inverse, sum.z * inverse, sum.w * inverse);
             } else {
                 *reinterpret_cast<float4*>(p.parts + ((uint64_t)slot * kRows + r) * HD + d) = sum;
@@ -613,70 +663,89 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
         }
         if (begins && !ends) {
             // The CTA whose run holds the unit's last block: run c is [total c / runs, total (c + 1) / runs).
-            const uint64_t last_block = at + sq.blocks - 1;
+            const uint64_t last_block = at - done.blocks + done.all_blocks - 1;
             uint32_t last = (uint32_t)(last_block * runs / total);
             while (total * (last + 1) / runs <= last_block) ++last;
             while (total * last / runs > last_block) --last;
-            cut = PartsHead{row, head, last, 0};
+            cut = PartsHead{done.row, done.head, last, 0};
         }
-        at += blocks;
+        if (!more) break;
+        if (!kBeside) {
+            __syncthreads();  // the sums have been read
+            begin_copies(w);
+        }
     }
     if (tid == 0) heads[blockIdx.x] = cut;
 }
 
-// Joins the parts of a unit that begins in CTA c's run and ends in a later one's: a warp per query head.
+// Joins the parts of a unit that begins in CTA c's run and ends in a later one's: a CTA per query head, whose warps take parts in turn, so that a
+// unit over many CTAs is joined in a few trips to memory.
 template <int HD>
-__global__ void __launch_bounds__(32 * kRows) attention_token_join_kernel(const float* __restrict__ parts, float* __restrict__ out, uint32_t n_heads, uint32_t group) {
-    constexpr int kPairs = HD / 64;
+__global__ void __launch_bounds__(256) attention_token_join_kernel(const float* __restrict__ parts, float* __restrict__ out, uint32_t n_heads, uint32_t group) {
+    constexpr int kPairs = HD / 64, kAtOnce = 4;
+    __shared__ float2 warp_stats[8];
+    __shared__ float warp_sums[8][HD];
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t lane = threadIdx.x & 31, r = threadIdx.x >> 5, c = blockIdx.x;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.y, c = blockIdx.x;
     const PartsHead cut = reinterpret_cast<const PartsHead*>(parts + (uint64_t)2 * kMostCtas * kRows * (HD + 2))[c];
-    if (cut.last == 0 || r >= group) return;
+    if (cut.last == 0) return;
     const float2* stats = reinterpret_cast<const float2*>(parts + (uint64_t)2 * kMostCtas * kRows * HD);
     const uint32_t n = cut.last - c + 1;
-    auto slot_of = [&](uint32_t i) { return 2 * (c + i) + (i == 0 ? 1 : 0); };
-    float top = -INFINITY;
-    for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, stats[slot_of(i) * kRows + r].x);
-    top = warp_max(top);
-    const float shift = top == -INFINITY ? 0.f : top;
-    float total = 0.f;
+    float top = -INFINITY, total = 0.f;
     float2 sum[kPairs];
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) sum[i] = make_float2(0.f, 0.f);
-    for (uint32_t i0 = 0; i0 < n; i0 += 32) {
-        float2 st = make_float2(-INFINITY, 0.f);
-        if (i0 + lane < n) st = stats[slot_of(i0 + lane) * kRows + r];
-        const float weight = st.x == -INFINITY ? 0.f : exp2f(st.x - shift);
-        total += weight * st.y;
-        const uint32_t many = min(32u, n - i0);
-#pragma unroll 4
-        for (uint32_t i = 0; i < many; ++i) {
-            const float w = __shfl_sync(0xffffffffu, weight, i);
-            const bool any = __shfl_sync(0xffffffffu, st.x, i) != -INFINITY;
-            const float2* from = reinterpret_cast<const float2*>(parts + ((uint64_t)slot_of(i0 + i) * kRows + r) * HD) + lane;
+    for (uint32_t first = warp; first < n; first += 8 * kAtOnce) {
+        float2 st[kAtOnce], v[kAtOnce][kPairs];
 #pragma unroll
-            for (int k = 0; k < kPairs; ++k) {
-                const float2 v = from[32 * k];
-                if (any) {
-                    sum[k].x += w * v.x;
-                    sum[k].y += w * v.y;
+        for (int k = 0; k < kAtOnce; ++k) {
+            const uint32_t i = first + 8 * k, at = (2 * (c + i) + (i == 0 ? 1 : 0)) * kRows + r;
+            st[k] = i < n ? stats[at] : make_float2(-INFINITY, 0.f);
+            const float2* from = reinterpret_cast<const float2*>(parts + (uint64_t)at * HD) + lane;
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j) v[k][j] = i < n ? from[32 * j] : make_float2(0.f, 0.f);
+        }
+        float now = top;
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) now = fmaxf(now, st[k].x);
+        const float shift = now == -INFINITY ? 0.f : now, fall = exp2f(top - shift);
+        top = now;
+        total *= fall;
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) sum[j] = make_float2(sum[j].x * fall, sum[j].y * fall);
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            const float weight = st[k].x == -INFINITY ? 0.f : exp2f(st[k].x - shift);
+            total += weight * st[k].y;
+            if (st[k].x != -INFINITY) {
+#pragma unroll
+                for (int j = 0; j < kPairs; ++j) {
+                    sum[j].x += weight * v[k][j].x;
+                    sum[j].y += weight * v[k][j].y;
                 }
             }
         }
     }
-    total = warp_sum(total);
-    const float inverse = top == -INFINITY && total == 0.f ? 0.f : 1.f / total;
-    float2* to = reinterpret_cast<float2*>(out + (uint64_t)cut.row * n_heads * HD + (cut.head * group + r) * HD) + lane;
+    if (lane == 0) warp_stats[warp] = make_float2(top, total);
 #pragma unroll
-    for (int k = 0; k < kPairs; ++k) to[32 * k] = make_float2(sum[k].x * inverse, sum[k].y * inverse);
-}
-
-template <int FMT, int HD>
-constexpr size_t token_smem_bytes() {
-    using R = Ring<FMT, HD>;
-    constexpr size_t rings = (size_t)kWarps * R::kSteps * R::kBytes, sums = (size_t)kWarps * kRows * (HD + 4) * 4;
-    return (size_t)(HD / 16) * 32 * 16 + (rings > sums ? rings : sums);
+    for (int j = 0; j < kPairs; ++j) *reinterpret_cast<float2*>(&warp_sums[warp][64 * j + 2 * lane]) = sum[j];
+    __syncthreads();
+    for (uint32_t d = tid; d < HD; d += 256) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = fmaxf(most, warp_stats[i].x);
+        const float shift = most == -INFINITY ? 0.f : most;
+        float all = 0.f, x = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 st = warp_stats[i];
+            const float weight = st.x == -INFINITY ? 0.f : exp2f(st.x - shift);
+            all += weight * st.y;
+            if (st.x != -INFINITY) x += weight * warp_sums[i][d];
+        }
+        out[(uint64_t)cut.row * n_heads * HD + (cut.head * group + r) * HD + d] = most == -INFINITY && all == 0.f ? 0.f : x / all;
+    }
 }
 
 uint32_t block_of(const KvPool& pool) {
@@ -699,17 +768,17 @@ uint32_t token_ctas(const KvPool& pool, const KvRows& rows) {
 
 template <int FMT, int HD, bool PACKED>
 cudaError_t launch_token_as(cudaStream_t stream, const TokenParams& p, uint32_t ctas) {
-    static_assert((token_smem_bytes<FMT, HD>() + 4096) * ctas_per_sm(HD) <= 228 * 1024, "shared memory of an SM");
-    cudaError_t e = ensure_dynamic_smem((const void*)attention_token_paged_kernel<FMT, HD, PACKED>, token_smem_bytes<FMT, HD>());
+    static_assert((token_smem_bytes<FMT, HD, PACKED>() + 4096) * ctas_per_sm(HD) <= 228 * 1024, "shared memory of an SM");
+    cudaError_t e = ensure_dynamic_smem((const void*)attention_token_paged_kernel<FMT, HD, PACKED>, token_smem_bytes<FMT, HD, PACKED>());
     if (e != cudaSuccess) return e;
-    return launch_dependent(attention_token_paged_kernel<FMT, HD, PACKED>, dim3(ctas), dim3(kThreads), token_smem_bytes<FMT, HD>(), stream, p);
+    return launch_dependent(attention_token_paged_kernel<FMT, HD, PACKED>, dim3(ctas), dim3(kThreads), token_smem_bytes<FMT, HD, PACKED>(), stream, p);
 }
 template <int FMT, int HD>
 cudaError_t launch_token(cudaStream_t stream, const TokenParams& p) {
     const uint32_t ctas = token_ctas(p.pool, p.rows);
     cudaError_t e = p.group <= 4 ? launch_token_as<FMT, HD, true>(stream, p, ctas) : launch_token_as<FMT, HD, false>(stream, p, ctas);
     if (e != cudaSuccess || ctas == 1) return e;
-    return launch_dependent(attention_token_join_kernel<HD>, dim3(ctas - 1), dim3(32 * kRows), 0, stream, static_cast<const float*>(p.parts), p.out, p.n_heads, p.group);
+    return launch_dependent(attention_token_join_kernel<HD>, dim3(ctas - 1, p.group), dim3(256), 0, stream, static_cast<const float*>(p.parts), p.out, p.n_heads, p.group);
 }
 
 uint64_t token_floats(uint32_t head_dim) {
