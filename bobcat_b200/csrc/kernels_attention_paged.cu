@@ -46,6 +46,7 @@ struct TokenParams {
     uint64_t q_stride, q_head_stride;
     uint32_t n_heads, group;
     uint32_t most;  // sequences of more rows are the other kernel's (kernels_attention_chunk.cu)
+    bool whole;     // units are not cut: each counts as one block, and there is nothing to join
 };
 // What the joining launch needs of the unit that begins in a CTA's run and goes on behind it; `last` is the CTA it ends in, 0 when there is none.
 struct PartsHead {
@@ -100,7 +101,7 @@ template <int FMT, int HD>
 struct Ring {
     // Positions of a step: two fragments where registers and shared memory hold them, which halves what a step costs beside its multiplies. A block, the
     // unit that work is counted in, is a step of each warp.
-    static constexpr uint32_t kStep = HD == 64 || (HD == 128 && FMT == BC_I8) ? 2 * kHalf : kHalf, kBlock = kStep * kWarps, kHalves = kStep / kHalf;
+    static constexpr uint32_t kStep = HD == 64 ? 2 * kHalf : kHalf, kBlock = kStep * kWarps, kHalves = kStep / kHalf;
     static constexpr uint32_t kRowBytes = FMT == BC_F16 ? 2 * HD : HD;
     static constexpr uint32_t kKeyPitch = kRowBytes == 64 ? 64 : kRowBytes + 64, kValuePitch = kRowBytes + 16;
     static constexpr uint32_t kValues = kStep * kKeyPitch, kScales = kValues + kStep * kValuePitch, kBytes = kScales + (FMT == BC_I8 ? 8 * kStep : 0);
@@ -109,9 +110,9 @@ struct Ring {
 // A sequence of the call: its rows, the positions it holds, the blocks its longest row takes.
 struct Seq {
     uint32_t row0, n, end, len;
-    uint32_t blocks;
+    uint32_t blocks, counted;  // of its longest row; of them, what a unit counts as
 };
-__device__ __forceinline__ Seq seq_at(const KvPool& pool, const KvRows& rows, uint32_t s, uint32_t most, uint32_t block) {
+__device__ __forceinline__ Seq seq_at(const KvPool& pool, const KvRows& rows, uint32_t s, uint32_t most, uint32_t block, bool whole) {
     Seq q;
     q.row0 = rows.starts[s];
     q.end = rows.starts[s + 1];
@@ -119,9 +120,10 @@ __device__ __forceinline__ Seq seq_at(const KvPool& pool, const KvRows& rows, ui
     q.len = rows.lens[s];
     const uint32_t held = min((uint64_t)q.len, (uint64_t)rows.max_pages << pool.page_shift);
     q.blocks = max(1u, (held + block - 1) / block);
+    q.counted = whole ? 1 : q.blocks;
     return q;
 }
-__device__ __forceinline__ uint64_t blocks_of(const KvPool& pool, const Seq& q) { return (uint64_t)q.n * pool.n_kv_heads * q.blocks; }
+__device__ __forceinline__ uint64_t blocks_of(const KvPool& pool, const Seq& q) { return (uint64_t)q.n * pool.n_kv_heads * q.counted; }
 
 __device__ __forceinline__ uint64_t warp_sum_u64(uint64_t v) {
 #pragma unroll
@@ -178,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
 
     // This CTA's run of blocks, and the sequence that it begins in. Every warp works it out for itself.
     uint64_t total = 0;
-    for (uint32_t s = lane; s < rows.n_seqs; s += 32) total += blocks_of(pool, seq_at(pool, rows, s, p.most, kBlock));
+    for (uint32_t s = lane; s < rows.n_seqs; s += 32) total += blocks_of(pool, seq_at(pool, rows, s, p.most, kBlock, p.whole));
     total = warp_sum_u64(total);
     const uint64_t runs = min((uint64_t)gridDim.x, total);  // none of them empty
     uint64_t at = blockIdx.x < runs ? total * blockIdx.x / runs : total;
@@ -191,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
     uint32_t seq = 0;
     uint64_t base = 0;  // blocks of the sequences before `seq`
     for (uint32_t s0 = 0; s0 < rows.n_seqs; s0 += 32) {
-        const uint64_t mine = s0 + lane < rows.n_seqs ? blocks_of(pool, seq_at(pool, rows, s0 + lane, p.most, kBlock)) : 0;
+        const uint64_t mine = s0 + lane < rows.n_seqs ? blocks_of(pool, seq_at(pool, rows, s0 + lane, p.most, kBlock, p.whole)) : 0;
         uint64_t upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -211,20 +213,21 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
 
     // The unit at `at`, and the blocks of it that are this CTA's. Rows of a head are neighbours.
     struct Work {
-        uint32_t seq, row, head, n_keys, block0, blocks, all_blocks;
+        uint32_t seq, row, head, n_keys, block0, blocks, counted, all_blocks;
     };
     auto find = [&]() {
         Work w;
-        Seq sq = seq_at(pool, rows, seq, p.most, kBlock);
+        Seq sq = seq_at(pool, rows, seq, p.most, kBlock, p.whole);
         while (base + blocks_of(pool, sq) <= at) {  // sequences without rows have no blocks
             base += blocks_of(pool, sq);
-            sq = seq_at(pool, rows, ++seq, p.most, kBlock);
+            sq = seq_at(pool, rows, ++seq, p.most, kBlock, p.whole);
         }
         const uint64_t in_seq = at - base;
-        const uint32_t which = (uint32_t)(in_seq / sq.blocks);
+        const uint32_t which = (uint32_t)(in_seq / sq.counted);
         w.seq = seq;
-        w.block0 = (uint32_t)(in_seq % sq.blocks);
-        w.blocks = (uint32_t)min((uint64_t)(sq.blocks - w.block0), end - at);
+        w.block0 = (uint32_t)(in_seq % sq.counted);
+        w.counted = (uint32_t)min((uint64_t)(sq.counted - w.block0), end - at);
+        w.blocks = p.whole ? sq.blocks : w.counted;
         w.all_blocks = sq.blocks;
         w.head = which / sq.n;
         w.row = sq.row0 + which % sq.n;
@@ -600,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
         }
         async::cp_async_wait<0>();
         const Work done = w;
-        at += done.blocks;
+        at += done.counted;
         const bool more = at < end;  // uniform in the CTA
         if (more) w = find();
         if (kBeside && more) begin_copies(w);
@@ -777,9 +780,14 @@ template <int FMT, int HD>
 cudaError_t launch_token(cudaStream_t stream, const TokenParams& p) {
     const uint32_t ctas = token_ctas(p.pool, p.rows);
     cudaError_t e = p.group <= 4 ? launch_token_as<FMT, HD, true>(stream, p, ctas) : launch_token_as<FMT, HD, false>(stream, p, ctas);
-    if (e != cudaSuccess || ctas == 1) return e;
+    if (e != cudaSuccess || ctas == 1 || p.whole) return e;
     return launch_dependent(attention_token_join_kernel<HD>, dim3(ctas - 1, p.group), dim3(256), 0, stream, static_cast<const float*>(p.parts), p.out, p.n_heads, p.group);
 }
+
+// Where tables cannot hold more than this many elements of a head's keys, units stay whole: what a CTA takes longer for the longest unit is less
+// than the joining launch (one sequence of 8 heads of 64: 301 positions 6.4 us, cut and joined 8.6; 1024 positions 8.3 and 8.6; 2001 11.7 and 9.1).
+constexpr uint64_t kWholeElements = 65536;
+bool whole_units(const KvRows& rows, const KvPool& pool) { return ((uint64_t)rows.max_pages << pool.page_shift) * pool.head_dim <= kWholeElements; }
 
 uint64_t token_floats(uint32_t head_dim) {
     return (uint64_t)2 * kMostCtas * kRows * (head_dim + 2) + (uint64_t)kMostCtas * sizeof(PartsHead) / 4;
@@ -796,7 +804,7 @@ uint64_t attention_paged_scratch_floats(uint32_t, uint32_t, uint32_t head_dim) {
 }
 
 int attention_paged_launches(const KvPool& pool, const KvRows& rows, uint32_t) {
-    const int tokens = token_ctas(pool, rows) == 1 ? 1 : 2;
+    const int tokens = token_ctas(pool, rows) == 1 || whole_units(rows, pool) ? 1 : 2;
     if (rows.max_queries <= kTokenRows) return tokens;
     return attention_chunk_launches() + (rows.n_seqs > 1 ? tokens : 0);
 }
@@ -806,7 +814,7 @@ cudaError_t attention_paged(cudaStream_t stream, const KvPool& pool, const KvRow
     if (rows.n_rows == 0 || rows.n_seqs == 0) return cudaSuccess;
     // What the caller says of the rows decides which kernels run; the rows themselves, on the device, which of them takes a sequence.
     const bool chunks = rows.max_queries > kTokenRows, tokens = !chunks || rows.n_seqs > 1;
-    const TokenParams p{pool, rows, q, out, scratch, q_stride, q_head_stride, n_heads, n_heads / pool.n_kv_heads, chunks ? kTokenRows : 0xffffffffu};
+    const TokenParams p{pool, rows, q, out, scratch, q_stride, q_head_stride, n_heads, n_heads / pool.n_kv_heads, chunks ? kTokenRows : 0xffffffffu, whole_units(rows, pool)};
     const bool half = pool.format == BC_F16;
     cudaError_t e = cudaSuccess;
     if (tokens) {
