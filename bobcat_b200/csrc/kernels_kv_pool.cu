@@ -1,14 +1,17 @@
 // Rows into the pages of a key/value pool, and back.
 //
 // Writing (8 bit). A row is the head_dim elements of one head at one position: d = f32(max |x| / 127), q = the whole number nearest to
-// x / d, ties to even, within +-127. The quotient is rounded exactly without a division per element: q0 = rint(x * (1 / d)) is at most one
-// off, and x - q0 d, which an fma gives without error (a multiple of both operands' last places, no longer than a float), says where x lies.
+// x / d, ties to even. One fma rounds x * (1 / d) to a whole number (added to 1.5 * 2^23 + 128, whose last byte is then the one stored); the product
+// is within 2^-16 of x / d, so only where it lies that near the middle between two numbers (one element in 5000 is taken to) does a second look
+// decide: x - q d, which an fma gives without error (a multiple of both operands' last places, no longer than a float), against d / 2.
 // Rows whose d is not a normal number (all elements below 127 * 2^-126) are stored as zeros; a row with an infinity or a NaN gets a scale of
 // NaN, so it reads as NaN throughout. Half pages store the elements rounded to nearest.
 //
 // What bounds it: bytes, 4 read and 1 (+ 4 / head_dim) or 2 written per element, and the look-up of a row's place before the
 // first store. A lane holds 8 elements (two 16-byte loads, one 8- or 16-byte store), a cell (one head's row of keys or of values) is
-// 8, 16 or 32 lanes. A CTA takes neighbouring token rows; its warps look the rows' places up while the first cells' loads are on their way.
+// 8, 16 or 32 lanes. A CTA takes neighbouring token rows; its warps look the rows' places up while the first cells' loads are on their way. Large
+// calls are bound by bytes as long as an element costs few instructions: with the exact test for every element 50 of them, and the
+// rows of eight prompts (32 008 of 2 x 8 heads of 128) took 117 us to write.
 
 #include "kv_pool.cuh"
 
@@ -21,6 +24,19 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr uint32_t kRowsPerCta = 8;  // at most: one warp looks up each
+
+// Cells of a token row, and how to divide by their number.
+struct Cells {
+    uint32_t per_row, magic, rows_per_cta;
+    __device__ __forceinline__ uint32_t row(uint32_t cell) const { return __umulhi(cell, magic); }  // cell * per_row < 2^32
+};
+
+// The larger magnitude; NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 
 // Places of the CTA's rows; the sequence look-up is a warp's.
 __device__ __forceinline__ void look_up(const KvPool& pool, const KvRows& rows, uint32_t row0, uint32_t n, uint2* place) {
@@ -45,31 +61,34 @@ struct Sources {
 
 template <int FMT, int HD>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constant__ KvPool pool, const __grid_constant__ KvRows rows,
-                                                            const __grid_constant__ Sources src, uint32_t rows_per_cta) {
+                                                            const __grid_constant__ Sources src, const __grid_constant__ Cells cells) {
     constexpr uint32_t kLanes = HD / 8, kCellsAtOnce = kThreads / kLanes;
     __shared__ uint2 place[kRowsPerCta];
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t row0 = blockIdx.x * rows_per_cta, n = min(rows_per_cta, rows.n_rows - row0);
-    const uint32_t per_row = 2 * pool.n_kv_heads, n_cells = n * per_row;
+    const uint32_t row0 = blockIdx.x * cells.rows_per_cta, n = min(cells.rows_per_cta, rows.n_rows - row0);
+    const uint32_t n_cells = n * cells.per_row;
     const uint32_t lane = threadIdx.x % kLanes, first = threadIdx.x / kLanes;
-    float x[8];
-    auto load = [&](uint32_t cell) {
-        const uint32_t row = cell / per_row, head = cell % per_row;
+    auto load = [&](uint32_t cell, float (&x)[8]) {
+        const uint32_t row = cells.row(cell), head = cell - row * cells.per_row;
         const bool value = head >= pool.n_kv_heads;
         const float* from = value ? src.v + (row0 + row) * src.v_stride + (head - pool.n_kv_heads) * HD : src.k + (row0 + row) * src.k_stride + head * HD;
         const float4 a = __ldcs(reinterpret_cast<const float4*>(from) + 2 * lane), b = __ldcs(reinterpret_cast<const float4*>(from) + 2 * lane + 1);
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
         x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
     };
-    if (first < n_cells) load(first);
+    float next[8] = {};
+    if (first < n_cells) load(first, next);
     look_up(pool, rows, row0, n, place);
     __syncthreads();
     for (uint32_t cell0 = 0; cell0 < n_cells; cell0 += kCellsAtOnce) {
         const uint32_t cell = cell0 + first;
         const bool mine = cell < n_cells;
-        if (cell0 > 0 && mine) load(cell);
-        const uint32_t row = mine ? cell / per_row : 0, head = cell % per_row;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = next[i];
+        if (cell + kCellsAtOnce < n_cells) load(cell + kCellsAtOnce, next);
+        const uint32_t row = mine ? cells.row(cell) : 0, head = mine ? cell - row * cells.per_row : 0;
         const bool value = head >= pool.n_kv_heads;
         const uint2 at = place[row];
         uint8_t* const to = value ? pool.v : pool.k;
@@ -83,28 +102,39 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constan
                 *reinterpret_cast<uint4*>(to + kv_row_at(pool, at.x, kv_head, at.y) + 16 * lane) = *reinterpret_cast<uint4*>(h);
             }
         } else {
-            uint32_t top = 0;  // magnitudes as bits: they order as the numbers do, with infinities and NaN on top
+            float top = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+            for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(x[i]));
 #pragma unroll
-            for (uint32_t o = kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-            float d = __fdiv_rn(__uint_as_float(top), 127.f);
-            if (d < 1.17549435e-38f) d = 0.f;
-            const bool finite = top < 0x7f800000u;
+            for (uint32_t o = kLanes / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+            float d = __fdiv_rn(top, 127.f);
+            const bool finite = top < INFINITY;
+            if (!(d >= 1.17549435e-38f)) d = 0.f;
             const float inverse = d > 0.f && finite ? __frcp_rn(d) : 0.f;
-            uint32_t bytes[2] = {0, 0};
+            constexpr float kMagic = 12583040.f;  // 1.5 * 2^23 + 128
+            uint32_t bytes[2] = {0x80808080u, 0x80808080u};
+            if (inverse > 0.f) {
+                float whole[8], furthest = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float q = 0.f;
-                if (inverse > 0.f) {
-                    q = rintf(x[i] * inverse);
-                    const float twice = 2.f * fmaf(-q, d, x[i]);
-                    const bool odd = (int)q & 1;
-                    if (twice > d || (twice == d && odd)) q += 1.f;
-                    if (twice < -d || (twice == -d && odd)) q -= 1.f;
-                    q = fminf(fmaxf(q, -127.f), 127.f);
+                for (int i = 0; i < 8; ++i) {
+                    whole[i] = fmaf(x[i], inverse, kMagic);
+                    furthest = fmaxf(furthest, fabsf(fmaf(x[i], inverse, kMagic - whole[i])));
                 }
-                bytes[i / 4] |= (uint32_t)((int)q + 128) << (8 * (i % 4));
+                if (furthest > 0.4999f) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float q = whole[i] - kMagic, twice = 2.f * fmaf(-q, d, x[i]);
+                        const bool odd = __float_as_uint(whole[i]) & 1;
+                        if (twice > d || (twice == d && odd)) whole[i] += 1.f;
+                        if (twice < -d || (twice == -d && odd)) whole[i] -= 1.f;
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t low = __byte_perm(__float_as_uint(whole[4 * h]), __float_as_uint(whole[4 * h + 1]), 0x0040);
+                    const uint32_t high = __byte_perm(__float_as_uint(whole[4 * h + 2]), __float_as_uint(whole[4 * h + 3]), 0x0040);
+                    bytes[h] = __byte_perm(low, high, 0x5410);
+                }
             }
             if (store) {
                 *reinterpret_cast<uint2*>(to + kv_row_at(pool, at.x, kv_head, at.y) + 8 * lane) = make_uint2(bytes[0], bytes[1]);
@@ -123,47 +153,53 @@ struct Targets {
 
 template <int FMT, int HD, typename Out>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant__ KvPool pool, const __grid_constant__ KvRows rows,
-                                                           const __grid_constant__ Targets dst, uint32_t rows_per_cta) {
+                                                           const __grid_constant__ Targets dst, const __grid_constant__ Cells cells) {
     constexpr uint32_t kLanes = HD / 8, kCellsAtOnce = kThreads / kLanes;
     constexpr int kAhead = 4;  // cells a lane has loads under way for
     __shared__ uint2 place[kRowsPerCta];
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t row0 = blockIdx.x * rows_per_cta, n = min(rows_per_cta, rows.n_rows - row0);
-    const uint32_t per_row = 2 * pool.n_kv_heads, n_cells = n * per_row;
+    const uint32_t row0 = blockIdx.x * cells.rows_per_cta, n = min(cells.rows_per_cta, rows.n_rows - row0);
+    const uint32_t n_cells = n * cells.per_row;
     const uint32_t lane = threadIdx.x % kLanes, first = threadIdx.x / kLanes;
     look_up(pool, rows, row0, n, place);
     __syncthreads();
     for (uint32_t cell0 = first; cell0 < n_cells; cell0 += kAhead * kCellsAtOnce) {
         uint4 raw[kAhead];
         float scale[kAhead];
+        Out* to[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-            const uint32_t cell = cell0 + j * kCellsAtOnce, row = cell / per_row, head = cell % per_row;
-            raw[j] = make_uint4(0, 0, 0, 0);
+            const uint32_t cell = cell0 + j * kCellsAtOnce;
+            raw[j] = FMT == BC_F16 ? make_uint4(0, 0, 0, 0) : make_uint4(0x80808080u, 0x80808080u, 0, 0);
             scale[j] = 0.f;
-            if (cell >= n_cells || place[row].x == kNoSlot) continue;
-            const uint8_t* from = head >= pool.n_kv_heads ? pool.v : pool.k;
-            const uint32_t kv_head = head >= pool.n_kv_heads ? head - pool.n_kv_heads : head;
+            to[j] = nullptr;
+            if (cell >= n_cells) continue;
+            const uint32_t row = cells.row(cell), head = cell - row * cells.per_row;
+            const bool value = head >= pool.n_kv_heads;
+            const uint2 at = place[row];
+            void* const base = value ? dst.v : dst.k;
+            if (!base || (at.x == kNoSlot && at.y == 1)) continue;
+            const uint32_t kv_head = value ? head - pool.n_kv_heads : head;
+            to[j] = static_cast<Out*>(base) + (row0 + row) * (value ? dst.v_stride : dst.k_stride) + kv_head * HD + 8 * lane;
+            if (at.x == kNoSlot) continue;
+            const uint8_t* const from = value ? pool.v : pool.k;
             if constexpr (FMT == BC_F16) {
-                raw[j] = *reinterpret_cast<const uint4*>(from + kv_row_at(pool, place[row].x, kv_head, place[row].y) + 16 * lane);
+                raw[j] = __ldcs(reinterpret_cast<const uint4*>(from + kv_row_at(pool, at.x, kv_head, at.y) + 16 * lane));
             } else {
-                const uint2 b = *reinterpret_cast<const uint2*>(from + kv_row_at(pool, place[row].x, kv_head, place[row].y) + 8 * lane);
+                const uint2 b = __ldcs(reinterpret_cast<const uint2*>(from + kv_row_at(pool, at.x, kv_head, at.y) + 8 * lane));
                 raw[j].x = b.x;
                 raw[j].y = b.y;
-                scale[j] = *reinterpret_cast<const float*>(from + kv_scale_at(pool, place[row].x, kv_head, place[row].y));
+                scale[j] = *reinterpret_cast<const float*>(from + kv_scale_at(pool, at.x, kv_head, at.y));
             }
         }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-            const uint32_t cell = cell0 + j * kCellsAtOnce, row = cell / per_row, head = cell % per_row;
-            if (cell >= n_cells) continue;
-            const uint2 at = place[row];
-            if (at.x == kNoSlot && at.y == 1) continue;
-            const bool value = head >= pool.n_kv_heads;
-            void* base = value ? dst.v : dst.k;
-            if (!base) continue;
-            Out* to = static_cast<Out*>(base) + (row0 + row) * (value ? dst.v_stride : dst.k_stride) + (value ? head - pool.n_kv_heads : head) * HD + 8 * lane;
+            if (!to[j]) continue;
+            if constexpr (FMT == BC_F16 && sizeof(Out) == 2) {
+                __stcs(reinterpret_cast<uint4*>(to[j]), raw[j]);
+                continue;
+            }
             float x[8];
             if constexpr (FMT == BC_F16) {
                 const __half2* h = reinterpret_cast<const __half2*>(&raw[j]);
@@ -176,41 +212,42 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
             } else {
                 const uint32_t words[2] = {raw[j].x, raw[j].y};
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = at.x == kNoSlot ? 0.f : (float)((int)(words[i / 4] >> (8 * (i % 4)) & 0xffu) - 128) * scale[j];
+                for (int i = 0; i < 8; ++i)  // the byte as the last of 2^23's
+                    x[i] = (__uint_as_float(__byte_perm(words[i / 4], 0x4b000000u, 0x7440 + i % 4)) - 8388736.f) * scale[j];
             }
             if constexpr (sizeof(Out) == 4) {
-                reinterpret_cast<float4*>(to)[0] = make_float4(x[0], x[1], x[2], x[3]);
-                reinterpret_cast<float4*>(to)[1] = make_float4(x[4], x[5], x[6], x[7]);
+                __stcs(reinterpret_cast<float4*>(to[j]), make_float4(x[0], x[1], x[2], x[3]));
+                __stcs(reinterpret_cast<float4*>(to[j]) + 1, make_float4(x[4], x[5], x[6], x[7]));
             } else {
                 __half2 h[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-                *reinterpret_cast<uint4*>(to) = *reinterpret_cast<uint4*>(h);
+                __stcs(reinterpret_cast<uint4*>(to[j]), *reinterpret_cast<uint4*>(h));
             }
         }
     }
 }
 
-// Token rows per CTA: a CTA works through at most about four rounds of its threads, fewer where that leaves SMs without one.
-uint32_t rows_per_cta(const KvPool& pool, const KvRows& rows) {
-    const uint32_t lanes_per_row = 2 * pool.n_kv_heads * (pool.head_dim / 8);
-    uint32_t n = 4 * kThreads / lanes_per_row;
+// Token rows per CTA: a CTA works through at most about eight rounds of its threads, fewer where that leaves SMs without one.
+Cells cells_of(const KvPool& pool, const KvRows& rows) {
+    const uint32_t per_row = 2 * pool.n_kv_heads, lanes_per_row = per_row * (pool.head_dim / 8);
+    uint32_t n = 8 * kThreads / lanes_per_row;
     if (n > kRowsPerCta) n = kRowsPerCta;
-    while (n > 1 && (rows.n_rows + n - 1) / n < 2 * (uint32_t)sm_count()) n /= 2;
-    return n < 1 ? 1 : n;
+    while (n > 1 && (rows.n_rows + n - 1) / n < 4 * (uint32_t)sm_count()) n /= 2;
+    return Cells{per_row, (uint32_t)(((1ull << 32) + per_row - 1) / per_row), n < 1 ? 1 : n};
 }
 
 template <int FMT, int HD>
 cudaError_t write_as(cudaStream_t stream, const KvPool& pool, const KvRows& rows, const Sources& src) {
-    const uint32_t n = rows_per_cta(pool, rows);
-    return launch_dependent(kv_write_kernel<FMT, HD>, dim3((rows.n_rows + n - 1) / n), dim3(kThreads), 0, stream, pool, rows, src, n);
+    const Cells cells = cells_of(pool, rows);
+    return launch_dependent(kv_write_kernel<FMT, HD>, dim3((rows.n_rows + cells.rows_per_cta - 1) / cells.rows_per_cta), dim3(kThreads), 0, stream, pool, rows, src, cells);
 }
 template <int FMT, int HD>
 cudaError_t read_as(cudaStream_t stream, const KvPool& pool, const KvRows& rows, const Targets& dst, bool half) {
-    const uint32_t n = rows_per_cta(pool, rows);
-    const dim3 grid((rows.n_rows + n - 1) / n);
-    return half ? launch_dependent(kv_read_kernel<FMT, HD, __half>, grid, dim3(kThreads), 0, stream, pool, rows, dst, n)
-                : launch_dependent(kv_read_kernel<FMT, HD, float>, grid, dim3(kThreads), 0, stream, pool, rows, dst, n);
+    const Cells cells = cells_of(pool, rows);
+    const dim3 grid((rows.n_rows + cells.rows_per_cta - 1) / cells.rows_per_cta);
+    return half ? launch_dependent(kv_read_kernel<FMT, HD, __half>, grid, dim3(kThreads), 0, stream, pool, rows, dst, cells)
+                : launch_dependent(kv_read_kernel<FMT, HD, float>, grid, dim3(kThreads), 0, stream, pool, rows, dst, cells);
 }
 
 }  // namespace
