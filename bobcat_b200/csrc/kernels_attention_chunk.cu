@@ -129,11 +129,11 @@ struct TileInfo {
     alignas(16) float dk[FMT == BC_I8 ? KT : 4];
     alignas(16) float dv[FMT == BC_I8 ? KT : 4];
 };
-// A tile's bytes as they lie in the pages.
+// A tile's bytes as they lie in the pages: its keys with both scales, which the scores' warps want first, and its values.
 template <uint32_t KT, int FMT, int HD>
-struct RawTile {
+struct RawKeys {
     static constexpr uint32_t kRowBytes = FMT == BC_F16 ? 2 * HD : HD;
-    uint8_t keys[KT * kRowBytes], values[KT * kRowBytes];
+    uint8_t keys[KT * kRowBytes];
     float dk[FMT == BC_I8 ? KT : 4], dv[FMT == BC_I8 ? KT : 4];
 };
 
@@ -229,13 +229,14 @@ struct Shared {
     static constexpr uint32_t kTileBytes = KT / 8 * (HD / 8) * kCore;
     uint8_t q_lo[HD == 256 ? kRows / 8 * (HD / 8) * kCore : 16];
     uint8_t keys[kStages][kTileBytes], values[kStages][kTileBytes];
-    alignas(16) RawTile<KT, FMT, HD> raw[kRaw];
+    alignas(16) RawKeys<KT, FMT, HD> raw_keys[kRaw];
+    alignas(16) uint8_t raw_values[kRaw][KT * RawKeys<KT, FMT, HD>::kRowBytes];
     TileInfo<KT, FMT> info[kRing];
     TileDesc desc[kDescRing];
     float most[2][kParts][kRows];  // [parity][part]: maxima of the parts of a row's scores; at a unit's ends, other exchanges
     uint32_t not_finite[FMT == BC_F16 ? kUnits : 1][FMT == BC_F16 ? HD : 1];  // by unit: the first position with such a value, of each element
     uint32_t any_not_finite[kUnits];
-    uint64_t bars[4 * kStages + 2 * kRaw + 10 + kDescRing];
+    uint64_t bars[4 * kStages + 4 * kRaw + 10 + kDescRing];
     uint64_t total, run_tiles;  // key tiles of the call, and of the CTA's run
     Place place;
     uint32_t tmem;
@@ -260,8 +261,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
     const uint64_t capacity = (uint64_t)p.rows.max_pages << pool.page_shift;
     const uint32_t per_tile = kRows / p.group;
     const uint32_t bars = smem_u32(sh.bars);
-    const uint32_t k_full = bars, k_free = k_full + 8 * ST, v_full = k_free + 8 * ST, v_free = v_full + 8 * ST, raw_full = v_free + 8 * ST, raw_free = raw_full + 8 * RAW;
-    const uint32_t s_full = raw_free + 8 * RAW, p_ready = s_full + 16, pv_full = p_ready + 16, pv_free = pv_full + 16, q_ready = pv_free + 8;
+    const uint32_t k_full = bars, k_free = k_full + 8 * ST, v_full = k_free + 8 * ST, v_free = v_full + 8 * ST, rk_full = v_free + 8 * ST, rk_free = rk_full + 8 * RAW;
+    const uint32_t rv_full = rk_free + 8 * RAW, rv_free = rv_full + 8 * RAW, s_full = rv_free + 8 * RAW, p_ready = s_full + 16, pv_full = p_ready + 16, pv_free = pv_full + 16, q_ready = pv_free + 8;
     const uint32_t rows_bar = q_ready + 8, unpack_bar = rows_bar + 8, described = unpack_bar + 8;
 
     pdl_launch_dependents();
@@ -273,8 +274,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             mbar_init(v_free + 8 * s, 1);
         }
         for (uint32_t r = 0; r < RAW; ++r) {
-            mbar_init(raw_full + 8 * r, 1);
-            mbar_init(raw_free + 8 * r, kUnpackWarps);
+            mbar_init(rk_full + 8 * r, 1);
+            mbar_init(rk_free + 8 * r, kUnpackWarps);
+            mbar_init(rv_full + 8 * r, 1);
+            mbar_init(rv_free + 8 * r, kUnpackWarps);
         }
         mbar_init(s_full, 1);
         mbar_init(s_full + 8, 1);
@@ -625,66 +628,78 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
         const uint32_t utid = tid - kRowThreads, uwarp = utid >> 5;
         constexpr uint32_t kPieces = KT * (HD / 8) / kUnpackThreads;           // pieces of 8 elements of a key that a thread unpacks
         constexpr uint32_t kBlocks = KT / 8 * (HD / 8) / kUnpackThreads;       // blocks of 8 positions x 8 elements of values
-        constexpr uint32_t kPiece = FMT == BC_F16 ? 16 : 8, kWords = kPiece / 4, kRowBytes = RawTile<KT, FMT, HD>::kRowBytes;
+        constexpr uint32_t kPiece = FMT == BC_F16 ? 16 : 8, kWords = kPiece / 4, kRowBytes = RawKeys<KT, FMT, HD>::kRowBytes;
         WarpsBarrier everyone{unpack_bar, 0, 14};
-        for (uint32_t j = 0; j < n_tiles; ++j) {
-            const uint32_t st = j % ST;
-            TileInfo<KT, FMT>& info = sh.info[j % kRing];
-            const RawTile<KT, FMT, HD>& raw = sh.raw[j % RAW];
-            await(alive, raw_full + 8 * (j % RAW), (j / RAW) & 1, dead, 10);
-            if (!alive) break;
+        // Keys one tile ahead of values: the next scores need no more, while the values' place waits for a product.
+        for (uint32_t i = 0; i <= n_tiles && n_tiles > 0; ++i) {
+            if (i < n_tiles) {
+                const uint32_t j = i, st = j % ST;
+                TileInfo<KT, FMT>& info = sh.info[j % kRing];
+                const RawKeys<KT, FMT, HD>& raw = sh.raw_keys[j % RAW];
+                await(alive, rk_full + 8 * (j % RAW), (j / RAW) & 1, dead, 10);
+                if (!alive) break;
+                const TileDesc& desc = sh.desc[j % kDescRing];
+                const uint32_t key0 = desc.key0, end = desc.end, groups = desc.groups;
+                auto key_there = [&](uint32_t key) { return (groups >> (key >> 4) & 1) && key0 + key < end; };
+                const bool whole = groups == (1u << KT / 16) - 1 && end - key0 >= KT;  // every position is there
+                // Free keys: their scores are done, so the rows' warps are done with the tile before those, and the ring's fourth is nobody's.
+                await(alive, k_free + 8 * st, ((j / ST) & 1) ^ 1, dead, 3);
+                if (!alive) break;
+                if constexpr (FMT == BC_F16) {
+                    if (desc.first) {
+                        const uint32_t slot = desc.unit % kUnits;
+                        for (uint32_t e = utid; e < HD; e += kUnpackThreads) sh.not_finite[slot][e] = 0xffffffffu;
+                        if (utid == 0) sh.any_not_finite[slot] = 0;
+                        everyone.sync(alive, dead);  // before any of them finds one
+                        if (!alive) break;
+                    }
+                }
+                // Masks and scales of the tile's positions.
+                const bool there = utid < KT && key_there(utid);
+                const uint32_t votes = __ballot_sync(0xffffffffu, there);
+                if (lane == 0 && uwarp < KT / 32) info.valid[uwarp] = votes;
+                if (utid == 0) info.masked = !whole || (int64_t)key0 + KT - 1 > desc.pos0;
+                if constexpr (FMT == BC_I8) {
+                    const float dv = there ? raw.dv[utid] : 0.f;
+                    if (utid < KT) {
+                        info.dk[utid] = there ? raw.dk[utid] : 0.f;
+                        info.dv[utid] = dv;
+                    }
+                    // The largest finite one.
+                    const uint32_t bits = __float_as_uint(dv) & 0x7fffffffu, largest = __reduce_max_sync(0xffffffffu, bits < 0x7f800000u ? bits : 0u);
+                    if (lane == 0) info.top_scale[uwarp] = largest;
+                }
+                {  // What is there of positions that are not is masked in the scores, whatever it is.
+                    const uint8_t* from = raw.keys + utid * kPiece;
+                    uint8_t* const to = sh.keys[st];
+#pragma unroll 4
+                    for (uint32_t n = 0; n < kPieces; ++n) {
+                        const uint32_t at = utid + n * kUnpackThreads, piece = at % (HD / 8), key = at / (HD / 8);
+                        uint4 w;
+                        if constexpr (FMT == BC_F16) {
+                            w = *reinterpret_cast<const uint4*>(from + n * kUnpackThreads * kPiece);
+                        } else {
+                            const uint2 b = *reinterpret_cast<const uint2*>(from + n * kUnpackThreads * kPiece);
+                            unpack_i8(b.x, w.x, w.y);
+                            unpack_i8(b.y, w.z, w.w);
+                        }
+                        *reinterpret_cast<uint4*>(to + (key >> 3) * kKeyStep + piece * kCore + (key & 7) * 16) = w;
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(k_full + 8 * st);
+                    mbar_arrive(rk_free + 8 * (j % RAW));
+                }
+            }
+            if (i == 0) continue;
+            const uint32_t j = i - 1, st = j % ST;
             const TileDesc& desc = sh.desc[j % kDescRing];
             const uint32_t key0 = desc.key0, end = desc.end, groups = desc.groups;
             auto key_there = [&](uint32_t key) { return (groups >> (key >> 4) & 1) && key0 + key < end; };
-            const bool whole = groups == (1u << KT / 16) - 1 && end - key0 >= KT;  // every position is there
-            // Free keys: their scores are done, so the rows' warps are done with the tile before those, and the ring's fourth is nobody's.
-            await(alive, k_free + 8 * st, ((j / ST) & 1) ^ 1, dead, 3);
-            if (!alive) break;
-            if constexpr (FMT == BC_F16) {
-                if (desc.first) {
-                    const uint32_t slot = desc.unit % kUnits;
-                    for (uint32_t i = utid; i < HD; i += kUnpackThreads) sh.not_finite[slot][i] = 0xffffffffu;
-                    if (utid == 0) sh.any_not_finite[slot] = 0;
-                    everyone.sync(alive, dead);  // before any of them finds one
-                    if (!alive) break;
-                }
-            }
-            // Masks and scales of the tile's positions.
-            const bool there = utid < KT && key_there(utid);
-            const uint32_t votes = __ballot_sync(0xffffffffu, there);
-            if (lane == 0 && uwarp < KT / 32) info.valid[uwarp] = votes;
-            if (utid == 0) info.masked = !whole || (int64_t)key0 + KT - 1 > desc.pos0;
-            if constexpr (FMT == BC_I8) {
-                const float dv = there ? raw.dv[utid] : 0.f;
-                if (utid < KT) {
-                    info.dk[utid] = there ? raw.dk[utid] : 0.f;
-                    info.dv[utid] = dv;
-                }
-                // The largest finite one.
-                const uint32_t bits = __float_as_uint(dv) & 0x7fffffffu, largest = __reduce_max_sync(0xffffffffu, bits < 0x7f800000u ? bits : 0u);
-                if (lane == 0) info.top_scale[uwarp] = largest;
-            }
-            {  // What is there of positions that are not is masked in the scores, whatever it is.
-                const uint8_t* from = raw.keys + utid * kPiece;
-                uint8_t* const to = sh.keys[st];
-#pragma unroll 4
-                for (uint32_t n = 0; n < kPieces; ++n) {
-                    const uint32_t i = utid + n * kUnpackThreads, piece = i % (HD / 8), key = i / (HD / 8);
-                    uint4 w;
-                    if constexpr (FMT == BC_F16) {
-                        w = *reinterpret_cast<const uint4*>(from + n * kUnpackThreads * kPiece);
-                    } else {
-                        const uint2 b = *reinterpret_cast<const uint2*>(from + n * kUnpackThreads * kPiece);
-                        unpack_i8(b.x, w.x, w.y);
-                        unpack_i8(b.y, w.z, w.w);
-                    }
-                    *reinterpret_cast<uint4*>(to + (key >> 3) * kKeyStep + piece * kCore + (key & 7) * 16) = w;
-                }
-            }
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(k_full + 8 * st);
-
+            const bool whole = groups == (1u << KT / 16) - 1 && end - key0 >= KT;
+            await(alive, rv_full + 8 * (j % RAW), (j / RAW) & 1, dead, 15);
             await(alive, v_free + 8 * st, ((j / ST) & 1) ^ 1, dead, 4);
             if (!alive) break;
             uint8_t* const to = sh.values[st];
@@ -693,8 +708,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             const bool apart = FMT == BC_F16 && (int64_t)key0 + KT - 1 > desc.pos0;
 #pragma unroll 1
             for (uint32_t n = 0; n < kBlocks; ++n) {
-                const uint32_t i = utid + n * kUnpackThreads, piece = i % (HD / 8), key = i / (HD / 8) * 8;
-                const uint8_t* from = raw.values + key * kRowBytes + piece * kPiece;
+                const uint32_t at = utid + n * kUnpackThreads, piece = at % (HD / 8), key = at / (HD / 8) * 8;
+                const uint8_t* from = sh.raw_values[j % RAW] + key * kRowBytes + piece * kPiece;
                 uint4* const core = reinterpret_cast<uint4*>(to + piece * kCore + (key >> 3) * kKeyStep);  // 8 elements x 8 positions
                 uint32_t v[8][kWords];
 #pragma unroll
@@ -764,7 +779,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(v_full + 8 * st);
-                mbar_arrive(raw_free + 8 * (j % RAW));
+                mbar_arrive(rv_free + 8 * (j % RAW));
             }
         }
     } else {
@@ -835,79 +850,99 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
         } else if (warp == kCopyWarp) {
             // ---- the walk through the run, and the pages' bytes: a lane per 16 positions of keys, values, and either's scales.
             Place& at = sh.place;
-            constexpr uint32_t kGroups = KT / 16, kRowBytes = RawTile<KT, FMT, HD>::kRowBytes;
+            constexpr uint32_t kGroups = KT / 16, kRowBytes = RawKeys<KT, FMT, HD>::kRowBytes;
             const uint32_t page_slots = (1u << pool.page_shift) - 1;
-            uint32_t issued = 0;
-            for (uint32_t j = 0; j < n_tiles; ++j) {
-                TileDesc& d = sh.desc[j % kDescRing];
-                if (lane == 0) {
-                    if (at.in_unit == at.unit.tiles) {
-                        at.cursor.take(p, capacity, KT, at.unit);
-                        at.in_unit = 0;
-                        ++at.unit_number;
+            uint32_t keys_issued = 0, values_issued = 0;
+            const uint32_t group = lane % kGroups, what = lane / kGroups;
+            uint64_t value_rows_at = ~0ull;  // of the tile before
+            for (uint32_t i = 0; i <= n_tiles && n_tiles > 0; ++i) {
+                uint64_t rows_at = ~0ull;
+                if (i < n_tiles) {
+                    const uint32_t j = i;
+                    TileDesc& d = sh.desc[j % kDescRing];
+                    if (lane == 0) {
+                        if (at.in_unit == at.unit.tiles) {
+                            at.cursor.take(p, capacity, KT, at.unit);
+                            at.in_unit = 0;
+                            ++at.unit_number;
+                        }
+                        const Unit& u = at.unit;
+                        const ChunkSeq& s = at.cursor.s;
+                        const uint32_t query0 = u.row_tile * per_tile;
+                        const int64_t pos = (int64_t)s.len - (s.end - s.row0) + query0;
+                        d.key0 = (u.tile0 + at.in_unit) * KT;
+                        d.end = s.held;
+                        d.row0 = s.row0 + query0;
+                        d.n = min(per_tile, s.n - query0);
+                        d.head = u.head;
+                        d.pos0 = (int32_t)min(pos, (int64_t)0x7fffffff);
+                        d.unit = at.unit_number;
+                        d.first = at.in_unit == 0;
+                        d.last = at.in_unit + 1 == u.tiles;
+                        d.begins = u.begins;
+                        d.ends = u.ends;
+                        if (s.held < s.len) leave_fault(pool, kFaultTable);
+                        if (u.begins && !u.ends && at.in_unit == 0) {
+                            // The CTA whose run holds the row tile's last key tile: run c is [total c / runs, total (c + 1) / runs).
+                            const uint64_t total = sh.total, runs = min((uint64_t)gridDim.x, total), last_tile = total * blockIdx.x / runs + j + at.cursor.count - 1;
+                            uint32_t last = (uint32_t)(last_tile * runs / total);
+                            while (total * (last + 1) / runs <= last_tile) ++last;
+                            while (total * last / runs > last_tile) --last;
+                            at.cut = ChunkHead{d.row0, d.n, d.head, last};
+                        }
+                        ++at.in_unit;
                     }
-                    const Unit& u = at.unit;
-                    const ChunkSeq& s = at.cursor.s;
-                    const uint32_t query0 = u.row_tile * per_tile;
-                    const int64_t pos = (int64_t)s.len - (s.end - s.row0) + query0;
-                    d.key0 = (u.tile0 + at.in_unit) * KT;
-                    d.end = s.held;
-                    d.row0 = s.row0 + query0;
-                    d.n = min(per_tile, s.n - query0);
-                    d.head = u.head;
-                    d.pos0 = (int32_t)min(pos, (int64_t)0x7fffffff);
-                    d.unit = at.unit_number;
-                    d.first = at.in_unit == 0;
-                    d.last = at.in_unit + 1 == u.tiles;
-                    d.begins = u.begins;
-                    d.ends = u.ends;
-                    if (s.held < s.len) leave_fault(pool, kFaultTable);
-                    if (u.begins && !u.ends && at.in_unit == 0) {
-                        // The CTA whose run holds the row tile's last key tile: run c is [total c / runs, total (c + 1) / runs).
-                        const uint64_t total = sh.total, runs = min((uint64_t)gridDim.x, total), last_tile = total * blockIdx.x / runs + j + at.cursor.count - 1;
-                        uint32_t last = (uint32_t)(last_tile * runs / total);
-                        while (total * (last + 1) / runs <= last_tile) ++last;
-                        while (total * last / runs > last_tile) --last;
-                        at.cut = ChunkHead{d.row0, d.n, d.head, last};
+                    __syncwarp();
+                    // Every lane looks up its group's page.
+                    const uint32_t key = d.key0 + 16 * group;
+                    uint32_t page = ~0u;
+                    if (key < d.end) {
+                        page = p.rows.table[(uint64_t)at.unit.seq * p.rows.max_pages + (key >> pool.page_shift)];
+                        if (page >= pool.n_pages) leave_fault(pool, kFaultPage);
                     }
-                    ++at.in_unit;
-                }
-                __syncwarp();
-                // Every lane looks up its group's page.
-                const uint32_t group = lane % kGroups, what = lane / kGroups, key = d.key0 + 16 * group;
-                uint32_t page = ~0u;
-                if (key < d.end && what < 4) {
-                    page = p.rows.table[(uint64_t)at.unit.seq * p.rows.max_pages + (key >> pool.page_shift)];
-                    if (page >= pool.n_pages) leave_fault(pool, kFaultPage);
-                }
-                const bool there = page < pool.n_pages;
-                const uint32_t groups = __ballot_sync(0xffffffffu, there) & ((1u << kGroups) - 1);
-                const uint32_t slot = j % RAW, bar = raw_full + 8 * slot;
-                await(alive, raw_free + 8 * slot, ((j / RAW) & 1) ^ 1, dead, 11);
-                if (!alive) break;
-                ++issued;
-                if (lane == 0) {
-                    d.groups = groups;
-                    mbar_arrive(described + 8 * (j % kDescRing));
-                    mbar_arrive_expect(bar, __popc(groups) * 16 * 2 * (kRowBytes + (FMT == BC_I8 ? 4 : 0)));
-                }
-                __syncwarp();
-                if (there) {
-                    RawTile<KT, FMT, HD>& raw = sh.raw[slot];
-                    const uint64_t rows_at = kv_row_at(pool, page, d.head, key & page_slots);
-                    if (what < 2) {
-                        bulk_load(smem_u32(what ? raw.values : raw.keys) + group * 16 * kRowBytes, (what ? pool.v : pool.k) + rows_at, 16 * kRowBytes, bar);
-                    } else if (FMT == BC_I8 && what < 4) {
-                        bulk_load(smem_u32(what == 3 ? raw.dv : raw.dk) + group * 64, (what == 3 ? pool.v : pool.k) + kv_scale_at(pool, page, d.head, key & page_slots), 64, bar);
+                    const bool there = page < pool.n_pages;
+                    const uint32_t groups = __ballot_sync(0xffffffffu, there) & ((1u << kGroups) - 1);
+                    if (there) rows_at = kv_row_at(pool, page, d.head, key & page_slots);
+                    const uint32_t slot = j % RAW, bar = rk_full + 8 * slot;
+                    await(alive, rk_free + 8 * slot, ((j / RAW) & 1) ^ 1, dead, 11);
+                    if (!alive) break;
+                    ++keys_issued;
+                    if (lane == 0) {
+                        d.groups = groups;
+                        mbar_arrive(described + 8 * (j % kDescRing));
+                        mbar_arrive_expect(bar, __popc(groups) * 16 * (kRowBytes + (FMT == BC_I8 ? 8 : 0)));
                     }
+                    __syncwarp();
+                    if (there) {
+                        RawKeys<KT, FMT, HD>& raw = sh.raw_keys[slot];
+                        if (what == 0)
+                            bulk_load(smem_u32(raw.keys) + group * 16 * kRowBytes, pool.k + rows_at, 16 * kRowBytes, bar);
+                        else if (FMT == BC_I8 && what < 3)
+                            bulk_load(smem_u32(what == 2 ? raw.dv : raw.dk) + group * 64, (what == 2 ? pool.v : pool.k) + kv_scale_at(pool, page, d.head, key & page_slots), 64, bar);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
+                if (i > 0) {
+                    const uint32_t j = i - 1, slot = j % RAW, bar = rv_full + 8 * slot;
+                    await(alive, rv_free + 8 * slot, ((j / RAW) & 1) ^ 1, dead, 16);
+                    if (!alive) break;
+                    ++values_issued;
+                    if (lane == 0) mbar_arrive_expect(bar, __popc(sh.desc[j % kDescRing].groups) * 16 * kRowBytes);
+                    __syncwarp();
+                    if (what == 0 && value_rows_at != ~0ull) bulk_load(smem_u32(sh.raw_values[slot]) + group * 16 * kRowBytes, pool.v + value_rows_at, 16 * kRowBytes, bar);
+                    __syncwarp();
+                }
+                value_rows_at = rows_at;
             }
             if (lane == 0) reinterpret_cast<ChunkHead*>(p.parts + (uint64_t)2 * kMostCtas * kRows * (HD + 2))[blockIdx.x] = alive ? at.cut : ChunkHead{0, 0, 0, 0};
             // Copies in flight end before the CTA does: the unpacking warps wait for them, or this one does when those gave up.
-            for (uint32_t r = 0; r < RAW && r < issued && *dead; ++r) {
-                const uint32_t j = issued - 1 - r;
-                mbar_wait(raw_full + 8 * (j % RAW), (j / RAW) & 1, kSpinLimit, &sh.never);
+            for (uint32_t r = 0; r < RAW && r < keys_issued && *dead; ++r) {
+                const uint32_t j = keys_issued - 1 - r;
+                mbar_wait(rk_full + 8 * (j % RAW), (j / RAW) & 1, kSpinLimit, &sh.never);
+            }
+            for (uint32_t r = 0; r < RAW && r < values_issued && *dead; ++r) {
+                const uint32_t j = values_issued - 1 - r;
+                mbar_wait(rv_full + 8 * (j % RAW), (j / RAW) & 1, kSpinLimit, &sh.never);
             }
         }
     }
