@@ -69,10 +69,11 @@ struct Unit {
     bool begins, ends;
 };
 
-// Walks a run of key tiles.
+// Walks a run: of key tiles, or of whole row tiles.
 struct Cursor {
     uint32_t seq, head, row_tile, at, count;
     uint64_t left;
+    bool whole;
     ChunkSeq s;
     __device__ __forceinline__ bool take(const ChunkParams& p, uint64_t capacity, uint32_t key_tile, Unit& u) {
         if (left == 0) return false;
@@ -94,11 +95,11 @@ struct Cursor {
         u.head = head;
         u.row_tile = row_tile;
         u.tile0 = at;
-        u.tiles = (uint32_t)min((uint64_t)(count - at), left);
+        u.tiles = whole ? count : (uint32_t)min((uint64_t)(count - at), left);
         u.begins = at == 0;
         at += u.tiles;
         u.ends = at == count;
-        left -= u.tiles;
+        left -= whole ? 1 : u.tiles;
         return true;
     }
 };
@@ -300,18 +301,35 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
         auto seq_at = [&](uint32_t s) {
             return chunk_seq(p.rows.starts[s], p.rows.starts[s + 1], p.rows.lens[s], capacity, p.rows.n_rows, p.fewest, per_tile, KT);
         };
-        uint64_t total = 0, run_tiles = 0;
+        uint64_t total = 0, units = 0, run_tiles = 0;
+        uint32_t longest = 0;
         Cursor cur{};
-        for (uint32_t s = lane; s < p.rows.n_seqs; s += 32) total += pool.n_kv_heads * seq_at(s).tiles_per_head();
+        for (uint32_t s = lane; s < p.rows.n_seqs; s += 32) {
+            const ChunkSeq sq = seq_at(s);
+            if (sq.row_tiles == 0) continue;
+            total += pool.n_kv_heads * sq.tiles_per_head();
+            units += (uint64_t)pool.n_kv_heads * sq.row_tiles;
+            longest = max(longest, sq.tiles(sq.row_tiles - 1));
+        }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        const uint64_t runs = min((uint64_t)gridDim.x, total);
+        for (int o = 16; o > 0; o >>= 1) {
+            total += __shfl_xor_sync(0xffffffffu, total, o);
+            units += __shfl_xor_sync(0xffffffffu, units, o);
+        }
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        // Runs of key tiles are equal but cut row tiles; runs of whole row tiles are not, and nothing is cut. A row tile costs about two key tiles beside its
+        // own (its queries, its sums), a cut one more to join. (512 rows of 8 heads from position 0, 128 row tiles of 1 to 4 key tiles: 30 us cut, 21
+        // whole.)
+        const uint64_t ctas = gridDim.x, units_each = (units + ctas - 1) / ctas;
+        cur.whole = units_each * (longest + 2) <= total / ctas + 2 * (units_each + 1) + 1;
+        const uint64_t counted = cur.whole ? units : total, runs = min(ctas, counted);
+        auto counted_of = [&](const ChunkSeq& sq) { return cur.whole ? (uint64_t)sq.row_tiles : sq.tiles_per_head(); };
         if (blockIdx.x < runs) {
-            const uint64_t begin = total * blockIdx.x / runs;
-            run_tiles = total * (blockIdx.x + 1) / runs - begin;
+            const uint64_t begin = counted * blockIdx.x / runs;
+            cur.left = counted * (blockIdx.x + 1) / runs - begin;
             uint64_t base = 0;
             for (uint32_t s0 = 0; s0 < p.rows.n_seqs; s0 += 32) {
-                const uint64_t mine = s0 + lane < p.rows.n_seqs ? pool.n_kv_heads * seq_at(s0 + lane).tiles_per_head() : 0;
+                const uint64_t mine = s0 + lane < p.rows.n_seqs ? pool.n_kv_heads * counted_of(seq_at(s0 + lane)) : 0;
                 uint64_t upto = mine;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -328,21 +346,32 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 base += __shfl_sync(0xffffffffu, upto, 31);
             }
             cur.s = seq_at(cur.seq);
-            const uint64_t per_head = cur.s.tiles_per_head(), in_seq = begin - base, in_head = in_seq % per_head;
+            const uint64_t per_head = counted_of(cur.s), in_seq = begin - base, in_head = in_seq % per_head;
             cur.head = (uint32_t)(in_seq / per_head);
-            // The last row tile that begins at or before in_head: 32 candidates at a time.
-            uint32_t lo = 0, span = cur.s.row_tiles;
-            while (span > 1) {
-                const uint32_t step = (span + 31) / 32, r = lo + lane * step;
-                const uint32_t below = __ballot_sync(0xffffffffu, lane * step < span && cur.s.tiles_before(r) <= in_head);
-                const uint32_t who = 31 - __clz(below);  // lane 0's holds
-                lo += who * step;
-                span = min(step, span - who * step);
+            if (cur.whole) {
+                cur.row_tile = (uint32_t)in_head;
+                cur.at = 0;
+            } else {
+                // The last row tile that begins at or before in_head: 32 candidates at a time.
+                uint32_t lo = 0, span = cur.s.row_tiles;
+                while (span > 1) {
+                    const uint32_t step = (span + 31) / 32, r = lo + lane * step;
+                    const uint32_t below = __ballot_sync(0xffffffffu, lane * step < span && cur.s.tiles_before(r) <= in_head);
+                    const uint32_t who = 31 - __clz(below);  // lane 0's holds
+                    lo += who * step;
+                    span = min(step, span - who * step);
+                }
+                cur.row_tile = lo;
+                cur.at = (uint32_t)(in_head - cur.s.tiles_before(lo));
             }
-            cur.row_tile = lo;
-            cur.at = (uint32_t)(in_head - cur.s.tiles_before(lo));
-            cur.count = cur.s.tiles(lo);
-            cur.left = run_tiles;
+            cur.count = cur.s.tiles(cur.row_tile);
+            run_tiles = cur.left;
+            if (cur.whole) {
+                run_tiles = 0;
+                Cursor ahead = cur;
+                Unit u;
+                while (ahead.take(p, capacity, KT, u)) run_tiles += u.tiles;
+            }
         }
         if (lane == 0) {
             sh.total = total;
@@ -381,12 +410,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             const bool there = query < d.n;
             const float4* from = reinterpret_cast<const float4*>(p.q + (there ? (uint64_t)(d.row0 + query) * p.q_stride + (uint64_t)(d.head * p.group + row % p.group) * p.q_head_stride
                                                                                : 0) + part * kSums);
+            float4 v[kSums / 4];  // every load under way before the first is waited for
             uint32_t top = 0;
-#pragma unroll 8
-            for (uint32_t i = 0; i < kSums / 4; ++i) {
-                const float4 v = there ? from[i] : make_float4(0.f, 0.f, 0.f, 0.f);
-                top = max(max(top, __float_as_uint(v.x) & 0x7fffffffu), max(__float_as_uint(v.y) & 0x7fffffffu, max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu)));
-            }
+#pragma unroll
+            for (uint32_t i = 0; i < kSums / 4; ++i) v[i] = there ? from[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (uint32_t i = 0; i < kSums / 4; ++i)
+                top = max(max(top, __float_as_uint(v[i].x) & 0x7fffffffu), max(__float_as_uint(v[i].y) & 0x7fffffffu, max(__float_as_uint(v[i].z) & 0x7fffffffu, __float_as_uint(v[i].w) & 0x7fffffffu)));
             sh.most[0][part][row] = __uint_as_float(top);
             rows_sync();
 #pragma unroll
@@ -396,14 +426,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             const uint32_t exponent = min(max(top >> 23, 1u), 253u);
             const float up = __uint_as_float((254u - exponent) << 23);
             factor = __uint_as_float(exponent << 23) * scale;
-#pragma unroll 2
+#pragma unroll
             for (uint32_t i = 0; i < kSums / 16; ++i) {  // 16 elements: 8 columns
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (uint32_t e = 0; e < 4; ++e) {
-                    const float4 v = there ? from[4 * i + e] : make_float4(0.f, 0.f, 0.f, 0.f);
-                    split_half2(v.x * up * 16384.f, v.y * up * 16384.f, hi[2 * e], lo[2 * e]);
-                    split_half2(v.z * up * 16384.f, v.w * up * 16384.f, hi[2 * e + 1], lo[2 * e + 1]);
+                    const float4 x = v[4 * i + e];
+                    split_half2(x.x * up * 16384.f, x.y * up * 16384.f, hi[2 * e], lo[2 * e]);
+                    split_half2(x.z * up * 16384.f, x.w * up * 16384.f, hi[2 * e + 1], lo[2 * e + 1]);
                 }
                 tmem_store_8(lanes + kQHi + part * (kSums / 2) + 8 * i, hi);
                 if constexpr (kQLoShared) {
@@ -596,9 +626,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             float keep = 0.f, grow = 0.f;
             for (uint32_t tile = 0; tile <= n_tiles && n_tiles > 0; ++tile) {
                 if (first) {
-                    // The next unit's queries go ahead of the last one's end: its scores are done.
+                    // The next unit's queries go ahead of the last one's end, whose scores are done, where registers hold both.
                     if (tile > 0) rows_sync();  // the maxima have been read
-                    if (tile < n_tiles && alive) load_queries(tile);
+                    if (HD < 256 && tile < n_tiles && alive) load_queries(tile);
                     if (tile > 0 && alive) {
                         add_product(tile - 1, keep, grow);
                         // A row's sums of probabilities meet.
@@ -609,6 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                         if (!alive) break;
                         store(sh.desc[(tile - 1) % kDescRing], first_sum, o, unit, part == 0);
                     }
+                    if (HD == 256 && tile < n_tiles && alive) load_queries(tile);
                     if (tile == n_tiles || !alive) break;
                     start_unit(tile);
                 }
@@ -965,51 +996,54 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
 }
 
 // Joins the parts of a unit that begins in CTA c's run: a warp to a row.
+constexpr uint32_t kJoinCtas = 8;  // to a cut row tile
 template <int HD>
 __global__ void __launch_bounds__(256) attention_chunk_join_kernel(const float* __restrict__ parts, float* __restrict__ out, uint32_t n_heads, uint32_t group) {
     constexpr int kPairs = HD / 64;
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5), c = blockIdx.x;
+    const uint32_t lane = threadIdx.x & 31, c = blockIdx.x;
     const ChunkHead cut = reinterpret_cast<const ChunkHead*>(parts + (uint64_t)2 * kMostCtas * kRows * (HD + 2))[c];
-    if (cut.last == 0 || r >= cut.n * group) return;
+    if (cut.last == 0) return;
     const float2* stats = reinterpret_cast<const float2*>(parts + (uint64_t)2 * kMostCtas * kRows * HD);
     const uint32_t n = cut.last - c + 1;
     auto slot_of = [&](uint32_t i) { return (uint64_t)(2 * (c + i) + (i == 0 ? 1 : 0)); };
-    float top = -INFINITY;
-    for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, stats[slot_of(i) * kRows + r].x);
-    top = warp_max(top);
-    const float shift = top == -INFINITY ? 0.f : top;
-    float total = 0.f;
-    float2 sum[kPairs];
+    for (uint32_t r = blockIdx.y * 8 + (threadIdx.x >> 5); r < cut.n * group; r += kJoinCtas * 8) {
+        float top = -INFINITY;
+        for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, stats[slot_of(i) * kRows + r].x);
+        top = warp_max(top);
+        const float shift = top == -INFINITY ? 0.f : top;
+        float total = 0.f;
+        float2 sum[kPairs];
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) sum[i] = make_float2(0.f, 0.f);
-    for (uint32_t i0 = 0; i0 < n; i0 += 32) {
-        float2 st = make_float2(-INFINITY, 0.f);
-        if (i0 + lane < n) st = stats[slot_of(i0 + lane) * kRows + r];
-        const float weight = st.x == -INFINITY ? 0.f : exp2f(st.x - shift);
-        total += weight * st.y;
-        const uint32_t many = min(32u, n - i0);
+        for (int i = 0; i < kPairs; ++i) sum[i] = make_float2(0.f, 0.f);
+        for (uint32_t i0 = 0; i0 < n; i0 += 32) {
+            float2 st = make_float2(-INFINITY, 0.f);
+            if (i0 + lane < n) st = stats[slot_of(i0 + lane) * kRows + r];
+            const float weight = st.x == -INFINITY ? 0.f : exp2f(st.x - shift);
+            total += weight * st.y;
+            const uint32_t many = min(32u, n - i0);
 #pragma unroll 4
-        for (uint32_t i = 0; i < many; ++i) {
-            const float w = __shfl_sync(0xffffffffu, weight, i);
-            const bool any = __shfl_sync(0xffffffffu, st.x, i) != -INFINITY;
-            const float2* from = reinterpret_cast<const float2*>(parts + (slot_of(i0 + i) * kRows + r) * HD) + lane;
+            for (uint32_t i = 0; i < many; ++i) {
+                const float w = __shfl_sync(0xffffffffu, weight, i);
+                const bool any = __shfl_sync(0xffffffffu, st.x, i) != -INFINITY;
+                const float2* from = reinterpret_cast<const float2*>(parts + (slot_of(i0 + i) * kRows + r) * HD) + lane;
 #pragma unroll
-            for (int k = 0; k < kPairs; ++k) {
-                const float2 v = from[32 * k];
-                if (any) {
-                    sum[k].x += w * v.x;
-                    sum[k].y += w * v.y;
+                for (int k = 0; k < kPairs; ++k) {
+                    const float2 v = from[32 * k];
+                    if (any) {
+                        sum[k].x += w * v.x;
+                        sum[k].y += w * v.y;
+                    }
                 }
             }
         }
-    }
-    total = warp_sum(total);
-    const float inverse = top == -INFINITY && total == 0.f ? 0.f : 1.f / total;
-    float2* to = reinterpret_cast<float2*>(out + (uint64_t)(cut.row0 + r / group) * n_heads * HD + (cut.head * group + r % group) * HD) + lane;
+        total = warp_sum(total);
+        const float inverse = top == -INFINITY && total == 0.f ? 0.f : 1.f / total;
+        float2* to = reinterpret_cast<float2*>(out + (uint64_t)(cut.row0 + r / group) * n_heads * HD + (cut.head * group + r % group) * HD) + lane;
 #pragma unroll
-    for (int k = 0; k < kPairs; ++k) to[32 * k] = make_float2(sum[k].x * inverse, sum[k].y * inverse);
+        for (int k = 0; k < kPairs; ++k) to[32 * k] = make_float2(sum[k].x * inverse, sum[k].y * inverse);
+    }
 }
 
 uint32_t chunk_ctas() {
@@ -1026,7 +1060,7 @@ cudaError_t launch_chunk(cudaStream_t stream, const ChunkParams& p) {
     const uint32_t ctas = chunk_ctas();
     e = launch_dependent(attention_chunk_kernel<FMT, HD>, dim3(ctas), dim3(kThreads), smem, stream, p);
     if (e != cudaSuccess || ctas == 1) return e;
-    return launch_dependent(attention_chunk_join_kernel<HD>, dim3(ctas - 1, kRows / 8), dim3(256), 0, stream, static_cast<const float*>(p.parts), p.out, p.n_heads, p.group);
+    return launch_dependent(attention_chunk_join_kernel<HD>, dim3(ctas - 1, kJoinCtas), dim3(256), 0, stream, static_cast<const float*>(p.parts), p.out, p.n_heads, p.group);
 }
 
 }  // namespace

@@ -795,9 +795,18 @@ uint64_t token_floats(uint32_t head_dim) {
 
 }  // namespace
 
-// Rows of a sequence up to which each is a unit of its own. The tensor-core kernel reads the positions once for all rows, and takes
-// the time of 128.
-constexpr uint32_t kTokenRows = 1;
+// Which kernel takes a sequence. The tensor-core kernel reads the positions once for all of a sequence's rows and takes the time of 128 of them: as long as
+// 2.5 rows here where contexts are long (8 sequences of 25000 positions, 8 heads of 64: 171 us; here 128 with 2 rows, 224 with 4), and 10 to 20 us beside that.
+// So sequences of up to two rows are always taken here, and all of a call's, with no second kernel, where what the tables can hold, 256 positions more
+// for a unit's beginning and end, times the rows beyond two, is what those 20 us read: (us, here and there) 8 sequences of up to 2900 positions with 5
+// rows 23 and 36, 64 of 500 with 4 rows 46 and 64, one of 1500 with 16 rows 17 and 26; past it 8 of 1100 with 16 rows 43 and 33, 64 of 100 with 8 rows 45 and 31.
+constexpr uint32_t kTokenRows = 2, kFewRows = 32;
+bool few_rows(const KvPool& pool, const KvRows& rows) {
+    if (rows.max_queries <= kTokenRows) return true;
+    const uint64_t positions = ((uint64_t)rows.max_pages << pool.page_shift) + 256;
+    const double elements = (double)positions * rows.n_seqs * pool.n_kv_heads * pool.head_dim * 2;
+    return rows.max_queries <= kFewRows && (rows.max_queries - kTokenRows) * elements <= (double)(1u << 27);
+}
 
 uint64_t attention_paged_scratch_floats(uint32_t, uint32_t, uint32_t head_dim) {
     return token_floats(head_dim) + attention_chunk_scratch_floats(head_dim);
@@ -805,7 +814,7 @@ uint64_t attention_paged_scratch_floats(uint32_t, uint32_t, uint32_t head_dim) {
 
 int attention_paged_launches(const KvPool& pool, const KvRows& rows, uint32_t) {
     const int tokens = token_ctas(pool, rows) == 1 || whole_units(rows, pool) ? 1 : 2;
-    if (rows.max_queries <= kTokenRows) return tokens;
+    if (few_rows(pool, rows)) return tokens;
     return attention_chunk_launches() + (rows.n_seqs > 1 ? tokens : 0);
 }
 
@@ -813,7 +822,7 @@ cudaError_t attention_paged(cudaStream_t stream, const KvPool& pool, const KvRow
                             float* scratch, float* out, uint32_t n_heads) {
     if (rows.n_rows == 0 || rows.n_seqs == 0) return cudaSuccess;
     // What the caller says of the rows decides which kernels run; the rows themselves, on the device, which of them takes a sequence.
-    const bool chunks = rows.max_queries > kTokenRows, tokens = !chunks || rows.n_seqs > 1;
+    const bool chunks = !few_rows(pool, rows), tokens = !chunks || rows.n_seqs > 1;
     const TokenParams p{pool, rows, q, out, scratch, q_stride, q_head_stride, n_heads, n_heads / pool.n_kv_heads, chunks ? kTokenRows : 0xffffffffu, whole_units(rows, pool)};
     const bool half = pool.format == BC_F16;
     cudaError_t e = cudaSuccess;
