@@ -1,4 +1,4 @@
-// The work of attention over pages for sequences of several new rows, as equal runs of key tiles: plain arithmetic, the same on
+// The work of attention over pages for sequences of several new rows, as equal runs: plain arithmetic, the same on
 // the host, which checks it, and in the kernel.
 //
 // A row tile is the query heads of `per_tile` neighbouring rows of one sequence and KV head. Row tile r sees the key tiles up to its last row's
@@ -31,6 +31,9 @@ __host__ __device__ inline uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a
     return sum;
 }
 
+// What a row tile counts beside its key tiles, ahead of them: its queries, its sums and the pipeline's start take about as long as two.
+constexpr uint32_t kRowTileCost = 2;
+
 struct ChunkSeq {
     uint32_t row0, n, end;   // rows row0 .. row0 + n - 1 are the sequence's; row `end` would be the position behind its last
     uint32_t len, held;      // positions, and those that its table can name
@@ -49,6 +52,8 @@ struct ChunkSeq {
     // Key tiles of row tiles 0 .. r - 1, r < row_tiles.
     __host__ __device__ uint64_t tiles_before(uint32_t r) const { return r + floor_sum(r, key_tile, per_tile, first() + per_tile - 1); }
     __host__ __device__ uint64_t tiles_per_head() const { return row_tiles == 0 ? 0 : tiles_before(row_tiles - 1) + tiles(row_tiles - 1); }
+    // What row tiles 0 .. r - 1 count as.
+    __host__ __device__ uint64_t counted_before(uint32_t r) const { return tiles_before(r) + (uint64_t)kRowTileCost * r; }
 };
 
 // n_rows: rows of the whole call; fewest: sequences of fewer rows are not these kernels' work.

@@ -66,18 +66,20 @@ struct ChunkHead {
 // A stretch of key tiles of one row tile.
 struct Unit {
     uint32_t seq, head, row_tile, tile0, tiles;
+    uint64_t last;  // where the row tile ends in the call's work: its last place
     bool begins, ends;
 };
 
-// Walks a run: of key tiles, or of whole row tiles.
+// Walks a run: of row tiles that count as their key tiles and kRowTileCost, or of whole ones that count as one.
 struct Cursor {
-    uint32_t seq, head, row_tile, at, count;
-    uint64_t left;
+    uint32_t seq, head, row_tile, count;
+    uint64_t at, left, end;  // in the row tile; of the run; the run's end
     bool whole;
     ChunkSeq s;
+    __device__ __forceinline__ uint64_t all() const { return whole ? 1 : (uint64_t)count + kRowTileCost; }
     __device__ __forceinline__ bool take(const ChunkParams& p, uint64_t capacity, uint32_t key_tile, Unit& u) {
         if (left == 0) return false;
-        if (at == count) {  // on to the next row tile
+        if (at == all()) {  // on to the next row tile
             at = 0;
             if (++row_tile == s.row_tiles) {
                 row_tile = 0;
@@ -86,7 +88,7 @@ struct Cursor {
                     do {
                         ++seq;
                         s = chunk_seq(p.rows.starts[seq], p.rows.starts[seq + 1], p.rows.lens[seq], capacity, p.rows.n_rows, p.fewest, s.per_tile, key_tile);
-                    } while (s.row_tiles == 0);  // tiles are left, so a sequence with some follows
+                    } while (s.row_tiles == 0);  // something is left, so a sequence with some follows
                 }
             }
             count = s.tiles(row_tile);
@@ -94,13 +96,16 @@ struct Cursor {
         u.seq = seq;
         u.head = head;
         u.row_tile = row_tile;
-        u.tile0 = at;
-        u.tiles = whole ? count : (uint32_t)min((uint64_t)(count - at), left);
-        u.begins = at == 0;
-        at += u.tiles;
-        u.ends = at == count;
-        left -= whole ? 1 : u.tiles;
-        return true;
+        u.last = end - left - at + all() - 1;
+        const uint64_t upto = min(all(), at + left);
+        u.tile0 = whole ? 0 : (uint32_t)(max(at, (uint64_t)kRowTileCost) - kRowTileCost);
+        const uint32_t tile1 = whole ? count : (uint32_t)(max(upto, (uint64_t)kRowTileCost) - kRowTileCost);
+        u.tiles = tile1 - u.tile0;
+        u.begins = u.tile0 == 0;
+        u.ends = tile1 == count;
+        left -= upto - at;
+        at = upto;
+        return u.tiles > 0;  // a run may end ahead of a row tile's first key tile
     }
 };
 
@@ -212,6 +217,25 @@ __device__ __forceinline__ uint32_t seen_bits(const TileInfo<KT, FMT>& info, uin
     return there & (n >= 16 ? 0xffffu : (1u << n) - 1);
 }
 
+// Four lanes' four pieces each: piece i of lane j becomes piece j of lane i. A row's memory is read and written four lanes at a time, 64 bytes, while a
+// thread works on a row of its own.
+__device__ __forceinline__ void quad_transpose(float4 (&v)[4], uint32_t lane) {
+#pragma unroll
+    for (int bit = 1; bit <= 2; bit <<= 1) {
+        const bool upper = lane & bit;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i & bit) continue;
+            float4 &a = v[i], &b = v[i | bit], give = upper ? a : b;
+            give.x = __shfl_xor_sync(0xffffffffu, give.x, bit);
+            give.y = __shfl_xor_sync(0xffffffffu, give.y, bit);
+            give.z = __shfl_xor_sync(0xffffffffu, give.z, bit);
+            give.w = __shfl_xor_sync(0xffffffffu, give.w, bit);
+            (upper ? a : b) = give;
+        }
+    }
+}
+
 // A barrier of several warps that a warp may leave: an mbarrier with an arrival of each.
 struct WarpsBarrier {
     uint32_t bar, phase;
@@ -238,7 +262,7 @@ struct Shared {
     uint32_t not_finite[FMT == BC_F16 ? kUnits : 1][FMT == BC_F16 ? HD : 1];  // by unit: the first position with such a value, of each element
     uint32_t any_not_finite[kUnits];
     uint64_t bars[4 * kStages + 4 * kRaw + 10 + kDescRing];
-    uint64_t total, run_tiles;  // key tiles of the call, and of the CTA's run
+    uint64_t counted, ahead[2];  // the call's work; key tiles ahead of the run's beginning, and of its end
     Place place;
     uint32_t tmem;
     int dead, never;            // whether a wait has run out; a flag that nobody raises
@@ -296,20 +320,21 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
     }
     if (warp == kMmaWarp) tmem_alloc(smem_u32(&sh.tmem), kTmemColumns);
     pdl_wait();
-    if (warp == kCopyWarp) {
-        // The run, and where it begins.
+    if (warp == kCopyWarp || warp == kCopyWarp + 1) {
+        // The run, and where it begins and ends.
         auto seq_at = [&](uint32_t s) {
             return chunk_seq(p.rows.starts[s], p.rows.starts[s + 1], p.rows.lens[s], capacity, p.rows.n_rows, p.fewest, per_tile, KT);
         };
-        uint64_t total = 0, units = 0, run_tiles = 0;
+        uint64_t total = 0, units = 0;
         uint32_t longest = 0;
-        Cursor cur{};
+        uint64_t my_tiles = 0, my_units = 0;  // of the lane's first sequence
         for (uint32_t s = lane; s < p.rows.n_seqs; s += 32) {
             const ChunkSeq sq = seq_at(s);
-            if (sq.row_tiles == 0) continue;
-            total += pool.n_kv_heads * sq.tiles_per_head();
-            units += (uint64_t)pool.n_kv_heads * sq.row_tiles;
-            longest = max(longest, sq.tiles(sq.row_tiles - 1));
+            const uint64_t tiles = pool.n_kv_heads * sq.tiles_per_head(), row_tiles = (uint64_t)pool.n_kv_heads * sq.row_tiles;
+            if (s == lane) my_tiles = tiles, my_units = row_tiles;
+            total += tiles;
+            units += row_tiles;
+            if (row_tiles > 0) longest = max(longest, sq.tiles(sq.row_tiles - 1));
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
@@ -317,38 +342,50 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             units += __shfl_xor_sync(0xffffffffu, units, o);
         }
         longest = __reduce_max_sync(0xffffffffu, longest);
-        // Runs of key tiles are equal but cut row tiles; runs of whole row tiles are not, and nothing is cut. A row tile costs about two key tiles beside its
-        // own (its queries, its sums), a cut one more to join. (512 rows of 8 heads from position 0, 128 row tiles of 1 to 4 key tiles: 30 us cut, 21
-        // whole.)
+        // Equal runs cut row tiles; runs of whole ones are not equal, but nothing is cut, which saves a row tile's cost and a part to join. (512 rows of 8
+        // heads from position 0, 128 row tiles of 1 to 4 key tiles: 33 us cut, 20 whole.)
         const uint64_t ctas = gridDim.x, units_each = (units + ctas - 1) / ctas;
-        cur.whole = units_each * (longest + 2) <= total / ctas + 2 * (units_each + 1) + 1;
-        const uint64_t counted = cur.whole ? units : total, runs = min(ctas, counted);
-        auto counted_of = [&](const ChunkSeq& sq) { return cur.whole ? (uint64_t)sq.row_tiles : sq.tiles_per_head(); };
-        if (blockIdx.x < runs) {
-            const uint64_t begin = counted * blockIdx.x / runs;
-            cur.left = counted * (blockIdx.x + 1) / runs - begin;
+        const bool whole = units_each * (longest + kRowTileCost) <= (total + kRowTileCost * units) / ctas + kRowTileCost + 1;
+        const uint64_t counted = whole ? units : total + kRowTileCost * units, runs = min(ctas, counted);
+        // Where the run begins, and the key tiles ahead of it; the other warp, where it ends.
+        const bool begin = warp == kCopyWarp;
+        const uint64_t place = blockIdx.x < runs ? counted * (blockIdx.x + (begin ? 0 : 1)) / runs : counted;
+        uint64_t ahead = place < counted ? 0 : total;
+        Cursor cur{};
+        cur.whole = whole;
+        if (place < counted) {
             uint64_t base = 0;
             for (uint32_t s0 = 0; s0 < p.rows.n_seqs; s0 += 32) {
-                const uint64_t mine = s0 + lane < p.rows.n_seqs ? pool.n_kv_heads * counted_of(seq_at(s0 + lane)) : 0;
-                uint64_t upto = mine;
+                uint64_t tiles = my_tiles, row_tiles = my_units;
+                if (s0 > 0) {
+                    tiles = row_tiles = 0;
+                    if (s0 + lane < p.rows.n_seqs) {
+                        const ChunkSeq sq = seq_at(s0 + lane);
+                        tiles = pool.n_kv_heads * sq.tiles_per_head();
+                        row_tiles = (uint64_t)pool.n_kv_heads * sq.row_tiles;
+                    }
+                }
+                const uint64_t mine = whole ? row_tiles : tiles + kRowTileCost * row_tiles;
+                uint64_t upto = mine, tiles_upto = tiles;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
-                    const uint64_t other = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (lane >= (uint32_t)o) upto += other;
+                    const uint64_t other = __shfl_up_sync(0xffffffffu, upto, o), other_tiles = __shfl_up_sync(0xffffffffu, tiles_upto, o);
+                    if (lane >= (uint32_t)o) upto += other, tiles_upto += other_tiles;
                 }
-                const uint32_t beyond = __ballot_sync(0xffffffffu, base + upto > begin);
+                const uint32_t beyond = __ballot_sync(0xffffffffu, base + upto > place);
+                const int who = beyond ? __ffs(beyond) - 1 : 31;
+                base += __shfl_sync(0xffffffffu, beyond ? upto - mine : upto, who);
+                ahead += __shfl_sync(0xffffffffu, beyond ? tiles_upto - tiles : tiles_upto, who);
                 if (beyond) {
-                    const int who = __ffs(beyond) - 1;
                     cur.seq = s0 + who;
-                    base += __shfl_sync(0xffffffffu, upto - mine, who);
                     break;
                 }
-                base += __shfl_sync(0xffffffffu, upto, 31);
             }
             cur.s = seq_at(cur.seq);
-            const uint64_t per_head = counted_of(cur.s), in_seq = begin - base, in_head = in_seq % per_head;
+            const uint64_t tiles_per_head = cur.s.tiles_per_head(), per_head = whole ? cur.s.row_tiles : tiles_per_head + (uint64_t)kRowTileCost * cur.s.row_tiles;
+            const uint64_t in_seq = place - base, in_head = in_seq % per_head;
             cur.head = (uint32_t)(in_seq / per_head);
-            if (cur.whole) {
+            if (whole) {
                 cur.row_tile = (uint32_t)in_head;
                 cur.at = 0;
             } else {
@@ -356,26 +393,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 uint32_t lo = 0, span = cur.s.row_tiles;
                 while (span > 1) {
                     const uint32_t step = (span + 31) / 32, r = lo + lane * step;
-                    const uint32_t below = __ballot_sync(0xffffffffu, lane * step < span && cur.s.tiles_before(r) <= in_head);
+                    const uint32_t below = __ballot_sync(0xffffffffu, lane * step < span && cur.s.counted_before(r) <= in_head);
                     const uint32_t who = 31 - __clz(below);  // lane 0's holds
                     lo += who * step;
                     span = min(step, span - who * step);
                 }
                 cur.row_tile = lo;
-                cur.at = (uint32_t)(in_head - cur.s.tiles_before(lo));
+                cur.at = in_head - cur.s.counted_before(lo);
             }
             cur.count = cur.s.tiles(cur.row_tile);
-            run_tiles = cur.left;
-            if (cur.whole) {
-                run_tiles = 0;
-                Cursor ahead = cur;
-                Unit u;
-                while (ahead.take(p, capacity, KT, u)) run_tiles += u.tiles;
-            }
+            ahead += cur.head * tiles_per_head + cur.s.tiles_before(cur.row_tile);
+            if (cur.at > kRowTileCost) ahead += cur.at - kRowTileCost;
+            cur.end = counted * (blockIdx.x + 1) / runs;
+            cur.left = cur.end - place;
         }
-        if (lane == 0) {
-            sh.total = total;
-            sh.run_tiles = run_tiles;
+        if (lane == 0) sh.ahead[begin ? 0 : 1] = ahead;
+        if (lane == 0 && begin) {
+            sh.counted = counted;
             sh.place.cut = ChunkHead{0, 0, 0, 0};
             sh.place.cursor = cur;
             sh.place.unit.tiles = sh.place.in_unit = 0;
@@ -386,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = sh.tmem;
-    const uint32_t n_tiles = (uint32_t)sh.run_tiles;
+    const uint32_t n_tiles = (uint32_t)(sh.ahead[1] - sh.ahead[0]);
     bool alive = true;
 
     if (warp < kRowWarps) {
@@ -408,15 +442,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             const TileDesc& d = sh.desc[tile % kDescRing];
             const uint32_t query = row / p.group;
             const bool there = query < d.n;
-            const float4* from = reinterpret_cast<const float4*>(p.q + (there ? (uint64_t)(d.row0 + query) * p.q_stride + (uint64_t)(d.head * p.group + row % p.group) * p.q_head_stride
-                                                                               : 0) + part * kSums);
-            float4 v[kSums / 4];  // every load under way before the first is waited for
+            const uint64_t mine = there ? (uint64_t)(d.row0 + query) * p.q_stride + (uint64_t)(d.head * p.group + row % p.group) * p.q_head_stride : ~0ull;
+            float4 v[kSums / 16][4];  // every load under way before the first is waited for
             uint32_t top = 0;
 #pragma unroll
-            for (uint32_t i = 0; i < kSums / 4; ++i) v[i] = there ? from[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (uint32_t r = 0; r < 4; ++r) {
+                const uint64_t from = __shfl_sync(0xffffffffu, mine, (lane & ~3u) + r);
 #pragma unroll
-            for (uint32_t i = 0; i < kSums / 4; ++i)
-                top = max(max(top, __float_as_uint(v[i].x) & 0x7fffffffu), max(__float_as_uint(v[i].y) & 0x7fffffffu, max(__float_as_uint(v[i].z) & 0x7fffffffu, __float_as_uint(v[i].w) & 0x7fffffffu)));
+                for (uint32_t i = 0; i < kSums / 16; ++i)
+                    v[i][r] = from != ~0ull ? *reinterpret_cast<const float4*>(p.q + from + part * kSums + 16 * i + 4 * (lane & 3)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < kSums / 16; ++i) quad_transpose(v[i], lane);
+#pragma unroll
+            for (uint32_t i = 0; i < kSums / 4; ++i) {
+                const float4 x = v[i / 4][i % 4];
+                top = max(max(top, __float_as_uint(x.x) & 0x7fffffffu), max(__float_as_uint(x.y) & 0x7fffffffu, max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu)));
+            }
             sh.most[0][part][row] = __uint_as_float(top);
             rows_sync();
 #pragma unroll
@@ -431,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (uint32_t e = 0; e < 4; ++e) {
-                    const float4 x = v[4 * i + e];
+                    const float4 x = v[i][e];
                     split_half2(x.x * up * 16384.f, x.y * up * 16384.f, hi[2 * e], lo[2 * e]);
                     split_half2(x.z * up * 16384.f, x.w * up * 16384.f, hi[2 * e + 1], lo[2 * e + 1]);
                 }
@@ -588,23 +630,33 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             const bool whole = desc.begins && desc.ends;
             const uint32_t slot = 2 * blockIdx.x + (desc.begins ? 1 : 0);
             if (whole) times *= top == -INFINITY && total == 0.f ? 0.f : 1.f / total;
-            float* to = (whole ? p.out + (uint64_t)(desc.row0 + row / p.group) * p.n_heads * HD + (desc.head * p.group + row % p.group) * HD
-                               : p.parts + ((uint64_t)slot * kRows + row) * HD) + first_element;
+            const uint64_t mine = row / p.group >= desc.n ? ~0ull
+                                  : whole ? (uint64_t)(desc.row0 + row / p.group) * p.n_heads * HD + (desc.head * p.group + row % p.group) * HD
+                                          : ((uint64_t)slot * kRows + row) * HD;
+            float* const to = (whole ? p.out : p.parts) + first_element + 4 * (lane & 3);
             const bool any = FMT == BC_F16 && sh.any_not_finite[desc.unit % kUnits];
-            if (row / p.group < desc.n) {
 #pragma unroll
-                for (uint32_t i = 0; i < HD / kParts / 2; i += 2) {
-                    float4 v = make_float4(sums[i].x * times, sums[i].y * times, sums[i + 1].x * times, sums[i + 1].y * times);
+            for (uint32_t i = 0; i < HD / kParts / 16; ++i) {
+                float4 v[4];
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    const float2 a = sums[8 * i + 2 * k], b = sums[8 * i + 2 * k + 1];
+                    v[k] = make_float4(a.x * times, a.y * times, b.x * times, b.y * times);
                     if constexpr (FMT == BC_F16) {
                         if (any) {
-                            const uint32_t* at = sh.not_finite[desc.unit % kUnits] + first_element + 2 * i;
-                            if ((int64_t)at[0] <= limit) v.x = __uint_as_float(0x7fc00000u);
-                            if ((int64_t)at[1] <= limit) v.y = __uint_as_float(0x7fc00000u);
-                            if ((int64_t)at[2] <= limit) v.z = __uint_as_float(0x7fc00000u);
-                            if ((int64_t)at[3] <= limit) v.w = __uint_as_float(0x7fc00000u);
+                            const uint32_t* at = sh.not_finite[desc.unit % kUnits] + first_element + 16 * i + 4 * k;
+                            if ((int64_t)at[0] <= limit) v[k].x = __uint_as_float(0x7fc00000u);
+                            if ((int64_t)at[1] <= limit) v[k].y = __uint_as_float(0x7fc00000u);
+                            if ((int64_t)at[2] <= limit) v[k].z = __uint_as_float(0x7fc00000u);
+                            if ((int64_t)at[3] <= limit) v[k].w = __uint_as_float(0x7fc00000u);
                         }
                     }
-                    *reinterpret_cast<float4*>(to + 2 * i) = v;
+                }
+                quad_transpose(v, lane);
+#pragma unroll
+                for (uint32_t r = 0; r < 4; ++r) {
+                    const uint64_t at = __shfl_sync(0xffffffffu, mine, (lane & ~3u) + r);
+                    if (at != ~0ull) *reinterpret_cast<float4*>(to + at + 16 * i) = v[r];
                 }
             }
             if (!whole && stats)
@@ -914,11 +966,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                         d.ends = u.ends;
                         if (s.held < s.len) leave_fault(pool, kFaultTable);
                         if (u.begins && !u.ends && at.in_unit == 0) {
-                            // The CTA whose run holds the row tile's last key tile: run c is [total c / runs, total (c + 1) / runs).
-                            const uint64_t total = sh.total, runs = min((uint64_t)gridDim.x, total), last_tile = total * blockIdx.x / runs + j + at.cursor.count - 1;
-                            uint32_t last = (uint32_t)(last_tile * runs / total);
-                            while (total * (last + 1) / runs <= last_tile) ++last;
-                            while (total * last / runs > last_tile) --last;
+                            // The CTA whose run holds the row tile's end: run c is [total c / runs, total (c + 1) / runs).
+                            const uint64_t total = sh.counted, runs = min((uint64_t)gridDim.x, total);
+                            uint32_t last = (uint32_t)(u.last * runs / total);
+                            while (total * (last + 1) / runs <= u.last) ++last;
+                            while (total * last / runs > u.last) --last;
                             at.cut = ChunkHead{d.row0, d.n, d.head, last};
                         }
                         ++at.in_unit;
