@@ -443,22 +443,42 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             const uint32_t query = row / p.group;
             const bool there = query < d.n;
             const uint64_t mine = there ? (uint64_t)(d.row0 + query) * p.q_stride + (uint64_t)(d.head * p.group + row % p.group) * p.q_head_stride : ~0ull;
-            float4 v[kSums / 16][4];  // every load under way before the first is waited for
+            uint64_t from[4];  // of the quad's rows
+#pragma unroll
+            for (uint32_t r = 0; r < 4; ++r) {
+                from[r] = __shfl_sync(0xffffffffu, mine, (lane & ~3u) + r);
+                if (from[r] != ~0ull) from[r] += part * kSums + 4 * (lane & 3);
+            }
+            // 32 elements at a time, in loops: twice the memory costs less than a thousand instructions in a line (heads of 256: 27000 cycles so, 8000 in loops).
+            using Block = float4[2][4];
+            auto load = [&](uint32_t block, Block& v) {
+#pragma unroll
+                for (uint32_t i = 0; i < 2; ++i)
+#pragma unroll
+                    for (uint32_t r = 0; r < 4; ++r)
+                        v[i][r] = from[r] != ~0ull ? *reinterpret_cast<const float4*>(p.q + from[r] + 32 * block + 16 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+            };
+            auto larger = [](uint32_t most, const float4& x) {
+                return max(max(most, __float_as_uint(x.x) & 0x7fffffffu), max(__float_as_uint(x.y) & 0x7fffffffu, max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu)));
+            };
+            Block v;
+            uint32_t tops[4] = {0, 0, 0, 0};  // of the quad's rows, this lane's elements
+#pragma unroll 1
+            for (uint32_t block = 0; block < kSums / 32; ++block) {
+                load(block, v);
+#pragma unroll
+                for (uint32_t i = 0; i < 2; ++i)
+#pragma unroll
+                    for (uint32_t r = 0; r < 4; ++r) tops[r] = larger(tops[r], v[i][r]);
+            }
             uint32_t top = 0;
 #pragma unroll
             for (uint32_t r = 0; r < 4; ++r) {
-                const uint64_t from = __shfl_sync(0xffffffffu, mine, (lane & ~3u) + r);
-#pragma unroll
-                for (uint32_t i = 0; i < kSums / 16; ++i)
-                    v[i][r] = from != ~0ull ? *reinterpret_cast<const float4*>(p.q + from + part * kSums + 16 * i + 4 * (lane & 3)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                tops[r] = max(tops[r], __shfl_xor_sync(0xffffffffu, tops[r], 1));
+                tops[r] = max(tops[r], __shfl_xor_sync(0xffffffffu, tops[r], 2));
+                if ((lane & 3) == r) top = tops[r];
             }
-#pragma unroll
-            for (uint32_t i = 0; i < kSums / 16; ++i) quad_transpose(v[i], lane);
-#pragma unroll
-            for (uint32_t i = 0; i < kSums / 4; ++i) {
-                const float4 x = v[i / 4][i % 4];
-                top = max(max(top, __float_as_uint(x.x) & 0x7fffffffu), max(__float_as_uint(x.y) & 0x7fffffffu, max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu)));
-            }
+            if (kSums > 32) load(0, v);
             sh.most[0][part][row] = __uint_as_float(top);
             rows_sync();
 #pragma unroll
@@ -468,23 +488,29 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             const uint32_t exponent = min(max(top >> 23, 1u), 253u);
             const float up = __uint_as_float((254u - exponent) << 23);
             factor = __uint_as_float(exponent << 23) * scale;
+#pragma unroll 1
+            for (uint32_t block = 0; block < kSums / 32; ++block) {
 #pragma unroll
-            for (uint32_t i = 0; i < kSums / 16; ++i) {  // 16 elements: 8 columns
-                uint32_t hi[8], lo[8];
+                for (uint32_t i = 0; i < 2; ++i) {  // 16 elements: 8 columns
+                    quad_transpose(v[i], lane);
+                    uint32_t hi[8], lo[8];
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) {
-                    const float4 x = v[i][e];
-                    split_half2(x.x * up * 16384.f, x.y * up * 16384.f, hi[2 * e], lo[2 * e]);
-                    split_half2(x.z * up * 16384.f, x.w * up * 16384.f, hi[2 * e + 1], lo[2 * e + 1]);
+                    for (uint32_t e = 0; e < 4; ++e) {
+                        const float4 x = v[i][e];
+                        split_half2(x.x * up * 16384.f, x.y * up * 16384.f, hi[2 * e], lo[2 * e]);
+                        split_half2(x.z * up * 16384.f, x.w * up * 16384.f, hi[2 * e + 1], lo[2 * e + 1]);
+                    }
+                    const uint32_t sixteen = 2 * block + i;
+                    tmem_store_8(lanes + kQHi + part * (kSums / 2) + 8 * sixteen, hi);
+                    if constexpr (kQLoShared) {
+                        uint8_t* to = sh.q_lo + (row >> 3) * kKeyStep + (part * (kSums / 8) + 2 * sixteen) * kCore + (row & 7) * 16;
+                        *reinterpret_cast<uint4*>(to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        *reinterpret_cast<uint4*>(to + kCore) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+                    } else {
+                        tmem_store_8(lanes + kQLo + part * (kSums / 2) + 8 * sixteen, lo);
+                    }
                 }
-                tmem_store_8(lanes + kQHi + part * (kSums / 2) + 8 * i, hi);
-                if constexpr (kQLoShared) {
-                    uint8_t* to = sh.q_lo + (row >> 3) * kKeyStep + (part * (kSums / 8) + 2 * i) * kCore + (row & 7) * 16;
-                    *reinterpret_cast<uint4*>(to) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                    *reinterpret_cast<uint4*>(to + kCore) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
-                } else {
-                    tmem_store_8(lanes + kQLo + part * (kSums / 2) + 8 * i, lo);
-                }
+                if (block + 1 < kSums / 32) load(block + 1, v);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             if (kQLoShared) fence_proxy_async();
@@ -642,15 +668,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 for (uint32_t k = 0; k < 4; ++k) {
                     const float2 a = sums[8 * i + 2 * k], b = sums[8 * i + 2 * k + 1];
                     v[k] = make_float4(a.x * times, a.y * times, b.x * times, b.y * times);
-                    if constexpr (FMT == BC_F16) {
-                        if (any) {
-                            const uint32_t* at = sh.not_finite[desc.unit % kUnits] + first_element + 16 * i + 4 * k;
-                            if ((int64_t)at[0] <= limit) v[k].x = __uint_as_float(0x7fc00000u);
-                            if ((int64_t)at[1] <= limit) v[k].y = __uint_as_float(0x7fc00000u);
-                            if ((int64_t)at[2] <= limit) v[k].z = __uint_as_float(0x7fc00000u);
-                            if ((int64_t)at[3] <= limit) v[k].w = __uint_as_float(0x7fc00000u);
-                        }
-                    }
                 }
                 quad_transpose(v, lane);
 #pragma unroll
@@ -658,6 +675,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                     const uint64_t at = __shfl_sync(0xffffffffu, mine, (lane & ~3u) + r);
                     if (at != ~0ull) *reinterpret_cast<float4*>(to + at + 16 * i) = v[r];
                 }
+            }
+            if (any) {  // after the quad's stores
+                __syncwarp();
+                const uint32_t* at = sh.not_finite[desc.unit % kUnits] + first_element;
+                if (mine != ~0ull)
+#pragma unroll 1
+                    for (uint32_t e = 0; e < HD / kParts; ++e)
+                        if ((int64_t)at[FMT == BC_F16 ? e : 0] <= limit) (whole ? p.out : p.parts)[mine + first_element + e] = __uint_as_float(0x7fc00000u);
             }
             if (!whole && stats)
                 *reinterpret_cast<float2*>(p.parts + (uint64_t)2 * kMostCtas * kRows * HD + ((uint64_t)slot * kRows + row) * 2) = make_float2(top, total);
