@@ -956,15 +956,21 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             }
             if (__all_sync(0xffffffffu, n_tiles > 0 && alive)) product(n_tiles - 1);
         } else if (warp == kCopyWarp) {
-            // ---- the walk through the run, and the pages' bytes: a lane per 16 positions of keys, values, and either's scales.
+            // ---- the walk through the run, and the pages' bytes: a lane per 16 positions of keys, values, and either's scales. What lies in one page
+            // is one copy, the first of its lanes': copies' number, not their bytes, is what the copying engine's time goes by (tiles of 128 positions
+            // in 32 copies kept everyone waiting).
             Place& at = sh.place;
             constexpr uint32_t kGroups = KT / 16, kRowBytes = RawKeys<KT, FMT, HD>::kRowBytes;
             const uint32_t page_slots = (1u << pool.page_shift) - 1;
             uint32_t keys_issued = 0, values_issued = 0;
             const uint32_t group = lane % kGroups, what = lane / kGroups;
+            const uint32_t segment = min(page_slots + 1, KT);  // positions of a copy
+            const bool leads = group * 16 % segment == 0;
+            uint32_t value_segments = 0;  // of the tile before
             uint64_t value_rows_at = ~0ull;  // of the tile before
             for (uint32_t i = 0; i <= n_tiles && n_tiles > 0; ++i) {
                 uint64_t rows_at = ~0ull;
+                uint32_t segments = 0;
                 if (i < n_tiles) {
                     const uint32_t j = i;
                     TileDesc& d = sh.desc[j % kDescRing];
@@ -1010,7 +1016,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                     }
                     const bool there = page < pool.n_pages;
                     const uint32_t groups = __ballot_sync(0xffffffffu, there) & ((1u << kGroups) - 1);
-                    if (there) rows_at = kv_row_at(pool, page, d.head, key & page_slots);
+                    segments = __popc(__ballot_sync(0xffffffffu, there && leads) & ((1u << kGroups) - 1));
+                    if (there && leads) rows_at = kv_row_at(pool, page, d.head, key & page_slots);
                     const uint32_t slot = j % RAW, bar = rk_full + 8 * slot;
                     await(alive, rk_free + 8 * slot, ((j / RAW) & 1) ^ 1, dead, 11);
                     if (!alive) break;
@@ -1018,15 +1025,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                     if (lane == 0) {
                         d.groups = groups;
                         mbar_arrive(described + 8 * (j % kDescRing));
-                        mbar_arrive_expect(bar, __popc(groups) * 16 * (kRowBytes + (FMT == BC_I8 ? 8 : 0)));
+                        mbar_arrive_expect(bar, segments * segment * (kRowBytes + (FMT == BC_I8 ? 8 : 0)));
                     }
                     __syncwarp();
-                    if (there) {
+                    if (there && leads) {
                         RawKeys<KT, FMT, HD>& raw = sh.raw_keys[slot];
                         if (what == 0)
-                            bulk_load(smem_u32(raw.keys) + group * 16 * kRowBytes, pool.k + rows_at, 16 * kRowBytes, bar);
+                            bulk_load(smem_u32(raw.keys) + group * 16 * kRowBytes, pool.k + rows_at, segment * kRowBytes, bar);
                         else if (FMT == BC_I8 && what < 3)
-                            bulk_load(smem_u32(what == 2 ? raw.dv : raw.dk) + group * 64, (what == 2 ? pool.v : pool.k) + kv_scale_at(pool, page, d.head, key & page_slots), 64, bar);
+                            bulk_load(smem_u32(what == 2 ? raw.dv : raw.dk) + group * 64, (what == 2 ? pool.v : pool.k) + kv_scale_at(pool, page, d.head, key & page_slots), segment * 4, bar);
                     }
                     __syncwarp();
                 }
@@ -1035,12 +1042,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                     await(alive, rv_free + 8 * slot, ((j / RAW) & 1) ^ 1, dead, 16);
                     if (!alive) break;
                     ++values_issued;
-                    if (lane == 0) mbar_arrive_expect(bar, __popc(sh.desc[j % kDescRing].groups) * 16 * kRowBytes);
+                    if (lane == 0) mbar_arrive_expect(bar, value_segments * segment * kRowBytes);
                     __syncwarp();
-                    if (what == 0 && value_rows_at != ~0ull) bulk_load(smem_u32(sh.raw_values[slot]) + group * 16 * kRowBytes, pool.v + value_rows_at, 16 * kRowBytes, bar);
+                    if (what == 0 && value_rows_at != ~0ull) bulk_load(smem_u32(sh.raw_values[slot]) + group * 16 * kRowBytes, pool.v + value_rows_at, segment * kRowBytes, bar);
                     __syncwarp();
                 }
                 value_rows_at = rows_at;
+                value_segments = segments;
             }
             if (lane == 0) reinterpret_cast<ChunkHead*>(p.parts + (uint64_t)2 * kMostCtas * kRows * (HD + 2))[blockIdx.x] = alive ? at.cut : ChunkHead{0, 0, 0, 0};
             // Copies in flight end before the CTA does: the unpacking warps wait for them, or this one does when those gave up.
