@@ -562,8 +562,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 }
             }
         };
-        // The tile's scores to probabilities, in place: of each 16 the upper halves, then the lower. 16 at a time, twice (for their maximum, then again), in loops:
-        // warps that run through a thousand instructions in a line wait for those more than for anything else.
+        // The tile's scores to probabilities, in place: of each 16 the upper halves, then the lower. 16 at a time, twice (for their maximum, then again), in loops of 16 and not
+        // more: roles run side by side, and what bounds all of them is that they fetch each other's instructions away (2048 rows over 10000 positions: 672 us; 730
+        // with two of them in a line, 950 with all four; scores kept in registers between the two, 10 % slower than read twice).
         auto take = [&](uint32_t tile, float& keep, float& grow) {
             const uint32_t buffer = tile & 1, scores_at = lanes + buffer * KT + first_score;
             const TileInfo<KT, FMT>& info = sh.info[tile % kRing];
@@ -572,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             tc_fence_after_sync();
             const int32_t see = (int32_t)max(min((int64_t)limit - sh.desc[tile % kDescRing].key0 - first_score, (int64_t)KT), (int64_t)-1);  // the last score seen
             float most[2] = {-INFINITY, -INFINITY};
-#pragma unroll 4
+#pragma unroll 1
             for (uint32_t c = 0; c < kScores; c += 16) {
                 float2 x[8];
                 load_scores(scores_at, info, see, c, x);
@@ -895,7 +896,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
         if (warp == kMmaWarp) {
             // ---- the tensor core. Lower halves first: what a sum cuts off grows with what is there already. Every loop and branch goes by a vote: the
             // compiler then keeps the descriptors in uniform registers, where the instruction wants them (without, an instruction took 106 cycles
-            // to issue, of the 64 that it runs).
+            // to issue, of the 64 that it runs). In loops too: unrolled, chunks of heads of 256 took 199 us, so 182.
             const uint32_t scores_idesc = umma_idesc_f16(kRows, KT), values_idesc = umma_idesc_f16(kRows, HD);
             const uint64_t q_lo = umma_desc(smem_u32(sh.q_lo), kCore, kKeyStep), keys0 = umma_desc(smem_u32(sh.keys), kCore, kKeyStep),
                            values0 = umma_desc(smem_u32(sh.values), kKeyStep, kCore);
@@ -909,9 +910,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 const uint64_t v = values0 + (j % ST) * (S::kTileBytes >> 4);
                 const uint32_t weights = tmem + (j & 1) * KT;
                 if (elect_one()) {
-#pragma unroll
+#pragma unroll 1
                     for (uint32_t part = 0; part < 2; ++part)
-#pragma unroll
+#pragma unroll 1
                         for (uint32_t ks = 0; ks < KT / 16; ++ks)
                             umma_f16_a_tmem(tmem + kPv, weights + ks * 16 + (part ^ 1) * 8, v + (uint64_t)(ks * 2 * kKeyStep >> 4), values_idesc, part | ks);
                 }
@@ -936,14 +937,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 const uint64_t keys = keys0 + (j % ST) * (S::kTileBytes >> 4);
                 const uint32_t to = tmem + (j & 1) * KT;
                 if (elect_one()) {
-#pragma unroll
+#pragma unroll 1
                     for (uint32_t ks = 0; ks < HD / 16; ++ks) {
                         if constexpr (kQLoShared)
                             umma_f16(to, q_lo + (uint64_t)(ks * 2 * kCore >> 4), keys + (uint64_t)(ks * 2 * kCore >> 4), scores_idesc, ks);
                         else
                             umma_f16_a_tmem(to, tmem + kQLo + ks * 8, keys + (uint64_t)(ks * 2 * kCore >> 4), scores_idesc, ks);
                     }
-#pragma unroll
+#pragma unroll 1
                     for (uint32_t ks = 0; ks < HD / 16; ++ks) umma_f16_a_tmem(to, tmem + kQHi + ks * 8, keys + (uint64_t)(ks * 2 * kCore >> 4), scores_idesc, 1);
                 }
                 __syncwarp();
