@@ -96,14 +96,17 @@ bc_status bc_buffer_at(bc_backend* b, void* ptr, size_t len, bc_buffer** out) {
         if (attributes.type != cudaMemoryTypeDevice || attributes.device != b->device)
             return fail(BC_ERR_ARGUMENT, "the pointer is not memory of device %d", b->device);
     }
-    bc_buffer* buffer = new (std::nothrow) bc_buffer();
-    if (!buffer) return fail(BC_ERR_ALLOCATION, "no memory for a buffer handle");
-    buffer->backend = b;
-    buffer->ptr = ptr;
-    buffer->len = len;
-    buffer->owned = false;
-    b->buffers.insert(buffer);
-    *out = buffer;
+    try {
+        std::unique_ptr<bc_buffer> buffer(new bc_buffer());
+        buffer->backend = b;
+        buffer->ptr = ptr;
+        buffer->len = len;
+        buffer->owned = false;
+        b->buffers.insert(buffer.get());
+        *out = buffer.release();
+    } catch (const std::bad_alloc&) {
+        return fail(BC_ERR_ALLOCATION, "no memory for a buffer handle");
+    }
     return BC_OK;
 }
 

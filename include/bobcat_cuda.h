@@ -250,7 +250,7 @@ typedef struct bc_kv_pool {
  * table[s][max_pages] names its pages; entries behind its last position are not read. The op takes up to n_rows rows; rows behind
  * starts[n_seqs] belong to no sequence and are left as they are, in every output. The words are read when the op runs, so a
  * captured call serves other lengths when it is replayed. max_queries, the most rows of one sequence as far as the caller knows, chooses
- * among kernels and changes no more than rounding when it is wrong. 1 to 65535 sequences, up to 2^24 rows.
+ * among kernels, with max_pages, and changes no more than rounding when it is wrong. 1 to 65535 sequences, up to 2^24 rows.
  * Rows that lie before a sequence's first position (more rows than positions) have no place: they are not written, read as zeros and attend to
  * nothing. A position behind the table or in a page that the pool does not have (its number is n_pages or more) is treated the same
  * way, as a key it is left out, and the wait for the recording (bc_wait, bc_end) returns BC_ERR_OUT_OF_BOUNDS. */
@@ -276,7 +276,7 @@ bc_status bc_op_kv_read(bc_backend* b, const bc_kv_pool* pool, const bc_kv_rows*
 /* Causal grouped-query attention of the rows over the pages: row r of sequence s sees positions 0 .. its own, which bc_op_kv_write has
  * stored. q is f32, token rows q_stride and heads q_head_stride elements apart (multiples of 4); out is [n_rows][n_heads * head_dim]
  * f32, zeros for a row that sees nothing; elements of positions that a row does not see have no part in it, whatever they are, and a value that is
- * not finite makes its element of the rows that see it not finite. Up to 8 query heads per KV head. Scores and sums are f32; operands keep 22 bits. `scratch` needs
+ * not finite makes its element of the rows that see it not finite. Up to 8 query heads per KV head. Scores and sums are f32; operands keep 22 bits. out does not overlap q. `scratch` needs
  * bc_attention_paged_scratch_floats floats (whatever the lengths), for the duration of the call: calls that may overlap, replayed graphs among
  * them, take one each. */
 size_t bc_attention_paged_scratch_floats(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);

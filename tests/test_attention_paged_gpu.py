@@ -383,3 +383,51 @@ def test_attention_refusals(cuda):
         other.close()
     cuda.attention_paged(pool, no_rows, q, scratch, out, 8, 512, 64)  # no rows: nothing to do
     cuda.end()
+
+
+@pytest.mark.parametrize("fmt", [F16, I8])
+@pytest.mark.parametrize("page_size, heads, kv, hd, seqs", [
+    (16, 4, 2, 64, [(1, 1), (2, 40), (5, 3)]),
+    (32, 8, 1, 64, [(3, 129)]),
+    (64, 6, 2, 128, [(4, 300), (1, 65), (0, 20), (8, 9)]),
+    (256, 8, 4, 128, [(2, 700)]),
+    (128, 7, 1, 256, [(2, 64), (3, 65), (1, 500)]),
+    (16, 5, 5, 256, [(9, 100), (1, 0)]),
+])
+def test_few_rows_either_way(cuda, fmt, page_size, heads, kv, hd, seqs):
+    """The caller's word on the rows chooses the kernel: both say the same, within the bound."""
+    news, lens = [n for n, _ in seqs], [length for _, length in seqs]
+    case = build(cuda, fmt, page_size, kv, hd, lens, seed=heads + hd + 40)
+    case.upload()
+    q = (np.random.default_rng(hd + 41).standard_normal((sum(news) + 2, heads * hd)) * 1.5).astype(np.float32)
+    for hint in (max(news), 32, 1000):
+        check(case, news, heads, q, attend(cuda, case, news, heads, q, rows=case.rows(news, n_rows=q.shape[0], max_queries=hint)))
+
+
+@pytest.mark.parametrize("fmt", [F16, I8])
+@pytest.mark.parametrize("kv, heads, hd, n_seqs, hint", [(1, 2, 64, 97, 1000), (2, 8, 64, 330, 1000), (1, 1, 128, 64, 1000), (1, 2, 64, 700, 3), (4, 8, 256, 40, 1000)])
+def test_many_sequences(cuda, fmt, kv, heads, hd, n_seqs, hint):
+    """More sequences than lanes that look for a run's beginning; many of them without rows, rows of most too few to fill a row tile."""
+    rng = np.random.default_rng(n_seqs)
+    news = [int(n) for n in rng.choice([0, 1, 1, 2, 3, 7, 40], size=n_seqs)]
+    news[0], news[-1], news[n_seqs // 2] = 0, 3, 150 if hint > 3 else 2
+    lens = [n + int(rng.integers(0, 60)) if n else 5 for n in news]
+    lens[1] = 900
+    case = Pool(cuda, fmt, 16, kv, hd, lens, rng)
+    case.fill_at_once(rng)
+    case.upload()
+    q = (rng.standard_normal((sum(news) + 1, heads * hd)) * 1.5).astype(np.float32)
+    check(case, news, heads, q, attend(cuda, case, news, heads, q, rows=case.rows(news, n_rows=q.shape[0], max_queries=hint)))
+
+
+@pytest.mark.parametrize("fmt", [F16, I8])
+@pytest.mark.parametrize("kv, hd", [(8, 64), (4, 256)])
+def test_row_tiles_cut_or_whole(cuda, fmt, kv, hd):
+    """Short prompts, whose row tiles stay whole, and one beside them that makes equal runs the better choice."""
+    rng = np.random.default_rng(hd)
+    for news, lens in (([300], [300]), ([300, 1, 90], [300, 4000, 2500])):
+        case = Pool(cuda, fmt, 32, kv, hd, lens, rng)
+        case.fill_at_once(rng)
+        case.upload()
+        q = (rng.standard_normal((sum(news), 2 * kv * hd)) * 1.5).astype(np.float32)
+        check(case, news, 2 * kv, q, attend(cuda, case, news, 2 * kv, q))

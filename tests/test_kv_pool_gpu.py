@@ -250,6 +250,29 @@ def test_buffers_over_memory_of_the_caller(cuda):
         cuda.buffer_at(host.data_ptr() // 256 * 256, 64)
 
 
+@pytest.mark.parametrize("n_seqs", [255, 256, 257, 300, 1023, 1056, 5000])
+def test_rows_find_their_sequence_among_many(cuda, n_seqs):
+    rng = np.random.default_rng(n_seqs)
+    news = [int(n) for n in rng.choice([0, 0, 1, 1, 2, 5], size=n_seqs)]
+    lens = [n + int(rng.integers(0, 20)) for n in news]
+    case = Pool(cuda, F16, 16, 1, 64, lens, rng)
+    pool, n = case.upload(), sum(news)
+    x = rng.standard_normal((n + 3, 64)).astype(np.float16).astype(np.float32)
+    starts = np.concatenate([[0], np.cumsum(news)])
+    rows, xb = case.rows(news, n_rows=n + 3), cuda.buffer_from(x)
+    back = cuda.buffer_from(np.full((n + 3, 64), 9.0, dtype=np.float32))
+    cuda.begin()
+    cuda.kv_write(pool, rows, xb, xb, 64, 64)
+    cuda.kv_read(pool, rows, back, None, False, 64, 64)
+    cuda.end()
+    for s, m in enumerate(news):
+        for i in range(m):
+            case.put(case.k_raw, s, lens[s] - m + i, x[starts[s] + i].reshape(1, 64))
+    assert np.array_equal(case.download()[0], case.k_raw)
+    got = cuda.read(back, np.zeros_like(x))
+    assert np.array_equal(got[:n], x[:n]) and (got[n:] == 9.0).all()
+
+
 def test_stored_is_what_the_formula_says():
     """The numpy form that the tests compare with: halfway cases to even, exact zeros."""
     held, scales = stored(np.array([[127.0, 0.5, 1.5, -2.5]], dtype=np.float32), I8)
