@@ -543,17 +543,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             if (lane == 0) mbar_arrive(pv_free);
         };
         // 16 scores of a tile from score c on, scaled and masked.
-        auto load_scores = [&](uint32_t scores_at, const TileInfo<KT, FMT>& info, int32_t see, uint32_t c, float2 (&x)[8]) {
+        // The scales are asked for ahead of the scores: nothing moves across a wait for tensor memory.
+        auto load_scores = [&](uint32_t scores_at, const TileInfo<KT, FMT>& info, bool masked, int32_t see, uint32_t c, float2 (&x)[8]) {
+            float4 d[4];
+            if constexpr (FMT == BC_I8) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) d[i] = *reinterpret_cast<const float4*>(info.dk + first_score + c + 4 * i);
+            }
             tmem_load_16(scores_at + c, reinterpret_cast<float(&)[16]>(x));
             if constexpr (FMT == BC_I8) {
 #pragma unroll
-                for (uint32_t i = 0; i < 8; i += 2) {
-                    const float4 d = *reinterpret_cast<const float4*>(info.dk + first_score + c + 2 * i);
-                    x[i] = mul2(x[i], make_float2(d.x, d.y));
-                    x[i + 1] = mul2(x[i + 1], make_float2(d.z, d.w));
+                for (uint32_t i = 0; i < 4; ++i) {
+                    x[2 * i] = mul2(x[2 * i], make_float2(d[i].x, d[i].y));
+                    x[2 * i + 1] = mul2(x[2 * i + 1], make_float2(d[i].z, d[i].w));
                 }
             }
-            if (info.masked) {
+            if (masked) {
                 const uint32_t bits = seen_bits(info, first_score + c, see - (int32_t)c);
 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i) {
@@ -572,11 +577,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
             if (!alive) return;
             tc_fence_after_sync();
             const int32_t see = (int32_t)max(min((int64_t)limit - sh.desc[tile % kDescRing].key0 - first_score, (int64_t)KT), (int64_t)-1);  // the last score seen
+            const bool masked = info.masked;
             float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
             for (uint32_t c = 0; c < kScores; c += 16) {
                 float2 x[8];
-                load_scores(scores_at, info, see, c, x);
+                load_scores(scores_at, info, masked, see, c, x);
 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i) most[i & 1] = fmaxf(most[i & 1], fmaxf(x[i].x, x[i].y));
             }
@@ -601,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
 #pragma unroll 1
             for (uint32_t c = 0; c < kScores; c += 16) {
                 float2 x[8];
-                load_scores(scores_at, info, see, c, x);
+                load_scores(scores_at, info, masked, see, c, x);
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i) {
@@ -612,12 +618,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_kernel(const __gr
                 }
                 if constexpr (FMT == BC_I8) {
 #pragma unroll
-                    for (uint32_t i = 0; i < 8; i += 2) {
-                        const float4 d = *reinterpret_cast<const float4*>(info.dv + first_score + c + 2 * i);
-                        x[i] = mul2(x[i], make_float2(d.x, d.y));
-                        x[i + 1] = mul2(x[i + 1], make_float2(d.z, d.w));
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        const float4 d = *reinterpret_cast<const float4*>(info.dv + first_score + c + 4 * i);
+                        x[2 * i] = mul2(x[2 * i], make_float2(d.x, d.y));
+                        x[2 * i + 1] = mul2(x[2 * i + 1], make_float2(d.z, d.w));
                     }
-                    if (info.masked) {  // a scale may be no number
+                    if (masked) {  // a scale may be no number
                         const uint32_t bits = seen_bits(info, first_score + c, see - (int32_t)c);
 #pragma unroll
                         for (uint32_t i = 0; i < 8; ++i) {
