@@ -307,22 +307,26 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
             copy_values(n);
         }
     };
+    // A warp's query head of a unit (PACKED: two warps a head), two elements of every 64 to a lane.
+    const uint32_t q_head = PACKED ? warp & 3 : warp;
+    float2 x[HD / 64];
+    auto load_query = [&](const Work& w) {
+#pragma unroll
+        for (int i = 0; i < HD / 64; ++i)
+            x[i] = q_head < p.group ? *reinterpret_cast<const float2*>(p.q + w.row * p.q_stride + (w.head * p.group + q_head) * p.q_head_stride + 64 * i + 2 * lane)
+                                    : make_float2(0.f, 0.f);
+    };
     Work w = find();
     begin_copies(w);
+    load_query(w);
     while (true) {
         // Query fragments in the order of a lane's key elements, a warp per query head (PACKED: two). A pair of elements is a word of hi and one of
         // lo parts.
         __syncthreads();  // the previous unit's fragments and sums have been read
-        const uint32_t q_head = PACKED ? warp & 3 : warp;
         {
-            float2 x[HD / 64];
             uint32_t most = 0;
 #pragma unroll
-            for (int i = 0; i < HD / 64; ++i) {
-                x[i] = q_head < p.group ? *reinterpret_cast<const float2*>(p.q + w.row * p.q_stride + (w.head * p.group + q_head) * p.q_head_stride + 64 * i + 2 * lane)
-                                      : make_float2(0.f, 0.f);
-                most = max(most, max(__float_as_uint(x[i].x) & 0x7fffffffu, __float_as_uint(x[i].y) & 0x7fffffffu));
-            }
+            for (int i = 0; i < HD / 64; ++i) most = max(most, max(__float_as_uint(x[i].x) & 0x7fffffffu, __float_as_uint(x[i].y) & 0x7fffffffu));
             most = __reduce_max_sync(0xffffffffu, most);
             const uint32_t exponent = min(max(most >> 23, 1u), 253u);
             const float up = __uint_as_float((254u - exponent) << 23);  // times 2^14 or 2^29 below: together they may pass the largest float
@@ -387,6 +391,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
         float top = -INFINITY, total_p = 0.f;  // of query head g, the sum over this lane's positions
         float unit = FMT == BC_I8 ? 0.f : 1.f, inverse_unit = unit;  // the sums of query head g are counted in these
 
+        // What comes next is looked up meanwhile.
+        const Work done = w;
+        at += done.counted;
+        const bool more = at < end;  // uniform in the CTA
+        if (more) w = find();
         for (uint32_t n = 0; n < n_steps; ++n) {
             const uint8_t* const here = ring + n % D * R::kBytes;
             // Positions of the step that exist, from its first on; halves whose page the pool does not have hold nothing.
@@ -602,11 +611,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
             }
         }
         async::cp_async_wait<0>();
-        const Work done = w;
-        at += done.counted;
-        const bool more = at < end;  // uniform in the CTA
-        if (more) w = find();
         if (kBeside && more) begin_copies(w);
+        if (more) load_query(w);
 
         // The warps' sums, joined through shared memory. Tile n's rows g and g + 8 are elements 2n' and 2n' + 1 of the lane's eight.
         total_p += __shfl_xor_sync(0xffffffffu, total_p, 1);
