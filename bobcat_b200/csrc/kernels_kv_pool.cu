@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constan
 
 // Reading. Rows of a sequence without a place (before its first position, behind the table, in no page of the pool) read as zeros; rows
 // of no sequence stay as they are. A lane takes two eights of a cell where what it writes of each is one store: what a cell costs beside its bytes counts
-// once (contexts of 104 000 positions of 2 x 4 heads of 256, 8 bits, as halves: 100 us, 115 with an eight); as floats, 206 us and 182, it takes one.
+// once (contexts of 104 000 positions of 2 x 4 heads of 256, 8 bits, as halves: 99 us, 115 with one eight); as floats, 206 us and 182, it takes one.
 struct Targets {
     void *k, *v;
     uint64_t k_stride, v_stride;
@@ -239,10 +239,11 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(const __grid_constant
     }
 }
 
-// Token rows per CTA: a CTA works through at most about eight rounds of its threads, fewer where that leaves SMs without one.
-Cells cells_of(const KvPool& pool, const KvRows& rows) {
+// Token rows per CTA: a CTA works through at most about `rounds` rounds of its threads, fewer where that leaves SMs without one. 104 000 positions of 2 x 4
+// heads of 256 are read as halves in 99 us in 4 rounds (115 in 2, 139 in one), as floats in 182 in 8 (196 in 4).
+Cells cells_of(const KvPool& pool, const KvRows& rows, uint32_t rounds) {
     const uint32_t per_row = 2 * pool.n_kv_heads, lanes_per_row = per_row * (pool.head_dim / 8);
-    uint32_t n = 8 * kThreads / lanes_per_row;
+    uint32_t n = rounds * kThreads / lanes_per_row;
     if (n > kRowsPerCta) n = kRowsPerCta;
     while (n > 1 && (rows.n_rows + n - 1) / n < 4 * (uint32_t)sm_count()) n /= 2;
     return Cells{per_row, (uint32_t)(((1ull << 32) + per_row - 1) / per_row), n < 1 ? 1 : n};
@@ -250,12 +251,12 @@ Cells cells_of(const KvPool& pool, const KvRows& rows) {
 
 template <int FMT, int HD>
 cudaError_t write_as(cudaStream_t stream, const KvPool& pool, const KvRows& rows, const Sources& src) {
-    const Cells cells = cells_of(pool, rows);
+    const Cells cells = cells_of(pool, rows, 4);
     return launch_dependent(kv_write_kernel<FMT, HD>, dim3((rows.n_rows + cells.rows_per_cta - 1) / cells.rows_per_cta), dim3(kThreads), 0, stream, pool, rows, src, cells);
 }
 template <int FMT, int HD>
 cudaError_t read_as(cudaStream_t stream, const KvPool& pool, const KvRows& rows, const Targets& dst, bool half) {
-    const Cells cells = cells_of(pool, rows);
+    const Cells cells = cells_of(pool, rows, half ? 4 : 8);
     const dim3 grid((rows.n_rows + cells.rows_per_cta - 1) / cells.rows_per_cta);
     return half ? launch_dependent(kv_read_kernel<FMT, HD, __half>, grid, dim3(kThreads), 0, stream, pool, rows, dst, cells)
                 : launch_dependent(kv_read_kernel<FMT, HD, float>, grid, dim3(kThreads), 0, stream, pool, rows, dst, cells);
