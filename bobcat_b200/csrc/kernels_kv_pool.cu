@@ -10,8 +10,8 @@
 // What bounds it: bytes, 4 read and 1 (+ 4 / head_dim) or 2 written per element, and the look-up of a row's place before the
 // first store. A lane holds 8 elements (two 16-byte loads, one 8- or 16-byte store), a cell (one head's row of keys or of values) is
 // 8, 16 or 32 lanes. A CTA takes neighbouring token rows; its warps look the rows' places up while the first cells' loads are on their way. Large
-// calls are bound by bytes as long as an element costs few instructions: with the exact test for every element 50 of them, and the
-// rows of eight prompts (32 008 of 2 x 8 heads of 128) took 117 us to write.
+// calls are bound by bytes as long as an element costs few instructions: the rows of eight prompts (32 008 of 2 x 8 heads of 128) take 60 us (262 MB read, 68 written:
+// 5.5 TB/s), with the exact test for every element, 50 instructions, 117.
 
 #include "kv_pool.cuh"
 
