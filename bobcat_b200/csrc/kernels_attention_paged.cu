@@ -110,13 +110,15 @@ struct Ring {
     static constexpr uint32_t kKeyPitch = kRowBytes == 64 ? 64 : kRowBytes + 64, kValuePitch = kRowBytes + 16;
     static constexpr uint32_t kValues = kStep * kKeyPitch, kScales = kValues + kStep * kValuePitch, kBytes = kScales + (FMT == BC_I8 ? 8 * kStep : 0);
     static constexpr uint32_t kSteps = kBytes <= 5632 ? 2 : 1;
+    // Blocks that a unit counts beside its own, ahead of them: its beginning and end take as long as these.
+    static constexpr uint32_t kUnitCost = FMT == BC_F16 ? 1 : 2;
 };
 // A sequence of the call: its rows, the positions it holds, the blocks its longest row takes.
 struct Seq {
     uint32_t row0, n, end, len;
     uint32_t blocks, counted;  // of its longest row; of them, what a unit counts as
 };
-__device__ __forceinline__ Seq seq_at(const KvPool& pool, const KvRows& rows, uint32_t s, uint32_t most, uint32_t block, bool whole) {
+__device__ __forceinline__ Seq seq_at(const KvPool& pool, const KvRows& rows, uint32_t s, uint32_t most, uint32_t block, uint32_t unit_cost, bool whole) {
     Seq q;
     q.row0 = rows.starts[s];
     q.end = rows.starts[s + 1];
@@ -124,7 +126,7 @@ __device__ __forceinline__ Seq seq_at(const KvPool& pool, const KvRows& rows, ui
     q.len = rows.lens[s];
     const uint32_t held = min((uint64_t)q.len, (uint64_t)rows.max_pages << pool.page_shift);
     q.blocks = max(1u, (held + block - 1) / block);
-    q.counted = whole ? 1 : q.blocks;
+    q.counted = whole ? 1 : q.blocks + unit_cost;
     return q;
 }
 __device__ __forceinline__ uint64_t blocks_of(const KvPool& pool, const Seq& q) { return (uint64_t)q.n * pool.n_kv_heads * q.counted; }
@@ -184,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
 
     // This CTA's run of blocks, and the sequence that it begins in. Every warp works it out for itself.
     uint64_t total = 0;
-    for (uint32_t s = lane; s < rows.n_seqs; s += 32) total += blocks_of(pool, seq_at(pool, rows, s, p.most, kBlock, p.whole));
+    for (uint32_t s = lane; s < rows.n_seqs; s += 32) total += blocks_of(pool, seq_at(pool, rows, s, p.most, kBlock, R::kUnitCost, p.whole));
     total = warp_sum_u64(total);
     const uint64_t runs = min((uint64_t)gridDim.x, total);  // none of them empty
     uint64_t at = blockIdx.x < runs ? total * blockIdx.x / runs : total;
@@ -197,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
     uint32_t seq = 0;
     uint64_t base = 0;  // blocks of the sequences before `seq`
     for (uint32_t s0 = 0; s0 < rows.n_seqs; s0 += 32) {
-        const uint64_t mine = s0 + lane < rows.n_seqs ? blocks_of(pool, seq_at(pool, rows, s0 + lane, p.most, kBlock, p.whole)) : 0;
+        const uint64_t mine = s0 + lane < rows.n_seqs ? blocks_of(pool, seq_at(pool, rows, s0 + lane, p.most, kBlock, R::kUnitCost, p.whole)) : 0;
         uint64_t upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -215,23 +217,26 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
     }
     PartsHead cut{0, 0, 0, 0};
 
-    // The unit at `at`, and the blocks of it that are this CTA's. Rows of a head are neighbours.
+    // The unit at `at`, and the blocks of it that are this CTA's: none where the run ends ahead of them. Rows of a head are neighbours.
     struct Work {
         uint32_t seq, row, head, n_keys, block0, blocks, counted, all_blocks;
+        uint64_t last;  // the unit's last place in the call's work
     };
     auto find = [&]() {
         Work w;
-        Seq sq = seq_at(pool, rows, seq, p.most, kBlock, p.whole);
+        Seq sq = seq_at(pool, rows, seq, p.most, kBlock, R::kUnitCost, p.whole);
         while (base + blocks_of(pool, sq) <= at) {  // sequences without rows have no blocks
             base += blocks_of(pool, sq);
-            sq = seq_at(pool, rows, ++seq, p.most, kBlock, p.whole);
+            sq = seq_at(pool, rows, ++seq, p.most, kBlock, R::kUnitCost, p.whole);
         }
         const uint64_t in_seq = at - base;
         const uint32_t which = (uint32_t)(in_seq / sq.counted);
         w.seq = seq;
-        w.block0 = (uint32_t)(in_seq % sq.counted);
-        w.counted = (uint32_t)min((uint64_t)(sq.counted - w.block0), end - at);
-        w.blocks = p.whole ? sq.blocks : w.counted;
+        const uint32_t from = (uint32_t)(in_seq % sq.counted), cost = p.whole ? 0 : R::kUnitCost;
+        w.counted = (uint32_t)min((uint64_t)(sq.counted - from), end - at);
+        w.block0 = max(from, cost) - cost;
+        w.blocks = p.whole ? sq.blocks : max(from + w.counted, cost) - cost - w.block0;
+        w.last = at - from + sq.counted - 1;
         w.all_blocks = sq.blocks;
         w.head = which / sq.n;
         w.row = sq.row0 + which % sq.n;
@@ -321,6 +326,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
                                     : make_float2(0.f, 0.f);
     };
     Work w = find();
+    if (w.blocks == 0) {
+        if (tid == 0) heads[blockIdx.x] = cut;
+        return;
+    }
     begin_copies(w);
     load_query(w);
     while (true) {
@@ -398,8 +407,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
         // What comes next is looked up meanwhile.
         const Work done = w;
         at += done.counted;
-        const bool more = at < end;  // uniform in the CTA
-        if (more) w = find();
+        bool more = at < end;  // uniform in the CTA
+        if (more) {
+            w = find();
+            more = w.blocks > 0;
+        }
         for (uint32_t n = 0; n < n_steps; ++n) {
             const uint8_t* const here = ring + n % D * R::kBytes;
             // Positions of the step that exist, from its first on; halves whose page the pool does not have hold nothing.
@@ -676,10 +688,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
         }
         if (begins && !ends) {
             // The CTA whose run holds the unit's last block: run c is [total c / runs, total (c + 1) / runs).
-            const uint64_t last_block = at - done.blocks + done.all_blocks - 1;
-            uint32_t last = (uint32_t)(last_block * runs / total);
-            while (total * (last + 1) / runs <= last_block) ++last;
-            while (total * last / runs > last_block) --last;
+            uint32_t last = (uint32_t)(done.last * runs / total);
+            while (total * (last + 1) / runs <= done.last) ++last;
+            while (total * last / runs > done.last) --last;
             cut = PartsHead{done.row, done.head, last, 0};
         }
         if (!more) break;
