@@ -266,7 +266,7 @@ struct Shared {
     float most[2][kParts][kRows];  // [parity][part]: maxima of the parts of a row's scores; at a unit's ends, other exchanges
     uint32_t not_finite[FMT == BC_F16 ? kUnits : 1][FMT == BC_F16 ? HD : 1];  // by unit: the first position with such a value, of each element
     uint32_t any_not_finite[kUnits];
-    uint64_t bars[4 * kStages + 4 * kRaw + 10 + kDescRing];
+    uint64_t bars[4 * kStages + 4 * kRaw + 13 + kDescRing];
     uint64_t counted, ahead[2];  // the call's work; key tiles ahead of the run's beginning, and of its end
     Place place;
     uint32_t tmem;
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
     const uint32_t bars = smem_u32(sh.bars);
     const uint32_t k_full = bars, k_free = k_full + 8 * ST, v_full = k_free + 8 * ST, v_free = v_full + 8 * ST, rk_full = v_free + 8 * ST, rk_free = rk_full + 8 * RAW;
     const uint32_t rv_full = rk_free + 8 * RAW, rv_free = rv_full + 8 * RAW, s_full = rv_free + 8 * RAW, p_ready = s_full + 16, pv_full = p_ready + 16, pv_free = pv_full + 16, q_ready = pv_free + 8;
-    const uint32_t rows_bar = q_ready + 8, unpack_bar = rows_bar + 8, described = unpack_bar + 8;
+    const uint32_t rows_bar = q_ready + 8, unpack_bar = rows_bar + 8 * 4, described = unpack_bar + 8;
 
     pdl_launch_dependents();
     if (tid == 0) {
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
         mbar_init(pv_full + 8, 1);
         mbar_init(pv_free, kRowWarps);
         mbar_init(q_ready, kRowWarps);
-        mbar_init(rows_bar, kRowWarps);
+        for (uint32_t w = 0; w < 4; ++w) mbar_init(rows_bar + 8 * w, kParts);
         mbar_init(unpack_bar, kUnpackWarps);
         for (uint32_t d = 0; d < kDescRing; ++d) mbar_init(described + 8 * d, 1);
         sh.dead = sh.never = 0;
@@ -436,8 +436,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
         const uint32_t lanes = tmem + ((warp & 3) << 21);
         const float scale = 1.4426950408889634f / sqrtf((float)HD) / 16384.f;
         float factor = 0.f;
-        WarpsBarrier everyone{rows_bar, 0, 13};
-        auto rows_sync = [&]() { everyone.sync(alive, dead); };
+        // The warps that share 32 rows wait for one another, and for nobody else's.
+        WarpsBarrier sharers{rows_bar + 8 * (warp & 3), 0, 13};
+        auto rows_sync = [&]() { sharers.sync(alive, dead); };
 
         // The next unit's queries, a thread half of a row: its largest element goes to 2^14 (see kernels_attention_paged.cu). The other half's
         // largest comes through shared memory.
