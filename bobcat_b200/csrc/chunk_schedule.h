@@ -13,17 +13,17 @@
 namespace bc {
 namespace k {
 
-// Sum over i = 0 .. n - 1 of floor((a i + b) / m).
-__host__ __device__ inline uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
+// Sum over i = 0 .. n - 1 of floor((a i + b) / m), of numbers with (a mod m) n + m below 2^32: divisions of 64 bits are most of a search's instructions.
+__host__ __device__ inline uint64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
     uint64_t sum = 0;
     while (n > 0) {
-        sum += a / m * (n * (n - 1) / 2) + b / m * n;
-        a %= m;
-        b %= m;
-        const uint64_t last = a * n + b;
+        const uint32_t of_a = a / m, of_b = b / m;
+        sum += of_a * ((uint64_t)n * (n - 1) / 2) + (uint64_t)of_b * n;
+        a -= of_a * m;
+        b -= of_b * m;
+        const uint32_t last = a * n + b, other = a;
         n = last / m;
-        b = last % m;
-        const uint64_t other = a;
+        b = last - n * m;
         a = m;
         m = other;
         if (m == 0) break;
@@ -39,15 +39,15 @@ struct ChunkSeq {
     uint32_t len, held;      // positions, and those that its table can name
     uint32_t per_tile, row_tiles, key_tile;
     // Position of the first row, for counting: within what the table holds.
-    __host__ __device__ uint64_t first() const {
+    __host__ __device__ uint32_t first() const {
         const uint32_t rows = end - row0;
         const uint32_t at = len > rows ? len - rows : 0;
         return at < held ? at : held;
     }
     // Key tiles of row tile r, one at least.
     __host__ __device__ uint32_t tiles(uint32_t r) const {
-        const uint64_t rows = (uint64_t)(r + 1) * per_tile;
-        return (uint32_t)((first() + (rows < n ? rows : n) - 1) / key_tile) + 1;
+        const uint32_t rows = (r + 1) * per_tile;
+        return (first() + (rows < n ? rows : n) - 1) / key_tile + 1;
     }
     // Key tiles of row tiles 0 .. r - 1, r < row_tiles.
     __host__ __device__ uint64_t tiles_before(uint32_t r) const { return r + floor_sum(r, key_tile, per_tile, first() + per_tile - 1); }

@@ -1018,6 +1018,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
                             at.cut = ChunkHead{d.row0, d.n, d.head, last};
                         }
                         ++at.in_unit;
+                        mbar_arrive(described + 8 * (j % kDescRing));  // but for the groups, which the copies' arrival shows
                     }
                     __syncwarp();
                     // Every lane looks up its group's page.
@@ -1037,7 +1038,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
                     ++keys_issued;
                     if (lane == 0) {
                         d.groups = groups;
-                        mbar_arrive(described + 8 * (j % kDescRing));
                         mbar_arrive_expect(bar, segments * segment * (kRowBytes + (FMT == BC_I8 ? 8 : 0)));
                     }
                     __syncwarp();

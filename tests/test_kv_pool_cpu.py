@@ -50,7 +50,7 @@ def schedule(tmp_path_factory):
     source.write_text("""
 #include "chunk_schedule.h"
 using namespace bc::k;
-extern "C" uint64_t sums(uint64_t n, uint64_t m, uint64_t a, uint64_t b) { return floor_sum(n, m, a, b); }
+extern "C" uint64_t sums(uint32_t n, uint32_t m, uint32_t a, uint32_t b) { return floor_sum(n, m, a, b); }
 extern "C" uint32_t sequence(uint32_t start, uint32_t end, uint32_t len, uint64_t capacity, uint32_t n_rows, uint32_t fewest, uint32_t per_tile, uint32_t key_tile,
                              uint32_t* tiles, uint64_t* before, uint64_t* counted, uint64_t* per_head) {
     const ChunkSeq s = chunk_seq(start, end, len, capacity, n_rows, fewest, per_tile, key_tile);
@@ -63,16 +63,16 @@ extern "C" uint32_t cost() { return kRowTileCost; }
     subprocess.run([compiler, "-O1", "-std=c++17", "-shared", "-fPIC", "-I", CSRC, "-I", "/usr/local/cuda/include", "-o", str(binary), str(source)], check=True)
     library = C.CDLL(str(binary))
     library.sums.restype = C.c_uint64
-    library.sums.argtypes = [C.c_uint64] * 4
+    library.sums.argtypes = [C.c_uint32] * 4
     library.sequence.argtypes = [C.c_uint32] * 3 + [C.c_uint64] + [C.c_uint32] * 4 + [C.c_void_p] * 4
     return library
 
 
 def test_sums_of_quotients(schedule):
-    for n in (0, 1, 2, 7, 100):
+    for n in (0, 1, 2, 7, 100, 5000):
         for m in (1, 3, 64, 128):
             for a in (0, 1, 16, 127, 300):
-                for b in (0, 5, 127, 1 << 40):
+                for b in (0, 5, 127, 1 << 31):
                     assert schedule.sums(n, m, a, b) == sum((a * i + b) // m for i in range(n))
 
 
