@@ -14,10 +14,10 @@
 // Queries and probabilities are A operands in tensor memory: both operands in shared memory would take its 128 bytes a cycle whole. (Heads of 256
 // leave room for the queries' upper halves alone.)
 //
-// Measured: 2048 rows of 32 heads of 128 behind 30 001 8-bit positions, 2.33 ms: 447 TFLOP/s of attention, twice that in half products (multiplies alone would take
+// Measured: 2048 rows of 32 heads of 128 behind 30 001 8-bit positions, 2.31 ms: 450 TFLOP/s of attention, twice that in half products (multiplies alone would take
 // 1.26 ms). A key tile takes 4700 cycles, its multiplies 2100 of them; the rest is the rows' warps, whose instructions bound it: 54 % of
 // the issue slots are used, 12 % of the waiting is for instructions. Tried and left: four threads to a row (2.48 ms: the instructions grow by a quarter), scores held in
-// registers between maximum and exponential (2.61 ms). 512 rows from position 0, 32 heads of 64, take 20 us, most of it one CTA's way through two tiles.
+// registers between maximum and exponential (2.61 ms). 512 rows from position 0, 32 heads of 64, take 18 us, most of it one CTA's way through two tiles.
 
 #include "async_utils.cuh"
 #include "chunk_schedule.h"
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
         }
         longest = __reduce_max_sync(0xffffffffu, longest);
         // Equal runs cut row tiles; runs of whole ones are not equal, but nothing is cut, which saves a row tile's cost and a part to join. (512 rows of 8
-        // heads from position 0, 128 row tiles of 1 to 4 key tiles: 33 us cut, 20 whole.)
+        // heads from position 0, 128 row tiles of 1 to 4 key tiles: 23 us cut, 19 whole.)
         const uint64_t ctas = gridDim.x, units_each = (units + ctas - 1) / ctas;
         const bool whole = units_each * (longest + kRowTileCost) <= (total + kRowTileCost * units) / ctas + kRowTileCost + 1;
         const uint64_t counted = whole ? units : total + kRowTileCost * units, runs = min(ctas, counted);

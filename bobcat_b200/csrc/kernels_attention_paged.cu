@@ -21,9 +21,10 @@
 // columns (hi in the first four, lo in the others, from rows of queries given twice), more take two multiplies. The tensor cores cut sums
 // off: what they add up is one step, and steps are added in f32, rounding.
 //
-// Measured: a token each of 64 sequences, 32 heads over 8 of 128, contexts of 500 to 8200: 8-bit pages, 589 MB, 117 us (5.0 TB/s), halves, 1.14 GB, 191 us
-// (6.0 TB/s). One sequence of 131 072 8-bit positions, 4 KV heads of 256: 273 MB in 51 us (5.4 TB/s). Of the 117 us about ten are the launch's beginning, the last
-// units and the join; a form without arithmetic took 114. One sequence of 301 positions: 6 us, all of it latency.
+// Measured: a token each of 64 sequences, 32 heads over 8 of 128, contexts of 500 to 8200: 8-bit pages, 589 MB, 112 us (5.3 TB/s; 116 where
+// units do not count two blocks beside their own, kUnitCost), halves, 1.14 GB, 190 us (6.0 TB/s). One sequence of 131 072 8-bit positions, 4 KV heads of 256: 273 MB in
+// 50 us (5.4 TB/s). Of the 112 us about ten are the launch's beginning and the join; CTAs of equal runs end 86 to 108 us after it. One sequence of 301
+// positions: 6 us, all of it latency.
 
 #include "async_utils.cuh"
 #include "kv_pool.cuh"
@@ -806,7 +807,7 @@ cudaError_t launch_token(cudaStream_t stream, const TokenParams& p) {
 }
 
 // Where tables cannot hold more than this many elements of a head's keys, units stay whole: what a CTA takes longer for the longest unit is less
-// than the joining launch (one sequence of 8 heads of 64: 301 positions 6.4 us, cut and joined 8.6; 1024 positions 8.3 and 8.6; 2001 11.7 and 9.1).
+// than the joining launch (one sequence of 8 heads of 64: 301 positions 6.3 us, cut and joined 7.7; 1024 positions 8.5 and 9.8; 2001 12.3 and 10.2).
 constexpr uint64_t kWholeElements = 65536;
 bool whole_units(const KvRows& rows, const KvPool& pool) { return ((uint64_t)rows.max_pages << pool.page_shift) * pool.head_dim <= kWholeElements; }
 
@@ -817,16 +818,17 @@ uint64_t token_floats(uint32_t head_dim) {
 }  // namespace
 
 // Which kernel takes a sequence. The tensor-core kernel reads the positions once for all of a sequence's rows and takes the time of 128 of them: as long as
-// 2.5 rows here where contexts are long (8 sequences of 25000 positions, 8 heads of 64: 171 us; here 128 with 2 rows, 224 with 4), and 10 to 20 us beside that.
-// So sequences of up to two rows are always taken here, and all of a call's, with no second kernel, where what the tables can hold, 256 positions more
-// for a unit's beginning and end, times the rows beyond two, is what those 20 us read: (us, here and there) 8 sequences of up to 2900 positions with 5
-// rows 23 and 36, 64 of 500 with 4 rows 46 and 64, one of 1500 with 16 rows 17 and 26; past it 8 of 1100 with 16 rows 43 and 33, 64 of 100 with 8 rows 45 and 31.
-constexpr uint32_t kTokenRows = 2, kFewRows = 32;
+// three rows here where contexts are long (8 sequences of 25000 positions, 8 heads of 64: 168 us; here 134 with 2 rows, 178 with 3, 252 with 4), and 10 to 20 us
+// beside that (8 of 5500 with 3 rows: 34 here, 55 there). So sequences of up to three rows are always taken here, and all of a call's, with no second
+// kernel, where what the tables can hold, 256 positions more for a unit's beginning and end, times the rows beyond three, is what those 20 us read: (us, here and
+// there) 8 sequences of up to 2900 positions with 2 to 5 rows 19 and 30, 64 of 500 with 4 rows 46 and 61, one of 1500 with 16 rows 16 and 21; past it 8 of 1100
+// with 16 rows 43 and 28, 64 of 100 with 8 rows 47 and 32.
+constexpr uint32_t kTokenRows = 3, kFewRows = 32;
 bool few_rows(const KvPool& pool, const KvRows& rows) {
     if (rows.max_queries <= kTokenRows) return true;
     const uint64_t positions = ((uint64_t)rows.max_pages << pool.page_shift) + 256;
     const double elements = (double)positions * rows.n_seqs * pool.n_kv_heads * pool.head_dim * 2;
-    return rows.max_queries <= kFewRows && (rows.max_queries - kTokenRows) * elements <= (double)(1u << 27);
+    return rows.max_queries <= kFewRows && (rows.max_queries - kTokenRows) * elements <= 1.1e8;
 }
 
 uint64_t attention_paged_scratch_floats(uint32_t, uint32_t, uint32_t head_dim) {
