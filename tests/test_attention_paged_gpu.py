@@ -300,7 +300,8 @@ def test_a_conversation(cuda, fmt):
 
 
 @pytest.mark.parametrize("fmt", [F16, I8])
-def test_captured_calls_follow_the_lengths(fmt):
+@pytest.mark.parametrize("hint", [64, 4])
+def test_captured_calls_follow_the_lengths(fmt, hint):
     """A step captured once and replayed after the lengths, the tables and the rows have changed on the device; a second graph beside it with a
     scratch of its own, on another stream."""
     torch = pytest.importorskip("torch")
@@ -317,7 +318,7 @@ def test_captured_calls_follow_the_lengths(fmt):
                  dict(table=case.table, starts=np.array([0, 1, 2, 3], dtype=np.uint32), lens=np.array([300, 150, 40], dtype=np.uint32)).items()}
         torch.cuda.synchronize()
         at = {n: cuda.buffer_at(t.data_ptr(), t.numel() * 4) for n, t in dict(words, q=q, out=out).items()}
-        rows = KvRows(3, 64, 64, case.max_pages, at["table"], at["starts"], at["lens"])
+        rows = KvRows(3, 64, hint, case.max_pages, at["table"], at["starts"], at["lens"])
         scratch = cuda.new_buffer(4 * cuda.attention_paged_scratch_floats(heads, kv, hd))
         call = lambda: cuda.attention_paged(case.pool, rows, at["q"], scratch, at["out"], heads, heads * hd, hd)  # noqa: E731
         cuda.begin()
