@@ -91,7 +91,10 @@ struct Cursor {
                 if (++head == p.pool.n_kv_heads) {
                     head = 0;
                     do {
-                        ++seq;
+                        if (++seq == p.rows.n_seqs) {
+                            left = 0;
+                            return false;
+                        }
                         s = chunk_seq(p.rows.starts[seq], p.rows.starts[seq + 1], p.rows.lens[seq], capacity, p.rows.n_rows, p.fewest, s.per_tile, key_tile);
                     } while (s.row_tiles == 0);  // something is left, so a sequence with some follows
                 }

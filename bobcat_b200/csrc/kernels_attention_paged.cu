@@ -4,8 +4,9 @@
 // Work. A unit is one row of one KV head: the group of up to 8 query heads that share the head, over the positions that the row sees.
 // Units are cut into blocks of 128 positions (256 of heads of 64), and the blocks of all units, in order, into equal runs, one to a CTA: however
 // the lengths differ, every CTA reads about the same number of positions, a block or two fewer for each unit that it begins, and lengths stay on
-// the device (a captured call serves whatever they become). (Twice as many runs, half as long: 117 us where these take 111.) A unit that lies in one CTA's run is written out by it; a unit that is cut leaves unnormalised sums with their maximum and sum of
-// exponentials, at most two to a CTA, and a second launch joins them in order.
+// the device (a captured call serves whatever they become).
+// (Twice as many runs, half as long: 117 us where these take 111.) A unit that lies in one CTA's run is written out by it; a unit that is cut leaves
+// unnormalised sums with their maximum and sum of exponentials, at most two to a CTA, and a second launch joins them in order.
 //
 // Arithmetic. Elements are exact in half precision (8-bit ones as whole numbers, their scales multiply scores and probabilities in f32).
 // A query element, and a probability times the value's scale, is split into two halves, value = hi + lo (about 22 bits), every product is half x
@@ -228,6 +229,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
         Seq sq = seq_at(pool, rows, seq, p.most, kBlock, R::kUnitCost, p.whole);
         while (base + blocks_of(pool, sq) <= at) {  // sequences without rows have no blocks
             base += blocks_of(pool, sq);
+            if (seq + 1 == rows.n_seqs) return Work{};
             sq = seq_at(pool, rows, ++seq, p.most, kBlock, R::kUnitCost, p.whole);
         }
         const uint64_t in_seq = at - base;

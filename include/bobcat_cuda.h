@@ -248,8 +248,8 @@ typedef struct bc_kv_pool {
 /* The rows of a call, in device memory of 32-bit words: starts[n_seqs + 1] ascends, sequence s has rows starts[s] .. starts[s + 1] - 1 (none,
  * one, or more); lens[s] is the number of positions it holds, its rows the last of them: row r is position lens[s] - (starts[s + 1] - r).
  * table[s][max_pages] names its pages; entries behind its last position are not read. The op takes up to n_rows rows; rows behind
- * starts[n_seqs] belong to no sequence and are left as they are, in every output. The words are read when the op runs, so a
- * captured call serves other lengths when it is replayed. max_queries, the most rows of one sequence as far as the caller knows, chooses
+ * starts[n_seqs] belong to no sequence and are left as they are, in every output. The words are read when the op runs, at any time until it
+ * ends, and stay as they are meanwhile; a captured call serves other lengths when it is replayed. max_queries, the most rows of one sequence as far as the caller knows, chooses
  * among kernels, with max_pages, and changes no more than rounding when it is wrong. 1 to 65535 sequences, up to 2^24 rows.
  * Rows that lie before a sequence's first position (more rows than positions) have no place: they are not written, read as zeros and attend to
  * nothing. A position behind the table or in a page that the pool does not have (its number is n_pages or more) is treated the same
