@@ -7,6 +7,7 @@
 #include <cstdarg>
 #include <cstring>
 #include <initializer_list>
+#include <new>
 
 namespace bc {
 
@@ -40,8 +41,7 @@ bc_status check_range(const bc_backend* backend, const bc_buffer* buffer, size_t
 
 namespace {
 
-// Per device: one word of mapped host memory per kernel file with bounded waits, and one for the key/value pool's kernels, for the life of
-// the process.
+// Per device: one word of mapped host memory per kernel file with bounded waits, for the life of the process.
 constexpr int kWaitWords = 8, kMaxDevices = 64;
 std::atomic<volatile int*> g_wait_words[kMaxDevices];
 
@@ -51,8 +51,8 @@ bc_status set_wait_words(int device) {
     std::lock_guard<std::mutex> lock(mutex);
     if (g_wait_words[device].load()) return BC_OK;
     int* words = nullptr;
-    BC_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&words), (kWaitWords + 1) * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable));
-    for (int i = 0; i <= kWaitWords; ++i) words[i] = 0;
+    BC_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&words), kWaitWords * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable));
+    for (int i = 0; i < kWaitWords; ++i) words[i] = 0;
     BC_CUDA(k::matvec_wait_word(words));
     BC_CUDA(k::matmul_wait_word(words + 1));
     BC_CUDA(k::matmul_half_wait_word(words + 2));
@@ -67,6 +67,14 @@ bc_status set_wait_words(int device) {
 
 }  // namespace
 
+// Whether a graph is being recorded from the stream's launches.
+bool is_capturing(cudaStream_t stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &status) == cudaSuccess) return status != cudaStreamCaptureStatusNone;
+    cudaGetLastError();
+    return true;
+}
+
 // A kernel whose bounded wait ran out leaves a code rather than hanging the device. Reading a code
 // clears it, so one failure is reported once and later healthy work is not blamed for it.
 bc_status kernel_wait_status() {
@@ -74,11 +82,7 @@ bc_status kernel_wait_status() {
     if (cudaGetDevice(&device) != cudaSuccess || device >= kMaxDevices) return BC_OK;
     volatile int* words = g_wait_words[device].load();
     if (!words) return BC_OK;
-    auto take = [&](int i) {
-        const int code = words[i];
-        if (code) words[i] = 0;
-        return code;
-    };
+    auto take = [&](int i) { return __atomic_exchange_n(const_cast<int*>(words + i), 0, __ATOMIC_RELAXED); };
     if (int code = take(0)) return fail(BC_ERR_EXECUTION, "a decode kernel gave up waiting for its weight stream or its input (code %d)", code);
     if (int code = take(1)) return fail(BC_ERR_EXECUTION, "a prefill kernel gave up waiting on its pipeline (code %d)", code);
     if (int code = take(2)) return fail(BC_ERR_EXECUTION, "a prefill kernel gave up waiting on its pipeline (code %d)", code);
@@ -87,16 +91,83 @@ bc_status kernel_wait_status() {
     if (int code = take(5)) return fail(BC_ERR_EXECUTION, "a product over experts gave up waiting on its pipeline (code %d)", code);
     if (int code = take(4)) return fail(BC_ERR_EXECUTION, "a product of few rows gave up waiting for its %s (code %d)", code == 2 ? "weights" : "sums", code);
     if (int code = take(7)) return fail(BC_ERR_EXECUTION, "attention over pages gave up waiting on its pipeline (code %d)", code);
-    if (int code = words[kWaitWords]) {
-        words[kWaitWords] = 0;
-        return fail(BC_ERR_OUT_OF_BOUNDS, code == 1 ? "a page table names a page that the pool does not have" : "a sequence holds more positions than its page table");
-    }
     return BC_OK;
 }
 
-int* page_fault_word(int device) {
-    volatile int* words = device < kMaxDevices ? g_wait_words[device].load() : nullptr;
-    return words ? const_cast<int*>(words) + kWaitWords : nullptr;
+namespace {
+
+// Words of mapped host memory that kernels of the key/value pool leave a fault in, handed out one at a time, zero. Their memory stays for the life of the process:
+// a captured graph may name one for as long as it exists.
+class FaultWords {
+  public:
+    int* take() {
+        std::lock_guard<std::mutex> lock(mutex_);
+        if (free_.empty()) {
+            int* words = nullptr;
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // another stream may be capturing, which this has no part in
+            cudaThreadExchangeStreamCaptureMode(&mode);
+            const cudaError_t e = cudaHostAlloc(reinterpret_cast<void**>(&words), kBlock * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+            cudaThreadExchangeStreamCaptureMode(&mode);
+            if (e != cudaSuccess) {
+                cudaGetLastError();
+                return nullptr;
+            }
+            free_.reserve(all_ += kBlock);  // give_back never allocates
+            for (size_t i = 0; i < kBlock; ++i) words[i] = 0, free_.push_back(words + i);
+        }
+        int* const word = free_.back();
+        free_.pop_back();
+        return word;
+    }
+    void give_back(int* word) {
+        std::lock_guard<std::mutex> lock(mutex_);
+        free_.push_back(word);
+    }
+
+  private:
+    static constexpr size_t kBlock = 1024;
+    std::mutex mutex_;
+    std::vector<int*> free_;
+    size_t all_ = 0;
+};
+FaultWords& fault_words() {
+    static FaultWords* words = new FaultWords();  // outlives backends that the process's end closes
+    return *words;
+}
+
+int read_fault(int* word) { return __atomic_exchange_n(word, 0, __ATOMIC_ACQUIRE); }
+
+bc_status page_fault_status(int code) {
+    if (!code) return BC_OK;
+    return fail(BC_ERR_OUT_OF_BOUNDS, code == 1 ? "a page table names a page that the pool does not have" : "a sequence holds more positions than its page table");
+}
+
+// What the recording's launches left, whose work has ended; the word goes back.
+int collect_page_fault(bc_backend* b, uint64_t ticket) {
+    auto word = b->page_faults.find(ticket);
+    if (word == b->page_faults.end()) return 0;
+    const int code = read_fault(word->second);
+    fault_words().give_back(word->second);
+    b->page_faults.erase(word);
+    return code;
+}
+
+}  // namespace
+
+int* page_fault_word(bc_backend* b) {
+    if (is_capturing(b->stream)) {
+        b->captured_page_ops = true;
+        return b->captured_page_fault;
+    }
+    try {
+        auto kept = b->page_faults.find(b->next_ticket);
+        if (kept != b->page_faults.end()) return kept->second;
+        int* const word = fault_words().take();
+        if (word) b->page_faults[b->next_ticket] = word;
+        return word;
+    } catch (const std::bad_alloc&) {
+        return nullptr;
+    }
 }
 
 }  // namespace bc
@@ -179,13 +250,6 @@ bc_status expand_for_many_tokens(bc_backend* b, bc_buffer* buffer, bool capturin
     return BC_OK;
 }
 
-bool is_capturing(cudaStream_t stream) {
-    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(stream, &status) == cudaSuccess) return status != cudaStreamCaptureStatusNone;
-    cudaGetLastError();
-    return true;
-}
-
 // The vectorised kernels read activations 16 bytes at a time: views of activation vectors must
 // start on a 16-byte boundary (cudaMalloc bases are 256-byte aligned, so only the offset matters).
 // Checked before any launch, because a misaligned vector load is a device fault, not a status code.
@@ -214,6 +278,11 @@ bc_status bc_backend_open(int32_t device, void* stream, bc_backend** out) {
     b->device = device;
     BC_TRY(b->activate());
     BC_TRY(set_wait_words(device));
+    try {
+        b->captured_page_fault = fault_words().take();
+    } catch (const std::bad_alloc&) {
+    }
+    if (!b->captured_page_fault) return fail(BC_ERR_ALLOCATION, "no host memory for a backend");
     if (stream) {
         b->stream = static_cast<cudaStream_t>(stream);
     } else {
@@ -246,6 +315,8 @@ void bc_backend_close(bc_backend* b) {
     if (b->pack) cudaFree(b->pack);
     if (b->partials) cudaFree(b->partials);
     if (b->owns_stream) cudaStreamDestroy(b->stream);
+    while (!b->page_faults.empty()) collect_page_fault(b, b->page_faults.begin()->first);
+    if (!b->captured_page_ops) fault_words().give_back(b->captured_page_fault);
     delete b;
 }
 
@@ -414,7 +485,10 @@ bc_status bc_wait(bc_backend* b, bc_ticket ticket, double* seconds) {
     cudaEventDestroy(end->second);
     b->tickets.erase(end);
     if (seconds) *seconds = ms * 1e-3;
-    return kernel_wait_status();
+    const int fault = collect_page_fault(b, ticket);
+    BC_TRY(kernel_wait_status());
+    BC_TRY(page_fault_status(fault));
+    return page_fault_status(read_fault(b->captured_page_fault));
 }
 
 bc_status bc_end(bc_backend* b, double* seconds) {
@@ -433,6 +507,7 @@ void bc_discard(bc_backend* b) {
         cudaEventDestroy(start->second);
         b->ticket_starts.erase(start);
     }
+    collect_page_fault(b, b->next_ticket);
     b->recording = false;
 }
 

@@ -65,6 +65,11 @@ struct bc_backend {
     cudaEvent_t record_start = nullptr;
     std::map<uint64_t, cudaEvent_t> tickets;  // ticket -> end-of-recording event
     std::map<uint64_t, cudaEvent_t> ticket_starts;
+    // Words that launches over a key/value pool leave a fault in (kv_pool.cuh): a recording's with its ticket, until its wait; one for all that were captured into
+    // graphs, which run at any time.
+    std::map<uint64_t, int*> page_faults;
+    int* captured_page_fault = nullptr;
+    bool captured_page_ops = false;
     std::set<bc_buffer*> buffers;
     std::set<bc_seq*> seqs;  // sequences recording onto this backend; closing the backend releases them
     uint64_t launches = 0;  // kernels launched through this backend
@@ -96,8 +101,9 @@ namespace bc {
 bc_status check_range(const bc_backend* backend, const bc_buffer* buffer, size_t offset, size_t needed, const char* op);
 // BC_ERR_EXECUTION when a kernel's bounded wait ran out since the last call; clears the record.
 bc_status kernel_wait_status();
-// The word of host memory that the key/value pool's kernels leave a fault in (kv_pool.cuh); null on a device that has none.
-int* page_fault_word(int device);
+// The word of host memory that a launch over the key/value pool leaves a fault in (kv_pool.cuh), of the open recording, or of the backend's captured
+// launches; null without memory.
+int* page_fault_word(bc_backend* b);
 
 }  // namespace bc
 

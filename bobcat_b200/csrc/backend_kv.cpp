@@ -59,8 +59,8 @@ bc_status pool_and_rows(bc_backend* b, const bc_kv_pool* pool, const bc_kv_rows*
     BC_TRY(aligned(op, "tables", rows->table_off, 4));
     BC_TRY(aligned(op, "starts", rows->starts_off, 4));
     BC_TRY(aligned(op, "lengths", rows->lens_off, 4));
-    int* fault = page_fault_word(b->device);
-    if (!fault) return fail(BC_ERR_UNSUPPORTED, "key/value pages on device %d", b->device);
+    int* fault = page_fault_word(b);
+    if (!fault) return fail(BC_ERR_ALLOCATION, "no host memory for the %s launch's faults", op);
     uint32_t shift = 0;
     while (1u << shift < pool->page_size) ++shift;
     *p = k::KvPool{pool->format, pool->n_pages, shift, pool->n_kv_heads, pool->head_dim, (uint32_t)row_bytes(pool->format, pool->head_dim), page,
