@@ -128,7 +128,7 @@ struct Place {
 struct TileDesc {
     uint32_t key0, end;       // the first position, and the position behind the sequence's last that its table can name
     uint32_t groups;          // of 16 positions, a bit each: in a page of the pool
-    uint32_t row0, n, head;   // the row tile's first row of the call, its rows, the KV head
+    uint32_t seq, row0, n, head;  // the sequence; the row tile's first row of the call, its rows, the KV head
     int32_t pos0;             // the position of its first row
     uint32_t unit;            // number within the run
     uint32_t first, last;     // of the unit
@@ -188,6 +188,11 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     float2 r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(r)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+    return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN if any is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -626,7 +631,46 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
                 float2 x[8];
                 load_scores(scores_at, info, masked, see, c, x);
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) most[i & 1] = fmaxf(most[i & 1], fmaxf(x[i].x, x[i].y));
+                for (uint32_t i = 0; i < 8; ++i)
+                    most[i & 1] = FMT == BC_F16 ? max3_nan(most[i & 1], x[i].x, x[i].y) : fmaxf(most[i & 1], fmaxf(x[i].x, x[i].y));
+            }
+            if constexpr (FMT == BC_F16) {
+                // A score that is no number, for the first time: of an infinite key, perhaps one whose score is minus infinity, which weighs nothing.
+                const bool some = (most[0] != most[0] || most[1] != most[1]) && total == total;
+                if (__builtin_expect(__any_sync(0xffffffffu, some), 0)) {
+                    const TileDesc& desc = sh.desc[tile % kDescRing];
+                    const uint32_t query = row / p.group;
+                    const bool mine = some && query < desc.n;
+                    const float* const q = p.q + (mine ? (uint64_t)(desc.row0 + query) * p.q_stride + (uint64_t)(desc.head * p.group + row % p.group) * p.q_head_stride : 0);
+                    most[0] = most[1] = -INFINITY;
+#pragma unroll 1
+                    for (uint32_t c = 0; c < kScores; c += 16) {
+                        float x[16];
+                        tmem_load_16(scores_at + c, x);
+                        const uint32_t bits = masked ? seen_bits(info, first_score + c, see - (int32_t)c) : 0xffffu;
+                        uint32_t nothing = 0;
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; ++i) nothing |= x[i] != x[i] ? 1u << i : 0u;
+                        nothing = mine ? nothing & bits : 0;
+                        for (uint32_t left = nothing; left; left &= left - 1) {
+                            const uint32_t i = __ffs(left) - 1, key = desc.key0 + first_score + c + i;
+                            const uint32_t page = p.rows.table[(uint64_t)desc.seq * p.rows.max_pages + (key >> pool.page_shift)];
+                            if (page >= pool.n_pages || !score_is_minus_infinity(q, pool.k + kv_row_at(pool, page, desc.head, key & ((1u << pool.page_shift) - 1)), HD))
+                                nothing &= ~(1u << i);
+                        }
+                        __syncwarp();
+                        uint32_t back[2][8];
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; ++i) {
+                            if (nothing >> i & 1) x[i] = -INFINITY;
+                            if (bits >> i & 1) most[i & 1] = fmaxf(most[i & 1], x[i]);
+                            back[i / 8][i % 8] = __float_as_uint(x[i]);
+                        }
+                        tmem_store_8(scores_at + c, back[0]);
+                        tmem_store_8(scores_at + c + 8, back[1]);
+                    }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                }
             }
             float now = fmaxf(top, fmaxf(most[0], most[1]) * factor);
             sh.most[tile & 1][part][row] = now;
@@ -1037,6 +1081,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
                         const int64_t pos = (int64_t)s.len - (s.end - s.row0) + query0;
                         d.key0 = (u.tile0 + at.in_unit) * KT;
                         d.end = s.held;
+                        d.seq = u.seq;
                         d.row0 = s.row0 + query0;
                         d.n = min(per_tile, s.n - query0);
                         d.head = u.head;

@@ -523,6 +523,23 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attention_token_pag
                 x[i] = exp2_fast(x[i] - down);  // the sums are lifted alike
                 total_step += x[i];
             }
+            if constexpr (FMT == BC_F16) {
+                // No number, for the first time: of an infinite key, perhaps one whose score is minus infinity, which weighs nothing.
+                const uint32_t q_head = PACKED ? g & 3 : g;
+                if (__builtin_expect(__any_sync(0xffffffffu, total_step != total_step && total_p == total_p && q_head < p.group), 0)) {
+                    total_step = 0.f;
+#pragma unroll
+                    for (int i = 0; i < kScores; ++i) {
+                        const uint32_t in_step = 16 * (i >> 2) + 2 * t + (i & 1) + 8 * (i >> 1 & 1), page = page_ids[warp][(n * kHalves + (i >> 2)) % 64];
+                        if (x[i] != x[i] && q_head < p.group && page < pool.n_pages &&
+                            score_is_minus_infinity(p.q + done.row * p.q_stride + (done.head * p.group + q_head) * p.q_head_stride,
+                                                    pool.k + kv_row_at(pool, page, done.head, (pos0 + n * kBlock + in_step) & slots), HD))
+                            x[i] = 0.f;
+                        total_step += x[i];
+                    }
+                    __syncwarp();
+                }
+            }
             total_p = total_p * factor + total_step;
             if constexpr (FMT == BC_I8) {
 #pragma unroll

@@ -66,5 +66,24 @@ __device__ __forceinline__ void unpack_i8(uint32_t w, uint32_t& lo, uint32_t& hi
     hi = *reinterpret_cast<uint32_t*>(&y);
 }
 
+// Whether the score of a query with a half key that is not finite is minus infinity: every infinite element's product with the query's is, and there is no NaN.
+// (Products of a query's halves with an infinity need not have its sign, and are no number where a half is zero.)
+__device__ __forceinline__ bool score_is_minus_infinity(const float* q, const uint8_t* key, uint32_t head_dim) {
+    bool minus = false;
+#pragma unroll 1
+    for (uint32_t e = 0; e < head_dim; e += 2) {
+        const uint32_t pair = *reinterpret_cast<const uint32_t*>(key + 2 * e);
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+            const uint32_t bits = pair >> (16 * i) & 0xffffu;
+            if ((bits & 0x7fffu) < 0x7c00u) continue;
+            const float x = q[e + i];
+            if ((bits & 0x7fffu) > 0x7c00u || !(bits >> 15 ? x > 0.f : x < 0.f)) return false;
+            minus = true;
+        }
+    }
+    return minus;
+}
+
 }  // namespace k
 }  // namespace bc
