@@ -252,9 +252,11 @@ typedef struct bc_kv_pool {
  * ends, and stay as they are meanwhile; a captured call serves other lengths when it is replayed. max_queries, the most rows of one sequence as far as the caller knows, chooses
  * among kernels, with max_pages, and changes no more than rounding when it is wrong. 1 to 65535 sequences, up to 2^24 rows.
  * Rows that lie before a sequence's first position (more rows than positions) have no place: they are not written, read as zeros and attend to
- * nothing. A position behind the table or in a page that the pool does not have (its number is n_pages or more) is treated the same
- * way, as a key it is left out, and the wait for the recording (bc_wait, bc_end) returns BC_ERR_OUT_OF_BOUNDS, once; other recordings, other
- * backends and steps of models do not. What a captured call meets when its graph runs is returned by the next wait for a recording of its backend. */
+ * nothing.
+ * A position behind the table, or in a page that the pool does not have (its number is n_pages or more), cannot be written, reads as zeros, and is left out as a
+ * key; the row of such a position attends to the keys up to its own position that are there, none of which gives zeros. The wait for the recording
+ * (bc_wait, bc_end) returns BC_ERR_OUT_OF_BOUNDS, once; other recordings, other backends and steps of models do not. What a captured call meets when its
+ * graph runs is returned by the next wait for a recording of its backend. */
 typedef struct bc_kv_rows {
     uint32_t n_seqs, n_rows, max_queries, max_pages;
     bc_buffer* table;
