@@ -1085,7 +1085,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
                         d.row0 = s.row0 + query0;
                         d.n = min(per_tile, s.n - query0);
                         d.head = u.head;
-                        d.pos0 = (int32_t)min(pos, (int64_t)0x7fffffff);
+                        d.pos0 = (int32_t)max(min(pos, (int64_t)0x7fffffff), -(int64_t)0x7fffffff);
                         d.unit = at.unit_number;
                         d.first = at.in_unit == 0;
                         d.last = at.in_unit + 1 == u.tiles;

@@ -1,11 +1,11 @@
-"""Lengths that the page table does not cover."""
+"""Lengths that the page table does not cover, and rows that a call does not take."""
 
 import numpy as np
 import pytest
 
-from bobcat_b200 import F16, I8, errors
+from bobcat_b200 import F16, I8, KvRows, errors
 from kv_pool_cases import Pool, attention
-from test_attention_paged_gpu import MARK
+from test_attention_paged_gpu import MARK, attend, check
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +53,30 @@ def test_rows_behind_the_table_are_not_written(cuda, fmt):
             case.put(case.v_raw, s, pos, x[row0 + pos, 128:].reshape(2, 64))
     k_now, v_now = case.download()
     assert np.array_equal(k_now, case.k_raw) and np.array_equal(v_now, case.v_raw)
+
+
+@pytest.mark.parametrize("hint", [1, 1000])
+@pytest.mark.parametrize("fmt", [F16, I8])
+@pytest.mark.parametrize("end", [41, 1 << 24, (1 << 31) + 5, (1 << 32) - 1])
+def test_rows_of_a_sequence_that_a_call_does_not_take(cuda, end, fmt, hint):
+    """A sequence of more rows than the call takes, and than positions: those that it takes lie before the first position, or at it."""
+    case = Pool(cuda, fmt, 16, 2, 64, [40], np.random.default_rng(75))
+    case.fill(np.random.default_rng(76))
+    case.upload()
+    q = np.random.default_rng(77).standard_normal((40, 4 * 64)).astype(np.float32)
+    c = cuda
+    rows = KvRows(1, 40, hint, case.max_pages, c.buffer_from(case.table), c.buffer_from(np.array([0, end], dtype=np.uint32)), c.buffer_from(np.array([40], dtype=np.uint32)))
+    got = attend(cuda, case, [40], 4, q, rows=rows)
+    if end == 41:  # row r is position r - 1
+        assert (got[0] == 0).all()
+        check(case, [39], 4, q[1:], got[1:], lens=[39])
+    else:
+        assert (got == 0).all()
+    back = cuda.buffer_from(np.full((40, 128), 9.0, dtype=np.float32))
+    cuda.begin()
+    cuda.kv_read(case.pool, rows, back, None, False, 128, 128)
+    cuda.end()
+    want = np.zeros((40, 128), dtype=np.float32)
+    if end == 41:
+        want[1:] = np.stack([case.get(case.k_raw, 0, pos, np.float32).reshape(-1) for pos in range(39)])
+    assert np.array_equal(cuda.read(back, np.zeros_like(want)), want)
