@@ -1,6 +1,8 @@
 // Bounds-checked op wrappers of the key/value pool, and buffers over memory of the caller's. What lies on the device (page tables, row
 // starts, lengths) is checked by the kernels: see kv_pool.cuh.
 
+#include <cuda.h>
+
 #include <new>
 
 #include "backend.h"
@@ -78,6 +80,28 @@ bc_status strided(bc_backend* b, bc_buffer* buffer, size_t offset, uint32_t n_ro
     return check_range(b, buffer, offset, n_rows ? ((size_t)(n_rows - 1) * stride + width) * element : 0, op);
 }
 
+// Whether [at, at + len) is allocated device memory. The driver, reached through cudaGetDriverEntryPoint, names one allocation or mapping at a time; a range
+// may lie over several neighbouring mappings.
+bool allocated(uintptr_t at, size_t len) {
+    using AddressRange = CUresult (*)(CUdeviceptr*, size_t*, CUdeviceptr);
+    static const AddressRange range_of = [] {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        const bool ok = cudaGetDriverEntryPoint("cuMemGetAddressRange", &fn, cudaEnableDefault, &found) == cudaSuccess && found == cudaDriverEntryPointSuccess;
+        return ok ? reinterpret_cast<AddressRange>(fn) : nullptr;
+    }();
+    while (len > 0) {
+        CUdeviceptr base = 0;
+        size_t size = 0;
+        if (!range_of || range_of(&base, &size, (CUdeviceptr)at) != CUDA_SUCCESS || at < base || at - base >= size) return false;
+        const size_t here = size - (at - base);
+        if (here >= len) return true;
+        at += here;
+        len -= here;
+    }
+    return true;
+}
+
 }  // namespace
 
 extern "C" {
@@ -95,6 +119,7 @@ bc_status bc_buffer_at(bc_backend* b, void* ptr, size_t len, bc_buffer** out) {
         }
         if (attributes.type != cudaMemoryTypeDevice || attributes.device != b->device)
             return fail(BC_ERR_ARGUMENT, "the pointer is not memory of device %d", b->device);
+        if (!allocated(reinterpret_cast<uintptr_t>(ptr), len)) return fail(BC_ERR_ARGUMENT, "the memory at the pointer ends before %zu bytes", len);
     }
     try {
         std::unique_ptr<bc_buffer> buffer(new bc_buffer());

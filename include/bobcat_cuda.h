@@ -98,8 +98,8 @@ size_t bc_buffer_len(const bc_buffer* buffer);
 /* The device address, for callers that share the buffer with their own CUDA code. */
 void* bc_buffer_device_ptr(bc_buffer* buffer);
 /* A buffer over `len` bytes of device memory of the caller's (another library's tensor), for ops that read or
- * write it in place. No counterpart in the reference, whose buffers share memory with the CPU. `ptr` is memory of the backend's device
- * and starts at a multiple of 256 bytes, as the backend's own buffers do (a view's offset reaches what lies behind); it stays the
+ * write it in place. No counterpart in the reference, whose buffers share memory with the CPU. `ptr` is memory of the backend's device,
+ * allocated for `len` bytes, and starts at a multiple of 256 bytes, as the backend's own buffers do (a view's offset reaches what lies behind); it stays the
  * caller's: bc_buffer_free and bc_backend_close wait for the stream and drop the handle alone. Ops run on the backend's stream, so work of
  * other streams on the memory has to be ordered with it by the caller. */
 bc_status bc_buffer_at(bc_backend* backend, void* ptr, size_t len, bc_buffer** out);
