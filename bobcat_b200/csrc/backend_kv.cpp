@@ -80,6 +80,24 @@ bc_status strided(bc_backend* b, bc_buffer* buffer, size_t offset, uint32_t n_ro
     return check_range(b, buffer, offset, n_rows ? ((size_t)(n_rows - 1) * stride + width) * element : 0, op);
 }
 
+// Floats from a view on.
+struct Floats {
+    uintptr_t at;
+    uint64_t n;
+};
+Floats floats_at(bc_buffer* buffer, size_t offset, uint64_t n) { return Floats{reinterpret_cast<uintptr_t>(buffer->ptr) + offset, n}; }
+bool overlap(const Floats& a, const Floats& b) { return a.at < b.at + 4 * b.n && b.at < a.at + 4 * a.n; }
+
+// Whether `x` lies over some head of strided rows, whose strides are no less than what they step over: heads ascend, so only the last one that begins before the end of
+// `x` can reach into it.
+bool over_heads(const Floats& x, uintptr_t first, uint32_t n_rows, uint64_t stride, uint32_t n_heads, uint64_t head_stride, uint32_t head_dim) {
+    const uintptr_t end = x.at + 4 * x.n;
+    if (end <= first) return false;
+    const uint64_t ahead = (end - first - 1) / 4, row = ahead / stride < n_rows ? ahead / stride : n_rows - 1, in_row = (ahead - row * stride) / head_stride;
+    const uint64_t head = in_row < n_heads ? in_row : n_heads - 1;
+    return first + 4 * (row * stride + head * head_stride + head_dim) > x.at;
+}
+
 // Whether [at, at + len) is allocated device memory. The driver, reached through cudaGetDriverEntryPoint, names one allocation or mapping at a time; a range
 // may lie over several neighbouring mappings.
 bool allocated(uintptr_t at, size_t len) {
@@ -189,6 +207,12 @@ bc_status bc_op_attention_paged(bc_backend* b, const bc_kv_pool* pool, const bc_
     BC_TRY(aligned("attention_paged", "scratch", s_off, 16));
     BC_TRY(check_range(b, scratch, s_off, bc_attention_paged_scratch_floats(n_heads, p.n_kv_heads, p.head_dim) * 4, "attention_paged"));
     if (r.n_rows == 0) return BC_OK;
+    const Floats outs = floats_at(out, out_off, (uint64_t)r.n_rows * n_heads * p.head_dim),
+                 parts = floats_at(scratch, s_off, bc_attention_paged_scratch_floats(n_heads, p.n_kv_heads, p.head_dim));
+    const uintptr_t queries = reinterpret_cast<uintptr_t>(at<const float>(q, q_off));
+    if (overlap(outs, parts) || over_heads(outs, queries, r.n_rows, q_stride, n_heads, q_head_stride, p.head_dim) ||
+        over_heads(parts, queries, r.n_rows, q_stride, n_heads, q_head_stride, p.head_dim))
+        return fail(BC_ERR_ARGUMENT, "the attention_paged launch has queries, scratch and results that overlap");
     return b->run("attention_paged", r.n_rows, r.n_seqs, 0, k::attention_paged_launches(p, r, n_heads), [&] {
         return k::attention_paged(b->stream, p, r, at<const float>(q, q_off), q_stride, q_head_stride, at<float>(scratch, s_off), at<float>(out, out_off), n_heads);
     });

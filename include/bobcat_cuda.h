@@ -280,7 +280,7 @@ bc_status bc_op_kv_read(bc_backend* b, const bc_kv_pool* pool, const bc_kv_rows*
  * stored. q is f32, token rows q_stride and heads q_head_stride elements apart (multiples of 4); out is [n_rows][n_heads * head_dim]
  * f32, zeros for a row that sees nothing; elements of positions that a row does not see have no part in it, whatever they are, and a value that is
  * not finite makes its element of the rows that see it not finite. A key that is not finite counts by the formula: where the score is minus infinity it weighs
- * nothing (a row all of whose scores are is zeros), else the rows that see it are NaN. Up to 8 query heads per KV head. out does not overlap q. Scores and sums are f32; operands keep 22
+ * nothing (a row all of whose scores are is zeros), else the rows that see it are NaN. Up to 8 query heads per KV head. q, scratch and out that overlap are refused. Scores and sums are f32; operands keep 22
  * bits: of a query element, or 2^-30 of its row's largest; of a probability, or 2^-40 of its row's largest; with 8-bit values, of a probability times the
  * values' scale, or 2^-32 of the largest of these that the row sees. (Sums of numbers above 2^80 may pass the largest float.) `scratch` needs
  * bc_attention_paged_scratch_floats floats (whatever the lengths), for the duration of the call: calls that may overlap, replayed graphs among
