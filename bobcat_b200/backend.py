@@ -77,6 +77,10 @@ class KvPool(_lib.KvPool):
         super().__init__(fmt, n_pages, page_size, n_kv_heads, head_dim, *_v(k), *_v(v))
         self.holds = (k, v)
 
+    def _now(self) -> "KvPool":
+        (self.k, self.k_off), (self.v, self.v_off) = map(_v, self.holds)  # of a buffer that was freed: none
+        return self
+
 
 class KvRows(_lib.KvRows):
     """The rows of a call over a pool (``bc_kv_rows``): page tables, row starts and lengths are views of 32-bit words."""
@@ -84,6 +88,10 @@ class KvRows(_lib.KvRows):
     def __init__(self, n_seqs: int, n_rows: int, max_queries: int, max_pages: int, table, starts, lens):
         super().__init__(n_seqs, n_rows, max_queries, max_pages, *_v(table), *_v(starts), *_v(lens))
         self.holds = (table, starts, lens)
+
+    def _now(self) -> "KvRows":
+        (self.table, self.table_off), (self.starts, self.starts_off), (self.lens, self.lens_off) = map(_v, self.holds)
+        return self
 
 
 class Readback:
@@ -256,13 +264,13 @@ class Cuda:
         return int(self._L.bc_kv_pool_bytes(fmt, n_pages, page_size, n_kv_heads, head_dim))
 
     def kv_write(self, pool: KvPool, rows: KvRows, k, v, k_stride, v_stride) -> None:
-        self._check(self._L.bc_op_kv_write(self._h, pool, rows, *_v(k), *_v(v), k_stride, v_stride))
+        self._check(self._L.bc_op_kv_write(self._h, pool._now(), rows._now(), *_v(k), *_v(v), k_stride, v_stride))
 
     def kv_read(self, pool: KvPool, rows: KvRows, k, v, out_half, k_stride, v_stride) -> None:
-        self._check(self._L.bc_op_kv_read(self._h, pool, rows, *_v(k), *_v(v), int(out_half), k_stride, v_stride))
+        self._check(self._L.bc_op_kv_read(self._h, pool._now(), rows._now(), *_v(k), *_v(v), int(out_half), k_stride, v_stride))
 
     def attention_paged(self, pool: KvPool, rows: KvRows, q, scratch, out, n_heads, q_stride, q_head_stride) -> None:
-        self._check(self._L.bc_op_attention_paged(self._h, pool, rows, *_v(q), *_v(scratch), *_v(out), n_heads, q_stride, q_head_stride))
+        self._check(self._L.bc_op_attention_paged(self._h, pool._now(), rows._now(), *_v(q), *_v(scratch), *_v(out), n_heads, q_stride, q_head_stride))
 
     def attention_paged_scratch_floats(self, n_heads, n_kv_heads, head_dim) -> int:
         return int(self._L.bc_attention_paged_scratch_floats(n_heads, n_kv_heads, head_dim))
