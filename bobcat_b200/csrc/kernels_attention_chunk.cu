@@ -19,6 +19,8 @@
 // the issue slots are used, 12 % of the waiting is for instructions. Tried and left: four threads to a row (2.48 ms: the instructions grow by a quarter), scores held in
 // registers between maximum and exponential (2.61 ms). 512 rows from position 0, 32 heads of 64, take 18 us, most of it one CTA's way through two tiles.
 
+#include <type_traits>
+
 #include "async_utils.cuh"
 #include "chunk_schedule.h"
 #include "kv_pool.cuh"
@@ -41,6 +43,7 @@ constexpr int kRowRegisters = 184, kUnpackRegisters = 96, kOtherRegisters = 48;
 constexpr uint32_t kCore = 144;                    // bytes from one core matrix to the next
 constexpr uint32_t kTmemColumns = 512;
 constexpr uint32_t kMostCtas = kChunkMostCtas;
+constexpr uint32_t kJoinCtas = 8;                  // of the joining launch, to a cut row tile
 constexpr uint32_t kSpinLimit = 1u << 22;
 constexpr uint32_t kRing = 4, kDescRing = 8;       // tiles whose scales and masks are kept; whose descriptions are
 
@@ -59,14 +62,22 @@ struct ChunkParams {
     KvRows rows;
     const float* q;
     float* out;
-    float* parts;  // [2 * CTA + which][kRows][HD] sums, then [2 * CTA + which][kRows] (maximum, sum), then a ChunkHead per CTA
+    float* parts;  // [2 * CTA + which][kRows][HD] sums, then [2 * CTA + which][kRows] (maximum, sum), then a ChunkHead per CTA, then a ChunkSpan
     uint64_t q_stride, q_head_stride;
     uint32_t n_heads, group, fewest;
 };
-// The unit that begins in a CTA's run and goes on behind it, for the joining launch; `last` is the CTA it ends in, 0 when there is none.
+// What a CTA leaves the joining launch: the unit that begins in its run and goes on behind it, `last` the CTA that this ends in, 0 when there is none; and whether
+// sums of a row that it has written whole are no number (kOdd).
 struct ChunkHead {
-    uint32_t row0, n, head, last;  // rows of the call from row0, n of them; KV head
+    uint32_t row0, n, head, last;  // rows of the call from row0, n of them (and kOdd); KV head
 };
+constexpr uint32_t kOdd = 1u << 31;
+// Its first unit and its last.
+struct ChunkSpan {
+    uint32_t seq[2], head[2], row_tile[2], unused[2];
+};
+__device__ __forceinline__ ChunkHead* chunk_heads(float* parts, uint32_t head_dim) { return reinterpret_cast<ChunkHead*>(parts + (uint64_t)2 * kMostCtas * kRows * (head_dim + 2)); }
+__device__ __forceinline__ ChunkSpan* chunk_spans(float* parts, uint32_t head_dim) { return reinterpret_cast<ChunkSpan*>(chunk_heads(parts, head_dim) + kMostCtas); }
 
 // A stretch of key tiles of one row tile.
 struct Unit {
@@ -123,12 +134,13 @@ struct Place {
     Unit unit;
     uint32_t in_unit, unit_number;
     ChunkHead cut;
+    ChunkSpan span;
 };
 // What a tile is, for every role.
 struct TileDesc {
     uint32_t key0, end;       // the first position, and the position behind the sequence's last that its table can name
     uint32_t groups;          // of 16 positions, a bit each: in a page of the pool
-    uint32_t seq, row0, n, head;  // the sequence; the row tile's first row of the call, its rows, the KV head
+    uint32_t row0, n, head;   // the row tile's first row of the call, its rows, the KV head
     int32_t pos0;             // the position of its first row
     uint32_t unit;            // number within the run
     uint32_t first, last;     // of the unit
@@ -188,11 +200,6 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     float2 r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(r)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
-    return r;
-}
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN if any is
-    float r;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -285,6 +292,7 @@ struct Shared {
     Place place;
     uint32_t tmem;
     int dead, never;            // whether a wait has run out; a flag that nobody raises
+    int odd;                    // whether sums of a row that was written whole are no number
 };
 
 template <int FMT, int HD>
@@ -334,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
         for (uint32_t w = 0; w < 4; ++w) mbar_init(rows_bar + 8 * w, kParts);
         mbar_init(unpack_bar, kUnpackWarps);
         for (uint32_t d = 0; d < kDescRing; ++d) mbar_init(described + 8 * d, 1);
-        sh.dead = sh.never = 0;
+        sh.dead = sh.never = sh.odd = 0;
         mbar_init_fence();
     }
     if (warp == kMmaWarp) tmem_alloc(smem_u32(&sh.tmem), kTmemColumns);
@@ -429,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
         if (lane == 0) sh.ahead[begin ? 0 : 1] = ahead;
         if (lane == 0 && begin) {
             sh.counted = counted;
-            sh.place.cut = ChunkHead{0, 0, 0, 0};
+            sh.place.cut = ChunkHead{};
             sh.place.cursor = cur;
             sh.place.unit.tiles = sh.place.in_unit = 0;
             sh.place.unit_number = ~0u;
@@ -591,27 +599,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
         // The tile's scores to probabilities, in place: of each 16 the upper halves, then the lower. 16 at a time, twice (for their maximum, then again), in loops of 16 and not
         // more: roles run side by side, and what bounds all of them is that they fetch each other's instructions away (2048 rows over 10000 positions: 672 us; 730
         // with two of them in a line, 950 with all four; scores kept in registers between the two, 10 % slower than read twice).
-        auto take = [&](uint32_t tile, float& keep, float& grow) {
-            const uint32_t buffer = tile & 1, scores_at = lanes + buffer * KT + first_score;
+        // PLAIN: every row sees all of the tile, and 8-bit values' weights are counted by tile (`differ`).
+        auto take = [&](auto plain, bool by_row, uint32_t tile, float& keep, float& grow) {
+            constexpr bool PLAIN = decltype(plain)::value, MAY_BY_ROW = !PLAIN && FMT == BC_I8;
+            const uint32_t scores_at = lanes + (tile & 1) * KT + first_score;
             const TileInfo<KT, FMT>& info = sh.info[tile % kRing];
-            await(alive, s_full + 8 * buffer, (tile >> 1) & 1, dead, 2);
-            if (!alive) return;
-            tc_fence_after_sync();
             const int32_t see = (int32_t)max(min((int64_t)limit - sh.desc[tile % kDescRing].key0 - first_score, (int64_t)KT), (int64_t)-1);  // the last score seen
-            const bool masked = info.masked;
-            // 8-bit values: weights, probabilities times scales, are counted in the power of two below the tile's largest scale, 2^14 to one, and are exact
-            // to 2^-25 of these. A row's largest weight is the smallest scale so far at the least. Where that is less than 2^-7 of the tile's largest scale,
-            // which may be of a position that a row does not see, or hardly, each row counts in the power of two below its own largest weight. So a
-            // weight keeps 22 bits, or 2^-32 of its row's largest. (That this may happen costs 3 % where it does not: 2.28 to 2.35 ms for the chunk above.)
-            uint32_t scale_bits = 0;
-            bool by_row = false;
+            const bool masked = !PLAIN && info.masked;
             float heaviest = -INFINITY;
-            if constexpr (FMT == BC_I8) {
-                const uint4 tops = *reinterpret_cast<const uint4*>(info.top_scale), lows = *reinterpret_cast<const uint4*>(info.low_scale);
-                scale_bits = max(max(tops.x, tops.y), max(tops.z, tops.w));
-                lowest = min(lowest, min(min(lows.x, lows.y), min(lows.z, lows.w)));
-                by_row = (scale_bits >> 23) > min(lowest >> 23, 220u) + 6;
-                if (__builtin_expect(by_row, 0)) {
+            if constexpr (MAY_BY_ROW) {
+                if (by_row) {
 #pragma unroll 1
                     for (uint32_t c = 0; c < kScores; c += 16) {
                         float2 x[8];
@@ -631,46 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
                 float2 x[8];
                 load_scores(scores_at, info, masked, see, c, x);
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i)
-                    most[i & 1] = FMT == BC_F16 ? max3_nan(most[i & 1], x[i].x, x[i].y) : fmaxf(most[i & 1], fmaxf(x[i].x, x[i].y));
-            }
-            if constexpr (FMT == BC_F16) {
-                // A score that is no number, for the first time: of an infinite key, perhaps one whose score is minus infinity, which weighs nothing.
-                const bool some = (most[0] != most[0] || most[1] != most[1]) && total == total;
-                if (__builtin_expect(__any_sync(0xffffffffu, some), 0)) {
-                    const TileDesc& desc = sh.desc[tile % kDescRing];
-                    const uint32_t query = row / p.group;
-                    const bool mine = some && query < desc.n;
-                    const float* const q = p.q + (mine ? (uint64_t)(desc.row0 + query) * p.q_stride + (uint64_t)(desc.head * p.group + row % p.group) * p.q_head_stride : 0);
-                    most[0] = most[1] = -INFINITY;
-#pragma unroll 1
-                    for (uint32_t c = 0; c < kScores; c += 16) {
-                        float x[16];
-                        tmem_load_16(scores_at + c, x);
-                        const uint32_t bits = masked ? seen_bits(info, first_score + c, see - (int32_t)c) : 0xffffu;
-                        uint32_t nothing = 0;
-#pragma unroll
-                        for (uint32_t i = 0; i < 16; ++i) nothing |= x[i] != x[i] ? 1u << i : 0u;
-                        nothing = mine ? nothing & bits : 0;
-                        for (uint32_t left = nothing; left; left &= left - 1) {
-                            const uint32_t i = __ffs(left) - 1, key = desc.key0 + first_score + c + i;
-                            const uint32_t page = p.rows.table[(uint64_t)desc.seq * p.rows.max_pages + (key >> pool.page_shift)];
-                            if (page >= pool.n_pages || !score_is_minus_infinity(q, pool.k + kv_row_at(pool, page, desc.head, key & ((1u << pool.page_shift) - 1)), HD))
-                                nothing &= ~(1u << i);
-                        }
-                        __syncwarp();
-                        uint32_t back[2][8];
-#pragma unroll
-                        for (uint32_t i = 0; i < 16; ++i) {
-                            if (nothing >> i & 1) x[i] = -INFINITY;
-                            if (bits >> i & 1) most[i & 1] = fmaxf(most[i & 1], x[i]);
-                            back[i / 8][i % 8] = __float_as_uint(x[i]);
-                        }
-                        tmem_store_8(scores_at + c, back[0]);
-                        tmem_store_8(scores_at + c + 8, back[1]);
-                    }
-                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                }
+                for (uint32_t i = 0; i < 8; ++i) most[i & 1] = fmaxf(most[i & 1], fmaxf(x[i].x, x[i].y));
             }
             float now = fmaxf(top, fmaxf(most[0], most[1]) * factor);
             sh.most[tile & 1][part][row] = now;
@@ -682,8 +640,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
             top = now;
             float down = kLift - shift, tile_unit = 1.f;
             if constexpr (FMT == BC_I8) {
-                int exponent = (int)(scale_bits >> 23) - 127;
-                if (__builtin_expect(by_row, 0)) exponent = (int)floorf(fmaxf(fmaxf(heaviest, sh.heaviest[tile & 1][part ^ 1][row]) - shift, -128.f));
+                const uint4 tops = *reinterpret_cast<const uint4*>(info.top_scale);
+                int exponent = (int)(max(max(tops.x, tops.y), max(tops.z, tops.w)) >> 23) - 127;
+                if (MAY_BY_ROW && by_row) exponent = (int)floorf(fmaxf(fmaxf(heaviest, sh.heaviest[tile & 1][part ^ 1][row]) - shift, -128.f));
                 exponent = min(max(exponent, -100), 100);
                 tile_unit = __uint_as_float((uint32_t)(exponent + 127) << 23);
                 down -= (float)exponent;
@@ -739,6 +698,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
                 unit = 1.f;
             }
         };
+        // 8-bit values: weights, probabilities times scales, are counted in the power of two below the tile's largest scale, 2^14 to one, and are exact to
+        // 2^-25 of these. A row's largest weight is the unit's smallest scale so far at the least. From where that is less than 2^-7 of a tile's largest scale,
+        // which may be of a position that a row does not see, or hardly, each row counts in the power of two below its own largest weight. So a
+        // weight keeps 22 bits, or 2^-32 of its row's largest.
+        auto differ = [&](uint32_t tile) {
+            if constexpr (FMT == BC_I8) {
+                const TileInfo<KT, FMT>& info = sh.info[tile % kRing];
+                const uint4 tops = *reinterpret_cast<const uint4*>(info.top_scale), lows = *reinterpret_cast<const uint4*>(info.low_scale);
+                lowest = min(lowest, min(min(lows.x, lows.y), min(lows.z, lows.w)));
+                return (max(max(tops.x, tops.y), max(tops.z, tops.w)) >> 23) > min(lowest >> 23, 220u) + 6;
+            } else {
+                return false;
+            }
+        };
         auto publish = [&](uint32_t tile) {
             tc_fence_before_sync();
             __syncwarp();
@@ -777,6 +750,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
                     for (uint32_t e = 0; e < HD / kParts; ++e)
                         if ((int64_t)at[FMT == BC_F16 ? e : 0] <= limit) (whole ? p.out : p.parts)[mine + first_element + e] = __uint_as_float(0x7fc00000u);
             }
+            if (FMT == BC_F16 && whole && mine != ~0ull && total != total) sh.odd = 1;
             if (!whole && stats)
                 *reinterpret_cast<float2*>(p.parts + (uint64_t)2 * kMostCtas * kRows * HD + ((uint64_t)slot * kRows + row) * 2) = make_float2(top, total);
         };
@@ -791,38 +765,49 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
             total = unit = 0.f;
             lowest = 0x7f7fffff;
         };
-        {
-            // All rows' threads take every tile; the last product is added to the sums when the next tile's probabilities are there.
-            bool first = true;
-            float keep = 0.f, grow = 0.f;
-            for (uint32_t tile = 0; tile <= n_tiles && n_tiles > 0; ++tile) {
-                if (first) {
-                    // The next unit's queries go ahead of the last one's end, whose scores are done, where registers hold both.
-                    if (tile > 0) rows_sync();  // the maxima have been read
-                    if (HD < 256 && tile < n_tiles && alive) load_queries(tile);
-                    if (tile > 0 && alive) {
-                        add_product(tile - 1, keep, grow);
-                        // A row's sums of probabilities meet.
-                        sh.most[0][part][row] = total;
-                        rows_sync();
-                        total = sh.most[0][0][row] + sh.most[0][1][row];
-                        rows_sync();  // the next unit writes there
-                        if (!alive) break;
-                        store(sh.desc[(tile - 1) % kDescRing], first_sum, o, unit, part == 0);
-                    }
-                    if (HD == 256 && tile < n_tiles && alive) load_queries(tile);
-                    if (tile == n_tiles || !alive) break;
-                    start_unit(tile);
-                }
+        // All rows' threads take every tile; the last product is added to the sums when the next tile's probabilities are there.
+        uint32_t tile = 0;
+        float keep = 0.f, grow = 0.f;
+        bool begins = true;  // the tile is its unit's first
+        // Tiles up to the unit's last; PLAIN: false at one that is not. Most of a long unit's are, and a loop for these alone is the shorter one.
+        auto take_tiles = [&](auto plain) {
+            while (true) {
+                await(alive, s_full + 8 * (tile & 1), (tile >> 1) & 1, dead, 2);
+                if (!alive) return true;
+                tc_fence_after_sync();
+                const bool by_row = differ(tile);
+                if (decltype(plain)::value && (by_row || sh.info[tile % kRing].masked)) return false;
                 float next_keep, next_grow;
-                take(tile, next_keep, next_grow);
-                if (!first && alive) add_product(tile - 1, keep, grow);  // before the next one may take its place
-                if (!alive) break;
+                take(plain, by_row, tile, next_keep, next_grow);
+                if (!begins && alive) add_product(tile - 1, keep, grow);  // before the next one may take its place
+                if (!alive) return true;
                 keep = next_keep;
                 grow = next_grow;
+                begins = false;
                 publish(tile);
-                first = sh.desc[tile % kDescRing].last;
+                if (sh.desc[tile++ % kDescRing].last) return true;
             }
+        };
+        while (n_tiles > 0) {
+            // The next unit's queries go ahead of the last one's end, whose scores are done, where registers hold both.
+            if (tile > 0) rows_sync();  // the maxima have been read
+            if (HD < 256 && tile < n_tiles && alive) load_queries(tile);
+            if (tile > 0 && alive) {
+                add_product(tile - 1, keep, grow);
+                // A row's sums of probabilities meet.
+                sh.most[0][part][row] = total;
+                rows_sync();
+                total = sh.most[0][0][row] + sh.most[0][1][row];
+                rows_sync();  // the next unit writes there
+                if (!alive) break;
+                store(sh.desc[(tile - 1) % kDescRing], first_sum, o, unit, part == 0);
+            }
+            if (HD == 256 && tile < n_tiles && alive) load_queries(tile);
+            if (tile == n_tiles || !alive) break;
+            start_unit(tile);
+            begins = true;
+            if (!take_tiles(std::true_type{})) take_tiles(std::false_type{});
+            if (!alive) break;
         }
     } else if (warp < kMmaWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kUnpackRegisters));
@@ -1073,7 +1058,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
                         if (at.in_unit == at.unit.tiles) {
                             at.cursor.take(p, capacity, KT, at.unit);
                             at.in_unit = 0;
-                            ++at.unit_number;
+                            if (++at.unit_number == 0) at.span = ChunkSpan{{at.unit.seq, 0}, {at.unit.head, 0}, {at.unit.row_tile, 0}, {}};
                         }
                         const Unit& u = at.unit;
                         const ChunkSeq& s = at.cursor.s;
@@ -1081,7 +1066,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
                         const int64_t pos = (int64_t)s.len - (s.end - s.row0) + query0;
                         d.key0 = (u.tile0 + at.in_unit) * KT;
                         d.end = s.held;
-                        d.seq = u.seq;
                         d.row0 = s.row0 + query0;
                         d.n = min(per_tile, s.n - query0);
                         d.head = u.head;
@@ -1146,7 +1130,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
                 value_rows_at = rows_at;
                 value_segments = segments;
             }
-            if (lane == 0) reinterpret_cast<ChunkHead*>(p.parts + (uint64_t)2 * kMostCtas * kRows * (HD + 2))[blockIdx.x] = alive ? at.cut : ChunkHead{0, 0, 0, 0};
+            if (lane == 0) {
+                chunk_heads(p.parts, HD)[blockIdx.x] = alive ? at.cut : ChunkHead{};
+                at.span.seq[1] = at.unit.seq, at.span.head[1] = at.unit.head, at.span.row_tile[1] = at.unit.row_tile;
+                chunk_spans(p.parts, HD)[blockIdx.x] = at.span;
+            }
             // Copies in flight end before the CTA does: the unpacking warps wait for them, or this one does when those gave up.
             for (uint32_t r = 0; r < RAW && r < keys_issued && *dead; ++r) {
                 const uint32_t j = keys_issued - 1 - r;
@@ -1161,6 +1149,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
     // Whoever waited for the last product has seen all multiplies end; after a wait that ran out, they get a limited time to.
     tc_fence_before_sync();
     __syncthreads();
+    if (FMT == BC_F16 && tid == 0 && sh.odd) chunk_heads(p.parts, HD)[blockIdx.x].n = sh.dead ? 0 : sh.place.cut.n | kOdd;
     if (warp == kMmaWarp) {
         if (sh.dead && n_tiles > 0) {
             if (elect_one()) {
@@ -1176,55 +1165,151 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
     }
 }
 
-// Joins the parts of a unit that begins in CTA c's run: a warp to a row.
-constexpr uint32_t kJoinCtas = 8;  // to a cut row tile
+// Attention of one query by a warp, in f32 throughout, with infinities as the formula has them. Rows whose sums are no number are done again by this: a half page may hold
+// an infinite key whose score is minus infinity, which weighs nothing, but a query's lower half times it may be plus infinity, or no number.
 template <int HD>
-__global__ void __launch_bounds__(256) attention_chunk_paged_join_kernel(const float* __restrict__ parts, float* __restrict__ out, uint32_t n_heads, uint32_t group) {
-    constexpr int kPairs = HD / 64;
-    pdl_launch_dependents();
-    pdl_wait();
-    const uint32_t lane = threadIdx.x & 31, c = blockIdx.x;
-    const ChunkHead cut = reinterpret_cast<const ChunkHead*>(parts + (uint64_t)2 * kMostCtas * kRows * (HD + 2))[c];
-    if (cut.last == 0) return;
-    const float2* stats = reinterpret_cast<const float2*>(parts + (uint64_t)2 * kMostCtas * kRows * HD);
-    const uint32_t n = cut.last - c + 1;
-    auto slot_of = [&](uint32_t i) { return (uint64_t)(2 * (c + i) + (i == 0 ? 1 : 0)); };
-    for (uint32_t r = blockIdx.y * 8 + (threadIdx.x >> 5); r < cut.n * group; r += kJoinCtas * 8) {
-        float top = -INFINITY;
-        for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, stats[slot_of(i) * kRows + r].x);
-        top = warp_max(top);
-        const float shift = top == -INFINITY ? 0.f : top;
-        float total = 0.f;
-        float2 sum[kPairs];
+__device__ __forceinline__ void attend_in_f32(const ChunkParams& p, uint32_t seq, uint32_t kv_head, const float* q, uint32_t n_keys, float* out) {
+    const KvPool& pool = p.pool;
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t* const table = p.rows.table + (uint64_t)seq * p.rows.max_pages;
+    float top = -INFINITY, total = 0.f;
+    float2 sum[HD / 64];
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) sum[i] = make_float2(0.f, 0.f);
-        for (uint32_t i0 = 0; i0 < n; i0 += 32) {
-            float2 st = make_float2(-INFINITY, 0.f);
-            if (i0 + lane < n) st = stats[slot_of(i0 + lane) * kRows + r];
-            const float weight = st.x == -INFINITY ? 0.f : exp2f(st.x - shift);
-            total += weight * st.y;
-            const uint32_t many = min(32u, n - i0);
-#pragma unroll 4
-            for (uint32_t i = 0; i < many; ++i) {
-                const float w = __shfl_sync(0xffffffffu, weight, i);
-                const bool any = __shfl_sync(0xffffffffu, st.x, i) != -INFINITY;
-                const float2* from = reinterpret_cast<const float2*>(parts + (slot_of(i0 + i) * kRows + r) * HD) + lane;
+    for (int i = 0; i < HD / 64; ++i) sum[i] = make_float2(0.f, 0.f);
+    for (uint32_t key0 = 0; key0 < n_keys; key0 += 32) {
+        const uint32_t key = key0 + lane, page = key < n_keys ? table[key >> pool.page_shift] : kNoSlot;
+        const bool there = page < pool.n_pages;
+        const uint64_t at = there ? kv_row_at(pool, page, kv_head, key & ((1u << pool.page_shift) - 1)) : 0;
+        float score = -INFINITY;
+        if (there) {
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+            for (int e = 0; e < HD; e += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(q + e);
+                const uint2 w = *reinterpret_cast<const uint2*>(pool.k + at + 2 * e);
+                const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+                s[0] = fmaf(x.x, a.x, s[0]);
+                s[1] = fmaf(x.y, a.y, s[1]);
+                s[2] = fmaf(x.z, b.x, s[2]);
+                s[3] = fmaf(x.w, b.y, s[3]);
+            }
+            score = ((s[0] + s[1]) + (s[2] + s[3])) * (1.4426950408889634f / sqrtf((float)HD));
+        }
+        if (__any_sync(0xffffffffu, !(score < INFINITY))) {  // so is the row
+            for (uint32_t e = lane; e < HD; e += 32) out[e] = __uint_as_float(0x7fc00000u);
+            return;
+        }
+        const float now = fmaxf(top, warp_max(score)), shift = now == -INFINITY ? 0.f : now, fall = exp2f(top - shift), weight = exp2f(score - shift);
+        top = now;
+        total = total * fall + weight;
 #pragma unroll
-                for (int k = 0; k < kPairs; ++k) {
-                    const float2 v = from[32 * k];
-                    if (any) {
-                        sum[k].x += w * v.x;
-                        sum[k].y += w * v.y;
-                    }
+        for (int i = 0; i < HD / 64; ++i) sum[i] = make_float2(sum[i].x * fall, sum[i].y * fall);
+        for (uint32_t left = __ballot_sync(0xffffffffu, there); left; left &= left - 1) {
+            const uint32_t who = __ffs(left) - 1;
+            const float w = __shfl_sync(0xffffffffu, weight, who);
+            const __half2* v = reinterpret_cast<const __half2*>(pool.v + __shfl_sync(0xffffffffu, at, who)) + lane;
+#pragma unroll
+            for (int i = 0; i < HD / 64; ++i) {
+                const float2 x = __half22float2(v[32 * i]);
+                sum[i].x = fmaf(w, x.x, sum[i].x);
+                sum[i].y = fmaf(w, x.y, sum[i].y);
+            }
+        }
+    }
+    total = warp_sum(total);
+    const float inverse = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int i = 0; i < HD / 64; ++i) reinterpret_cast<float2*>(out)[32 * i + lane] = make_float2(sum[i].x * inverse, sum[i].y * inverse);
+}
+
+// A row's query head again. (Not in line, nor what follows: the joining launch is short, and most of its time is its beginning.)
+template <int HD>
+__device__ __noinline__ void again(const ChunkParams& p, uint32_t seq, uint32_t row, uint32_t head) {
+    const uint32_t back = p.rows.starts[seq + 1] - row, len = p.rows.lens[seq];
+    const uint32_t held = (uint32_t)min((uint64_t)len, (uint64_t)p.rows.max_pages << p.pool.page_shift), n_keys = back <= len ? min(len - back + 1, held) : 0;
+    attend_in_f32<HD>(p, seq, head / p.group, p.q + row * p.q_stride + head * p.q_head_stride, n_keys, p.out + ((uint64_t)row * p.n_heads + head) * HD);
+}
+// The rows of CTA c's units whose sums are no number, by kJoinCtas CTAs; of units that were cut the launch's joining takes care.
+template <int HD>
+__device__ __noinline__ void again_where_whole(const ChunkParams& p, uint32_t c, uint32_t ctas) {
+    const uint32_t lane = threadIdx.x & 31, warp = blockIdx.y * 8 + (threadIdx.x >> 5), per_tile = kRows / p.group;
+    const ChunkHead* const heads = chunk_heads(p.parts, HD);
+    const ChunkSpan span = chunk_spans(p.parts, HD)[c];
+    for (uint32_t seq = span.seq[0]; seq <= span.seq[1]; ++seq) {
+        const ChunkSeq s = chunk_seq(p.rows.starts[seq], p.rows.starts[seq + 1], p.rows.lens[seq], (uint64_t)p.rows.max_pages << p.pool.page_shift, p.rows.n_rows, p.fewest, per_tile, 128);
+        const bool first = seq == span.seq[0], last = seq == span.seq[1];
+        for (uint32_t head = first ? span.head[0] : 0; head <= (last ? span.head[1] : p.pool.n_kv_heads - 1); ++head) {
+            const uint32_t tile1 = last && head == span.head[1] ? min(s.row_tiles, span.row_tile[1] + 1) : s.row_tiles;
+            for (uint32_t tile = first && head == span.head[0] ? span.row_tile[0] : 0; tile < tile1; ++tile) {
+                const uint32_t row0 = s.row0 + tile * per_tile, n = min(per_tile, s.n - tile * per_tile);
+                bool joined = false;
+                for (uint32_t k = lane; k < ctas; k += 32) joined |= heads[k].last != 0 && heads[k].head == head && heads[k].row0 == row0;
+                if (__any_sync(0xffffffffu, joined)) continue;
+                for (uint32_t r = warp; r < n * p.group; r += 8 * kJoinCtas) {
+                    const uint32_t row = row0 + r / p.group, q_head = head * p.group + r % p.group;
+                    const float x = p.out[((uint64_t)row * p.n_heads + q_head) * HD + lane];
+                    if (__any_sync(0xffffffffu, x != x)) again<HD>(p, seq, row, q_head);
                 }
             }
         }
-        total = warp_sum(total);
-        const float inverse = top == -INFINITY && total == 0.f ? 0.f : 1.f / total;
-        float2* to = reinterpret_cast<float2*>(out + (uint64_t)(cut.row0 + r / group) * n_heads * HD + (cut.head * group + r % group) * HD) + lane;
-#pragma unroll
-        for (int k = 0; k < kPairs; ++k) to[32 * k] = make_float2(sum[k].x * inverse, sum[k].y * inverse);
     }
+}
+
+// Joins the parts of a unit that begins in CTA c's run: a warp to a row. Rows of halves whose sums are no number are done again.
+template <int FMT, int HD>
+__global__ void __launch_bounds__(256, HD == 64 ? 8 : 6) attention_chunk_paged_join_kernel(const __grid_constant__ ChunkParams p, uint32_t ctas) {
+    constexpr int kPairs = HD / 64;
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x;
+    const ChunkHead cut = chunk_heads(p.parts, HD)[c];
+    if (cut.last != 0) {
+        const float2* stats = reinterpret_cast<const float2*>(p.parts + (uint64_t)2 * kMostCtas * kRows * HD);
+        const uint32_t n = cut.last - c + 1;
+        auto slot_of = [&](uint32_t i) { return (uint64_t)(2 * (c + i) + (i == 0 ? 1 : 0)); };
+        for (uint32_t r = blockIdx.y * 8 + warp; r < (cut.n & ~kOdd) * p.group; r += kJoinCtas * 8) {
+            float top = -INFINITY;
+            for (uint32_t i = lane; i < n; i += 32) top = fmaxf(top, stats[slot_of(i) * kRows + r].x);
+            top = warp_max(top);
+            const float shift = top == -INFINITY ? 0.f : top;
+            float total = 0.f;
+            float2 sum[kPairs];
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) sum[i] = make_float2(0.f, 0.f);
+            for (uint32_t i0 = 0; i0 < n; i0 += 32) {
+                float2 st = make_float2(-INFINITY, 0.f);
+                if (i0 + lane < n) st = stats[slot_of(i0 + lane) * kRows + r];
+                const float weight = st.x == -INFINITY ? 0.f : exp2f(st.x - shift);
+                total += weight * st.y;
+                const uint32_t many = min(32u, n - i0);
+#pragma unroll 4
+                for (uint32_t i = 0; i < many; ++i) {
+                    const float w = __shfl_sync(0xffffffffu, weight, i);
+                    const bool any = __shfl_sync(0xffffffffu, st.x, i) != -INFINITY;
+                    const float2* from = reinterpret_cast<const float2*>(p.parts + (slot_of(i0 + i) * kRows + r) * HD) + lane;
+#pragma unroll
+                    for (int k = 0; k < kPairs; ++k) {
+                        const float2 v = from[32 * k];
+                        if (any) {
+                            sum[k].x += w * v.x;
+                            sum[k].y += w * v.y;
+                        }
+                    }
+                }
+            }
+            total = warp_sum(total);
+            const uint32_t row = cut.row0 + r / p.group, head = cut.head * p.group + r % p.group;
+            if (FMT == BC_F16 && total != total) {
+                again<HD>(p, seq_of_row(p.rows, row), row, head);
+                continue;
+            }
+            const float inverse = top == -INFINITY && total == 0.f ? 0.f : 1.f / total;
+            float2* to = reinterpret_cast<float2*>(p.out + ((uint64_t)row * p.n_heads + head) * HD) + lane;
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) to[32 * k] = make_float2(sum[k].x * inverse, sum[k].y * inverse);
+        }
+    }
+    if (FMT == BC_F16 && cut.n & kOdd) again_where_whole<HD>(p, c, ctas);
 }
 
 uint32_t chunk_ctas() {
@@ -1240,17 +1325,17 @@ cudaError_t launch_chunk(cudaStream_t stream, const ChunkParams& p) {
     if (e != cudaSuccess) return e;
     const uint32_t ctas = chunk_ctas();
     e = launch_dependent(attention_chunk_paged_kernel<FMT, HD>, dim3(ctas), dim3(kThreads), smem, stream, p);
-    if (e != cudaSuccess || ctas == 1) return e;
-    return launch_dependent(attention_chunk_paged_join_kernel<HD>, dim3(ctas - 1, kJoinCtas), dim3(256), 0, stream, static_cast<const float*>(p.parts), p.out, p.n_heads, p.group);
+    if (e != cudaSuccess) return e;
+    return launch_dependent(attention_chunk_paged_join_kernel<FMT, HD>, dim3(ctas, kJoinCtas), dim3(256), 0, stream, p, ctas);
 }
 
 }  // namespace
 
 uint64_t attention_chunk_scratch_floats(uint32_t head_dim) {
-    return (uint64_t)2 * kMostCtas * kRows * (head_dim + 2) + (uint64_t)kMostCtas * sizeof(ChunkHead) / 4;
+    return (uint64_t)2 * kMostCtas * kRows * (head_dim + 2) + (uint64_t)kMostCtas * (sizeof(ChunkHead) + sizeof(ChunkSpan)) / 4;
 }
 
-int attention_chunk_launches() { return chunk_ctas() == 1 ? 1 : 2; }
+int attention_chunk_launches() { return 2; }
 
 cudaError_t attention_chunk(cudaStream_t stream, const KvPool& pool, const KvRows& rows, const float* q, uint64_t q_stride, uint64_t q_head_stride, float* scratch,
                             float* out, uint32_t n_heads, uint32_t fewest) {

@@ -5,8 +5,8 @@ import numpy as np
 import pytest
 
 from bobcat_b200 import F16
-from kv_pool_cases import attention
-from test_attention_paged_gpu import attend, build
+from kv_pool_cases import Pool, attention
+from test_attention_paged_gpu import MARK, attend, build
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,30 @@ def test_a_key_that_is_no_number_and_rows_all_of_whose_scores_are_minus_infinity
     want, bound = attention(q[3:150].reshape(147, 2, hd), k, v, 0)
     assert (np.abs(got[3:150] - want) <= bound).all()
     assert np.isnan(got[150:]).all()
+
+
+@pytest.mark.parametrize("hint", [1, 1000])
+@pytest.mark.parametrize("heads, kv, hd", [(16, 8, 64), (8, 8, 128), (14, 2, 256)])
+def test_infinite_keys_of_long_contexts(cuda, heads, kv, hd, hint):
+    """Row tiles over many CTAs and whole ones, beside single tokens: what the contexts hold ahead of the rows weighs nothing on any of them."""
+    rng = np.random.default_rng(66)
+    news, lens = [70, 1, 300, 2, 33], [6000, 4000, 310, 900, 2500]
+    special = [[3, 127, 128, 5000], [64], [2], [0, 800], [31, 1000, 2000]]
+    case = Pool(cuda, F16, 64, kv, hd, lens, rng)
+    case.fill_at_once(rng)
+    for s, positions in enumerate(special):
+        for pos in positions:
+            key = rng.standard_normal((kv, hd)).astype(np.float32)
+            key[:, 7] = INF
+            case.put(case.k_raw, s, pos, key)
+    case.upload()
+    q = (rng.standard_normal((sum(news) + 1, heads, hd)) * 1.5).astype(np.float32)
+    q[..., 7] = -np.abs(q[..., 7])
+    got = attend(cuda, case, news, heads, q.reshape(len(q), -1), rows=case.rows(news, n_rows=len(q), max_queries=hint)).reshape(len(q), heads, hd)
+    at = 0
+    for s, n in enumerate(news):
+        k, v = (np.delete(case.context(raw, s, lens[s]), special[s], axis=0) for raw in (case.k_raw, case.v_raw))
+        want, bound = attention(q[at:at + n], k, v, lens[s] - n - len(special[s]))
+        assert (np.abs(got[at:at + n] - want) <= bound).all(), s
+        at += n
+    assert (got[at:] == MARK).all()
