@@ -71,5 +71,55 @@ __host__ __device__ inline ChunkSeq chunk_seq(uint32_t start, uint32_t end, uint
     return s;
 }
 
+// A stretch of key tiles of one row tile.
+struct ChunkUnit {
+    uint32_t seq, head, row_tile, tile0, tiles;
+    uint64_t last;  // where the row tile ends in the call's work: its last place
+    bool begins, ends;
+};
+
+// Walks a run: of row tiles that count as their key tiles and kRowTileCost, or of whole ones that count as one.
+struct ChunkCursor {
+    uint32_t seq, head, row_tile, count;
+    uint64_t at, left, end;  // in the row tile; of the run; the run's end
+    bool whole;
+    ChunkSeq s;
+    __host__ __device__ uint64_t all() const { return whole ? 1 : (uint64_t)count + kRowTileCost; }
+    // The next stretch; false where the run has none, as where it ends ahead of a row tile's first key tile, or the sequences have ended before it.
+    __host__ __device__ bool take(const uint32_t* starts, const uint32_t* lens, uint32_t n_seqs, uint32_t n_rows, uint32_t n_kv_heads, uint64_t capacity, uint32_t fewest, ChunkUnit& u) {
+        if (left == 0) return false;
+        if (at == all()) {  // on to the next row tile
+            at = 0;
+            if (++row_tile >= s.row_tiles) {
+                row_tile = 0;
+                if (++head >= n_kv_heads) {
+                    head = 0;
+                    do {
+                        if (++seq >= n_seqs) {
+                            left = 0;
+                            return false;
+                        }
+                        s = chunk_seq(starts[seq], starts[seq + 1], lens[seq], capacity, n_rows, fewest, s.per_tile, s.key_tile);
+                    } while (s.row_tiles == 0);
+                }
+            }
+            count = s.tiles(row_tile);
+        }
+        u.seq = seq;
+        u.head = head;
+        u.row_tile = row_tile;
+        u.last = end - left - at + all() - 1;
+        const uint64_t upto = at + left < all() ? at + left : all();
+        u.tile0 = whole || at < kRowTileCost ? 0 : (uint32_t)(at - kRowTileCost);
+        const uint32_t tile1 = whole ? count : upto < kRowTileCost ? 0 : (uint32_t)(upto - kRowTileCost);
+        u.tiles = tile1 - u.tile0;
+        u.begins = u.tile0 == 0;
+        u.ends = tile1 == count;
+        left -= upto - at;
+        at = upto;
+        return u.tiles > 0;
+    }
+};
+
 }  // namespace k
 }  // namespace bc

@@ -503,7 +503,7 @@ cudaError_t attention_paged(cudaStream_t stream, const KvPool& pool, const KvRow
 // Its sequences of `fewest` rows and more on the tensor cores (kernels_attention_chunk.cu). Codes of its waits: rows on 1: a product with values,
 // 2: scores, 9: a tile's description; unpacking on 3: free keys, 4: free values; multiplies on 5: probabilities, 6: values, 7: keys,
 // 8: queries, 12: the last product's reading; copies on 11 and 16: room for keys' and values'
-// bytes; unpacking on 10 and 15: those; rows and unpacking on one another: 13, 14.
+// bytes; unpacking on 10 and 15: those; rows and unpacking on one another: 13, 14. 17: a run that ended ahead of its tiles.
 cudaError_t attention_chunk_wait_word(int* word);
 uint64_t attention_chunk_scratch_floats(uint32_t head_dim);
 int attention_chunk_launches();

@@ -79,59 +79,10 @@ struct ChunkSpan {
 __device__ __forceinline__ ChunkHead* chunk_heads(float* parts, uint32_t head_dim) { return reinterpret_cast<ChunkHead*>(parts + (uint64_t)2 * kMostCtas * kRows * (head_dim + 2)); }
 __device__ __forceinline__ ChunkSpan* chunk_spans(float* parts, uint32_t head_dim) { return reinterpret_cast<ChunkSpan*>(chunk_heads(parts, head_dim) + kMostCtas); }
 
-// A stretch of key tiles of one row tile.
-struct Unit {
-    uint32_t seq, head, row_tile, tile0, tiles;
-    uint64_t last;  // where the row tile ends in the call's work: its last place
-    bool begins, ends;
-};
-
-// Walks a run: of row tiles that count as their key tiles and kRowTileCost, or of whole ones that count as one.
-struct Cursor {
-    uint32_t seq, head, row_tile, count;
-    uint64_t at, left, end;  // in the row tile; of the run; the run's end
-    bool whole;
-    ChunkSeq s;
-    __device__ __forceinline__ uint64_t all() const { return whole ? 1 : (uint64_t)count + kRowTileCost; }
-    __device__ __forceinline__ bool take(const ChunkParams& p, uint64_t capacity, uint32_t key_tile, Unit& u) {
-        if (left == 0) return false;
-        if (at == all()) {  // on to the next row tile
-            at = 0;
-            if (++row_tile == s.row_tiles) {
-                row_tile = 0;
-                if (++head == p.pool.n_kv_heads) {
-                    head = 0;
-                    do {
-                        if (++seq == p.rows.n_seqs) {
-                            left = 0;
-                            return false;
-                        }
-                        s = chunk_seq(p.rows.starts[seq], p.rows.starts[seq + 1], p.rows.lens[seq], capacity, p.rows.n_rows, p.fewest, s.per_tile, key_tile);
-                    } while (s.row_tiles == 0);  // something is left, so a sequence with some follows
-                }
-            }
-            count = s.tiles(row_tile);
-        }
-        u.seq = seq;
-        u.head = head;
-        u.row_tile = row_tile;
-        u.last = end - left - at + all() - 1;
-        const uint64_t upto = min(all(), at + left);
-        u.tile0 = whole ? 0 : (uint32_t)(max(at, (uint64_t)kRowTileCost) - kRowTileCost);
-        const uint32_t tile1 = whole ? count : (uint32_t)(max(upto, (uint64_t)kRowTileCost) - kRowTileCost);
-        u.tiles = tile1 - u.tile0;
-        u.begins = u.tile0 == 0;
-        u.ends = tile1 == count;
-        left -= upto - at;
-        at = upto;
-        return u.tiles > 0;  // a run may end ahead of a row tile's first key tile
-    }
-};
-
 // Where the first loading warp is in the run.
 struct Place {
-    Cursor cursor;
-    Unit unit;
+    ChunkCursor cursor;
+    ChunkUnit unit;
     uint32_t in_unit, unit_number;
     ChunkHead cut;
     ChunkSpan span;
@@ -378,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
         const bool begin = warp == kCopyWarp;
         const uint64_t place = blockIdx.x < runs ? counted * (blockIdx.x + (begin ? 0 : 1)) / runs : counted;
         uint64_t ahead = place < counted ? 0 : total;
-        Cursor cur{};
+        ChunkCursor cur{};
         cur.whole = whole;
         if (place < counted) {
             uint64_t base = 0;
@@ -1054,13 +1005,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
                 if (i < n_tiles) {
                     const uint32_t j = i;
                     TileDesc& d = sh.desc[j % kDescRing];
+                    bool some = true;
+                    if (lane == 0 && at.in_unit == at.unit.tiles) {
+                        some = at.cursor.take(p.rows.starts, p.rows.lens, p.rows.n_seqs, p.rows.n_rows, pool.n_kv_heads, capacity, p.fewest, at.unit);
+                        at.in_unit = 0;
+                        if (++at.unit_number == 0) at.span = ChunkSpan{{at.unit.seq, 0}, {at.unit.head, 0}, {at.unit.row_tile, 0}, {}};
+                    }
+                    // The run's tiles have been counted. One that ends before, since the call's words have changed since, is given up.
+                    alive = __all_sync(0xffffffffu, some);
+                    if (!alive) {
+                        if (lane == 0) give_up(dead, 17);
+                        break;
+                    }
                     if (lane == 0) {
-                        if (at.in_unit == at.unit.tiles) {
-                            at.cursor.take(p, capacity, KT, at.unit);
-                            at.in_unit = 0;
-                            if (++at.unit_number == 0) at.span = ChunkSpan{{at.unit.seq, 0}, {at.unit.head, 0}, {at.unit.row_tile, 0}, {}};
-                        }
-                        const Unit& u = at.unit;
+                        const ChunkUnit& u = at.unit;
                         const ChunkSeq& s = at.cursor.s;
                         const uint32_t query0 = u.row_tile * per_tile;
                         const int64_t pos = (int64_t)s.len - (s.end - s.row0) + query0;
