@@ -69,6 +69,10 @@ def _v(view):
     return view.buffer._h, view.offset
 
 
+def _buffers_of(*views) -> tuple:
+    return tuple(v if isinstance(v, Buffer) else v.buffer for v in views if v is not None)
+
+
 class KvPool(_lib.KvPool):
     """Pages of keys and values that sequences share (``bc_kv_pool``): ``k`` and ``v`` are views of
     ``Cuda.kv_pool_bytes`` bytes each."""
@@ -76,9 +80,13 @@ class KvPool(_lib.KvPool):
     def __init__(self, fmt: int, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, k, v):
         super().__init__(fmt, n_pages, page_size, n_kv_heads, head_dim, *_v(k), *_v(v))
         self.holds = (k, v)
+        self._buffers = _buffers_of(k, v)
 
     def _now(self) -> "KvPool":
-        (self.k, self.k_off), (self.v, self.v_off) = map(_v, self.holds)  # of a buffer that was freed: none
+        for b in self._buffers:  # one that was freed meanwhile is no buffer
+            if b._h is None:
+                (self.k, self.k_off), (self.v, self.v_off) = map(_v, self.holds)
+                break
         return self
 
 
@@ -88,9 +96,13 @@ class KvRows(_lib.KvRows):
     def __init__(self, n_seqs: int, n_rows: int, max_queries: int, max_pages: int, table, starts, lens):
         super().__init__(n_seqs, n_rows, max_queries, max_pages, *_v(table), *_v(starts), *_v(lens))
         self.holds = (table, starts, lens)
+        self._buffers = _buffers_of(table, starts, lens)
 
     def _now(self) -> "KvRows":
-        (self.table, self.table_off), (self.starts, self.starts_off), (self.lens, self.lens_off) = map(_v, self.holds)
+        for b in self._buffers:
+            if b._h is None:
+                (self.table, self.table_off), (self.starts, self.starts_off), (self.lens, self.lens_off) = map(_v, self.holds)
+                break
         return self
 
 
