@@ -499,7 +499,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
         };
         float2 o[kSums / 2];
         float top = 0.f, total = 0.f, unit = 0.f;
-        uint32_t lowest = 0;  // 8-bit values: the smallest scale so far
+        uint32_t lowest = 0;   // 8-bit values: the smallest scale so far
+        float heaviest = 0.f;  // of the row's largest exponential times scale so far, no more than the logarithm (where scales differ)
         int32_t limit = 0;  // the last position that the row sees, negative for none
         // Sums become o keep + product grow.
         auto add_product = [&](uint32_t tile, float keep, float grow) {
@@ -557,22 +558,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
             const TileInfo<KT, FMT>& info = sh.info[tile % kRing];
             const int32_t see = (int32_t)max(min((int64_t)limit - sh.desc[tile % kDescRing].key0 - first_score, (int64_t)KT), (int64_t)-1);  // the last score seen
             const bool masked = !PLAIN && info.masked;
-            float heaviest = -INFINITY;
-            if constexpr (MAY_BY_ROW) {
-                if (by_row) {
-#pragma unroll 1
-                    for (uint32_t c = 0; c < kScores; c += 16) {
-                        float2 x[8];
-                        load_scores(scores_at, info, masked, see, c, x);
-#pragma unroll
-                        for (uint32_t i = 0; i < 8; ++i) {
-                            const float2 d = *reinterpret_cast<const float2*>(info.dv + first_score + c + 2 * i);
-                            heaviest = fmaxf(heaviest, fmaxf(fmaf(x[i].x, factor, log2_fast(d.x)), fmaf(x[i].y, factor, log2_fast(d.y))));
-                        }
-                    }
-                    sh.heaviest[tile & 1][part][row] = heaviest;
-                }
-            }
             float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
             for (uint32_t c = 0; c < kScores; c += 16) {
@@ -581,19 +566,46 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i) most[i & 1] = fmaxf(most[i & 1], fmaxf(x[i].x, x[i].y));
             }
-            float now = fmaxf(top, fmaxf(most[0], most[1]) * factor);
-            sh.most[tile & 1][part][row] = now;
+            float tile_top = fmaxf(most[0], most[1]) * factor;
+            sh.most[tile & 1][part][row] = tile_top;
             rows_sync();
             if (!alive) return;
-            now = fmaxf(now, sh.most[tile & 1][part ^ 1][row]);
+            tile_top = fmaxf(tile_top, sh.most[tile & 1][part ^ 1][row]);
+            const float now = fmaxf(top, tile_top);
             const float shift = now == -INFINITY ? 0.f : now;
-            const float fall = exp2_fast(top - shift);
+            const float fall = exp2_fast(top - shift), before = top;
             top = now;
             float down = kLift - shift, tile_unit = 1.f;
             if constexpr (FMT == BC_I8) {
                 const uint4 tops = *reinterpret_cast<const uint4*>(info.top_scale);
                 int exponent = (int)(max(max(tops.x, tops.y), max(tops.z, tops.w)) >> 23) - 127;
-                if (MAY_BY_ROW && by_row) exponent = (int)floorf(fmaxf(fmaxf(heaviest, sh.heaviest[tile & 1][part ^ 1][row]) - shift, -128.f));
+                if constexpr (MAY_BY_ROW) {
+                    if (by_row) {
+                        const uint4 lows = *reinterpret_cast<const uint4*>(info.low_scale);
+                        auto exponent_of = [](uint32_t bits) { return bits ? (float)(int)(bits >> 23) - 127.f : -INFINITY; };
+                        heaviest = fmaxf(heaviest, fmaxf(before + exponent_of(lowest), tile_top + exponent_of(min(min(lows.x, lows.y), min(lows.z, lows.w)))));
+                        // The same for both threads of a row, so for both warps.
+                        if (__any_sync(0xffffffffu, now + (float)(exponent - 6) > heaviest || exponent >= 100)) {
+                            float mine = -INFINITY;
+#pragma unroll 1
+                            for (uint32_t c = 0; c < kScores; c += 16) {
+                                float2 x[8];
+                                load_scores(scores_at, info, masked, see, c, x);
+#pragma unroll
+                                for (uint32_t i = 0; i < 8; ++i) {
+                                    const float2 d = *reinterpret_cast<const float2*>(info.dv + first_score + c + 2 * i);
+                                    mine = fmaxf(mine, fmaxf(fmaf(x[i].x, factor, log2_fast(d.x)), fmaf(x[i].y, factor, log2_fast(d.y))));
+                                }
+                            }
+                            sh.heaviest[tile & 1][part][row] = mine;
+                            rows_sync();
+                            if (!alive) return;
+                            mine = floorf(fmaxf(mine, sh.heaviest[tile & 1][part ^ 1][row]) - shift);
+                            heaviest = fmaxf(heaviest, mine + shift);
+                            exponent = (int)fmaxf(mine, -128.f);
+                        }
+                    }
+                }
                 exponent = min(max(exponent, -100), 100);
                 tile_unit = __uint_as_float((uint32_t)(exponent + 127) << 23);
                 down -= (float)exponent;
@@ -651,8 +663,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
         };
         // 8-bit values: weights, probabilities times scales, are counted in the power of two below the tile's largest scale, 2^14 to one, and are exact to
         // 2^-25 of these. A row's largest weight is the unit's smallest scale so far at the least. From where that is less than 2^-7 of a tile's largest scale,
-        // which may be of a position that a row does not see, or hardly, each row counts in the power of two below its own largest weight. So a
-        // weight keeps 22 bits, or 2^-32 of its row's largest.
+        // which may be of a position that a row does not see, or hardly, rows look closer: the largest weight is at least a tile's largest probability times its
+        // smallest scale; where 32 rows find one for which that is too little, too, each counts in the power of two below its own largest weight.
+        // So a weight keeps 22 bits, or 2^-32 of its row's largest.
         auto differ = [&](uint32_t tile) {
             if constexpr (FMT == BC_I8) {
                 const TileInfo<KT, FMT>& info = sh.info[tile % kRing];
@@ -715,6 +728,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
             top = -INFINITY;
             total = unit = 0.f;
             lowest = 0x7f7fffff;
+            heaviest = -INFINITY;
         };
         // All rows' threads take every tile; the last product is added to the sums when the next tile's probabilities are there.
         uint32_t tile = 0;

@@ -113,3 +113,22 @@ def test_value_rows_of_zeros_and_of_every_size(cuda, hd, kv, heads, hint):
     case.upload()
     q = (rng.standard_normal((695, heads * hd)) * 1.5).astype(np.float32)
     within(case, attend(cuda, case, [695], heads, q, rows=case.rows([695], max_queries=hint)), q, 5, heads, 700)
+
+
+@pytest.mark.parametrize("hint", [1, 1000])
+@pytest.mark.parametrize("hd, kv, heads", SHAPES)
+@pytest.mark.parametrize("gap", [0.0, 8.0, 25.0])
+def test_a_first_position_of_small_values(cuda, gap, hd, kv, heads, hint):
+    """What prompts begin with often has small values and takes most of the probability, of some heads' queries: the others' share is what the rows are about, in
+    every tile behind it."""
+    case = build(cuda, I8, 32, kv, hd, [1500], seed=58)
+    rng = np.random.default_rng(59)
+    key = (rng.standard_normal((kv, hd)) * 0.1).astype(np.float32)
+    key[:, 0] = gap * np.sqrt(hd) / 4.0
+    case.put(case.k_raw, 0, 0, key)
+    case.put(case.v_raw, 0, 0, (rng.standard_normal((kv, hd)) * 1e-6).astype(np.float32))
+    case.put(case.v_raw, 0, 700, (rng.standard_normal((kv, hd)) * 1e7).astype(np.float32))
+    case.upload()
+    q = rng.standard_normal((300, heads, hd)).astype(np.float32)
+    q[:, ::2, 0] = 4.0
+    within(case, attend(cuda, case, [300], heads, q.reshape(300, -1), rows=case.rows([300], max_queries=hint)), q, 1200, heads, 1500)
