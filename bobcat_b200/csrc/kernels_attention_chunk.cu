@@ -10,14 +10,15 @@
 // copies, a page's share each. Four warps unpack them and, of values, transpose them, into the no-swizzle K-major operand layout; its 128-byte core matrices
 // lie 144 bytes apart, so that what neighbouring lanes store falls in distinct banks. One warp issues the multiplies. Eight warps own the rows, a thread
 // half of a row's scores and half of its sums: they exchange the rows' maxima through shared memory, turn scores into probabilities in place in
-// tensor memory, and add the previous tile's product to their sums, while the scores of the next tile run.
+// tensor memory, and add the previous tile's product to their sums, while the scores of the next tile run. Tiles that every row sees whole have a loop of
+// their own (2048 rows behind 30 001 positions: 2.12 ms, 2.37 in one loop with the masks and with weights by row).
 // Queries and probabilities are A operands in tensor memory: both operands in shared memory would take its 128 bytes a cycle whole. (Heads of 256
 // leave room for the queries' upper halves alone.)
 //
-// Measured: 2048 rows of 32 heads of 128 behind 30 001 8-bit positions, 2.31 ms: 450 TFLOP/s of attention, twice that in half products (multiplies alone would take
-// 1.26 ms). A key tile takes 4700 cycles, its multiplies 2100 of them; the rest is the rows' warps, whose instructions bound it: 54 % of
-// the issue slots are used, 12 % of the waiting is for instructions. Tried and left: four threads to a row (2.48 ms: the instructions grow by a quarter), scores held in
-// registers between maximum and exponential (2.61 ms). 512 rows from position 0, 32 heads of 64, take 18 us, most of it one CTA's way through two tiles.
+// Measured: 2048 rows of 32 heads of 128 behind 30 001 8-bit positions, 2.12 ms: 490 TFLOP/s of attention, twice that in half products (multiplies alone would take
+// 1.26 ms). A key tile takes 4300 cycles, its multiplies 2100 of them; the rest is the rows' warps, whose instructions bound it: 58 % of the issue slots
+// are used. Tried and left, against 2.31 ms then: four threads to a row (2.48: the instructions grow by a quarter), scores held in registers between
+// maximum and exponential (2.61). 512 rows from position 0, 32 heads of 64, take 19 us, most of it one CTA's way through two tiles.
 
 #include <type_traits>
 

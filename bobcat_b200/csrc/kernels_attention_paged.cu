@@ -5,7 +5,7 @@
 // Units are cut into blocks of 128 positions (256 of heads of 64), and the blocks of all units, in order, into equal runs, one to a CTA: however
 // the lengths differ, every CTA reads about the same number of positions, a block or two fewer for each unit that it begins, and lengths stay on
 // the device (a captured call serves whatever they become).
-// (Twice as many runs, half as long: 117 us where these take 111.) A unit that lies in one CTA's run is written out by it; a unit that is cut leaves
+// (Twice as many runs, half as long: 5 % slower.) A unit that lies in one CTA's run is written out by it; a unit that is cut leaves
 // unnormalised sums with their maximum and sum of exponentials, at most two to a CTA, and a second launch joins them in order.
 //
 // Arithmetic. Elements are exact in half precision (8-bit ones as whole numbers, their scales multiply scores and probabilities in f32).
@@ -22,9 +22,9 @@
 // columns (hi in the first four, lo in the others, from rows of queries given twice), more take two multiplies. The tensor cores cut sums
 // off: what they add up is one step, and steps are added in f32, rounding.
 //
-// Measured: a token each of 64 sequences, 32 heads over 8 of 128, contexts of 500 to 8200: 8-bit pages, 589 MB, 112 us (5.3 TB/s; 116 where
-// units do not count two blocks beside their own, kUnitCost), halves, 1.14 GB, 190 us (6.0 TB/s). One sequence of 131 072 8-bit positions, 4 KV heads of 256: 273 MB in
-// 50 us (5.4 TB/s). Of the 112 us about ten are the launch's beginning and the join; CTAs of equal runs end 86 to 108 us after it. One sequence of 301
+// Measured: a token each of 64 sequences, 32 heads over 8 of 128, contexts of 500 to 8200: 8-bit pages, 589 MB, 112 to 120 us by the
+// device (5.2 to 4.9 TB/s; 4 more where units do not count two blocks beside their own, kUnitCost), halves, 1.14 GB, 190 to 199 us (6.0 to 5.8 TB/s). One sequence of 131 072 8-bit positions, 4 KV heads of 256: 273 MB in
+// 51 to 53 us (5.4 to 5.1 TB/s). Of the 112 us about ten are the launch's beginning and the join; CTAs of equal runs end 86 to 108 us after it. One sequence of 301
 // positions: 6 us, all of it latency.
 
 #include "async_utils.cuh"
@@ -841,7 +841,9 @@ uint64_t token_floats(uint32_t head_dim) {
 // beside that (8 of 5500 with 3 rows: 34 here, 55 there). So sequences of up to three rows are always taken here, and all of a call's, with no second
 // kernel, where what the tables can hold, 256 positions more for a unit's beginning and end, times the rows beyond three, is what those 20 us read: (us, here and
 // there) 8 sequences of up to 2900 positions with 2 to 5 rows 19 and 30, 64 of 500 with 4 rows 46 and 61, one of 1500 with 16 rows 16 and 21; past it 8 of 1100
-// with 16 rows 43 and 28, 64 of 100 with 8 rows 47 and 32.
+// with 16 rows 43 and 28, 64 of 100 with 8 rows 47 and 32. All these are 8 heads of 64. On nine layouts (halves and 8 bits; heads of 64, 128 and 256; one to eight query heads a KV head),
+// 4, 8 and 16 rows of 1 to 64 sequences of 500 to 5000 positions, 103 of 108 choices are the quicker form or within 10 % of it; the worst are 8 sequences of 5000 half positions of 8 heads of
+// 128 with 4 rows (80 here, 65 there) and 64 of 500, 2 heads of 64 of 7 query heads each, with 8 (30 and 23).
 constexpr uint32_t kTokenRows = 3, kFewRows = 32;
 bool few_rows(const KvPool& pool, const KvRows& rows) {
     if (rows.max_queries <= kTokenRows) return true;

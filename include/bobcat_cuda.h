@@ -245,18 +245,21 @@ typedef struct bc_kv_pool {
     bc_buffer* v;
     size_t v_off;
 } bc_kv_pool;
-/* The rows of a call, in device memory of 32-bit words: starts[n_seqs + 1] ascends, sequence s has rows starts[s] .. starts[s + 1] - 1 (none,
- * one, or more); lens[s] is the number of positions it holds, its rows the last of them: row r is position lens[s] - (starts[s + 1] - r).
- * table[s][max_pages] names its pages; entries behind its last position are not read. The op takes up to n_rows rows; rows behind
- * starts[n_seqs] belong to no sequence and are left as they are, in every output. The words are read when the op runs, at any time until it
- * ends, and stay as they are meanwhile; a captured call serves other lengths when it is replayed. max_queries, the most rows of one sequence as far as the caller knows, chooses
- * among kernels, with max_pages, and changes no more than rounding when it is wrong. 1 to 65535 sequences, up to 2^24 rows.
- * Rows that lie before a sequence's first position (more rows than positions) have no place: they are not written, read as zeros and attend to
- * nothing.
- * A position behind the table, or in a page that the pool does not have (its number is n_pages or more), cannot be written, reads as zeros, and is left out as a
- * key; the row of such a position attends to the keys up to its own position that are there, none of which gives zeros. The wait for the recording
- * (bc_wait, bc_end) returns BC_ERR_OUT_OF_BOUNDS, once; other recordings, other backends and steps of models do not. What a captured call meets when its
- * graph runs is returned by the next wait for a recording of its backend. */
+/* The rows of a call, in device memory of 32-bit words.
+ * starts[n_seqs + 1] ascends: sequence s has rows starts[s] .. starts[s + 1] - 1 (none, one, or more). lens[s] is the number of positions
+ * that it holds, its rows the last of them: row r is position lens[s] - (starts[s + 1] - r). table[s][max_pages] names its pages; entries
+ * behind its last position are not read. The op takes up to n_rows rows; rows behind starts[n_seqs] belong to no sequence and are left as
+ * they are, in every output. 1 to 65535 sequences, up to 2^24 rows.
+ * The words are read when the op runs, at any time until it ends, and stay as they are meanwhile; a captured call serves other lengths when
+ * it is replayed.
+ * max_queries, the most rows of one sequence as far as the caller knows, chooses among kernels, with max_pages. Where it is wrong, results
+ * change in rounding alone, and in whether an element that is not finite is an infinity or a NaN.
+ * Rows that lie before a sequence's first position (more rows than positions) have no place: they are not written, read as zeros and attend
+ * to nothing.
+ * A position behind the table, or in a page that the pool does not have (its number is n_pages or more), cannot be written, reads as zeros,
+ * and is left out as a key; the row of such a position attends to the keys up to its own position that are there (zeros where none is).
+ * The wait for the recording (bc_wait, bc_end) returns BC_ERR_OUT_OF_BOUNDS, once; other recordings, other backends and steps of models do
+ * not. What a captured call meets when its graph runs is returned by the next wait for a recording of its backend. */
 typedef struct bc_kv_rows {
     uint32_t n_seqs, n_rows, max_queries, max_pages;
     bc_buffer* table;
@@ -277,14 +280,16 @@ bc_status bc_op_kv_write(bc_backend* b, const bc_kv_pool* pool, const bc_kv_rows
 bc_status bc_op_kv_read(bc_backend* b, const bc_kv_pool* pool, const bc_kv_rows* rows, bc_buffer* k, size_t k_off, bc_buffer* v, size_t v_off,
                         int32_t out_half, uint32_t k_stride, uint32_t v_stride);
 /* Causal grouped-query attention of the rows over the pages: row r of sequence s sees positions 0 .. its own, which bc_op_kv_write has
- * stored. q is f32, token rows q_stride and heads q_head_stride elements apart (multiples of 4); out is [n_rows][n_heads * head_dim]
- * f32, zeros for a row that sees nothing; elements of positions that a row does not see have no part in it, whatever they are, and a value that is
- * not finite makes its element of the rows that see it not finite. A key that is not finite counts by the formula: where the score is minus infinity it weighs
- * nothing (a row all of whose scores are is zeros), else the rows that see it are NaN. Up to 8 query heads per KV head. q, scratch and out that overlap are refused. Scores and sums are f32; operands keep 22
- * bits: of a query element, or 2^-30 of its row's largest; of a probability, or 2^-40 of its row's largest; with 8-bit values, of a probability times the
- * values' scale, or 2^-32 of the largest of these that the row sees. (Sums of numbers above 2^80 may pass the largest float.) `scratch` needs
- * bc_attention_paged_scratch_floats floats (whatever the lengths), for the duration of the call: calls that may overlap, replayed graphs among
- * them, take one each. */
+ * stored. q is f32, token rows q_stride and heads q_head_stride elements apart (multiples of 4); out is [n_rows][n_heads * head_dim] f32,
+ * zeros for a row that sees nothing. Up to 8 query heads per KV head.
+ * Elements of positions that a row does not see have no part in it, whatever they are. A value that is not finite makes its element of the
+ * rows that see it not finite. A key that is not finite counts by the formula: where the score is minus infinity it weighs nothing (a row
+ * all of whose scores are is zeros), else the rows that see it are NaN.
+ * Scores and sums are f32. Operands keep 22 bits: of a query element, or 2^-30 of its row's largest; of a probability, or 2^-40 of its row's
+ * largest; with 8-bit values, of a probability times the values' scale, or 2^-32 of the largest of these that the row sees. Sums of numbers
+ * above 2^80 may pass the largest float.
+ * `scratch` needs bc_attention_paged_scratch_floats floats (whatever the lengths), for the duration of the call: calls that may overlap,
+ * replayed graphs among them, take one each. q, scratch and out that overlap are refused. */
 size_t bc_attention_paged_scratch_floats(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim);
 bc_status bc_op_attention_paged(bc_backend* b, const bc_kv_pool* pool, const bc_kv_rows* rows, bc_buffer* q, size_t q_off, bc_buffer* scratch,
                                 size_t s_off, bc_buffer* out, size_t out_off, uint32_t n_heads, uint32_t q_stride, uint32_t q_head_stride);
