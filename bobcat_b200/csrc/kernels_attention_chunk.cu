@@ -1024,9 +1024,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
                     if (lane == 0 && at.in_unit == at.unit.tiles) {
                         some = at.cursor.take(p.rows.starts, p.rows.lens, p.rows.n_seqs, p.rows.n_rows, pool.n_kv_heads, capacity, p.fewest, at.unit);
                         at.in_unit = 0;
-                        if (++at.unit_number == 0) at.span = ChunkSpan{{at.unit.seq, 0}, {at.unit.head, 0}, {at.unit.row_tile, 0}, {}};
+                        if (++at.unit_number == 0 && FMT == BC_F16) at.span = ChunkSpan{{at.unit.seq, 0}, {at.unit.head, 0}, {at.unit.row_tile, 0}, {}};
                     }
-                    // The run's tiles have been counted. One that ends before, since the call's words have changed since, is given up.
+                    // The run's tiles have been counted. One that ends before, since the call's words have changed since, is given up here: what the cursor holds then
+                    // describes no rows of the call.
                     alive = __all_sync(0xffffffffu, some);
                     if (!alive) {
                         if (lane == 0) give_up(dead, 17);
@@ -1105,8 +1106,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_chunk_paged_kernel(cons
             }
             if (lane == 0) {
                 chunk_heads(p.parts, HD)[blockIdx.x] = alive ? at.cut : ChunkHead{};
-                at.span.seq[1] = at.unit.seq, at.span.head[1] = at.unit.head, at.span.row_tile[1] = at.unit.row_tile;
-                chunk_spans(p.parts, HD)[blockIdx.x] = at.span;
+                if constexpr (FMT == BC_F16) {
+                    at.span.seq[1] = at.unit.seq, at.span.head[1] = at.unit.head, at.span.row_tile[1] = at.unit.row_tile;
+                    chunk_spans(p.parts, HD)[blockIdx.x] = at.span;
+                }
             }
             // Copies in flight end before the CTA does: the unpacking warps wait for them, or this one does when those gave up.
             for (uint32_t r = 0; r < RAW && r < keys_issued && *dead; ++r) {
