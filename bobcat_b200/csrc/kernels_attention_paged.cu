@@ -81,25 +81,6 @@ __device__ __forceinline__ void mma_i8(uint32_t (&c)[4], const uint4& a, uint32_
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                  : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float exp2_fast(float x) {  // results below the normal numbers are zero
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {  // two in one instruction
-    float2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(reinterpret_cast<uint64_t&>(r))
-        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
-    return r;
-}
-__device__ __forceinline__ void split_half2(float x, float y, uint32_t& hi, uint32_t& lo) {
-    __half2 h = __floats2half2_rn(x, y);
-    float2 back = __half22float2(h);
-    __half2 l = __floats2half2_rn(x - back.x, y - back.y);
-    hi = *reinterpret_cast<uint32_t*>(&h);
-    lo = *reinterpret_cast<uint32_t*>(&l);
-}
 
 // A warp's ring: steps under way, and where a step's keys, values and scales lie in it. Two rows of keys that a load's phase covers fall 64
 // bytes apart, four of values (every other one) 32.

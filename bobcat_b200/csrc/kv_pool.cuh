@@ -66,6 +66,28 @@ __device__ __forceinline__ void unpack_i8(uint32_t w, uint32_t& lo, uint32_t& hi
     hi = *reinterpret_cast<uint32_t*>(&y);
 }
 
+// Arithmetic of both kernels of attention over pages.
+__device__ __forceinline__ float exp2_fast(float x) {  // results below the normal numbers are zero
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {  // two in one instruction
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)), "l"(reinterpret_cast<uint64_t&>(c)));
+    return r;
+}
+// (x, y) as halves and what they leave over, as halves.
+__device__ __forceinline__ void split_half2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    __half2 h = __floats2half2_rn(x, y);
+    float2 back = __half22float2(h);
+    __half2 l = __floats2half2_rn(x - back.x, y - back.y);
+    hi = *reinterpret_cast<uint32_t*>(&h);
+    lo = *reinterpret_cast<uint32_t*>(&l);
+}
+
 // Whether the score of a query with a half key that is not finite is minus infinity: every infinite element's product with the query's is, and there is no NaN.
 // (Products of a query's halves with an infinity need not have its sign, and are no number where a half is zero.)
 __device__ __forceinline__ bool score_is_minus_infinity(const float* q, const uint8_t* key, uint32_t head_dim) {
